@@ -354,6 +354,123 @@ PFC_API int pfk_matmul_tf32x3_static(const float* a, const float* b, float* c, i
  * usable.  No counterpart in the reference. */
 PFC_API int pfk_check_bounded_wait(int* err, int64_t limit_us, void* stream);
 
+/* ---- token generation over a paged key-value cache ------------------------ */
+/* The pieces of a decoder layer's step for new tokens: products with 4-bit
+ * weights, rotary positions, appending keys and values to a paged cache, and
+ * attention of one new token per sequence over that cache.  They have no
+ * counterpart in the reference.  dtype is PFC_DTYPE_FLOAT32, FLOAT16 or
+ * BFLOAT16; strides count elements and the last axis is contiguous.  Each
+ * call launches on `stream` on the current device, allocates nothing, does
+ * not synchronise and may be captured into a CUDA graph.  Arguments that the
+ * host can see are checked and refused with PFC_ERR_INVALID_ARGUMENT; page
+ * numbers, slots and lengths are device data, which the kernels check: they
+ * skip a bad one and set the cache's `err`. */
+
+/* Rotary positions: pair i of a head's first rotary_dim values is turned by
+ * the angle positions * inv_freq[i], taken in 64 bits, and its cosine and
+ * sine are multiplied by `factor`.  The values behind rotary_dim are copied. */
+typedef struct pfk_rotary {
+    const double* inv_freq; /* device, rotary_dim / 2 angles per position */
+    int64_t rotary_dim;     /* even, at most head_dim; 0: no rotation */
+    int interleaved;        /* 0: pairs (i, i + rotary_dim/2); 1: pairs (2i, 2i + 1) */
+    float factor;
+} pfk_rotary;
+
+typedef struct pfk_rope_params {
+    int dtype;
+    int inverse; /* 1: turn by the negative angle (the gradient with respect to x) */
+    int64_t batch, tokens, heads, head_dim; /* head_dim at most 1024 */
+    int64_t x_sb, x_st, x_sh;               /* strides of x over batch, token, head */
+    int64_t y_sb, y_st, y_sh;
+    const int64_t* positions; /* of (b, t) at positions[b*p_sb + t*p_st] */
+    int64_t p_sb, p_st;
+    pfk_rotary rotary;
+} pfk_rope_params;
+/* y = x rotated; y may be x itself (same pointer and strides), and may not
+ * overlap it otherwise. */
+PFC_API int pfk_rope(const void* x, void* y, const pfk_rope_params* p, void* stream);
+
+/* A paged cache: token `o` of page `p` of head `h` is at
+ * p*page_stride + o*token_stride + h*head_stride of k and of v.  Slot
+ * numbers are page * page_size + o. */
+typedef struct pfk_paged_cache {
+    int dtype;
+    void* k;
+    void* v;
+    int64_t num_pages, page_size, heads, head_dim; /* num_pages * page_size below 2^31 */
+    int64_t page_stride, token_stride, head_stride;
+    int* err; /* device int or NULL: set to PFC_ERR_INVALID_ARGUMENT when a kernel meets a slot, page or
+                 length outside the cache (what it names is then skipped) */
+} pfk_paged_cache;
+
+typedef struct pfk_paged_append_params {
+    pfk_paged_cache cache;
+    int64_t tokens;
+    const void* k; /* [tokens][heads][head_dim] */
+    int64_t k_st, k_sh;
+    const void* v;
+    int64_t v_st, v_sh;
+    const void* q; /* [tokens][q_heads][head_dim], rotated into q_out (which may be q); NULL: none */
+    void* q_out;
+    int64_t q_heads, q_st, q_sh, qo_st, qo_sh;
+    const int64_t* slots;     /* [tokens]; negative: the token is skipped, its q_out row left as it was */
+    const int64_t* positions; /* [tokens]; may be NULL without rotation */
+    pfk_rotary rotary;        /* of k and q; rotary_dim 0: copied as they are */
+} pfk_paged_append_params;
+/* Stores rotated keys, values as they are, and rotated queries in one pass.
+ * The slots of one call are distinct; of tokens that name the same slot, any
+ * one's values may remain. */
+PFC_API int pfk_paged_append(const pfk_paged_append_params* p, void* stream);
+
+typedef struct pfk_paged_attention_params {
+    pfk_paged_cache cache; /* head_dim a multiple of 8 and at most 256; k, v and the strides multiples of 16 bytes */
+    int64_t batch, q_heads; /* q_heads a multiple of the cache's heads */
+    const void* q;          /* [batch][q_heads][head_dim] */
+    int64_t q_sb, q_sh;
+    void* out; /* [batch][q_heads][head_dim] */
+    int64_t o_sb, o_sh;
+    float* lse; /* [batch][q_heads] dense: natural log of the sum of exp(score), or NULL */
+    const int32_t* block_table; /* page of tokens [i*page_size, (i+1)*page_size) of sequence b at [b*table_stride + i] */
+    int64_t table_stride, table_width;
+    const int32_t* seq_lens; /* [batch]; 0: out is 0 and lse -infinity */
+    int64_t window;          /* only the last `window` tokens are seen; 0: all */
+    float scale;             /* of q.k */
+    void* workspace;         /* pfk_paged_attention_workspace bytes, 16-byte aligned, not shared by calls that may
+                                overlap; its contents are neither read from earlier calls nor kept */
+    size_t workspace_bytes;
+} pfk_paged_attention_params;
+PFC_API int pfk_paged_attention_workspace(const pfk_paged_attention_params* p, size_t* bytes);
+/* out[b,h] = sum_j softmax_j(scale * q[b,h].k[j]) v[j] over the tokens j of
+ * sequence b, with key-value head h / (q_heads / heads).  Infinite or NaN
+ * values in a seen row make that sequence's result NaN; what lies in a page
+ * outside the seen tokens has no effect. */
+PFC_API int pfk_paged_attention(const pfk_paged_attention_params* p, void* stream);
+
+/* Arranges 4-bit weights for pfk_linear_w4.  packed: [outer][(inner+1)/2]
+ * bytes, column 2i in the low half of byte i.  weight: [outer][ru(inner)/8]
+ * words, ru = round up to 128: block b of 128 columns is 16 words; word
+ * 4*t + j holds columns 128b + 32j + 8t ... + 7, the columns in the order
+ * 0, 2, 4, 6, 1, 3, 5, 7 from the lowest nibble up. */
+PFC_API int pfk_w4_arrange(const uint8_t* packed, int64_t outer, int64_t inner, uint32_t* weight, void* stream);
+
+typedef struct pfk_linear_w4_params {
+    int dtype; /* of x, y and bias */
+    int64_t rows, inner, outer;
+    int64_t group;  /* columns that share a scale: 32, 64 or a multiple of 128 */
+    const void* x;  /* [rows][inner] */
+    int64_t x_st;
+    void* y; /* [rows][outer] */
+    int64_t y_st;
+    const uint32_t* weight; /* pfk_w4_arrange's output, 16-byte aligned */
+    const void* scales;     /* [outer][ceil(inner/group)] dense */
+    int scale_dtype;
+    const uint8_t* zeros; /* [outer][ceil(inner/group)], 0..15, or NULL: 8 */
+    const void* bias;     /* [outer] or NULL */
+} pfk_linear_w4_params;
+/* y[m,n] = sum_k x[m,k] * (w[n,k] - zero) * scale (+ bias[n]), accumulated in
+ * fp32 from products that are not rounded before. */
+PFC_API int pfk_linear_w4(const pfk_linear_w4_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,10 +5,11 @@ tensors, graph nodes, ops, nn modules, device selection and `eval`, with
 'cuda[:N]' as the device.  Evaluation runs on sm_100a GPUs through
 libpyflame_cuda.so (include/pyflame_cuda.h); there is no CPU evaluation path.
 """
-from . import autograd, ir, nn, serving
+from . import autograd, decoding, ir, nn, serving
 from .backend import (Backend, CudaExecutor, DeviceInfo, ExecutionResult, Executor, ExecutorConfig, MemoryStats,
                       cuda_device_count, cuda_get_device, cuda_get_device_info, cuda_is_available, cuda_set_device,
                       cuda_synchronize)
+from .decoding import Linear4bit, PagedKVCache, RotaryEmbedding, rotary_frequencies
 from .device import device_info, eval, get_device, set_device, set_precision, synchronize
 from .ir import DType, Graph, Node, NodeType, OpType, TensorSpec, dtype_name, dtype_size
 from .tensor import (Tensor, abs, arange, broadcast_to, cat, clamp, cos, exp, from_numpy, full, gelu,

@@ -62,6 +62,43 @@ class PoolParamsC(C.Structure):
 
 _P = C.c_void_p
 _I64 = C.c_int64
+
+
+class RotaryC(C.Structure):
+    _fields_ = [("inv_freq", _P), ("rotary_dim", _I64), ("interleaved", C.c_int), ("factor", C.c_float)]
+
+
+class RopeParamsC(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("inverse", C.c_int)] + [(n, _I64) for n in (
+        "batch", "tokens", "heads", "head_dim", "x_sb", "x_st", "x_sh", "y_sb", "y_st", "y_sh")] + [
+        ("positions", _P), ("p_sb", _I64), ("p_st", _I64), ("rotary", RotaryC)]
+
+
+class PagedCacheC(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("k", _P), ("v", _P)] + [(n, _I64) for n in (
+        "num_pages", "page_size", "heads", "head_dim", "page_stride", "token_stride", "head_stride")] + [("err", _P)]
+
+
+class PagedAppendParamsC(C.Structure):
+    _fields_ = [("cache", PagedCacheC), ("tokens", _I64), ("k", _P), ("k_st", _I64), ("k_sh", _I64), ("v", _P),
+                ("v_st", _I64), ("v_sh", _I64), ("q", _P), ("q_out", _P)] + [(n, _I64) for n in (
+                    "q_heads", "q_st", "q_sh", "qo_st", "qo_sh")] + [
+        ("slots", _P), ("positions", _P), ("rotary", RotaryC)]
+
+
+class PagedAttentionParamsC(C.Structure):
+    _fields_ = [("cache", PagedCacheC), ("batch", _I64), ("q_heads", _I64), ("q", _P), ("q_sb", _I64),
+                ("q_sh", _I64), ("out", _P), ("o_sb", _I64), ("o_sh", _I64), ("lse", _P), ("block_table", _P),
+                ("table_stride", _I64), ("table_width", _I64), ("seq_lens", _P), ("window", _I64),
+                ("scale", C.c_float), ("workspace", _P), ("workspace_bytes", C.c_size_t)]
+
+
+class LinearW4ParamsC(C.Structure):
+    _fields_ = [("dtype", C.c_int)] + [(n, _I64) for n in ("rows", "inner", "outer", "group")] + [
+        ("x", _P), ("x_st", _I64), ("y", _P), ("y_st", _I64), ("weight", _P), ("scales", _P),
+        ("scale_dtype", C.c_int), ("zeros", _P), ("bias", _P)]
+
+
 # name -> (restype, argtypes); the list is the C-ABI of include/pyflame_cuda.h
 SIGNATURES = {
     "pfc_cuda_is_available": (C.c_int, []),
@@ -106,6 +143,12 @@ SIGNATURES = {
     "pfk_pool2d": (C.c_int, [_P, _P, C.POINTER(PoolParamsC), _P]),
     "pfk_matmul_tf32x3_static": (C.c_int, [_P, _P, _P, _I64, _I64, _I64, _P, _P]),
     "pfk_check_bounded_wait": (C.c_int, [_P, _I64, _P]),
+    "pfk_rope": (C.c_int, [_P, _P, C.POINTER(RopeParamsC), _P]),
+    "pfk_paged_append": (C.c_int, [C.POINTER(PagedAppendParamsC), _P]),
+    "pfk_paged_attention_workspace": (C.c_int, [C.POINTER(PagedAttentionParamsC), C.POINTER(C.c_size_t)]),
+    "pfk_paged_attention": (C.c_int, [C.POINTER(PagedAttentionParamsC), _P]),
+    "pfk_w4_arrange": (C.c_int, [_P, _I64, _I64, _P, _P]),
+    "pfk_linear_w4": (C.c_int, [C.POINTER(LinearW4ParamsC), _P]),
 }
 
 _lib = None

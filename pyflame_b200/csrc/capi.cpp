@@ -505,4 +505,43 @@ int pfk_pool2d(const float* x, float* y, const pfk_pool_params* p, void* stream)
   });
 }
 
+int pfk_rope(const void* x, void* y, const pfk_rope_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_rope(x, y, *p, as_stream(stream));
+  });
+}
+
+int pfk_paged_append(const pfk_paged_append_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_paged_append(*p, as_stream(stream));
+  });
+}
+
+int pfk_paged_attention_workspace(const pfk_paged_attention_params* p, size_t* bytes) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p && bytes, "null argument");
+    *bytes = pfb::paged_attention_workspace(*p);
+  });
+}
+
+int pfk_paged_attention(const pfk_paged_attention_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_paged_attention(*p, as_stream(stream));
+  });
+}
+
+int pfk_w4_arrange(const uint8_t* packed, int64_t outer, int64_t inner, uint32_t* weight, void* stream) {
+  return guarded([&] { pfb::launch_w4_arrange(packed, outer, inner, weight, as_stream(stream)); });
+}
+
+int pfk_linear_w4(const pfk_linear_w4_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_linear_w4(*p, as_stream(stream));
+  });
+}
+
 }  // extern "C"

@@ -5,6 +5,8 @@
 
 #include <cstdint>
 
+#include "../../../include/pyflame_cuda.h"
+
 namespace pfb {
 
 struct GemmLaunch {
@@ -253,5 +255,14 @@ struct BnFoldLaunch {
   float* shift = nullptr;
 };
 void launch_bn_fold(const BnFoldLaunch& L, cudaStream_t stream);
+
+// Token generation over a paged key-value cache (the C ABI's parameter
+// structs; each launcher checks what the host can see of them).
+void launch_rope(const void* x, void* y, const pfk_rope_params& p, cudaStream_t stream);
+void launch_paged_append(const pfk_paged_append_params& p, cudaStream_t stream);
+size_t paged_attention_workspace(const pfk_paged_attention_params& p);
+void launch_paged_attention(const pfk_paged_attention_params& p, cudaStream_t stream);
+void launch_w4_arrange(const uint8_t* packed, int64_t outer, int64_t inner, uint32_t* weight, cudaStream_t stream);
+void launch_linear_w4(const pfk_linear_w4_params& p, cudaStream_t stream);
 
 }  // namespace pfb

@@ -1,0 +1,454 @@
+"""Token generation over a paged key-value cache.
+
+The steps of a decoder layer for new tokens, on CUDA tensors of torch (the
+memory that `CudaExecutor.execute_device` also takes), in float32, float16 or
+bfloat16:
+
+  Linear4bit        x W^T (+ bias) with 4-bit weights and group scales
+  RotaryEmbedding   rotary positions of queries and keys, and their gradient
+  PagedKVCache      append(): store new keys and values, rotated on the way;
+                    attend(): attention of one new token per sequence
+
+They are hand-written kernels of libpyflame_cuda.so (the pfk_* entry points of
+include/pyflame_cuda.h).  Every call runs on torch's current stream of its
+tensors' device, does not synchronise, and may be captured into a CUDA graph
+(each captured call has its own workspace, from torch's allocator).  Arguments
+are checked on the host; a wrong one raises ValueError or TypeError.  Page
+numbers, slots and lengths are device data: a kernel that meets a bad one skips
+it and sets the cache's error flag, which `PagedKVCache.check()` raises.
+
+The calls take part in no autograd graph of torch and refuse tensors that
+require a gradient; RotaryEmbedding.backward is the rotation's gradient.  They
+have no counterpart in PyFlame.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional
+
+import numpy as np
+
+from . import _native as N
+from .ir import DType
+
+_codes = None
+
+
+def _code(dtype) -> int:
+    """pfc_dtype of a torch dtype that the kernels take."""
+    global _codes
+    if _codes is None:
+        import torch
+        _codes = {torch.float32: int(DType.float32), torch.float16: int(DType.float16),
+                  torch.bfloat16: int(DType.bfloat16)}
+    c = _codes.get(dtype)
+    if c is None:
+        raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
+    return c
+
+
+def _check(name: str, t, shape, dtype, device, last_contiguous: bool = True, output: bool = False) -> None:
+    """`shape` holds None where any size will do."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: dtype must be {dtype}, not {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name}: is on {t.device}, not on {device}")
+    if len(t.shape) != len(shape) or any(w is not None and w != s for w, s in zip(shape, t.shape)):
+        raise ValueError(f"{name}: shape must be {[('any' if w is None else w) for w in shape]}, not {list(t.shape)}")
+    if last_contiguous and t.shape and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last axis must be contiguous")
+    if t.requires_grad:
+        import torch
+        if torch.is_grad_enabled():
+            raise RuntimeError(f"{name}: requires a gradient, which this call does not record (detach it)")
+    if output and any(st == 0 and s > 1 for s, st in zip(t.shape, t.stride())):
+        raise ValueError(f"{name}: an output may not have elements that share memory")
+
+
+def _cuda(t, name: str):
+    if t.device.type != "cuda":
+        raise ValueError(f"{name}: must be on a CUDA device, not on {t.device}")
+    return t.device
+
+
+def _call(fn, device, *args) -> None:
+    """One entry point on the current stream of `device`."""
+    import torch
+    cuda = torch.cuda
+    stream = C.c_void_p(cuda.current_stream(device).cuda_stream)
+    if cuda.current_device() == device.index:
+        N.check(fn(*args, stream))
+    else:
+        with cuda.device(device):
+            N.check(fn(*args, stream))
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None):
+    """(inv_freq, factor): the angle per position of each of rotary_dim / 2
+    pairs, as float64, and the factor on cosines and sines.
+
+    `scaling` stretches the positions of a model to longer contexts:
+      {"type": "linear", "factor": f}   every frequency divided by f
+      {"type": "ntk", "factor": f}      the base multiplied by f^(d / (d - 2)): the lowest frequency is divided by f,
+                                        the highest kept
+      {"type": "yarn", "factor": f, "original_max_position": n [, "beta_fast": 32, "beta_slow": 1,
+       "attention_factor": 0.1 ln f + 1]}
+                                        pairs that turn more than beta_fast times in n positions keep their frequency,
+                                        those below beta_slow turns are divided by f, a ramp between them
+    """
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even and not negative")
+    if not (base > 0 and math.isfinite(base)) or base == 1.0:
+        raise ValueError("base must be positive, finite and not 1")
+    i = np.arange(rotary_dim // 2, dtype=np.float64)
+    factor = 1.0
+    if scaling is None:
+        return base ** (-2.0 * i / max(1, rotary_dim)), factor
+    kind, f = scaling.get("type"), float(scaling.get("factor", 0.0))
+    known = {"linear": {"type", "factor"}, "ntk": {"type", "factor"},
+             "yarn": {"type", "factor", "original_max_position", "beta_fast", "beta_slow", "attention_factor"}}
+    if kind not in known:
+        raise ValueError(f"scaling type must be one of {sorted(known)}, not {kind!r}")
+    if set(scaling) - known[kind]:
+        raise ValueError(f"{kind} scaling has no {sorted(set(scaling) - known[kind])}")
+    if not (f >= 1.0 and math.isfinite(f)):
+        raise ValueError("scaling factor must be at least 1")
+    if kind == "ntk":
+        if rotary_dim <= 2:
+            raise ValueError("ntk scaling needs rotary_dim above 2")
+        base = base * f ** (rotary_dim / (rotary_dim - 2))
+    inv = base ** (-2.0 * i / max(1, rotary_dim))
+    if kind == "linear":
+        inv = inv / f
+    if kind == "yarn":
+        n = float(scaling.get("original_max_position", 0))
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+        if not n > 0 or not fast > slow > 0:
+            raise ValueError("yarn scaling needs original_max_position > 0 and beta_fast > beta_slow > 0")
+
+        def pair_of(turns):  # the pair that turns so often in n positions
+            return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
+        ramp = np.clip((i - low) / max(high - low, 0.001), 0.0, 1.0)
+        inv = inv * (1.0 - ramp) + inv / f * ramp
+        factor = float(scaling.get("attention_factor", 0.1 * math.log(f) + 1.0))
+    return inv, factor
+
+
+class RotaryEmbedding:
+    """Rotary positions of the first `rotary_dim` values of a head.
+
+    layout "half" turns the pairs (i, i + rotary_dim/2), "interleaved" the
+    pairs (2i, 2i + 1), by position * inv_freq[i].  Angles are formed and
+    reduced in 64 bits, so far positions lose nothing.  `inv_freq` (a sequence
+    of rotary_dim / 2 numbers) replaces base and scaling (rotary_frequencies).
+    """
+
+    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, layout: str = "half",
+                 scaling: Optional[dict] = None, inv_freq=None, factor: float = 1.0, device="cuda"):
+        import torch
+        rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
+        if not 1 <= head_dim <= 1024:
+            raise ValueError("head_dim must be 1 to 1024")
+        if not 0 <= rotary_dim <= head_dim or rotary_dim % 2:
+            raise ValueError("rotary_dim must be even and at most head_dim")
+        if layout not in ("half", "interleaved"):
+            raise ValueError("layout must be 'half' or 'interleaved'")
+        if inv_freq is None:
+            inv_freq, scaled = rotary_frequencies(rotary_dim, base, scaling)
+            factor = factor * scaled
+        elif scaling is not None:
+            raise ValueError("inv_freq and scaling exclude each other")
+        inv_freq = np.asarray(inv_freq, dtype=np.float64)
+        if inv_freq.shape != (rotary_dim // 2,):
+            raise ValueError(f"inv_freq must hold {rotary_dim // 2} numbers")
+        self.head_dim, self.rotary_dim, self.layout, self.factor = int(head_dim), rotary_dim, layout, float(factor)
+        # a copy of the caller's: the device's table may not change with it
+        self.inv_freq = torch.from_numpy(inv_freq.copy()).to(torch.device(device))
+        _cuda(self.inv_freq, "device")
+        self.device = self.inv_freq.device
+        self._c = N.RotaryC(self.inv_freq.data_ptr(), rotary_dim, int(layout == "interleaved"), self.factor)
+
+    def _run(self, x, positions, out, inverse: int):
+        import torch
+        _cuda(x, "x")
+        dims = len(x.shape)
+        if dims not in (3, 4):
+            raise ValueError("x must be [tokens, heads, head_dim] or [batch, tokens, heads, head_dim]")
+        code = _code(x.dtype)
+        _check("x", x, (None,) * (dims - 1) + (self.head_dim,), x.dtype, self.device)
+        xs = x.stride()
+        batch, tokens, heads = (1,) * (4 - dims) + tuple(x.shape[:-1])
+        if len(positions.shape) == 2 and dims == 4:
+            _check("positions", positions, (batch, tokens), torch.int64, self.device, False)
+            p_sb, p_st = positions.stride()
+        else:
+            _check("positions", positions, (tokens,), torch.int64, self.device, False)
+            p_sb, p_st = 0, positions.stride(0)
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        else:
+            _check("out", out, x.shape, x.dtype, self.device, output=True)
+            if out.data_ptr() == x.data_ptr() and out.stride() != xs and x.numel():
+                raise ValueError("out: shares x's memory with other strides")
+        ys = out.stride()
+        p = N.RopeParamsC(code, inverse, batch, tokens, heads, self.head_dim, xs[0] if dims == 4 else 0, xs[-3], xs[-2],
+                          ys[0] if dims == 4 else 0, ys[-3], ys[-2], positions.data_ptr(), p_sb, p_st, self._c)
+        _call(N.lib().pfk_rope, self.device, x.data_ptr(), out.data_ptr(), C.byref(p))
+        return out
+
+    def apply(self, x, positions, out=None):
+        """x rotated.  x: [tokens, heads, head_dim] or [batch, tokens, heads,
+        head_dim], any strides with a contiguous head; positions: int64
+        [tokens] (shared by a batch) or [batch, tokens].  `out` may be x."""
+        return self._run(x, positions, out, 0)
+
+    def backward(self, dy, positions, out=None):
+        """The gradient with respect to x, given the gradient dy with respect
+        to apply(x, positions): the rotation by the negative angles."""
+        return self._run(dy, positions, out, 1)
+
+
+# ---------------------------------------------------------------------------
+# paged cache
+# ---------------------------------------------------------------------------
+
+class PagedKVCache:
+    """Keys and values of many sequences in pages of `page_size` tokens.
+
+    `k` and `v` are [num_pages, page_size, num_heads, head_dim]; token i of a
+    sequence is at offset i % page_size of page block_table[sequence, i //
+    page_size].  Which pages a sequence owns is the caller's bookkeeping.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, num_heads: int, head_dim: int, dtype=None, device="cuda"):
+        import torch
+        dtype = torch.float32 if dtype is None else dtype
+        _code(dtype)
+        shape = (int(num_pages), int(page_size), int(num_heads), int(head_dim))
+        if any(s < 1 for s in shape):
+            raise ValueError("sizes must be positive")
+        self._take(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+
+    @classmethod
+    def from_tensors(cls, k, v) -> "PagedKVCache":
+        """A cache in the caller's tensors, [num_pages, page_size, num_heads,
+        head_dim] with the same strides and a contiguous head (heads stored
+        before tokens: the permuted view)."""
+        self = cls.__new__(cls)
+        self._take(k, v)
+        return self
+
+    def _take(self, k, v):
+        import torch
+        device = _cuda(k, "k")
+        code = _code(k.dtype)
+        _check("k", k, (None,) * 4, k.dtype, device, output=True)
+        _check("v", v, tuple(k.shape), k.dtype, device, output=True)
+        if k.stride() != v.stride():
+            raise ValueError("k and v must have the same strides")
+        if k.numel() == 0:
+            raise ValueError("sizes must be positive")
+        if k.shape[0] * k.shape[1] > 0x7FFFFFFF:
+            raise ValueError("a cache holds fewer than 2^31 tokens")
+        self.k, self.v, self.device, self.dtype = k, v, device, k.dtype
+        self.num_pages, self.page_size, self.num_heads, self.head_dim = k.shape
+        self._err = torch.zeros(1, dtype=torch.int32, device=device)
+        self._c = N.PagedCacheC(code, k.data_ptr(), v.data_ptr(), *k.shape, *k.stride()[:3], self._err.data_ptr())
+        self._workspace = {}
+        self._no_rotary = N.RotaryC(None, 0, 0, 1.0)
+
+    def append(self, k, v, slots, positions=None, rotary: Optional[RotaryEmbedding] = None, q=None, q_out=None):
+        """Store new tokens: k, v [tokens, num_heads, head_dim] at `slots`
+        (int64 [tokens], page * page_size + offset; negative: the token is
+        skipped).  With `rotary`, keys and queries q [tokens, q_heads,
+        head_dim] are rotated by `positions` (int64 [tokens]); returns the
+        rotated queries (`q_out`, which may be q, or a new tensor, whose rows
+        of skipped tokens are 0).  The slots of one call are distinct."""
+        import torch
+        n, h, d = len(k), self.num_heads, self.head_dim
+        _check("k", k, (n, h, d), self.dtype, self.device)
+        _check("v", v, (n, h, d), self.dtype, self.device)
+        _check("slots", slots, (n,), torch.int64, self.device)
+        if (rotary is None) != (positions is None):
+            raise ValueError("positions and rotary go together")
+        turn, at = self._no_rotary, None
+        if rotary is not None:
+            if rotary.head_dim != d or rotary.device != self.device:
+                raise ValueError("rotary: is for another head_dim or device")
+            _check("positions", positions, (n,), torch.int64, self.device)
+            turn, at = rotary._c, positions.data_ptr()
+        ks, vs = k.stride(), v.stride()
+        p = N.PagedAppendParamsC(self._c, n, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1])
+        if q is not None:
+            _check("q", q, (n, None, d), self.dtype, self.device)
+            if q_out is None:
+                q_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+            else:
+                _check("q_out", q_out, q.shape, self.dtype, self.device, output=True)
+                if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride() and q.numel():
+                    raise ValueError("q_out: shares q's memory with other strides")
+            qs, os = q.stride(), q_out.stride()
+            p.q, p.q_out, p.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
+            p.q_st, p.q_sh, p.qo_st, p.qo_sh = qs[0], qs[1], os[0], os[1]
+            if not p.q_heads:
+                p.q = p.q_out = None
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        p.slots, p.positions, p.rotary = slots.data_ptr(), at, turn
+        _call(N.lib().pfk_paged_append, self.device, C.byref(p))
+        return q_out
+
+    def attend(self, q, block_table, seq_lens, scale: Optional[float] = None, window: int = 0, out=None,
+               return_lse: bool = False):
+        """Attention of one new token per sequence, its own key among the
+        cached: q [batch, q_heads, head_dim] (q_heads a multiple of num_heads;
+        query head h reads key-value head h // (q_heads / num_heads)),
+        block_table int32 [batch, pages], seq_lens int32 [batch].  `scale`
+        (1/sqrt(head_dim) by default) multiplies the scores; `window` > 0: only
+        a sequence's last `window` tokens are seen.  A sequence of length 0
+        gives 0.  With return_lse also the natural logarithm of the sum of
+        exp(score), float32 [batch, q_heads] (-inf for length 0)."""
+        import torch
+        if len(q.shape) != 3:
+            raise ValueError("q must be [batch, q_heads, head_dim]")
+        batch, heads, d = q.shape
+        _check("q", q, (None, None, self.head_dim), self.dtype, self.device)
+        if heads == 0 or heads % self.num_heads:
+            raise ValueError(f"q: {heads} heads are not a multiple of {self.num_heads}")
+        _check("block_table", block_table, (batch, None), torch.int32, self.device)
+        _check("seq_lens", seq_lens, (batch,), torch.int32, self.device)
+        if window < 0:
+            raise ValueError("window must not be negative")
+        scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+        if out is None:
+            out = torch.empty((batch, heads, d), dtype=q.dtype, device=q.device)
+        else:
+            _check("out", out, (batch, heads, d), self.dtype, self.device, output=True)
+        lse = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        qs, os = q.stride(), out.stride()
+        p = N.PagedAttentionParamsC(self._c, batch, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+                                    lse.data_ptr() if return_lse else None, block_table.data_ptr(),
+                                    block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), int(window), scale)
+        need = self._workspace.get((batch, heads))
+        if need is None:
+            size = C.c_size_t(0)
+            with torch.cuda.device(self.device):
+                N.check(N.lib().pfk_paged_attention_workspace(C.byref(p), C.byref(size)))
+            need = self._workspace[batch, heads] = size.value
+        # a workspace per call, from torch's allocator: calls on several streams and captured graphs share none
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        p.workspace, p.workspace_bytes = work.data_ptr(), need
+        _call(N.lib().pfk_paged_attention, self.device, C.byref(p))
+        return (out, lse) if return_lse else out
+
+    def check(self) -> None:
+        """Wait for the device and raise PfcError if a call met a slot, page
+        or length outside the cache since the last check."""
+        code = int(self._err.item())
+        if code:
+            self._err.zero_()
+            raise N.PfcError(code, "a call met a slot, page or length outside the paged cache")
+
+
+# ---------------------------------------------------------------------------
+# 4-bit weights
+# ---------------------------------------------------------------------------
+
+class Linear4bit:
+    """y = x W^T + bias with W[n, k] = (q[n, k] - zeros[n, k // group]) *
+    scales[n, k // group], q from 0 to 15.
+
+    packed: uint8 [out_features, (in_features + 1) // 2], column 2i in the low
+    half of byte i; scales: float32, float16 or bfloat16 [out_features,
+    ceil(in_features / group_size)]; zeros: uint8 of the same shape, 0 to 15,
+    or None for 8; bias: [out_features] of the type of x, or None; group_size:
+    32, 64 or a multiple of 128.  The constructor lays the weights out for the
+    kernel once.  For single tokens and batches of up to some tens of rows;
+    more rows read the weights again for every 64 (21 in float32).
+    """
+
+    def __init__(self, packed, scales, zeros=None, bias=None, in_features: Optional[int] = None, group_size: int = 128):
+        import torch
+        device = _cuda(packed, "packed")
+        if len(packed.shape) != 2 or 0 in packed.shape:
+            raise ValueError("packed must be [out_features, (in_features + 1) // 2]")
+        n = packed.shape[0]
+        k = 2 * packed.shape[1] if in_features is None else int(in_features)
+        if group_size not in (32, 64) and (group_size < 128 or group_size % 128):
+            raise ValueError("group_size must be 32, 64 or a multiple of 128")
+        groups = -(-k // group_size)
+        _check("packed", packed, (n, (k + 1) // 2), torch.uint8, device)
+        self.scale_code = _code(scales.dtype)
+        _check("scales", scales, (n, groups), scales.dtype, device)
+        if zeros is not None:
+            _check("zeros", zeros, (n, groups), torch.uint8, device)
+            if int(zeros.max()) > 15:
+                raise ValueError("zeros must be 0 to 15")
+            zeros = zeros.contiguous()
+        if bias is not None:
+            _code(bias.dtype)
+            _check("bias", bias, (n,), bias.dtype, device, False)
+            bias = bias.contiguous()
+        self.in_features, self.out_features, self.group_size = k, n, int(group_size)
+        self.device, self.scales, self.zeros, self.bias = device, scales.contiguous(), zeros, bias
+        self.weight = torch.empty((n, -(-k // 128) * 16), dtype=torch.int32, device=device)
+        packed = packed.contiguous()
+        _call(N.lib().pfk_w4_arrange, device, packed.data_ptr(), n, k, self.weight.data_ptr())
+
+    @classmethod
+    def quantize(cls, weight, group_size: int = 128, bias=None, symmetric: bool = False, scale_dtype=None) -> "Linear4bit":
+        """Weights [out_features, in_features] rounded to 4 bits: the nearest
+        of 16 evenly spaced values that cover each group's range and 0
+        (symmetric: 15 steps around 8)."""
+        import torch
+        _cuda(weight, "weight")
+        n, k = weight.shape
+        groups = -(-k // group_size)
+        w = torch.zeros((n, groups * group_size), dtype=torch.float32, device=weight.device)
+        w[:, :k] = weight
+        w = w.view(n, groups, group_size)
+        if symmetric:
+            scale = w.abs().amax(-1) / 7.0
+        else:
+            low, high = w.amin(-1).clamp(max=0.0), w.amax(-1).clamp(min=0.0)
+            scale = (high - low) / 15.0
+        scales = scale.to(torch.float16 if scale_dtype is None else scale_dtype)
+        s = scales.float()
+        step = torch.where(s > 0, s, torch.ones_like(s))
+        zeros = None if symmetric else (-low / step).round().clamp(0, 15)
+        z = 8.0 if symmetric else zeros[..., None]
+        q = ((w / step[..., None]).round() + z).clamp(0, 15).to(torch.uint8).view(n, -1)[:, :(k + 1) // 2 * 2]
+        if q.shape[1] % 2:
+            q = torch.nn.functional.pad(q, (0, 1))
+        packed = q[:, 0::2] | (q[:, 1::2] << 4)
+        return cls(packed, scales, None if symmetric else zeros.to(torch.uint8), bias, k, group_size)
+
+    def __call__(self, x, out=None):
+        """x: [..., in_features], the rows at any one stride."""
+        import torch
+        _cuda(x, "x")
+        code = _code(x.dtype)
+        _check("x", x, (None,) * (len(x.shape) - 1) + (self.in_features,), x.dtype, self.device)
+        if self.bias is not None and self.bias.dtype != x.dtype:
+            raise TypeError(f"x: dtype must be the bias's, {self.bias.dtype}, not {x.dtype}")
+        rows = x if len(x.shape) == 2 else x.reshape(-1, self.in_features)
+        shape = tuple(x.shape[:-1]) + (self.out_features,)
+        if out is None:
+            out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        else:
+            _check("out", out, shape, x.dtype, self.device, output=True)
+        flat = out if len(shape) == 2 else out.view(-1, self.out_features)
+        p = N.LinearW4ParamsC(code, rows.shape[0], self.in_features, self.out_features, self.group_size,
+                              rows.data_ptr(), rows.stride(0), flat.data_ptr(), flat.stride(0), self.weight.data_ptr(),
+                              self.scales.data_ptr(), self.scale_code,
+                              None if self.zeros is None else self.zeros.data_ptr(),
+                              None if self.bias is None else self.bias.data_ptr())
+        _call(N.lib().pfk_linear_w4, self.device, C.byref(p))
+        return out
