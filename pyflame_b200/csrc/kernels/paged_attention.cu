@@ -7,33 +7,36 @@
 // query heads share a key-value head), so memory bounds it as long as the
 // products run on the tensor cores and the loads never pause.
 //
-// Work.  A unit is one sequence, one key-value head and 8 or 16 of its query
-// heads; its keys are cut into tiles of 64.  The tiles of all units form one
+// Work.  A unit is one sequence, one key-value head and up to 16 of its query
+// heads; its keys are cut into tiles of 64 (32 for wide fp32 heads).  The tiles of all units form one
 // list, and each of a fixed number of CTAs (one wave) takes an equal run of
 // it, whatever the sequences' lengths: lengths are device data, so the host
 // could not balance them.  A CTA that has a whole unit writes its output; a
 // unit that is shared leaves (m, sum, o) of each share in the workspace, and
 // a second small kernel joins the shares in the order of the list, so that
-// results do not depend on timing.
+// results do not depend on timing and nothing has to be zero beforehand.
 //
 // Tile.  Each of a CTA's 4 warps takes 16 keys at a time, straight from
-// global memory into the registers of mma.sync operands, without shared
-// memory: S^T = K Q^T has the keys as its rows, and since the order of the
-// summed axis is free as long as both operands agree, a lane's fragment of K
-// is 16 consecutive bytes of two key rows.  O^T = V^T P^T has the values'
-// axis as its rows: a lane loads 16 bytes of each of its 4 keys and pairs
-// them with byte permutes.  P is turned from the first product's accumulator
-// layout into the second's operand layout by movmatrix.  A group of 8 query
-// heads fills the 8 columns of the instruction; tcgen05 would need 128 rows
-// of one operand in shared memory for the same, and the products are far from
-// being the limit.
+// global memory into registers, without shared memory: lane (g, t) = (lane /
+// 4, lane % 4) holds 16-byte pieces of the key rows g and g + 8 and of the
+// value rows 2t, 2t + 1, 8 + 2t and 9 + 2t.  Those are the operand registers
+// of mma.sync: S^T = K Q^T has the keys as its rows, and since the order of
+// the summed axis is free as long as both operands agree, a fragment of K is
+// 16 consecutive bytes; O^T = V^T P^T has the values' axis as its rows, whose
+// pairs of keys come from byte permutes.  P is turned from the first
+// product's accumulator layout into the second's operand layout by movmatrix.
+// A group of 8 query heads fills the 8 columns of the instruction; tcgen05
+// would need 128 rows of one operand in shared memory for the same, and the
+// products are far from being the limit.  The next step's keys are loaded as
+// soon as this step's scores are done, its values as soon as the products are.
 //
 // Types.  16-bit: Q, K, V enter exactly; P is split into a high and a low
 // part, so its rounding (2^-16 and less) stays below that of the output. fp16
 // P is scaled by 2^14 to keep small weights out of its subnormal range.
-// fp32: both operands are split into tf32 high and low parts, three products
-// (the dropped low-low term is below 2^-22 of the product).  Scores, maxima,
-// sums and outputs are held in fp32.
+// fp32, up to 4 query heads a key-value head: fp32 FMAs on the CUDA cores.
+// fp32, more: both operands are split into tf32 high and low parts, three
+// products (the dropped low-low term is below 2^-22 of the product).  Scores,
+// maxima, sums and outputs are held in fp32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -52,7 +55,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTile = 16 * kWarps;  // keys
 constexpr unsigned kNone = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -80,10 +82,11 @@ struct Args {
   long long most;  // tokens that the table has room for
   int window;
   float scale;
-  // workspace: [0] tile count, then each unit's first tile, the shares'
-  // maxima and sums [ctas][2][heads], and their outputs [ctas][2][heads][D]
-  long long* starts;
-  float* stats;
+  // workspace: a record of each CTA (the unit that began there and goes on in
+  // later CTAs, if there is one), the shares' maxima and sums
+  // [ctas][2][heads], and their outputs [ctas][2][heads][D]
+  int4* records;  // row, unit, last CTA, whether there is one
+  float2* stats;
   float* parts;
   int ctas;
   int heads;  // of a full unit: min(group, unit_heads)
@@ -93,6 +96,7 @@ struct Span {
   int begin, end, tiles;  // seen keys, and the tiles that cover them
 };
 
+template <int TILE>
 __device__ __forceinline__ Span span_of(const Args& a, int b) {
   long long n = a.seq_lens[b];
   if (n < 0 || n > a.most) {
@@ -102,7 +106,7 @@ __device__ __forceinline__ Span span_of(const Args& a, int b) {
   Span s;
   s.end = (int)n;
   s.begin = a.window > 0 && n > a.window ? (int)n - a.window : 0;
-  s.tiles = n ? (s.end + kTile - 1) / kTile - s.begin / kTile : 0;
+  s.tiles = n ? (s.end + TILE - 1) / TILE - s.begin / TILE : 0;
   return s;
 }
 
@@ -192,34 +196,44 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 __device__ __forceinline__ unsigned word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
 
+__device__ __forceinline__ unsigned long long divide(unsigned long long a, unsigned long long b) {
+  return ((a | b) >> 32) ? a / b : (unsigned)a / (unsigned)b;
+}
+
 // DP: head_dim rounded up to the size that the registers are laid out for.
-// NT: 8-column blocks of query heads.
-template <typename T, int DP, int NT>
+// CORES: fp32 on the CUDA cores, NT the query heads of a unit (1, 2 or 4);
+// otherwise on the tensor cores, NT blocks of 8 query heads.
+template <typename T, int DP, int NT, bool CORES>
 struct Layout {
   static constexpr int kVec = Traits<T>::kVec;
   static constexpr int kQ = DP / (4 * kVec);  // 16-byte chunks of a K row that a lane holds
   static constexpr int kV = DP / (8 * kVec);  // of a V row
+  static constexpr int kHeads = CORES ? NT : NT * 8;
   static constexpr int kPitch = DP + 4;
-  static constexpr size_t q_bytes = (size_t)kQ * NT * 32 * 16 * (sizeof(T) == 4 ? 2 : 1);
-  static constexpr size_t o_bytes = (size_t)kWarps * NT * 8 * kPitch * 4;
-  static constexpr size_t m_bytes = (size_t)2 * kWarps * NT * 8 * 4;
+  // a step's keys in blocks of 8: 16 fp32 rows of 256 do not fit the registers
+  static constexpr int kRows = CORES && DP > 128 ? 1 : 2;
+  static constexpr int kTile = 8 * kRows * kWarps;  // keys of a CTA's step
+  static constexpr size_t q_bytes = CORES ? (size_t)NT * DP * 4 : (size_t)kQ * NT * 32 * 16 * (sizeof(T) == 4 ? 2 : 1);
+  static constexpr size_t o_bytes = (size_t)kWarps * kHeads * kPitch * 4;
+  static constexpr size_t m_bytes = (size_t)2 * kWarps * kHeads * 4;
   static constexpr size_t smem = q_bytes + o_bytes + m_bytes;
 };
 
-template <typename T, int DP, int NT>
+template <typename T, int DP, int NT, bool CORES>
 __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
-  using L = Layout<T, DP, NT>;
+  using L = Layout<T, DP, NT, CORES>;
   using Tr = Traits<T>;
-  constexpr int VEC = L::kVec;
+  constexpr int VEC = L::kVec, HEADS = L::kHeads;
   constexpr bool k32 = sizeof(T) == 4;
   extern __shared__ __align__(16) char smem[];
-  uint4* qs = reinterpret_cast<uint4*>(smem);  // [split][nt][chunk][lane]
+  uint4* qs = reinterpret_cast<uint4*>(smem);  // [split][nt][chunk][lane], or [head][DP] floats
   float* os = reinterpret_cast<float*>(smem + L::q_bytes);
   float* ms = reinterpret_cast<float*>(smem + L::q_bytes + L::o_bytes);  // [warp][head] maxima, then sums
-  float* ls = ms + kWarps * NT * 8;
-  __shared__ long long scan[kWarps + 1];
+  float* ls = ms + kWarps * HEADS;
+  __shared__ long long scan[kWarps];
   __shared__ int found_row;
   __shared__ long long found_before;
+  __shared__ Span found_span;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -227,24 +241,11 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
 
   // the list of tiles: its length, and the row that holds this CTA's first
   const int per_row = a.kv_heads * a.chunks;
-  long long total = 0;
-  for (int b = tid; b < a.batch; b += kThreads) total += (long long)span_of(a, b).tiles * per_row;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-  if (lane == 0) scan[warp] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += scan[w];
-  if (blockIdx.x == 0 && tid == 0) a.starts[0] = total;
-  const long long t0 = total * blockIdx.x / a.ctas, t1 = total * (blockIdx.x + 1) / a.ctas;
-  if (t0 >= t1) return;
-  long long before = 0;
-  for (int base = 0;; base += kThreads) {
-    __syncthreads();
-    const int b = base + tid;
-    const long long mine = b < a.batch ? (long long)span_of(a, b).tiles * per_row : 0;
-    long long sum = mine;
+  Span mine = {0, 0, 0};
+  auto scan_rows = [&](int b) -> long long {  // tiles of the rows before b in its block of rows; scan: warps' sums
+    mine = b < a.batch ? span_of<L::kTile>(a, b) : Span{0, 0, 0};
+    const long long own = (long long)mine.tiles * per_row;
+    long long sum = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long up = __shfl_up_sync(~0u, sum, o);
@@ -252,68 +253,71 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
     }
     if (lane == 31) scan[warp] = sum;
     __syncthreads();
-    long long start = before;
+    long long start = sum - own;
     for (int w = 0; w < warp; ++w) start += scan[w];
-    start += sum - mine;
-    if (mine > 0 && t0 >= start && t0 < start + mine) {
-      found_row = b;
-      found_before = start;
+    return start;
+  };
+  auto scanned = [&]() -> long long { return scan[0] + scan[1] + scan[2] + scan[3]; };
+  static_assert(kWarps == 4, "scanned() adds four warps' sums");
+  long long total = 0, start = 0;
+  if (a.batch > kThreads) {
+    for (int b = tid; b < a.batch; b += kThreads) total += (long long)span_of<L::kTile>(a, b).tiles * per_row;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+    if (lane == 0) scan[warp] = total;
+    __syncthreads();
+    total = scanned();
+  } else {
+    start = scan_rows(tid);
+    total = scanned();
+  }
+  // runs of total / ctas tiles, the first ones a tile longer
+  const long long run = (long long)divide(total, a.ctas), longer = total - run * a.ctas;
+  const long long t0 = run * blockIdx.x + min((long long)blockIdx.x, longer);
+  const long long t1 = t0 + run + (blockIdx.x < longer ? 1 : 0);
+  if (t0 >= t1) {
+    if (tid == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  long long before = 0;
+  for (int base = 0;; base += kThreads) {
+    if (a.batch > kThreads) {
+      __syncthreads();
+      start = scan_rows(base + tid);
     }
-    for (int w = 0; w < kWarps; ++w) before += scan[w];
+    if (t0 >= before + start && t0 < before + start + (long long)mine.tiles * per_row) {
+      found_row = base + tid;
+      found_before = before + start;
+      found_span = mine;
+    }
+    before += scanned();
     if (before > t0) break;  // total > t0: some block of rows gets there
   }
   __syncthreads();
   int row = found_row;
-  Span sp = span_of(a, row);
-  int unit = (int)((t0 - found_before) / sp.tiles);  // of the row
+  Span sp = found_span;
+  int unit = (int)divide(t0 - found_before, sp.tiles);  // of the row
   int tile = (int)((t0 - found_before) - (long long)unit * sp.tiles);
+  int4 record = make_int4(0, 0, 0, 0);
 
   const float scale2 = a.scale * kLog2e;
   for (long long at = t0; at < t1;) {
-    while (sp.tiles == 0) sp = span_of(a, ++row);
+    while (sp.tiles == 0) sp = span_of<L::kTile>(a, ++row);
     const int count = (int)min((long long)(sp.tiles - tile), t1 - at);
     const int head = unit / a.chunks;
     const int first_q = head * a.group + (unit - head * a.chunks) * a.unit_heads;
     const int heads = min(a.unit_heads, (head + 1) * a.group - first_q);
 
-    // Q in the order of the second operand's registers
-    __syncthreads();  // the previous piece's reads of shared memory are over
-    {
-      const T* qp = (const T*)a.q + (long long)row * a.q_sb + (long long)first_q * a.q_sh;
-      for (int i = tid; i < NT * L::kQ * 32; i += kThreads) {
-        const int l = i & 31, c = (i >> 5) % L::kQ, nt = (i >> 5) / L::kQ;
-        const int h = nt * 8 + (l >> 2), d0 = (c * 4 + (l & 3)) * VEC;
-        if constexpr (k32) {
-          uint4 hi = {}, lo = {};
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : 0.f;
-          split(x[0], hi.x, lo.x);
-          split(x[1], hi.y, lo.y);
-          split(x[2], hi.z, lo.z);
-          split(x[3], hi.w, lo.w);
-          qs[i] = hi;
-          qs[NT * L::kQ * 32 + i] = lo;
-        } else {
-          T x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : Tr::from(0.f);
-          qs[i] = *reinterpret_cast<uint4*>(x);
-        }
-      }
-    }
-    __syncthreads();
-
     const char* kp = a.k + head * a.head_bytes;
     const char* vp = a.v + head * a.head_bytes;
     const int* table = a.table + (long long)row * a.table_stride;
     const int lo_key = sp.begin, hi_key = sp.end;
-    const int first_key = (sp.begin / kTile + tile) * kTile + warp * 16;
+    const int first_key = (sp.begin / L::kTile + tile) * L::kTile + warp * 8 * L::kRows;
 
-    // place of one of a step's 16 keys (lane & 15) in the cache, in units
+    // place of one of the warp's keys of a step (lane modulo their number) in the cache, in units
     auto place = [&](int step) -> unsigned {
       if (step >= count) return kNone;
-      const int key = first_key + step * kTile + (lane & 15);
+      const int key = first_key + step * L::kTile + (lane & (8 * L::kRows - 1));
       if (key < lo_key || key >= hi_key) return kNone;
       const unsigned p = a.by_page.div((unsigned)key);
       const unsigned page = (unsigned)table[p];
@@ -323,10 +327,10 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
       }
       return page * a.page_units + ((unsigned)key - p * a.by_page.d) * a.token_units;
     };
-    uint4 kr[2][L::kQ], vr[4][L::kV];
-    auto load_k = [&](unsigned where, bool (&seen)[2]) {
+    uint4 kr[L::kRows][L::kQ], vr[2 * L::kRows][L::kV];
+    auto load_k = [&](unsigned where, bool (&seen)[L::kRows]) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+      for (int r = 0; r < L::kRows; ++r) {
         const unsigned u = __shfl_sync(~0u, where, g + 8 * r);
         seen[r] = u != kNone;
         const char* p = kp + (unsigned long long)u * a.unit_bytes + t * 16;
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
     };
     auto load_v = [&](unsigned where) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int r = 0; r < 2 * L::kRows; ++r) {
         const unsigned u = __shfl_sync(~0u, where, 2 * t + (r & 1) + 8 * (r >> 1));
         const char* p = vp + (unsigned long long)u * a.unit_bytes + g * 16;
 #pragma unroll
@@ -349,151 +353,272 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
         }
       }
     };
+    bool seen[L::kRows];
+    unsigned next = place(0);
+    load_k(next, seen);
+    load_v(next);
+    next = place(1);
 
-    // per lane: query heads nt*8 + 2t and + 1
-    float m[NT][2], l[NT][2], o[NT][L::kV][VEC / 2][4];
+    // Q in the order of the second operand's registers
+    __syncthreads();  // the previous piece's reads of shared memory are over
+    {
+      const T* qp = (const T*)a.q + (long long)row * a.q_sb + (long long)first_q * a.q_sh;
+      if constexpr (CORES) {
+        for (int i = tid; i < NT * DP; i += kThreads) {
+          const int h = i / DP, d = i - h * DP;
+          reinterpret_cast<float*>(qs)[i] = h < heads && d < a.head_dim ? qp[h * a.q_sh + d] : 0.f;
+        }
+      } else {
+        for (int i = tid; i < NT * L::kQ * 32; i += kThreads) {
+          const int l = i & 31, c = (i >> 5) % L::kQ, nt = (i >> 5) / L::kQ;
+          const int h = nt * 8 + (l >> 2), d0 = (c * 4 + (l & 3)) * VEC;
+          if constexpr (k32) {
+            uint4 hi = {}, lo = {};
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : 0.f;
+            split(x[0], hi.x, lo.x);
+            split(x[1], hi.y, lo.y);
+            split(x[2], hi.z, lo.z);
+            split(x[3], hi.w, lo.w);
+            qs[i] = hi;
+            qs[NT * L::kQ * 32 + i] = lo;
+          } else {
+            alignas(16) T x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : Tr::from(0.f);
+            qs[i] = *reinterpret_cast<uint4*>(x);
+          }
+        }
+      }
+    }
+    __syncthreads();
+
+    // Running maxima, sums and outputs.  On the tensor cores a lane has query
+    // heads nt*8 + 2t and + 1, of o the value pairs 2j, 2j + 1 of its chunk;
+    // on the CUDA cores every head, of o its own keys' part.
+    constexpr int MH = CORES ? 1 : 2;
+    float m[NT][MH], l[NT][MH], o[NT][L::kV][VEC / 2][CORES ? 2 : 4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MH; ++i) {
+        m[nt][i] = -INFINITY;
+        l[nt][i] = 0.f;
+      }
 #pragma unroll
       for (int c = 0; c < L::kV; ++c)
 #pragma unroll
         for (int j = 0; j < VEC / 2; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[nt][c][j][r] = 0.f;
+          for (int r = 0; r < (CORES ? 2 : 4); ++r) o[nt][c][j][r] = 0.f;
     }
-    bool seen[2];
-    unsigned here = place(0);
-    load_k(here, seen);
-    load_v(here);
-    unsigned next = place(1);
     for (int step = 0; step < count; ++step) {
-      float s[NT][4];
+      bool live[L::kRows];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int r = 0; r < L::kRows; ++r) live[r] = seen[r];
+      if constexpr (CORES) {
+        float s[NT][L::kRows];  // of keys g (and g + 8), the same in a quad's lanes
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[nt][r] = 0.f;
+        for (int h = 0; h < NT; ++h) {
+          float even[L::kRows], odd[L::kRows];
 #pragma unroll
-        for (int c = 0; c < L::kQ; ++c) {
-          const uint4 b = qs[(nt * L::kQ + c) * 32 + lane];
-          if constexpr (k32) {
-            const uint4 bl = qs[(NT * L::kQ + nt * L::kQ + c) * 32 + lane];
+          for (int r = 0; r < L::kRows; ++r) even[r] = odd[r] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              unsigned h0, h1, h2, h3, l0, l1, l2, l3;
-              split(__uint_as_float(word(kr[0][c], 2 * e)), h0, l0);
-              split(__uint_as_float(word(kr[1][c], 2 * e)), h1, l1);
-              split(__uint_as_float(word(kr[0][c], 2 * e + 1)), h2, l2);
-              split(__uint_as_float(word(kr[1][c], 2 * e + 1)), h3, l3);
-              mma_tf32(s[nt], l0, l1, l2, l3, word(b, 2 * e), word(b, 2 * e + 1));
-              mma_tf32(s[nt], h0, h1, h2, h3, word(bl, 2 * e), word(bl, 2 * e + 1));
-              mma_tf32(s[nt], h0, h1, h2, h3, word(b, 2 * e), word(b, 2 * e + 1));
+          for (int c = 0; c < L::kQ; ++c) {
+            const float4 q = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(qs) + h * DP + (c * 4 + t) * 4);
+#pragma unroll
+            for (int r = 0; r < L::kRows; ++r) {
+              even[r] = fmaf(q.x, __uint_as_float(kr[r][c].x), even[r]);
+              odd[r] = fmaf(q.y, __uint_as_float(kr[r][c].y), odd[r]);
+              even[r] = fmaf(q.z, __uint_as_float(kr[r][c].z), even[r]);
+              odd[r] = fmaf(q.w, __uint_as_float(kr[r][c].w), odd[r]);
             }
-          } else {
-            Tr::mma(s[nt], kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, b.x, b.y);
-            Tr::mma(s[nt], kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, b.z, b.w);
           }
+#pragma unroll
+          for (int r = 0; r < L::kRows; ++r) s[h][r] = even[r] + odd[r];
         }
-      }
-      const bool seen0 = seen[0], seen1 = seen[1];
-      if (step + 1 < count) load_k(next, seen);
-
-      unsigned pt[NT][4];  // P as the second operand: 16-bit hi, lo of keys 0-7 and 8-15; fp32 its four values
+        if (step + 1 < count) load_k(next, seen);
+        float p[NT][2 * L::kRows];  // of the lane's value rows
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float x[4];
+        for (int h = 0; h < NT; ++h) {
+          float top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = (r < 2 ? seen0 : seen1) ? s[nt][r] * scale2 : -INFINITY;
-        float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
-        bool moved = false;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 4));
-          top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 8));
-          top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 16));
-          moved |= top[i] > m[nt][i];
-        }
-        if (__any_sync(~0u, moved)) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float to = fmaxf(m[nt][i], top[i]);
-            const float f = to == -INFINITY ? 1.f : exp2_fast(m[nt][i] - to);
-            m[nt][i] = to;
-            l[nt][i] *= f;
+          for (int r = 0; r < L::kRows; ++r) {
+            s[h][r] += __shfl_xor_sync(~0u, s[h][r], 1);
+            s[h][r] += __shfl_xor_sync(~0u, s[h][r], 2);
+            s[h][r] = live[r] ? s[h][r] * scale2 : -INFINITY;
+            top = fmaxf(top, s[h][r]);
+          }
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+          if (top > m[h][0]) {  // the same in all lanes
+            const float f = exp2_fast(m[h][0] - top);
+            m[h][0] = top;
+            l[h][0] *= f;
 #pragma unroll
             for (int c = 0; c < L::kV; ++c)
 #pragma unroll
               for (int j = 0; j < VEC / 2; ++j) {
-                o[nt][c][j][i] *= f;
-                o[nt][c][j][i + 2] *= f;
+                o[h][c][j][0] *= f;
+                o[h][c][j][1] *= f;
               }
           }
-        }
-        float p[4];
+          const float base = m[h][0] == -INFINITY ? 0.f : m[h][0];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float base = m[nt][r & 1] == -INFINITY ? 0.f : m[nt][r & 1];
-          p[r] = exp2_fast(x[r] - base + Tr::kShift);
-          l[nt][r & 1] += p[r];
-        }
-        if constexpr (k32) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const unsigned u0 = __float_as_uint(p[2 * i]), u1 = __float_as_uint(p[2 * i + 1]);
-            const unsigned lo = transpose8x8(__byte_perm(u0, u1, 0x5410));
-            const unsigned hi = transpose8x8(__byte_perm(u0, u1, 0x7632));
-            pt[nt][2 * i] = __byte_perm(lo, hi, 0x5410);      // key 8i + 2t of head g
-            pt[nt][2 * i + 1] = __byte_perm(lo, hi, 0x7632);  // key 8i + 2t + 1
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const unsigned hi = Tr::pack(p[2 * i], p[2 * i + 1]);
-            const float2 back = Tr::unpack(hi);
-            pt[nt][2 * i] = transpose8x8(hi);
-            pt[nt][2 * i + 1] = transpose8x8(Tr::pack(p[2 * i] - back.x, p[2 * i + 1] - back.y));
+          for (int r = 0; r < L::kRows; ++r) {
+            const float e = exp2_fast(s[h][r] - base);
+            l[h][0] += e;
+            p[h][2 * r] = __shfl_sync(~0u, e, 8 * t);
+            p[h][2 * r + 1] = __shfl_sync(~0u, e, 8 * t + 4);
           }
         }
-      }
+#pragma unroll
+        for (int c = 0; c < L::kV; ++c)
+#pragma unroll
+          for (int h = 0; h < NT; ++h)
+#pragma unroll
+            for (int r = 0; r < 2 * L::kRows; ++r)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                o[h][c][e >> 1][e & 1] = fmaf(p[h][r], __uint_as_float(word(vr[r][c], e)), o[h][c][e >> 1][e & 1]);
+      } else {
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          // several accumulators, added at the end: a chain of instructions on
+          // one would wait for each
+          constexpr int CH = k32 ? 3 : 2;
+          float acc[CH][4];
+#pragma unroll
+          for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][r] = 0.f;
+#pragma unroll
+          for (int c = 0; c < L::kQ; ++c) {
+            if (c * 4 * VEC >= a.head_dim) continue;
+            const uint4 b = qs[(nt * L::kQ + c) * 32 + lane];
+            if constexpr (k32) {
+              const uint4 bl = qs[(NT * L::kQ + nt * L::kQ + c) * 32 + lane];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                unsigned h0, h1, h2, h3, l0, l1, l2, l3;
+                split(__uint_as_float(word(kr[0][c], 2 * e)), h0, l0);
+                split(__uint_as_float(word(kr[1][c], 2 * e)), h1, l1);
+                split(__uint_as_float(word(kr[0][c], 2 * e + 1)), h2, l2);
+                split(__uint_as_float(word(kr[1][c], 2 * e + 1)), h3, l3);
+                mma_tf32(acc[1], l0, l1, l2, l3, word(b, 2 * e), word(b, 2 * e + 1));
+                mma_tf32(acc[CH - 1], h0, h1, h2, h3, word(bl, 2 * e), word(bl, 2 * e + 1));
+                mma_tf32(acc[0], h0, h1, h2, h3, word(b, 2 * e), word(b, 2 * e + 1));
+              }
+            } else {
+              Tr::mma(acc[0], kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, b.x, b.y);
+              Tr::mma(acc[1], kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, b.z, b.w);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[nt][r] = acc[0][r] + (k32 ? acc[1][r] + acc[CH - 1][r] : acc[1][r]);
+        }
+        if (step + 1 < count) load_k(next, seen);
+
+        unsigned pt[NT][4];  // P as the second operand: 16-bit hi, lo of keys 0-7 and 8-15; fp32 its four values
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float x[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = live[r >> 1] ? s[nt][r] * scale2 : -INFINITY;
+          float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+          bool moved = false;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 4));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 8));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 16));
+            moved |= top[i] > m[nt][i];
+          }
+          if (__any_sync(~0u, moved)) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float to = fmaxf(m[nt][i], top[i]);
+              const float f = to == -INFINITY ? 1.f : exp2_fast(m[nt][i] - to);
+              m[nt][i] = to;
+              l[nt][i] *= f;
+#pragma unroll
+              for (int c = 0; c < L::kV; ++c)
+#pragma unroll
+                for (int j = 0; j < VEC / 2; ++j) {
+                  o[nt][c][j][i] *= f;
+                  o[nt][c][j][i + 2] *= f;
+                }
+            }
+          }
+          float p[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float base = m[nt][r & 1] == -INFINITY ? 0.f : m[nt][r & 1];
+            p[r] = exp2_fast(x[r] - base + Tr::kShift);
+            l[nt][r & 1] += p[r];
+          }
+          if constexpr (k32) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const unsigned u0 = __float_as_uint(p[2 * i]), u1 = __float_as_uint(p[2 * i + 1]);
+              const unsigned lo = transpose8x8(__byte_perm(u0, u1, 0x5410));
+              const unsigned hi = transpose8x8(__byte_perm(u0, u1, 0x7632));
+              pt[nt][2 * i] = __byte_perm(lo, hi, 0x5410);      // key 8i + 2t of head g
+              pt[nt][2 * i + 1] = __byte_perm(lo, hi, 0x7632);  // key 8i + 2t + 1
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const unsigned hi = Tr::pack(p[2 * i], p[2 * i + 1]);
+              const float2 back = Tr::unpack(hi);
+              pt[nt][2 * i] = transpose8x8(hi);
+              pt[nt][2 * i + 1] = transpose8x8(Tr::pack(p[2 * i] - back.x, p[2 * i + 1] - back.y));
+            }
+          }
+        }
 
 #pragma unroll
-      for (int c = 0; c < L::kV; ++c) {
-        if constexpr (k32) {
+        for (int c = 0; c < L::kV; ++c) {
+          if (c * 8 * VEC >= a.head_dim) continue;
+          if constexpr (k32) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {  // keys 8i ... 8i + 7
-            unsigned bh[NT][2], bl[NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              split(__uint_as_float(pt[nt][2 * i]), bh[nt][0], bl[nt][0]);
-              split(__uint_as_float(pt[nt][2 * i + 1]), bh[nt][1], bl[nt][1]);
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              unsigned h0, h1, h2, h3, l0, l1, l2, l3;
-              split(__uint_as_float(word(vr[2 * i][c], 2 * j)), h0, l0);
-              split(__uint_as_float(word(vr[2 * i][c], 2 * j + 1)), h1, l1);
-              split(__uint_as_float(word(vr[2 * i + 1][c], 2 * j)), h2, l2);
-              split(__uint_as_float(word(vr[2 * i + 1][c], 2 * j + 1)), h3, l3);
+            for (int i = 0; i < 2; ++i) {  // keys 8i ... 8i + 7
+              unsigned bh[NT][2], bl[NT][2];
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma_tf32(o[nt][c][j], l0, l1, l2, l3, bh[nt][0], bh[nt][1]);
-                mma_tf32(o[nt][c][j], h0, h1, h2, h3, bl[nt][0], bl[nt][1]);
-                mma_tf32(o[nt][c][j], h0, h1, h2, h3, bh[nt][0], bh[nt][1]);
+                split(__uint_as_float(pt[nt][2 * i]), bh[nt][0], bl[nt][0]);
+                split(__uint_as_float(pt[nt][2 * i + 1]), bh[nt][1], bl[nt][1]);
+              }
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                unsigned h0, h1, h2, h3, l0, l1, l2, l3;
+                split(__uint_as_float(word(vr[2 * i][c], 2 * j)), h0, l0);
+                split(__uint_as_float(word(vr[2 * i][c], 2 * j + 1)), h1, l1);
+                split(__uint_as_float(word(vr[2 * i + 1][c], 2 * j)), h2, l2);
+                split(__uint_as_float(word(vr[2 * i + 1][c], 2 * j + 1)), h3, l3);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  mma_tf32(o[nt][c][j], l0, l1, l2, l3, bh[nt][0], bh[nt][1]);
+                  mma_tf32(o[nt][c][j], h0, h1, h2, h3, bl[nt][0], bl[nt][1]);
+                  mma_tf32(o[nt][c][j], h0, h1, h2, h3, bh[nt][0], bh[nt][1]);
+                }
               }
             }
-          }
-        } else {
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const unsigned a0 = __byte_perm(word(vr[0][c], j), word(vr[1][c], j), 0x5410);
-            const unsigned a1 = __byte_perm(word(vr[0][c], j), word(vr[1][c], j), 0x7632);
-            const unsigned a2 = __byte_perm(word(vr[2][c], j), word(vr[3][c], j), 0x5410);
-            const unsigned a3 = __byte_perm(word(vr[2][c], j), word(vr[3][c], j), 0x7632);
+            for (int j = 0; j < 4; ++j) {
+              const unsigned a0 = __byte_perm(word(vr[0][c], j), word(vr[1][c], j), 0x5410);
+              const unsigned a1 = __byte_perm(word(vr[0][c], j), word(vr[1][c], j), 0x7632);
+              const unsigned a2 = __byte_perm(word(vr[2][c], j), word(vr[3][c], j), 0x5410);
+              const unsigned a3 = __byte_perm(word(vr[2][c], j), word(vr[3][c], j), 0x7632);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              Tr::mma(o[nt][c][j], a0, a1, a2, a3, pt[nt][1], pt[nt][3]);
-              Tr::mma(o[nt][c][j], a0, a1, a2, a3, pt[nt][0], pt[nt][2]);
+              for (int nt = 0; nt < NT; ++nt) {
+                Tr::mma(o[nt][c][j], a0, a1, a2, a3, pt[nt][1], pt[nt][3]);
+                Tr::mma(o[nt][c][j], a0, a1, a2, a3, pt[nt][0], pt[nt][2]);
+              }
             }
           }
         }
@@ -508,19 +633,31 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < MH; ++i) {
+        const int h = warp * HEADS + (CORES ? nt : nt * 8 + 2 * t + i);
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[nt][i] += __shfl_xor_sync(~0u, l[nt][i], off);
-        if (g == 0) {
-          ms[warp * NT * 8 + nt * 8 + 2 * t + i] = m[nt][i];
-          ls[warp * NT * 8 + nt * 8 + 2 * t + i] = l[nt][i];
+        if (CORES ? lane == 0 : g == 0) {
+          ms[h] = m[nt][i];
+          ls[h] = l[nt][i];
         }
 #pragma unroll
         for (int c = 0; c < L::kV; ++c)
 #pragma unroll
-          for (int j = 0; j < VEC / 2; ++j)
-            *reinterpret_cast<float2*>(os + (size_t)(warp * NT * 8 + nt * 8 + 2 * t + i) * L::kPitch + (c * 8 + g) * VEC + 2 * j) =
-                make_float2(o[nt][c][j][i], o[nt][c][j][i + 2]);
+          for (int j = 0; j < VEC / 2; ++j) {
+            float2 pair;
+            if constexpr (CORES) {  // the quad's lanes have different keys of the same values
+              pair = make_float2(o[nt][c][j][0], o[nt][c][j][1]);
+#pragma unroll
+              for (int off = 1; off < 4; off <<= 1) {
+                pair.x += __shfl_xor_sync(~0u, pair.x, off);
+                pair.y += __shfl_xor_sync(~0u, pair.y, off);
+              }
+            } else {
+              pair = make_float2(o[nt][c][j][i], o[nt][c][j][CORES ? 0 : i + 2]);
+            }
+            if (!CORES || t == j) *reinterpret_cast<float2*>(os + (size_t)h * L::kPitch + (c * 8 + g) * VEC + 2 * j) = pair;
+          }
       }
     }
     __syncthreads();
@@ -531,173 +668,207 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
       const int h = i / a.head_dim, d = i - h * a.head_dim;
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ms[w * NT * 8 + h]);
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ms[w * HEADS + h]);
       float v = 0.f, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float mw = ms[w * NT * 8 + h];
+        const float mw = ms[w * HEADS + h];
         const float f = mw == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : exp2_fast(mw - top);
-        v += f * os[(size_t)(w * NT * 8 + h) * L::kPitch + d];
-        sum += f * ls[w * NT * 8 + h];
+        v += f * os[(size_t)(w * HEADS + h) * L::kPitch + d];
+        sum += f * ls[w * HEADS + h];
       }
       if (whole) {
-        ((T*)a.out)[(long long)row * a.o_sb + (first_q + h) * a.o_sh + d] = Tr::from(sum == 0.f ? 0.f : v / sum);
+        ((T*)a.out)[(long long)row * a.o_sb + (long long)(first_q + h) * a.o_sh + d] = Tr::from(sum == 0.f ? 0.f : v / sum);
         if (d == 0 && a.lse)
           a.lse[(long long)row * a.q_heads + first_q + h] = sum == 0.f ? -INFINITY : (top + log2f(sum) - Tr::kShift) * kLn2;
       } else {
         a.parts[(share + h) * a.head_dim + d] = v;
-        if (d == 0) {
-          a.stats[2 * (share + h)] = top;
-          a.stats[2 * (share + h) + 1] = sum;
-        }
+        if (d == 0) a.stats[share + h] = make_float2(top, sum);
       }
     }
-    if (tile == 0 && tid == 0) a.starts[1 + (long long)row * per_row + unit] = at;
+    if (tile == 0 && !whole) {  // the CTA that has the unit's last tile
+      const long long last = at + sp.tiles - 1, edge = longer * (run + 1);
+      record = make_int4(row, unit, (int)(last < edge ? divide(last, run + 1) : longer + divide(last - edge, run)), 1);
+    }
     at += count;
     tile = 0;
     if (++unit == per_row) {
       unit = 0;
       sp.tiles = 0;
-      if (at < t1) sp = span_of(a, ++row);
+      if (at < t1) sp = span_of<L::kTile>(a, ++row);
     }
   }
+  if (tid == 0) a.records[blockIdx.x] = record;
 }
 
-// One CTA per sequence and query head: joins the shares of a unit that
-// several CTAs had, in the order of the list; writes empty sequences.
+constexpr int kJoinThreads = 256;
+constexpr int kMostCtas = 4096;
+
+// CTA (c, h): joins the shares of query head h of the unit that began in CTA
+// c of the first kernel and went on, in the order of the list; and writes
+// the outputs of sequence c if it is empty.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) join_kernel(const Args a) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
   using Tr = Traits<T>;
-  __shared__ float tops[kWarps], sums[kWarps];
-  __shared__ float acc[kWarps][256];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x / a.q_heads, qh = blockIdx.x % a.q_heads;
-  T* out = (T*)a.out + (long long)b * a.o_sb + (long long)qh * a.o_sh;
-  const Span sp = span_of(a, b);
-  if (sp.tiles == 0) {
-    for (int d = tid; d < a.head_dim; d += kThreads) out[d] = Tr::from(0.f);
-    if (tid == 0 && a.lse) a.lse[(long long)b * a.q_heads + qh] = -INFINITY;
-    return;
+  __shared__ float weights[kMostCtas];
+  __shared__ float red[kJoinThreads / 32];
+  __shared__ float4 acc[kJoinThreads];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c0 = blockIdx.x;
+  if (c0 < a.batch && span_of<64>(a, c0).tiles == 0) {
+    for (int qh = blockIdx.y; qh < a.q_heads; qh += gridDim.y) {
+      for (int d = tid; d < a.head_dim; d += kJoinThreads)
+        ((T*)a.out)[(long long)c0 * a.o_sb + (long long)qh * a.o_sh + d] = Tr::from(0.f);
+      if (tid == 0 && a.lse) a.lse[(long long)c0 * a.q_heads + qh] = -INFINITY;
+    }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int head = qh / a.group, in_group = qh - head * a.group;
-  const int unit = head * a.chunks + in_group / a.unit_heads, h = in_group % a.unit_heads;
-  const long long total = a.starts[0];
-  const long long first = a.starts[1 + (long long)b * a.kv_heads * a.chunks + unit];
-  const long long last = first + sp.tiles - 1;
-  // the CTA that has tile x: the largest c with floor(total * c / ctas) <= x
-  const int c0 = (int)(((first + 1) * a.ctas + total - 1) / total) - 1;
-  const int c1 = (int)(((last + 1) * a.ctas + total - 1) / total) - 1;
-  if (c0 == c1) return;  // written whole
-  auto share_of = [&](int c) -> long long {
-    const long long t0 = total * c / a.ctas, t1 = total * (c + 1) / a.ctas;
-    return t0 == t1 ? -1 : ((long long)c * 2 + (t0 <= first ? 1 : 0)) * a.heads + h;
-  };
-  float top = -INFINITY;
-  for (int c = c0 + tid; c <= c1; c += kThreads) {
-    const long long s = share_of(c);
-    if (s >= 0) top = fmaxf(top, a.stats[2 * s]);
-  }
+  if (c0 >= a.ctas) return;
+  const int4 rec = a.records[c0];
+  if (!rec.w) return;
+  const int b = rec.x, head = rec.y / a.chunks, h = blockIdx.y;
+  const int qh = head * a.group + (rec.y - head * a.chunks) * a.unit_heads + h;
+  if (qh >= (head + 1) * a.group) return;
+  const int shares = rec.z - c0 + 1;
+  // the first share is slot 1 of its CTA, the others slot 0 of theirs
+  auto share = [&](int i) -> long long { return ((long long)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * a.heads + h; };
+  const int cols = a.head_dim / 4;                        // of 4 values
+  const int across = cols <= 16 ? 16 : cols <= 32 ? 32 : 64;  // threads of a share
+  const int groups = kJoinThreads / across, gi = tid / across, col = tid % across;
+
+  float top = -INFINITY, sum = 0.f;
+  for (int i = tid; i < shares; i += kJoinThreads) top = fmaxf(top, a.stats[share(i)].x);
 #pragma unroll
   for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, off));
-  if (lane == 0) tops[warp] = top;
+  if (lane == 0) red[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, tops[w]);
-  float sum = 0.f, v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  for (int c = c0 + warp; c <= c1; c += kWarps) {
-    const long long s = share_of(c);
-    if (s < 0) continue;
-    const float mc = a.stats[2 * s];
-    const float f = mc == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : exp2_fast(mc - top);
-    sum += f * a.stats[2 * s + 1];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (lane + 32 * e < a.head_dim) v[e] += f * a.parts[s * a.head_dim + lane + 32 * e];
+  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[w]);
+  __syncthreads();
+  for (int i = tid; i < shares; i += kJoinThreads) {
+    const float2 st = a.stats[share(i)];
+    const float f = st.x == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : exp2_fast(st.x - top);
+    weights[i] = f;
+    sum += f * st.y;
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[warp][lane + 32 * e] = v[e];
-  if (lane == 0) sums[warp] = sum;
+  for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(~0u, sum, off);
+  if (lane == 0) red[warp] = sum;
   __syncthreads();
   sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum += sums[w];
-  for (int d = tid; d < a.head_dim; d += kThreads) {
-    float x = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) x += acc[w][d];
-    out[d] = Tr::from(sum == 0.f ? 0.f : x / sum);
+  for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[w];
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col < cols) {
+#pragma unroll 4
+    for (int i = gi; i < shares; i += groups) {
+      const float4 x = *reinterpret_cast<const float4*>(a.parts + share(i) * a.head_dim + col * 4);
+      const float f = weights[i];
+      v.x = fmaf(f, x.x, v.x);
+      v.y = fmaf(f, x.y, v.y);
+      v.z = fmaf(f, x.z, v.z);
+      v.w = fmaf(f, x.w, v.w);
+    }
   }
-  if (tid == 0 && a.lse) a.lse[(long long)b * a.q_heads + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum) - Tr::kShift) * kLn2;
+  acc[tid] = v;
+  __syncthreads();
+  if (gi == 0 && col < cols) {
+    for (int w = 1; w < groups; ++w) {
+      const float4 x = acc[w * across + col];
+      v.x += x.x;
+      v.y += x.y;
+      v.z += x.z;
+      v.w += x.w;
+    }
+    T* out = (T*)a.out + (long long)b * a.o_sb + (long long)qh * a.o_sh + col * 4;
+    const float r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = Tr::from(sum == 0.f ? 0.f : r[e] / sum);
+    if (col == 0 && a.lse) a.lse[(long long)b * a.q_heads + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum) - Tr::kShift) * kLn2;
+  }
 }
 
 // CTAs of one wave of a kernel on the current device, asked once per device.
-template <typename T, int DP, int NT>
+template <class K>
 int wave() {
   static std::once_flag once[64];
   static int ctas[64];
   const int dev = current_device();
   std::call_once(once[dev], [dev] {
-    using L = Layout<T, DP, NT>;
-    PFB_CUDA(cudaFuncSetAttribute(attend_kernel<T, DP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem));
+    PFB_CUDA(cudaFuncSetAttribute(K::run, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)K::L::smem));
     int per = 0;
-    PFB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attend_kernel<T, DP, NT>, kThreads, L::smem));
-    ctas[dev] = std::max(1, per) * device_sm_count(dev);
+    PFB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, K::run, kThreads, K::L::smem));
+    ctas[dev] = std::min(std::max(1, per) * device_sm_count(dev), kMostCtas);
   });
   return ctas[dev];
 }
 
-template <typename T, int DP, int NT>
+template <class K>
 void launch_sized(Args& a, cudaStream_t stream) {
-  attend_kernel<T, DP, NT><<<(unsigned)a.ctas, kThreads, Layout<T, DP, NT>::smem, stream>>>(a);
+  K::run<<<(unsigned)a.ctas, kThreads, K::L::smem, stream>>>(a);
   PFB_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((int64_t)a.batch * a.q_heads));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)std::max(a.ctas, a.batch), (unsigned)a.heads);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  PFB_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<T>, (const Args&)a));
+  PFB_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<typename K::T>, (const Args&)a));
 }
 
-template <typename T_, int DP_, int NT_>
+template <typename T_, int DP, int NT, bool CORES>
 struct Kernel {
   using T = T_;
-  static constexpr int DP = DP_, NT = NT_;
+  using L = Layout<T, DP, NT, CORES>;
+  static constexpr auto run = attend_kernel<T, DP, NT, CORES>;
 };
 
-// Query heads of a unit: two column blocks hold 16, but their accumulators
-// fit the registers only with 16-bit types and head_dim up to 128.
+// Query heads of a unit, as many as the registers hold: on the tensor cores
+// two column blocks (16 heads) only with 16-bit types and head_dim up to 128;
+// on the CUDA cores up to 4, of wide heads up to 2.
 int unit_heads(const pfk_paged_attention_params& p) {
-  return p.q_heads / p.cache.heads > 8 && p.cache.dtype != PFC_DTYPE_FLOAT32 && p.cache.head_dim <= 128 ? 16 : 8;
+  const int64_t group = p.q_heads / p.cache.heads;
+  const bool wide = p.cache.head_dim > 128;
+  if (p.cache.dtype != PFC_DTYPE_FLOAT32) return group > 8 && !wide ? 16 : 8;
+  if (group <= 1) return 1;
+  if (group <= 2 || wide) return 2;
+  return group <= 4 ? 4 : 8;
 }
 
-// Calls f(Kernel<T, DP, NT>()) for the call's type and sizes.
+template <class F>
+void dispatch32(int heads, int64_t head_dim, F&& f) {
+  if (head_dim > 128) {
+    heads == 1 ? f(Kernel<float, 256, 1, true>()) : f(Kernel<float, 256, 2, true>());
+  } else if (head_dim > 64) {
+    if (heads == 1) f(Kernel<float, 128, 1, true>());
+    else if (heads == 2) f(Kernel<float, 128, 2, true>());
+    else if (heads == 4) f(Kernel<float, 128, 4, true>());
+    else f(Kernel<float, 128, 1, false>());
+  } else {
+    if (heads == 1) f(Kernel<float, 64, 1, true>());
+    else if (heads == 2) f(Kernel<float, 64, 2, true>());
+    else if (heads == 4) f(Kernel<float, 64, 4, true>());
+    else f(Kernel<float, 64, 1, false>());
+  }
+}
+
+template <typename T, class F>
+void dispatch16(int heads, int64_t head_dim, F&& f) {
+  if (head_dim > 128) f(Kernel<T, 256, 1, false>());
+  else if (head_dim > 64) heads == 16 ? f(Kernel<T, 128, 2, false>()) : f(Kernel<T, 128, 1, false>());
+  else heads == 16 ? f(Kernel<T, 64, 2, false>()) : f(Kernel<T, 64, 1, false>());
+}
+
+// Calls f(Kernel<...>()) for the call's type and sizes.
 template <class F>
 void dispatch(const pfk_paged_attention_params& p, F&& f) {
-  const bool wide = unit_heads(p) == 16;
+  const int heads = unit_heads(p);
   const int64_t d = p.cache.head_dim;
-  switch (p.cache.dtype) {
-    case PFC_DTYPE_FLOAT32:
-      if (d <= 64) f(Kernel<float, 64, 1>());
-      else if (d <= 128) f(Kernel<float, 128, 1>());
-      else f(Kernel<float, 256, 1>());
-      break;
-    case PFC_DTYPE_FLOAT16:
-      if (d <= 64) wide ? f(Kernel<__half, 64, 2>()) : f(Kernel<__half, 64, 1>());
-      else if (d <= 128) wide ? f(Kernel<__half, 128, 2>()) : f(Kernel<__half, 128, 1>());
-      else f(Kernel<__half, 256, 1>());
-      break;
-    default:
-      if (d <= 64) wide ? f(Kernel<__nv_bfloat16, 64, 2>()) : f(Kernel<__nv_bfloat16, 64, 1>());
-      else if (d <= 128) wide ? f(Kernel<__nv_bfloat16, 128, 2>()) : f(Kernel<__nv_bfloat16, 128, 1>());
-      else f(Kernel<__nv_bfloat16, 256, 1>());
-  }
+  if (p.cache.dtype == PFC_DTYPE_FLOAT16) dispatch16<__half>(heads, d, f);
+  else if (p.cache.dtype == PFC_DTYPE_BFLOAT16) dispatch16<__nv_bfloat16>(heads, d, f);
+  else dispatch32(heads, d, f);
 }
 
 void check(const pfk_paged_attention_params& p) {
@@ -719,18 +890,16 @@ void check(const pfk_paged_attention_params& p) {
 
 struct Plan {
   int ctas, heads;
-  int64_t units, stats_at, parts_at, bytes;
+  int64_t stats_at, parts_at, bytes;
 };
 
 Plan plan_of(const pfk_paged_attention_params& p) {
   Plan w;
   const int64_t group = p.q_heads / p.cache.heads;
-  const int most = unit_heads(p);
-  w.heads = (int)std::min<int64_t>(group, most);
-  dispatch(p, [&](auto k) { w.ctas = wave<typename decltype(k)::T, decltype(k)::DP, decltype(k)::NT>(); });
-  w.units = p.batch * p.cache.heads * ceil_div(group, most);
-  w.stats_at = round_up((1 + w.units) * 8, 16);
-  w.parts_at = round_up(w.stats_at + (int64_t)w.ctas * 2 * w.heads * 2 * 4, 16);
+  w.heads = (int)std::min<int64_t>(group, unit_heads(p));
+  dispatch(p, [&](auto k) { w.ctas = wave<decltype(k)>(); });
+  w.stats_at = (int64_t)w.ctas * 16;
+  w.parts_at = round_up(w.stats_at + (int64_t)w.ctas * 2 * w.heads * 8, 16);
   w.bytes = w.parts_at + (int64_t)w.ctas * 2 * w.heads * p.cache.head_dim * 4;
   return w;
 }
@@ -793,16 +962,16 @@ void launch_paged_attention(const pfk_paged_attention_params& p, cudaStream_t st
   a.table = p.block_table;
   a.table_stride = p.table_stride;
   a.seq_lens = p.seq_lens;
-  a.most = std::min<int64_t>(p.table_width * c.page_size, INT32_MAX - kTile);
+  a.most = std::min<int64_t>(p.table_width * c.page_size, INT32_MAX - 64);
   a.window = (int)std::min<int64_t>(p.window, INT32_MAX);
   a.scale = p.scale;
   char* ws = (char*)p.workspace;
-  a.starts = (long long*)ws;
-  a.stats = (float*)(ws + w.stats_at);
+  a.records = (int4*)ws;
+  a.stats = (float2*)(ws + w.stats_at);
   a.parts = (float*)(ws + w.parts_at);
   a.ctas = w.ctas;
   a.heads = w.heads;
-  dispatch(p, [&](auto k) { launch_sized<typename decltype(k)::T, decltype(k)::DP, decltype(k)::NT>(a, stream); });
+  dispatch(p, [&](auto k) { launch_sized<decltype(k)>(a, stream); });
 }
 
 }  // namespace pfb

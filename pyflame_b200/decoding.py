@@ -72,16 +72,36 @@ def _cuda(t, name: str):
     return t.device
 
 
+_device = _stream = None
+
+
 def _call(fn, device, *args) -> None:
-    """One entry point on the current stream of `device`."""
-    import torch
-    cuda = torch.cuda
-    stream = C.c_void_p(cuda.current_stream(device).cuda_stream)
-    if cuda.current_device() == device.index:
-        N.check(fn(*args, stream))
+    """One entry point on torch's current stream of `device`."""
+    global _device, _stream
+    if _device is None:
+        import torch
+        # what torch.cuda.current_device() and current_stream().cuda_stream read, without their 2 us of Python
+        _device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    index = device.index
+    if _device() == index:
+        N.check(fn(*args, _stream(index)))
     else:
-        with cuda.device(device):
-            N.check(fn(*args, stream))
+        import torch
+        with torch.cuda.device(device):
+            N.check(fn(*args, _stream(index)))
+
+
+class _Plans(dict):
+    """What a call's checks found, by everything about its tensors that they
+    look at (types, shapes, strides, devices; never addresses or contents), so
+    that a loop of like calls is checked once."""
+
+    def keep(self, key, plan, *tensors):
+        if not any(t.requires_grad for t in tensors if t is not None):  # refused or not by the grad mode of each call
+            if len(self) >= 512:
+                self.clear()
+            self[key] = plan
+        return plan
 
 
 # ---------------------------------------------------------------------------
@@ -174,8 +194,9 @@ class RotaryEmbedding:
         _cuda(self.inv_freq, "device")
         self.device = self.inv_freq.device
         self._c = N.RotaryC(self.inv_freq.data_ptr(), rotary_dim, int(layout == "interleaved"), self.factor)
+        self._plans = _Plans()
 
-    def _run(self, x, positions, out, inverse: int):
+    def _plan(self, x, positions, out, inverse: int):
         import torch
         _cuda(x, "x")
         dims = len(x.shape)
@@ -183,7 +204,6 @@ class RotaryEmbedding:
             raise ValueError("x must be [tokens, heads, head_dim] or [batch, tokens, heads, head_dim]")
         code = _code(x.dtype)
         _check("x", x, (None,) * (dims - 1) + (self.head_dim,), x.dtype, self.device)
-        xs = x.stride()
         batch, tokens, heads = (1,) * (4 - dims) + tuple(x.shape[:-1])
         if len(positions.shape) == 2 and dims == 4:
             _check("positions", positions, (batch, tokens), torch.int64, self.device, False)
@@ -191,15 +211,27 @@ class RotaryEmbedding:
         else:
             _check("positions", positions, (tokens,), torch.int64, self.device, False)
             p_sb, p_st = 0, positions.stride(0)
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        else:
+        if out is not None:
             _check("out", out, x.shape, x.dtype, self.device, output=True)
-            if out.data_ptr() == x.data_ptr() and out.stride() != xs and x.numel():
-                raise ValueError("out: shares x's memory with other strides")
-        ys = out.stride()
+        xs = x.stride()
+        ys = torch.empty(x.shape, device="meta").stride() if out is None else out.stride()
         p = N.RopeParamsC(code, inverse, batch, tokens, heads, self.head_dim, xs[0] if dims == 4 else 0, xs[-3], xs[-2],
-                          ys[0] if dims == 4 else 0, ys[-3], ys[-2], positions.data_ptr(), p_sb, p_st, self._c)
+                          ys[0] if dims == 4 else 0, ys[-3], ys[-2], None, p_sb, p_st, self._c)
+        return p, x.is_contiguous(), out is not None and tuple(xs) != tuple(ys) and x.numel() > 0
+
+    def _run(self, x, positions, out, inverse: int):
+        import torch
+        key = (inverse, x.dtype, x.shape, x.stride(), x.device, x.requires_grad, positions.dtype, positions.shape,
+               positions.stride(), positions.device)
+        if out is not None:
+            key += (out.dtype, out.shape, out.stride(), out.device, out.requires_grad)
+        plan = self._plans.get(key) or self._plans.keep(key, self._plan(x, positions, out, inverse), x, out)
+        if out is None:
+            out = torch.empty_like(x) if plan[1] else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif plan[2] and out.data_ptr() == x.data_ptr():
+            raise ValueError("out: shares x's memory with other strides")
+        p = N.RopeParamsC.from_buffer_copy(plan[0])
+        p.positions = positions.data_ptr()
         _call(N.lib().pfk_rope, self.device, x.data_ptr(), out.data_ptr(), C.byref(p))
         return out
 
@@ -261,7 +293,7 @@ class PagedKVCache:
         self.num_pages, self.page_size, self.num_heads, self.head_dim = k.shape
         self._err = torch.zeros(1, dtype=torch.int32, device=device)
         self._c = N.PagedCacheC(code, k.data_ptr(), v.data_ptr(), *k.shape, *k.stride()[:3], self._err.data_ptr())
-        self._workspace = {}
+        self._plans = _Plans()
         self._no_rotary = N.RotaryC(None, 0, 0, 1.0)
 
     def append(self, k, v, slots, positions=None, rotary: Optional[RotaryEmbedding] = None, q=None, q_out=None):
@@ -272,38 +304,59 @@ class PagedKVCache:
         rotated queries (`q_out`, which may be q, or a new tensor, whose rows
         of skipped tokens are 0).  The slots of one call are distinct."""
         import torch
+        key = ("append", k.dtype, k.shape, k.stride(), k.device, k.requires_grad, v.dtype, v.shape, v.stride(), v.device,
+               v.requires_grad, slots.dtype, slots.shape, slots.stride(), slots.device)
+        if rotary is not None and positions is not None:
+            key += (rotary.head_dim, rotary.device, positions.dtype, positions.shape, positions.stride(), positions.device)
+        if q is not None:
+            key += (q.dtype, q.shape, q.stride(), q.device, q.requires_grad)
+        if q_out is not None:
+            key += (q_out.dtype, q_out.shape, q_out.stride(), q_out.device, q_out.requires_grad)
+        key += (rotary is None, positions is None, q is None, q_out is None)
+        plan = self._plans.get(key) or self._plans.keep(
+            key, self._append_plan(k, v, slots, positions, rotary, q, q_out), k, v, q, q_out)
+        p = N.PagedAppendParamsC.from_buffer_copy(plan[0])
+        p.k, p.v, p.slots = k.data_ptr(), v.data_ptr(), slots.data_ptr()
+        if rotary is not None:
+            p.positions, p.rotary = positions.data_ptr(), rotary._c
+        if q is not None:
+            if q_out is None:
+                q_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+            elif plan[1] and q_out.data_ptr() == q.data_ptr():
+                raise ValueError("q_out: shares q's memory with other strides")
+            if p.q_heads:
+                p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
+        _call(N.lib().pfk_paged_append, self.device, C.byref(p))
+        return q_out
+
+    def _append_plan(self, k, v, slots, positions, rotary, q, q_out):
+        import torch
         n, h, d = len(k), self.num_heads, self.head_dim
         _check("k", k, (n, h, d), self.dtype, self.device)
         _check("v", v, (n, h, d), self.dtype, self.device)
         _check("slots", slots, (n,), torch.int64, self.device)
         if (rotary is None) != (positions is None):
             raise ValueError("positions and rotary go together")
-        turn, at = self._no_rotary, None
         if rotary is not None:
             if rotary.head_dim != d or rotary.device != self.device:
                 raise ValueError("rotary: is for another head_dim or device")
             _check("positions", positions, (n,), torch.int64, self.device)
-            turn, at = rotary._c, positions.data_ptr()
-        ks, vs = k.stride(), v.stride()
-        p = N.PagedAppendParamsC(self._c, n, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1])
+        ks, vs, other = k.stride(), v.stride(), False
+        p = N.PagedAppendParamsC(self._c, n, None, ks[0], ks[1], None, vs[0], vs[1])
+        p.rotary = self._no_rotary
         if q is not None:
             _check("q", q, (n, None, d), self.dtype, self.device)
-            if q_out is None:
-                q_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-            else:
+            qs = os = q.stride()
+            if q_out is not None:
                 _check("q_out", q_out, q.shape, self.dtype, self.device, output=True)
-                if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride() and q.numel():
-                    raise ValueError("q_out: shares q's memory with other strides")
-            qs, os = q.stride(), q_out.stride()
-            p.q, p.q_out, p.q_heads = q.data_ptr(), q_out.data_ptr(), q.shape[1]
-            p.q_st, p.q_sh, p.qo_st, p.qo_sh = qs[0], qs[1], os[0], os[1]
-            if not p.q_heads:
-                p.q = p.q_out = None
+                os = q_out.stride()
+                other = tuple(qs) != tuple(os) and q.numel() > 0
+            else:
+                os = torch.empty(q.shape, device="meta").stride()
+            p.q_heads, p.q_st, p.q_sh, p.qo_st, p.qo_sh = q.shape[1], qs[0], qs[1], os[0], os[1]
         elif q_out is not None:
             raise ValueError("q_out without q")
-        p.slots, p.positions, p.rotary = slots.data_ptr(), at, turn
-        _call(N.lib().pfk_paged_append, self.device, C.byref(p))
-        return q_out
+        return p, other
 
     def attend(self, q, block_table, seq_lens, scale: Optional[float] = None, window: int = 0, out=None,
                return_lse: bool = False):
@@ -316,6 +369,29 @@ class PagedKVCache:
         gives 0.  With return_lse also the natural logarithm of the sum of
         exp(score), float32 [batch, q_heads] (-inf for length 0)."""
         import torch
+        key = ("attend", scale, window, return_lse, q.dtype, q.shape, q.stride(), q.device, q.requires_grad, block_table.dtype,
+               block_table.shape, block_table.stride(), block_table.device, seq_lens.dtype, seq_lens.shape, seq_lens.stride(),
+               seq_lens.device)
+        if out is not None:
+            key += (out.dtype, out.shape, out.stride(), out.device, out.requires_grad)
+        plan = self._plans.get(key) or self._plans.keep(
+            key, self._attend_plan(q, block_table, seq_lens, scale, window, out), q, out)
+        if out is None:
+            out = torch.empty_like(q) if plan[1] else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        p = N.PagedAttentionParamsC.from_buffer_copy(plan[0])
+        p.q, p.out, p.block_table, p.seq_lens = q.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
+        lse = None
+        if return_lse:
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+            p.lse = lse.data_ptr()
+        # a workspace per call, from torch's allocator: calls on several streams and captured graphs share none
+        work = torch.empty(p.workspace_bytes, dtype=torch.uint8, device=q.device)
+        p.workspace = work.data_ptr()
+        _call(N.lib().pfk_paged_attention, self.device, C.byref(p))
+        return (out, lse) if return_lse else out
+
+    def _attend_plan(self, q, block_table, seq_lens, scale, window, out):
+        import torch
         if len(q.shape) != 3:
             raise ValueError("q must be [batch, q_heads, head_dim]")
         batch, heads, d = q.shape
@@ -327,26 +403,17 @@ class PagedKVCache:
         if window < 0:
             raise ValueError("window must not be negative")
         scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-        if out is None:
-            out = torch.empty((batch, heads, d), dtype=q.dtype, device=q.device)
-        else:
+        if out is not None:
             _check("out", out, (batch, heads, d), self.dtype, self.device, output=True)
-        lse = torch.empty((batch, heads), dtype=torch.float32, device=q.device) if return_lse else None
-        qs, os = q.stride(), out.stride()
-        p = N.PagedAttentionParamsC(self._c, batch, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
-                                    lse.data_ptr() if return_lse else None, block_table.data_ptr(),
-                                    block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), int(window), scale)
-        need = self._workspace.get((batch, heads))
-        if need is None:
-            size = C.c_size_t(0)
-            with torch.cuda.device(self.device):
-                N.check(N.lib().pfk_paged_attention_workspace(C.byref(p), C.byref(size)))
-            need = self._workspace[batch, heads] = size.value
-        # a workspace per call, from torch's allocator: calls on several streams and captured graphs share none
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        p.workspace, p.workspace_bytes = work.data_ptr(), need
-        _call(N.lib().pfk_paged_attention, self.device, C.byref(p))
-        return (out, lse) if return_lse else out
+        qs = q.stride()
+        os = torch.empty(q.shape, device="meta").stride() if out is None else out.stride()
+        p = N.PagedAttentionParamsC(self._c, batch, heads, None, qs[0], qs[1], None, os[0], os[1], None, None,
+                                    block_table.stride(0), block_table.shape[1], None, int(window), scale)
+        size = C.c_size_t(0)
+        with torch.cuda.device(self.device):
+            N.check(N.lib().pfk_paged_attention_workspace(C.byref(p), C.byref(size)))
+        p.workspace_bytes = size.value
+        return p, q.is_contiguous()
 
     def check(self) -> None:
         """Wait for the device and raise PfcError if a call met a slot, page
@@ -399,6 +466,7 @@ class Linear4bit:
         self.in_features, self.out_features, self.group_size = k, n, int(group_size)
         self.device, self.scales, self.zeros, self.bias = device, scales.contiguous(), zeros, bias
         self.weight = torch.empty((n, -(-k // 128) * 16), dtype=torch.int32, device=device)
+        self._plans = _Plans()
         packed = packed.contiguous()
         _call(N.lib().pfk_w4_arrange, device, packed.data_ptr(), n, k, self.weight.data_ptr())
 
@@ -433,22 +501,35 @@ class Linear4bit:
     def __call__(self, x, out=None):
         """x: [..., in_features], the rows at any one stride."""
         import torch
+        key = (x.dtype, x.shape, x.stride(), x.device, x.requires_grad)
+        if out is not None:
+            key += (out.dtype, out.shape, out.stride(), out.device, out.requires_grad)
+        plan = self._plans.get(key) or self._plans.keep(key, self._plan(x, out), x, out)
+        if plan[2]:
+            x = x.reshape(-1, self.in_features)
+        if out is None:
+            out = torch.empty(plan[1], dtype=x.dtype, device=x.device)
+        p = N.LinearW4ParamsC.from_buffer_copy(plan[0])
+        p.x, p.y = x.data_ptr(), out.data_ptr()
+        _call(N.lib().pfk_linear_w4, self.device, C.byref(p))
+        return out
+
+    def _plan(self, x, out):
         _cuda(x, "x")
         code = _code(x.dtype)
+        if len(x.shape) < 1:
+            raise ValueError("x must be [..., in_features]")
         _check("x", x, (None,) * (len(x.shape) - 1) + (self.in_features,), x.dtype, self.device)
         if self.bias is not None and self.bias.dtype != x.dtype:
             raise TypeError(f"x: dtype must be the bias's, {self.bias.dtype}, not {x.dtype}")
         rows = x if len(x.shape) == 2 else x.reshape(-1, self.in_features)
         shape = tuple(x.shape[:-1]) + (self.out_features,)
-        if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=x.device)
-        else:
+        y_st = self.out_features
+        if out is not None:
             _check("out", out, shape, x.dtype, self.device, output=True)
-        flat = out if len(shape) == 2 else out.view(-1, self.out_features)
-        p = N.LinearW4ParamsC(code, rows.shape[0], self.in_features, self.out_features, self.group_size,
-                              rows.data_ptr(), rows.stride(0), flat.data_ptr(), flat.stride(0), self.weight.data_ptr(),
-                              self.scales.data_ptr(), self.scale_code,
+            y_st = (out if len(shape) == 2 else out.view(-1, self.out_features)).stride(0)
+        p = N.LinearW4ParamsC(code, rows.shape[0], self.in_features, self.out_features, self.group_size, None,
+                              rows.stride(0), None, y_st, self.weight.data_ptr(), self.scales.data_ptr(), self.scale_code,
                               None if self.zeros is None else self.zeros.data_ptr(),
                               None if self.bias is None else self.bias.data_ptr())
-        _call(N.lib().pfk_linear_w4, self.device, C.byref(p))
-        return out
+        return p, shape, len(x.shape) != 2
