@@ -217,10 +217,12 @@ struct Layout {
   static constexpr size_t o_bytes = (size_t)kWarps * kHeads * kPitch * 4;
   static constexpr size_t m_bytes = (size_t)2 * kWarps * kHeads * 4;
   static constexpr size_t smem = q_bytes + o_bytes + m_bytes;
+  // CTAs that share an SM: as many warps' loads in flight as the registers hold
+  static constexpr int kResident = sizeof(T) == 2 ? (DP <= 64 ? (NT == 1 ? 4 : 3) : DP <= 128 && NT == 1 ? 3 : 2) : DP <= 64 ? 3 : 2;
 };
 
 template <typename T, int DP, int NT, bool CORES>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident)) attend_kernel(const Args a) {
   using L = Layout<T, DP, NT, CORES>;
   using Tr = Traits<T>;
   constexpr int VEC = L::kVec, HEADS = L::kHeads;
@@ -271,10 +273,12 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
     start = scan_rows(tid);
     total = scanned();
   }
-  // runs of total / ctas tiles, the first ones a tile longer
-  const long long run = (long long)divide(total, a.ctas), longer = total - run * a.ctas;
-  const long long t0 = run * blockIdx.x + min((long long)blockIdx.x, longer);
-  const long long t1 = t0 + run + (blockIdx.x < longer ? 1 : 0);
+  // runs of total / ctas tiles, the longer ones spread evenly (neighbouring
+  // CTAs share an SM: 505 us for 487 with the longer runs first)
+  const int ctas = (int)min((long long)a.ctas, total);
+  const long long c = min((int)blockIdx.x, ctas);
+  const long long t0 = ctas ? (long long)divide(total * c, ctas) : 0;
+  const long long t1 = c < ctas ? (long long)divide(total * (c + 1), ctas) : t0;
   if (t0 >= t1) {
     if (tid == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
@@ -301,63 +305,83 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
   int4 record = make_int4(0, 0, 0, 0);
 
   const float scale2 = a.scale * kLog2e;
+
+  // The loads run ahead of the products and over the borders of units: ahead
+  // stands at the step after the next, whose place in the cache it looks up.
+  struct {
+    long long at;
+    int row, unit, tile, begin, end, tiles;
+  } ahead = {t0, row, unit, tile, sp.begin, sp.end, sp.tiles};
+  struct Place {
+    unsigned where;  // of one of the warp's keys (lane modulo their number), in units
+    int head;
+  };
+  auto place = [&]() -> Place {
+    Place p = {kNone, 0};
+    if (ahead.at >= t1) return p;
+    p.head = ahead.unit / a.chunks;
+    const int key = (ahead.begin / L::kTile + ahead.tile) * L::kTile + warp * 8 * L::kRows + (lane & (8 * L::kRows - 1));
+    if (key >= ahead.begin && key < ahead.end) {
+      const unsigned i = a.by_page.div((unsigned)key);
+      const unsigned page = (unsigned)a.table[(long long)ahead.row * a.table_stride + i];
+      if (page < a.num_pages) p.where = page * a.page_units + ((unsigned)key - i * a.by_page.d) * a.token_units;
+      else if (a.err) *a.err = PFC_ERR_INVALID_ARGUMENT;
+    }
+    ++ahead.at;
+    if (++ahead.tile == ahead.tiles) {
+      ahead.tile = 0;
+      if (++ahead.unit == per_row) {
+        ahead.unit = 0;
+        if (ahead.at < t1) {
+          Span n;
+          do n = span_of<L::kTile>(a, ++ahead.row);
+          while (n.tiles == 0);  // there is one: the list goes on
+          ahead.begin = n.begin;
+          ahead.end = n.end;
+          ahead.tiles = n.tiles;
+        }
+      }
+    }
+    return p;
+  };
+  uint4 kr[L::kRows][L::kQ], vr[2 * L::kRows][L::kV];
+  unsigned ku[L::kRows], vu[2 * L::kRows];  // places of the rows that are loaded next
+  const char *kp, *vp;
+  auto aim = [&](const Place& p) {
+#pragma unroll
+    for (int r = 0; r < L::kRows; ++r) ku[r] = __shfl_sync(~0u, p.where, g + 8 * r);
+#pragma unroll
+    for (int r = 0; r < 2 * L::kRows; ++r) vu[r] = __shfl_sync(~0u, p.where, 2 * t + (r & 1) + 8 * (r >> 1));
+    kp = a.k + p.head * a.head_bytes + t * 16;
+    vp = a.v + p.head * a.head_bytes + g * 16;
+  };
+  auto load_k = [&](int c) {
+#pragma unroll
+    for (int r = 0; r < L::kRows; ++r) {
+      kr[r][c] = make_uint4(0, 0, 0, 0);
+      if (ku[r] != kNone && (c * 4 + t) * VEC < a.head_dim) kr[r][c] = load16(kp + ku[r] * a.unit_bytes + c * 64);
+    }
+  };
+  auto load_v = [&](int c) {
+#pragma unroll
+    for (int r = 0; r < 2 * L::kRows; ++r) {
+      vr[r][c] = make_uint4(0, 0, 0, 0);
+      if (vu[r] != kNone && (c * 8 + g) * VEC < a.head_dim) vr[r][c] = load16(vp + vu[r] * a.unit_bytes + c * 128);
+    }
+  };
+  aim(place());
+#pragma unroll
+  for (int c = 0; c < L::kQ; ++c) load_k(c);
+#pragma unroll
+  for (int c = 0; c < L::kV; ++c) load_v(c);
+  Place next = place();
+
   for (long long at = t0; at < t1;) {
     while (sp.tiles == 0) sp = span_of<L::kTile>(a, ++row);
     const int count = (int)min((long long)(sp.tiles - tile), t1 - at);
     const int head = unit / a.chunks;
     const int first_q = head * a.group + (unit - head * a.chunks) * a.unit_heads;
     const int heads = min(a.unit_heads, (head + 1) * a.group - first_q);
-
-    const char* kp = a.k + head * a.head_bytes;
-    const char* vp = a.v + head * a.head_bytes;
-    const int* table = a.table + (long long)row * a.table_stride;
-    const int lo_key = sp.begin, hi_key = sp.end;
-    const int first_key = (sp.begin / L::kTile + tile) * L::kTile + warp * 8 * L::kRows;
-
-    // place of one of the warp's keys of a step (lane modulo their number) in the cache, in units
-    auto place = [&](int step) -> unsigned {
-      if (step >= count) return kNone;
-      const int key = first_key + step * L::kTile + (lane & (8 * L::kRows - 1));
-      if (key < lo_key || key >= hi_key) return kNone;
-      const unsigned p = a.by_page.div((unsigned)key);
-      const unsigned page = (unsigned)table[p];
-      if (page >= a.num_pages) {
-        if (a.err) *a.err = PFC_ERR_INVALID_ARGUMENT;
-        return kNone;
-      }
-      return page * a.page_units + ((unsigned)key - p * a.by_page.d) * a.token_units;
-    };
-    uint4 kr[L::kRows][L::kQ], vr[2 * L::kRows][L::kV];
-    auto load_k = [&](unsigned where, bool (&seen)[L::kRows]) {
-#pragma unroll
-      for (int r = 0; r < L::kRows; ++r) {
-        const unsigned u = __shfl_sync(~0u, where, g + 8 * r);
-        seen[r] = u != kNone;
-        const char* p = kp + (unsigned long long)u * a.unit_bytes + t * 16;
-#pragma unroll
-        for (int c = 0; c < L::kQ; ++c) {
-          kr[r][c] = make_uint4(0, 0, 0, 0);
-          if (seen[r] && (c * 4 + t) * VEC < a.head_dim) kr[r][c] = load16(p + c * 64);
-        }
-      }
-    };
-    auto load_v = [&](unsigned where) {
-#pragma unroll
-      for (int r = 0; r < 2 * L::kRows; ++r) {
-        const unsigned u = __shfl_sync(~0u, where, 2 * t + (r & 1) + 8 * (r >> 1));
-        const char* p = vp + (unsigned long long)u * a.unit_bytes + g * 16;
-#pragma unroll
-        for (int c = 0; c < L::kV; ++c) {
-          vr[r][c] = make_uint4(0, 0, 0, 0);
-          if (u != kNone && (c * 8 + g) * VEC < a.head_dim) vr[r][c] = load16(p + c * 128);
-        }
-      }
-    };
-    bool seen[L::kRows];
-    unsigned next = place(0);
-    load_k(next, seen);
-    load_v(next);
-    next = place(1);
 
     // Q in the order of the second operand's registers
     __syncthreads();  // the previous piece's reads of shared memory are over
@@ -416,7 +440,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
     for (int step = 0; step < count; ++step) {
       bool live[L::kRows];
 #pragma unroll
-      for (int r = 0; r < L::kRows; ++r) live[r] = seen[r];
+      for (int r = 0; r < L::kRows; ++r) live[r] = ku[r] != kNone;
+      aim(next);
       if constexpr (CORES) {
         float s[NT][L::kRows];  // of keys g (and g + 8), the same in a quad's lanes
 #pragma unroll
@@ -434,11 +459,11 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
               even[r] = fmaf(q.z, __uint_as_float(kr[r][c].z), even[r]);
               odd[r] = fmaf(q.w, __uint_as_float(kr[r][c].w), odd[r]);
             }
+            if (h == NT - 1) load_k(c);
           }
 #pragma unroll
           for (int r = 0; r < L::kRows; ++r) s[h][r] = even[r] + odd[r];
         }
-        if (step + 1 < count) load_k(next, seen);
         float p[NT][2 * L::kRows];  // of the lane's value rows
 #pragma unroll
         for (int h = 0; h < NT; ++h) {
@@ -475,7 +500,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
           }
         }
 #pragma unroll
-        for (int c = 0; c < L::kV; ++c)
+        for (int c = 0; c < L::kV; ++c) {
 #pragma unroll
           for (int h = 0; h < NT; ++h)
 #pragma unroll
@@ -483,13 +508,16 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 o[h][c][e >> 1][e & 1] = fmaf(p[h][r], __uint_as_float(word(vr[r][c], e)), o[h][c][e >> 1][e & 1]);
+          load_v(c);
+        }
       } else {
         float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          // several accumulators, added at the end: a chain of instructions on
-          // one would wait for each
-          constexpr int CH = k32 ? 3 : 2;
+          // fp32 has 48 instructions on a score and keeps three accumulators,
+          // so as not to wait for each; 16-bit types have 8 (two accumulators
+          // measured 505 us for 423 at 128 sequences of 5000 keys)
+          constexpr int CH = k32 ? 3 : 1;
           float acc[CH][4];
 #pragma unroll
           for (int i = 0; i < CH; ++i)
@@ -497,7 +525,6 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
             for (int r = 0; r < 4; ++r) acc[i][r] = 0.f;
 #pragma unroll
           for (int c = 0; c < L::kQ; ++c) {
-            if (c * 4 * VEC >= a.head_dim) continue;
             const uint4 b = qs[(nt * L::kQ + c) * 32 + lane];
             if constexpr (k32) {
               const uint4 bl = qs[(NT * L::kQ + nt * L::kQ + c) * 32 + lane];
@@ -508,19 +535,19 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
                 split(__uint_as_float(word(kr[1][c], 2 * e)), h1, l1);
                 split(__uint_as_float(word(kr[0][c], 2 * e + 1)), h2, l2);
                 split(__uint_as_float(word(kr[1][c], 2 * e + 1)), h3, l3);
-                mma_tf32(acc[1], l0, l1, l2, l3, word(b, 2 * e), word(b, 2 * e + 1));
+                mma_tf32(acc[CH / 2], l0, l1, l2, l3, word(b, 2 * e), word(b, 2 * e + 1));
                 mma_tf32(acc[CH - 1], h0, h1, h2, h3, word(bl, 2 * e), word(bl, 2 * e + 1));
                 mma_tf32(acc[0], h0, h1, h2, h3, word(b, 2 * e), word(b, 2 * e + 1));
               }
             } else {
               Tr::mma(acc[0], kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, b.x, b.y);
-              Tr::mma(acc[1], kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, b.z, b.w);
+              Tr::mma(acc[0], kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, b.z, b.w);
             }
+            if (nt == NT - 1) load_k(c);
           }
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[nt][r] = acc[0][r] + (k32 ? acc[1][r] + acc[CH - 1][r] : acc[1][r]);
+          for (int r = 0; r < 4; ++r) s[nt][r] = k32 ? acc[0][r] + (acc[CH / 2][r] + acc[CH - 1][r]) : acc[0][r];
         }
-        if (step + 1 < count) load_k(next, seen);
 
         unsigned pt[NT][4];  // P as the second operand: 16-bit hi, lo of keys 0-7 and 8-15; fp32 its four values
 #pragma unroll
@@ -582,7 +609,6 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
 
 #pragma unroll
         for (int c = 0; c < L::kV; ++c) {
-          if (c * 8 * VEC >= a.head_dim) continue;
           if constexpr (k32) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {  // keys 8i ... 8i + 7
@@ -621,12 +647,10 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
               }
             }
           }
+          load_v(c);
         }
       }
-      if (step + 1 < count) {
-        load_v(next);
-        next = place(step + 2);
-      }
+      next = place();
     }
 
     // join the warps
@@ -687,8 +711,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const Args a) {
       }
     }
     if (tile == 0 && !whole) {  // the CTA that has the unit's last tile
-      const long long last = at + sp.tiles - 1, edge = longer * (run + 1);
-      record = make_int4(row, unit, (int)(last < edge ? divide(last, run + 1) : longer + divide(last - edge, run)), 1);
+      // tile x is in the last CTA c with floor(total c / ctas) <= x
+      record = make_int4(row, unit, (int)divide((at + sp.tiles) * ctas + total - 1, total) - 1, 1);
     }
     at += count;
     tile = 0;
