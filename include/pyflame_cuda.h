@@ -446,26 +446,38 @@ PFC_API int pfk_paged_attention_workspace(const pfk_paged_attention_params* p, s
  * outside the seen tokens has no effect. */
 PFC_API int pfk_paged_attention(const pfk_paged_attention_params* p, void* stream);
 
-/* Arranges 4-bit weights for pfk_linear_w4.  packed: [outer][(inner+1)/2]
- * bytes, column 2i in the low half of byte i.  weight: [outer][ru(inner)/8]
- * words, ru = round up to 128: block b of 128 columns is 16 words; word
- * 4*t + j holds columns 128b + 32j + 8t ... + 7, the columns in the order
- * 0, 2, 4, 6, 1, 3, 5, 7 from the lowest nibble up. */
-PFC_API int pfk_w4_arrange(const uint8_t* packed, int64_t outer, int64_t inner, uint32_t* weight, void* stream);
+/* Lays 4-bit weights out for pfk_linear_w4, once.
+ * weight: ceil(outer/16) * ceil(inner/128) blocks of 16 rows and 128 columns,
+ * those of the same rows together, 256 words each: word 16r + 4t + j holds
+ * columns 32j + 8t ... + 7 of row r, in the order 0, 2, 4, 6, 1, 3, 5, 7 from
+ * the lowest nibble up.
+ * meta: a word per row and group, the scale's float32 bits with the zero in
+ * the lowest four; for groups of 32 and 64 in the order of the weights'
+ * blocks, [16][128/group] each, for larger ones [ceil(outer/16)][groups][16].
+ * What lies behind the last row or column is 0. */
+typedef struct pfk_w4_arrange_params {
+    int64_t inner, outer;
+    int64_t group;          /* columns that share a scale: 32, 64 or a multiple of 128 */
+    const uint8_t* packed;  /* [outer][(inner+1)/2], column 2i in the low half of byte i */
+    const uint16_t* scales; /* [outer][ceil(inner/group)] */
+    int scale_dtype;        /* FLOAT16 or BFLOAT16 */
+    const uint8_t* zeros;   /* the same shape, 0..15, or NULL: 8 */
+    uint32_t* weight;
+    uint32_t* meta;
+} pfk_w4_arrange_params;
+PFC_API int pfk_w4_arrange(const pfk_w4_arrange_params* p, void* stream);
 
 typedef struct pfk_linear_w4_params {
     int dtype; /* of x, y and bias */
     int64_t rows, inner, outer;
-    int64_t group;  /* columns that share a scale: 32, 64 or a multiple of 128 */
-    const void* x;  /* [rows][inner] */
+    int64_t group;
+    const void* x; /* [rows][inner] */
     int64_t x_st;
     void* y; /* [rows][outer] */
     int64_t y_st;
-    const uint32_t* weight; /* pfk_w4_arrange's output, 16-byte aligned */
-    const void* scales;     /* [outer][ceil(inner/group)] dense */
-    int scale_dtype;
-    const uint8_t* zeros; /* [outer][ceil(inner/group)], 0..15, or NULL: 8 */
-    const void* bias;     /* [outer] or NULL */
+    const uint32_t* weight; /* pfk_w4_arrange's, 16-byte aligned */
+    const uint32_t* meta;
+    const void* bias;       /* [outer] or NULL */
 } pfk_linear_w4_params;
 /* y[m,n] = sum_k x[m,k] * (w[n,k] - zero) * scale (+ bias[n]), accumulated in
  * fp32 from products that are not rounded before. */

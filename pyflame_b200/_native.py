@@ -93,10 +93,14 @@ class PagedAttentionParamsC(C.Structure):
                 ("scale", C.c_float), ("workspace", _P), ("workspace_bytes", C.c_size_t)]
 
 
+class W4ArrangeParamsC(C.Structure):
+    _fields_ = [("inner", _I64), ("outer", _I64), ("group", _I64), ("packed", _P), ("scales", _P),
+                ("scale_dtype", C.c_int), ("zeros", _P), ("weight", _P), ("meta", _P)]
+
+
 class LinearW4ParamsC(C.Structure):
     _fields_ = [("dtype", C.c_int)] + [(n, _I64) for n in ("rows", "inner", "outer", "group")] + [
-        ("x", _P), ("x_st", _I64), ("y", _P), ("y_st", _I64), ("weight", _P), ("scales", _P),
-        ("scale_dtype", C.c_int), ("zeros", _P), ("bias", _P)]
+        ("x", _P), ("x_st", _I64), ("y", _P), ("y_st", _I64), ("weight", _P), ("meta", _P), ("bias", _P)]
 
 
 # name -> (restype, argtypes); the list is the C-ABI of include/pyflame_cuda.h
@@ -147,7 +151,7 @@ SIGNATURES = {
     "pfk_paged_append": (C.c_int, [C.POINTER(PagedAppendParamsC), _P]),
     "pfk_paged_attention_workspace": (C.c_int, [C.POINTER(PagedAttentionParamsC), C.POINTER(C.c_size_t)]),
     "pfk_paged_attention": (C.c_int, [C.POINTER(PagedAttentionParamsC), _P]),
-    "pfk_w4_arrange": (C.c_int, [_P, _I64, _I64, _P, _P]),
+    "pfk_w4_arrange": (C.c_int, [C.POINTER(W4ArrangeParamsC), _P]),
     "pfk_linear_w4": (C.c_int, [C.POINTER(LinearW4ParamsC), _P]),
 }
 

@@ -533,8 +533,11 @@ int pfk_paged_attention(const pfk_paged_attention_params* p, void* stream) {
   });
 }
 
-int pfk_w4_arrange(const uint8_t* packed, int64_t outer, int64_t inner, uint32_t* weight, void* stream) {
-  return guarded([&] { pfb::launch_w4_arrange(packed, outer, inner, weight, as_stream(stream)); });
+int pfk_w4_arrange(const pfk_w4_arrange_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_w4_arrange(*p, as_stream(stream));
+  });
 }
 
 int pfk_linear_w4(const pfk_linear_w4_params* p, void* stream) {

@@ -262,7 +262,7 @@ void launch_rope(const void* x, void* y, const pfk_rope_params& p, cudaStream_t 
 void launch_paged_append(const pfk_paged_append_params& p, cudaStream_t stream);
 size_t paged_attention_workspace(const pfk_paged_attention_params& p);
 void launch_paged_attention(const pfk_paged_attention_params& p, cudaStream_t stream);
-void launch_w4_arrange(const uint8_t* packed, int64_t outer, int64_t inner, uint32_t* weight, cudaStream_t stream);
+void launch_w4_arrange(const pfk_w4_arrange_params& p, cudaStream_t stream);
 void launch_linear_w4(const pfk_linear_w4_params& p, cudaStream_t stream);
 
 }  // namespace pfb

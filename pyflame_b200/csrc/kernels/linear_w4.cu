@@ -14,11 +14,25 @@
 // a nibble pair OR-ed into the mantissas of two 16-bit numbers is 2^7 + q
 // (2^10 + q in fp16), from which 2^7 + z is subtracted exactly.
 //
-// A CTA of 8 warps takes 16 output rows; its warps take the blocks of 128
-// columns in turn and add their sums through shared memory in a fixed order.
-// In a block a lane holds 16 bytes of two weight rows: the words of the
-// arranged layout give each lane 8 columns of each of the four 32-column
-// groups, so that no instruction mixes two groups.
+// A lane holds 16 bytes of each of two weight rows in a block of 128 columns:
+// the arranged layout gives it 8 columns of each of the four 32-column groups,
+// so that no instruction mixes two groups, and puts a warp's 1 KB together
+// (with whole rows in turn every load was eight pieces of 64 bytes: 22 us for
+// TIME_UP at 16384 x 4096).
+//
+// Two shapes of CTA, 8 warps each:
+//   few rows of x (8 columns of the instruction): the warps share the columns
+//   of 16 weight rows, or in pairs those of 64; a CTA keeps its part of x and
+//   walks over row tiles, so x is staged once;
+//   more: 128 weight rows (4 warps of 32, so that a fragment of x read from
+//   shared memory serves two instructions), two warps share the columns, x in
+//   chunks through two buffers.
+// Weights, scales and zeros reach a warp through a ring of its own in shared
+// memory, filled by asynchronous copies several steps ahead.  Where the rows
+// alone do not fill the device, the CTAs of a cluster share the columns and
+// add their sums through distributed shared memory, in the order of their
+// ranks: results do not depend on timing and nothing needs a workspace.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -36,11 +50,10 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kBlock = 128;            // columns of a warp's step
-constexpr int kStep = kBlock * kWarps; // of a CTA's step
-constexpr int kPad = 32;               // values between rows of x in shared memory: rows start 64 bytes apart mod 128
-constexpr int kRing = 4;               // blocks in flight per warp
-constexpr size_t kStageMax = 96 * 1024;
+constexpr int kBlock = 128;  // columns of a warp's step
+constexpr int kPad = 32;     // values between rows of x in shared memory: rows start 64 bytes apart mod 128
+constexpr int kSmemMost = 220 * 1024;
+constexpr int kSmemHalf = 112 * 1024;  // two CTAs an SM
 
 struct Args {
   const void* x;
@@ -48,17 +61,19 @@ struct Args {
   void* y;
   long long y_st;
   const uint4* weight;
-  const void* scales;
-  const uint8_t* zeros;
+  const unsigned* meta;
   const void* bias;
   int rows, inner, outer;
-  int blocks;    // of 128 columns
-  int groups;    // of a row
+  int blocks;        // of 128 columns
+  int part_blocks;   // of a cluster's CTA
+  int row_blocks;    // of 16 weight rows
+  int groups;        // of a row, for groups of 128 and more
   int group_blocks;  // blocks that share a scale, for groups of 128 and more
-  int scale_dtype;
-  int chunk;     // rows of x that a CTA takes
-  int tile;      // columns of x in shared memory, a multiple of kStep
-  int vector;    // rows of x are 16-byte aligned
+  int chunk;         // rows of x that a CTA takes
+  int tile;          // columns of x in a buffer
+  int whole;         // the CTA's columns of x fit one buffer, staged once
+  int vector;        // rows of x are 16-byte aligned
+  int tiles;         // of weight rows
 };
 
 template <typename T>
@@ -66,15 +81,20 @@ struct Num {  // 16-bit type of the products, its magic number for 4-bit integer
   using N = __nv_bfloat16;
   using N2 = __nv_bfloat162;
   static constexpr unsigned kMagic = 0x43004300u;  // 128
-  static constexpr float kBase = 128.f;
   static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
   static __device__ __forceinline__ N of(float v) { return __float2bfloat16_rn(v); }
-  static __device__ __forceinline__ N2 both(float v) { return __float2bfloat162_rn(v); }
   static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  // c = the product, with nothing added
+  static __device__ __forceinline__ void mma_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
   }
 };
 template <>
@@ -82,64 +102,93 @@ struct Num<__half> {
   using N = __half;
   using N2 = __half2;
   static constexpr unsigned kMagic = 0x64006400u;  // 1024
-  static constexpr float kBase = 1024.f;
   static constexpr int kParts = 1;
   static __device__ __forceinline__ N of(float v) { return __float2half_rn(v); }
-  static __device__ __forceinline__ N2 both(float v) { return __float2half2_rn(v); }
   static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  // c = the product, with nothing added
+  static __device__ __forceinline__ void mma_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  }
 };
 
-__device__ __forceinline__ float load_float(const void* p, long long i, int dtype) {
-  if (dtype == PFC_DTYPE_FLOAT32) return ((const float*)p)[i];
-  if (dtype == PFC_DTYPE_FLOAT16) return __half2float(((const __half*)p)[i]);
-  return __bfloat162float(((const __nv_bfloat16*)p)[i]);
+// A group's word: the scale's fp32 bits (of fp16 or bf16, so the lowest 13 are
+// 0), with the zero in the lowest four.
+__device__ __forceinline__ float scale_of(unsigned meta) { return __uint_as_float(meta & ~15u); }
+
+// (u & 0x000f000f) | magic in one instruction: two nibbles as 16-bit numbers
+// (written out, it became two: only one of the constants fits the instruction)
+__device__ __forceinline__ unsigned with_magic(unsigned u, unsigned magic) {
+  unsigned r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(u), "r"(0x000f000fu), "r"(magic));
+  return r;
 }
 
-__device__ __forceinline__ uint4 load_weight(const uint4* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
+// c += s * p in pairs
+__device__ __forceinline__ void fma2(float& c0, float& c1, float s, float p0, float p1) {
+  asm("{\n\t.reg .b64 c, s, p;\n\tmov.b64 c, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 p, {%3, %4};\n\t"
+      "fma.rn.f32x2 c, s, p, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "+f"(c0), "+f"(c1)
+      : "f"(s), "f"(p0), "f"(p1));
+}
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
 __device__ __forceinline__ unsigned word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
 
-// The columns [k0, k0 + tile) of the CTA's rows of x into shared memory, as
-// 16-bit parts: part p of row r in row p*rows + r; zeros behind the last.
+// `width` columns of the CTA's rows of x from column k0 on into a buffer, as
+// 16-bit parts: part p of row r in row p*rows + r; zeros behind the last
+// column.  16-bit rows that are aligned go by asynchronous copies, to be
+// waited for; width is a multiple of 128.
 template <typename T>
-__device__ __forceinline__ void stage(const Args& a, typename Num<T>::N* xs, int first, int rows, int k0) {
-  using NT = Num<T>;
-  const int pitch = a.tile + kPad;
-  const int width = min(a.tile, a.blocks * kBlock - k0);
-  for (int i = threadIdx.x * 8; i < rows * width; i += kThreads * 8) {  // width is a multiple of 128
-    const int r = i / width, c = i - r * width, k = k0 + c;
-    const T* src = (const T*)a.x + (long long)(first + r) * a.x_st + k;
+__device__ __noinline__ void stage(const T* x, long long x_st, int inner, int vector, typename Num<T>::N* xs, int pitch,
+                                   int rows, int k0, int width) {
+  using M = Num<T>;
+  const int pieces = (width + 255) / 256;  // a warp takes 256 columns of a row at a time
+  for (int i = threadIdx.x >> 5; i < rows * pieces; i += kWarps) {
+    const int r = i / pieces, c = (i - r * pieces) * 256 + (threadIdx.x & 31) * 8, k = k0 + c;
+    if (c >= width) continue;
+    const T* src = x + r * x_st + k;
+    if constexpr (M::kParts == 1) {
+      if (vector && k + 8 <= inner) {
+        copy16(xs + r * pitch + c, src);
+        continue;
+      }
+    }
     alignas(16) T v[8];
-    if (a.vector && k + 8 <= a.inner) {
+    if (M::kParts > 1 && vector && k + 8 <= inner) {
 #pragma unroll
       for (int e = 0; e < (int)sizeof(T) / 2; ++e) reinterpret_cast<uint4*>(v)[e] = reinterpret_cast<const uint4*>(src)[e];
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = k + e < a.inner ? src[e] : T(0.f);
+      for (int e = 0; e < 8; ++e) v[e] = k + e < inner ? src[e] : T(0.f);
     }
-    alignas(16) typename NT::N part[8];
-    if constexpr (NT::kParts == 1) {
+    if constexpr (M::kParts == 1) {
       *reinterpret_cast<uint4*>(xs + r * pitch + c) = *reinterpret_cast<uint4*>(v);
     } else {
+      alignas(16) typename M::N part[8];
       float rest[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) rest[e] = v[e];
 #pragma unroll
-      for (int p = 0; p < NT::kParts; ++p) {
+      for (int p = 0; p < M::kParts; ++p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          part[e] = NT::of(rest[e]);
+          part[e] = M::of(rest[e]);
           const float left = rest[e] - __bfloat162float(part[e]);
           rest[e] = isfinite(left) ? left : 0.f;  // an infinity or NaN is the first part
         }
@@ -150,158 +199,348 @@ __device__ __forceinline__ void stage(const Args& a, typename Num<T>::N* xs, int
 }
 
 // NT: 8-column blocks of x rows (times parts).  G: columns that share a scale
-// within a block: 32, 64, or 128 for groups of 128 and more.
-template <typename T, int NT, int G>
-__global__ void __launch_bounds__(kThreads) linear_kernel(const Args a) {
+// within a block: 32, 64, or 128 for groups of 128 and more.  MT: 16-row
+// blocks of a warp.  RW: warps along the weight rows; the others share the
+// columns.
+template <typename T, int NT, int G, int MT, int RW>
+struct Shape {
+  static constexpr int kAcross = kWarps / RW;       // warps along the columns
+  static constexpr int kRows = 16 * MT * RW;        // weight rows of a tile
+  static constexpr int kStep = kBlock * kAcross;    // columns of a CTA's step
+  static constexpr int kDepth = MT > 1 ? 4 : 6;     // slots of a warp's ring; all but one are on their way
+  static constexpr int kWords = kBlock / G;         // meta words of a block's row
+  static constexpr int kSlot = MT * (1024 + 64 * kWords);
+  static constexpr int kRing = kDepth * kSlot;
+  static constexpr int kPitch = NT * 8 + 1;
+  static constexpr size_t ring_bytes = (size_t)kWarps * kRing;
+  static constexpr size_t red_bytes = (size_t)kAcross * kRows * kPitch * 4;
+};
+
+template <typename T, int NT, int G, int MT, int RW>
+__global__ void __launch_bounds__(kThreads, MT > 1 ? 1 : 2) linear_kernel(const Args a) {
   using M = Num<T>;
   using N = typename M::N;
   using N2 = typename M::N2;
+  using S = Shape<T, NT, G, MT, RW>;
+  constexpr int MW = S::kWords, D = S::kDepth;
+  namespace cg = cooperative_groups;
   extern __shared__ __align__(16) char smem[];
-  N* xs = reinterpret_cast<N*>(smem);
-  float* red = reinterpret_cast<float*>(smem);  // after the last step: [warp][16][NT * 8 + 1]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int first = blockIdx.y * a.chunk, rows = min(a.chunk, a.rows - first);
+  char* ring = smem + warp * S::kRing;
+  N* xs = reinterpret_cast<N*>(smem + S::ring_bytes + (MT > 1 ? 0 : S::red_bytes));
+  float* red = reinterpret_cast<float*>(smem + S::ring_bytes);  // [across][rows][kPitch]; of a single tile in x's place
+  const int rw = warp % RW, kw = warp / RW;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const long long first = (long long)blockIdx.y * a.chunk;
+  const int rows = (int)min((long long)a.chunk, a.rows - first);
   const int cols = rows * M::kParts, pitch = a.tile + kPad;
-  const int n0 = blockIdx.x * 16;
-  // weight rows g and g + 8; rows behind the last repeat it and are not stored
-  const int na = min(n0 + g, a.outer - 1), nb = min(n0 + g + 8, a.outer - 1);
-  const uint4* wa = a.weight + (long long)na * a.blocks * 4 + t;
-  const uint4* wb = a.weight + (long long)nb * a.blocks * 4 + t;
-  const long long sa = (long long)na * a.groups, sb = (long long)nb * a.groups;
-  const int steps = (a.blocks + kWarps - 1) / kWarps;
+  const int b0 = rank * a.part_blocks, b1 = min(b0 + a.part_blocks, a.blocks);  // this CTA's blocks
+  const int steps = (a.part_blocks + S::kAcross - 1) / S::kAcross;              // of a tile, the same in all warps
+  const int stride = gridDim.x / ranks;
+  const int per_buffer = a.tile / S::kStep;
+  const size_t buffer = (size_t)cols * pitch;
 
-  uint4 ring[kRing][2];
-  auto fetch = [&](int step, uint4 (&w)[2]) {
-    const int kb = step * kWarps + warp;
-    w[0] = w[1] = make_uint4(0, 0, 0, 0);
-    if (kb < a.blocks) {
-      w[0] = load_weight(wa + (long long)kb * 4);
-      w[1] = load_weight(wb + (long long)kb * 4);
+  auto stage_from = [&](int step) {  // the buffer's columns from a step of the tile on
+    const int k = (b0 + step * S::kAcross) * kBlock;
+    const int width = min(a.tile, (b1 - b0) * kBlock - step * S::kStep);
+    if (width > 0)
+      stage<T>((const T*)a.x + first * a.x_st, a.x_st, a.inner, a.vector, xs + (a.whole ? 0 : (step / per_buffer & 1) * buffer), pitch, rows, k, width);
+  };
+  stage_from(0);
+  commit();
+
+  // of the next fetch: its tile, the step there, its block, its slot, and
+  // where the weights and words of its rows are (the host checked that these
+  // offsets fit 32 bits)
+  int f_tile = (int)blockIdx.x / ranks, f_step = 0, f_block, f_slot = 0;
+  unsigned f_w[MT], f_m[MT];
+  auto aim = [&]() {
+    f_block = b0 + kw;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      // blocks of 16 rows behind the last repeat it and are not stored
+      const unsigned n = min(f_tile * S::kRows / 16 + rw * MT + mt, a.row_blocks - 1);
+      f_w[mt] = (n * a.blocks + f_block) * 64 + lane;
+      f_m[mt] = G == 128 ? n * a.groups * 16 : (n * a.blocks + f_block) * 16 * MW;
+    }
+  };
+  aim();
+  auto fetch = [&]() {
+    char* to = ring + f_slot * S::kSlot;
+    if (f_block < b1) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        copy16(to + mt * 1024 + lane * 16, a.weight + f_w[mt]);
+        copy16(to + mt * 1024 + 512 + lane * 16, a.weight + f_w[mt] + 32);
+        if (lane < 4 * MW)
+          copy16(to + MT * 1024 + mt * 64 * MW + lane * 16,
+                 a.meta + f_m[mt] + (G == 128 ? 16 * (a.group_blocks == 1 ? f_block : f_block / a.group_blocks) : 0) + lane * 4);
+      }
+    }
+    commit();  // empty or not: the waits count groups
+    f_slot = f_slot + 1 == D ? 0 : f_slot + 1;
+    f_block += S::kAcross;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      f_w[mt] += S::kAcross * 64;
+      if (G != 128) f_m[mt] += S::kAcross * 16 * MW;
+    }
+    if (++f_step == steps) {
+      f_step = 0;
+      f_tile += stride;
+      if (f_tile < a.tiles) aim();
+      else f_block = b1, f_step = INT32_MIN;  // nothing more
     }
   };
 #pragma unroll
-  for (int i = 0; i < kRing; ++i) fetch(i, ring[i]);
+  for (int i = 0; i < D - 1; ++i) fetch();
 
-  float acc[NT][4];
+  int at[NT];  // the lane's columns of x; those behind the last repeat it, and what they give is not read
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) acc[nt][r] = 0.f;
+  for (int nt = 0; nt < NT; ++nt) at[nt] = min(nt * 8 + g, cols - 1) * pitch;
+  int slot = 0;
 
-  const int per_tile = a.tile / kStep;
-  for (int base = 0; base < steps; base += kRing) {
+  for (int tile = (int)blockIdx.x / ranks; tile < a.tiles; tile += stride) {
+    const bool again = tile != (int)blockIdx.x / ranks;
+    float acc[MT][NT][4];
 #pragma unroll
-    for (int i = 0; i < kRing; ++i) {
-      const int step = base + i;
-      if (step < steps) {
-        if (step % per_tile == 0) {
-          __syncthreads();
-          stage<T>(a, xs, first, rows, step * kStep);
-          __syncthreads();
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[mt][nt][r] = 0.f;
+    int in_buffer = a.whole && again ? 1 : 0;  // steps into the buffer; 0: wait for it
+    const N* xk = xs + kw * kBlock + t * 8;
+    for (int step = 0; step < steps; ++step) {
+      if (in_buffer == 0) {
+        // This buffer was staged per_buffer steps ago, before as many groups
+        // of the ring: the wait for this step's slot covers it unless that is
+        // fewer than stay pending.
+        if ((again && step == 0) || per_buffer < D - 2) wait_copies<0>();
+        else wait_copies<D - 2>();
+        __syncthreads();  // this buffer is filled, and the other one's reads are over
+        if (!a.whole) {
+          if (step) xk += ((step / per_buffer & 1) ? (long long)buffer : -(long long)buffer) - per_buffer * S::kStep;
+          if (step + per_buffer < steps) {
+            stage_from(step + per_buffer);
+            commit();
+          }
         }
-        const int kb = step * kWarps + warp;
-        if (kb < a.blocks) {
-          const N* xk = xs + g * pitch + (kb * kBlock - step / per_tile * a.tile) + t * 8;
-          float part[NT][4];
+      }
+      wait_copies<D - 2>();
+      __syncwarp();  // the slot's words are there for all lanes, and the slot before it has been read
+      fetch();
+      if (b0 + step * S::kAcross + kw < b1) {
+        const uint4* ws = reinterpret_cast<const uint4*>(ring + slot * S::kSlot) + lane;
+        const unsigned* mp = reinterpret_cast<const unsigned*>(ring + slot * S::kSlot + MT * 1024) + g * MW;
+        uint4 w[MT][2];
+        unsigned meta[MT][2][MW];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {  // 32 columns
-            if (j * 32 % G == 0) {
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) part[nt][r] = 0.f;
+          for (int h = 0; h < 2; ++h) {
+            w[mt][h] = ws[mt * 64 + h * 32];
+            const unsigned* m = mp + (mt * 16 + h * 8) * MW;
+            if constexpr (MW == 4) {
+              const uint4 u = *reinterpret_cast<const uint4*>(m);
+              meta[mt][h][0] = u.x, meta[mt][h][MW / 4] = u.y, meta[mt][h][MW / 2] = u.z, meta[mt][h][MW - 1] = u.w;
+            } else if constexpr (MW == 2) {
+              const uint2 u = *reinterpret_cast<const uint2*>(m);
+              meta[mt][h][0] = u.x, meta[mt][h][MW - 1] = u.y;
+            } else {
+              meta[mt][h][0] = *m;
             }
-            const int group = G == 128 ? kb / a.group_blocks : (kb * kBlock + j * 32) / G;
-            const bool real = group < a.groups;  // groups of padding have no scale; their x is zero
-            const N2 za = M::both(M::kBase + (real && a.zeros ? (float)a.zeros[sa + group] : 8.f));
-            const N2 zb = M::both(M::kBase + (real && a.zeros ? (float)a.zeros[sb + group] : 8.f));
-            const unsigned ua = word(ring[i][0], j), ub = word(ring[i][1], j);
-            unsigned qa[4], qb[4];
+          }
+        float part[MT][NT][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const unsigned pa = ((ua >> (4 * e)) & 0x000f000fu) | M::kMagic, pb = ((ub >> (4 * e)) & 0x000f000fu) | M::kMagic;
-              const N2 da = __hsub2(*reinterpret_cast<const N2*>(&pa), za), db = __hsub2(*reinterpret_cast<const N2*>(&pb), zb);
-              qa[e] = *reinterpret_cast<const unsigned*>(&da);
-              qb[e] = *reinterpret_cast<const unsigned*>(&db);
-            }
-            const unsigned f1[4] = {qa[0], qb[0], qa[1], qb[1]}, f2[4] = {qa[2], qb[2], qa[3], qb[3]};
+        for (int j = 0; j < 4; ++j) {  // 32 columns
+          unsigned f1[MT][4], f2[MT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint4 b = make_uint4(0, 0, 0, 0);
-              if (nt * 8 + g < cols) b = *reinterpret_cast<const uint4*>(xk + nt * 8 * pitch + j * 32);
-              M::mma(part[nt], f1, b.x, b.y);
-              M::mma(part[nt], f2, b.z, b.w);
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const unsigned zz = (meta[mt][h][j * 32 / G] & 15u) * 0x10001u + M::kMagic;
+              const N2 z = *reinterpret_cast<const N2*>(&zz);
+              const unsigned u = word(w[mt][h], j);
+              unsigned q[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const unsigned p = with_magic(u >> (4 * e), M::kMagic);
+                const N2 d = __hsub2(*reinterpret_cast<const N2*>(&p), z);
+                q[e] = *reinterpret_cast<const unsigned*>(&d);
+              }
+              f1[mt][h] = q[0];
+              f1[mt][h + 2] = q[1];
+              f2[mt][h] = q[2];
+              f2[mt][h + 2] = q[3];
             }
-            if ((j + 1) * 32 % G == 0) {
-              const float ca = real ? load_float(a.scales, sa + group, a.scale_dtype) : 0.f;
-              const float cb = real ? load_float(a.scales, sb + group, a.scale_dtype) : 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint4 b = *reinterpret_cast<const uint4*>(xk + at[nt] + j * 32);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              if (j * 32 % G == 0) M::mma_first(part[mt][nt], f1[mt], b.x, b.y);
+              else M::mma(part[mt][nt], f1[mt], b.x, b.y);
+              M::mma(part[mt][nt], f2[mt], b.z, b.w);
+            }
+          }
+          if ((j + 1) * 32 % G == 0) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              const float ca = scale_of(meta[mt][0][j * 32 / G]), cb = scale_of(meta[mt][1][j * 32 / G]);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                acc[nt][0] = fmaf(ca, part[nt][0], acc[nt][0]);
-                acc[nt][1] = fmaf(ca, part[nt][1], acc[nt][1]);
-                acc[nt][2] = fmaf(cb, part[nt][2], acc[nt][2]);
-                acc[nt][3] = fmaf(cb, part[nt][3], acc[nt][3]);
+                fma2(acc[mt][nt][0], acc[mt][nt][1], ca, part[mt][nt][0], part[mt][nt][1]);
+                fma2(acc[mt][nt][2], acc[mt][nt][3], cb, part[mt][nt][2], part[mt][nt][3]);
               }
             }
           }
         }
-        fetch(step + kRing, ring[i]);
       }
+      slot = slot + 1 == D ? 0 : slot + 1;
+      xk += S::kStep;
+      if (++in_buffer == per_buffer && !a.whole) in_buffer = 0;
     }
-  }
 
-  // add the warps' sums: accumulator (row g or g + 8, column 2t or 2t + 1)
-  __syncthreads();
-  constexpr int kPitch = NT * 8 + 1;
+    // the tile is done: add the warps' sums, accumulator (row g or g + 8,
+    // column 2t or 2t + 1), then the cluster's
+    const int n0 = tile * S::kRows;
+    __syncthreads();  // the previous tile's sums have been read, and all of x
+    if (MT == 1 && !a.whole && tile + stride < a.tiles) {
+      stage_from(0);
+      commit();
+    }
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      red[(warp * 16 + g + 8 * (r >> 1)) * kPitch + nt * 8 + 2 * t + (r & 1)] = acc[nt][r];
-  __syncthreads();
-  for (int i = tid; i < 16 * rows; i += kThreads) {
-    const int m = i >> 4, n = i & 15;
-    if (n0 + n >= a.outer) continue;
-    float v = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int p = M::kParts - 1; p >= 0; --p)
+        for (int r = 0; r < 4; ++r)
+          red[(kw * S::kRows + (rw * MT + mt) * 16 + g + 8 * (r >> 1)) * S::kPitch + nt * 8 + 2 * t + (r & 1)] = acc[mt][nt][r];
+    __syncthreads();
+    if (ranks > 1) {
+      if constexpr (S::kAcross > 1) {
+        for (int j = tid; j < S::kRows * cols; j += kThreads) {
+          const int n = j % S::kRows, c = j / S::kRows;
+          float v = red[n * S::kPitch + c];
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += red[(w * 16 + n) * kPitch + p * rows + m];
-    if (a.bias) v += (float)((const T*)a.bias)[n0 + n];
-    ((T*)a.y)[(long long)(first + m) * a.y_st + n0 + n] = T(v);
+          for (int w = 1; w < S::kAcross; ++w) v += red[(w * S::kRows + n) * S::kPitch + c];
+          red[n * S::kPitch + c] = v;  // read and written by this thread alone
+        }
+      }
+      cluster.sync();
+    }
+    // a rank writes its share of the tile's outputs
+    for (int j = tid + rank * kThreads; j < S::kRows * rows; j += kThreads * ranks) {
+      const int m = j / S::kRows, n = j % S::kRows;
+      if (n0 + n >= a.outer) continue;
+      float v = 0.f;
+#pragma unroll
+      for (int p = M::kParts - 1; p >= 0; --p) {
+        if (ranks > 1) {
+          for (int r = 0; r < ranks; ++r) v += cluster.map_shared_rank(red, r)[n * S::kPitch + p * rows + m];
+        } else {
+#pragma unroll
+          for (int w = 0; w < S::kAcross; ++w) v += red[(w * S::kRows + n) * S::kPitch + p * rows + m];
+        }
+      }
+      if (a.bias) v += (float)((const T*)a.bias)[n0 + n];
+      ((T*)a.y)[(long long)(first + m) * a.y_st + n0 + n] = T(v);
+    }
+    if (ranks > 1) cluster.sync();  // the others' reads of this CTA's sums are over
   }
 }
 
-__global__ void arrange_kernel(const uint8_t* packed, long long pitch, int inner, int blocks, long long words, uint32_t* weight) {
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += (long long)gridDim.x * blockDim.x) {
-    const int w = (int)(i & 15), t = w >> 2, j = w & 3;
-    const long long row = (i >> 4) / blocks;
-    const int col = (int)((i >> 4) - row * blocks) * kBlock + j * 32 + t * 8;
+struct ArrangeArgs {
+  const uint8_t* packed;
+  const unsigned short* scales;
+  const uint8_t* zeros;
+  uint32_t* weight;
+  uint32_t* meta;
+  long long words, metas;  // of the outputs
+  int inner, outer, blocks, groups, group, bf16;
+};
+
+__global__ void arrange_kernel(const ArrangeArgs a) {
+  const long long step = (long long)gridDim.x * blockDim.x, start = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long pitch = (a.inner + 1) / 2;
+  for (long long i = start; i < a.words; i += step) {
+    const int j = (int)(i & 3), t = (int)(i >> 2 & 3), r = (int)(i >> 4 & 15);  // r: half * 8 + g
+    const long long rb = (i >> 8) / a.blocks, row = rb * 16 + r;
+    const int col = (int)((i >> 8) - rb * a.blocks) * kBlock + j * 32 + t * 8;
     uint32_t u = 0;
     for (int e = 0; e < 8; ++e) {
       const int k = col + e;
-      const unsigned q = k < inner ? (packed[row * pitch + (k >> 1)] >> (4 * (k & 1))) & 15u : 0u;
+      const unsigned q = row < a.outer && k < a.inner ? (a.packed[row * pitch + (k >> 1)] >> (4 * (k & 1))) & 15u : 0u;
       // even columns in nibbles 0-3, odd ones in 4-7
       u |= q << (4 * ((e >> 1) + 4 * (e & 1)));
     }
-    weight[i] = u;
+    a.weight[i] = u;
+  }
+  const int mw = a.group < kBlock ? kBlock / a.group : 1;             // words of a row in a step
+  const int along = a.group < kBlock ? a.blocks : a.groups;           // steps
+  for (long long i = start; i < a.metas; i += step) {
+    const long long rb = i / mw / 16 / along, row = rb * 16 + i / mw % 16;
+    const int m = (int)(i / mw / 16 - rb * along) * mw + (int)(i % mw);  // the group
+    uint32_t u = 0;
+    if (row < a.outer && m < a.groups) {
+      const unsigned short b = a.scales[row * a.groups + m];
+      const float f = a.bf16 ? __uint_as_float((unsigned)b << 16) : __half2float(__ushort_as_half(b));
+      // a NaN stays one without its lowest bits
+      u = (isnan(f) ? 0x7fc00000u : __float_as_uint(f)) | (a.zeros ? a.zeros[row * a.groups + m] & 15u : 8u);
+    }
+    a.meta[i] = u;
   }
 }
 
-template <typename T, int NT, int G>
-void launch_sized(const Args& a, cudaStream_t stream) {
+template <typename T, int NT, int G, int MT, int RW>
+void launch_sized(Args a, cudaStream_t stream) {
+  using S = Shape<T, NT, G, MT, RW>;
+  const auto kernel = linear_kernel<T, NT, G, MT, RW>;
   static std::once_flag once[64];
-  const int dev = current_device();
-  constexpr size_t kMost = kStageMax + 64 * 1024;
-  std::call_once(once[dev], [] {
-    PFB_CUDA(cudaFuncSetAttribute(linear_kernel<T, NT, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost));
+  const int dev = current_device(), sms = device_sm_count(dev);
+  std::call_once(once[dev], [&] {
+    PFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
   });
-  const int rows = std::min(a.chunk, a.rows);
-  const size_t smem = std::max<size_t>((size_t)rows * Num<T>::kParts * (a.tile + kPad) * 2, (size_t)kWarps * 16 * (NT * 8 + 1) * 4);
-  PFB_CHECK_ARG(smem <= kMost, "linear w4: tile does not fit");
-  const dim3 grid((unsigned)ceil_div(a.outer, 16), (unsigned)ceil_div(a.rows, a.chunk));
-  linear_kernel<T, NT, G><<<grid, kThreads, smem, stream>>>(a);
-  PFB_CUDA(cudaGetLastError());
+  a.tiles = (int)ceil_div(a.outer, S::kRows);
+  const int64_t slots = (MT > 1 ? 1 : 2) * (int64_t)sms;
+  // the columns are shared as long as that fills the device and leaves each
+  // CTA two steps
+  int ranks = 1;
+  while (ranks < 8 && (int64_t)a.tiles * ranks * 2 <= slots && a.blocks >= ranks * 2 * 2 * S::kAcross) ranks *= 2;
+  a.part_blocks = (int)ceil_div(a.blocks, ranks);
+  const int cols = a.chunk * Num<T>::kParts;
+  const int64_t mine = round_up((int64_t)a.part_blocks * kBlock, S::kStep);
+  auto bytes = [&](int64_t width) { return (int64_t)cols * (width + kPad) * 2; };
+  // a CTA's part of x in one buffer, where as many CTAs still fit an SM
+  constexpr int64_t fixed = (int64_t)S::ring_bytes + (MT > 1 ? 0 : (int64_t)S::red_bytes);
+  constexpr int64_t room = (MT > 1 ? (int64_t)kSmemMost : kSmemHalf) - fixed;
+  a.whole = bytes(mine) <= room;
+  int64_t width = mine;
+  if (!a.whole) {
+    width = S::kStep;
+    while (width + S::kStep < mine && width < 2048 && 2 * bytes(width + S::kStep) <= room) width += S::kStep;
+  }
+  a.tile = (int)width;
+  const int64_t x_bytes = (a.whole ? 1 : 2) * bytes(width);
+  const int64_t smem = fixed + (MT > 1 ? std::max<int64_t>(x_bytes, S::red_bytes) : x_bytes);
+  PFB_CHECK_ARG(smem <= kSmemMost, "linear w4: tile does not fit");
+  // a CTA walks over row tiles (few rows of x), keeping x
+  const int64_t wave = std::max<int64_t>(1, slots / ranks);
+  const int64_t across = MT > 1 ? a.tiles : std::min<int64_t>(a.tiles, wave);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(across * ranks), (unsigned)ceil_div(a.rows, a.chunk));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  PFB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const Args&)a));
 }
 
 template <typename T>
@@ -311,45 +550,67 @@ void launch_typed(Args& a, int64_t group, cudaStream_t stream) {
   const int64_t chunks = ceil_div(a.rows, most);
   a.chunk = (int)ceil_div(a.rows, chunks);
   const int cols = a.chunk * parts;
-  // all of x, or as many steps of it as the stage holds
-  const int64_t whole = round_up((int64_t)a.blocks * kBlock, kStep);
-  const int64_t fits = std::max<int64_t>(kStep, (int64_t)(kStageMax / (2 * cols)) / kStep * kStep);
-  a.tile = (int)std::min(whole, fits);
-  auto grouped = [&](auto nt) {
-    constexpr int NT = decltype(nt)::value;
-    if (group == 32) launch_sized<T, NT, 32>(a, stream);
-    else if (group == 64) launch_sized<T, NT, 64>(a, stream);
-    else launch_sized<T, NT, 128>(a, stream);
+  auto grouped = [&](auto nt, auto mt, auto rw) {
+    constexpr int NT = decltype(nt)::value, MT = decltype(mt)::value, RW = decltype(rw)::value;
+    if (group == 32) launch_sized<T, NT, 32, MT, RW>(a, stream);
+    else if (group == 64) launch_sized<T, NT, 64, MT, RW>(a, stream);
+    else launch_sized<T, NT, 128, MT, RW>(a, stream);
   };
-  if (cols <= 8) grouped(std::integral_constant<int, 1>());
-  else if (cols <= 16) grouped(std::integral_constant<int, 2>());
-  else if (cols <= 32) grouped(std::integral_constant<int, 4>());
-  else grouped(std::integral_constant<int, 8>());
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I3 = std::integral_constant<int, 3>;
+  using I4 = std::integral_constant<int, 4>;
+  using I6 = std::integral_constant<int, 6>;
+  using I8 = std::integral_constant<int, 8>;
+  // with enough weight rows for one wave of 64-row tiles the warps take rows
+  // of their own and join only in pairs, once a tile; so do they where all of
+  // x does not fit beside the ring
+  const bool tall = ceil_div(a.outer, 64) >= device_sm_count(current_device()) || (int64_t)cols * a.blocks * kBlock * 2 > 40 * 1024;
+  if (cols <= 8) tall ? grouped(I1(), I1(), I4()) : grouped(I1(), I1(), I1());
+  else if (cols <= 16) grouped(I2(), I2(), I4());
+  else if (cols <= 24) grouped(I3(), I2(), I4());
+  else if (cols <= 32) grouped(I4(), I2(), I4());
+  else if (cols <= 48) grouped(I6(), I2(), I4());
+  else grouped(I8(), I2(), I4());
+}
+
+void check_group(int64_t group) {
+  PFB_CHECK_ARG(group == 32 || group == 64 || (group >= 128 && group % 128 == 0 && group <= INT32_MAX),
+                "linear w4: group must be 32, 64 or a multiple of 128");
 }
 
 }  // namespace
 
-void launch_w4_arrange(const uint8_t* packed, int64_t outer, int64_t inner, uint32_t* weight, cudaStream_t stream) {
-  PFB_CHECK_ARG(outer >= 0 && inner >= 0 && outer <= (1 << 28) && inner <= (1 << 28), "w4 arrange: bad size");
-  if (outer == 0 || inner == 0) return;
-  PFB_CHECK_ARG(packed && weight, "w4 arrange: null pointer");
-  const int64_t blocks = ceil_div(inner, kBlock), words = outer * blocks * 16;
-  arrange_kernel<<<(unsigned)std::min<int64_t>(ceil_div(words, 256), 148 * 16), 256, 0, stream>>>(
-      packed, (inner + 1) / 2, (int)inner, (int)blocks, words, weight);
+void launch_w4_arrange(const pfk_w4_arrange_params& p, cudaStream_t stream) {
+  PFB_CHECK_ARG(p.outer >= 0 && p.inner >= 0 && p.outer <= (1 << 28) && p.inner <= (1 << 28), "w4 arrange: bad size");
+  check_group(p.group);
+  PFB_CHECK_ARG(p.scale_dtype == PFC_DTYPE_FLOAT16 || p.scale_dtype == PFC_DTYPE_BFLOAT16,
+                "w4 arrange: scale_dtype must be float16 or bfloat16");
+  if (p.outer == 0 || p.inner == 0) return;
+  PFB_CHECK_ARG(p.packed && p.scales && p.weight && p.meta, "w4 arrange: null pointer");
+  ArrangeArgs a = {p.packed, p.scales, p.zeros, p.weight, p.meta, 0, 0, (int)p.inner, (int)p.outer};
+  a.blocks = (int)ceil_div(p.inner, kBlock);
+  a.groups = (int)ceil_div(p.inner, p.group);
+  a.group = (int)p.group;
+  a.bf16 = p.scale_dtype == PFC_DTYPE_BFLOAT16;
+  const int64_t row_blocks = ceil_div(p.outer, 16);
+  a.words = row_blocks * a.blocks * 256;
+  a.metas = row_blocks * 16 * (p.group < kBlock ? a.blocks * (kBlock / p.group) : a.groups);
+  arrange_kernel<<<(unsigned)std::min<int64_t>(ceil_div(a.words, 256), 148 * 16), 256, 0, stream>>>(a);
   PFB_CUDA(cudaGetLastError());
 }
 
 void launch_linear_w4(const pfk_linear_w4_params& p, cudaStream_t stream) {
   check_decode_dtype(p.dtype);
-  check_decode_dtype(p.scale_dtype);
   PFB_CHECK_ARG(p.rows >= 0 && p.rows <= (1 << 20), "linear w4: rows must be 0 to 2^20");
   PFB_CHECK_ARG(p.inner >= 1 && p.inner <= (1 << 28) && p.outer >= 1 && p.outer <= (1 << 28),
                 "linear w4: inner and outer must be 1 to 2^28");
-  PFB_CHECK_ARG(p.group == 32 || p.group == 64 || (p.group >= 128 && p.group % 128 == 0 && p.group <= INT32_MAX),
-                "linear w4: group must be 32, 64 or a multiple of 128");
+  check_group(p.group);
+  PFB_CHECK_ARG(round_up(p.outer, 16) * ceil_div(p.inner, kBlock) * 4 < (1ll << 32), "linear w4: weights of 64 GiB or more");
   if (p.rows == 0) return;
-  PFB_CHECK_ARG(p.x && p.y && p.weight && p.scales, "linear w4: null pointer");
-  PFB_CHECK_ARG((uintptr_t)p.weight % 16 == 0, "linear w4: weight must be 16-byte aligned");
+  PFB_CHECK_ARG(p.x && p.y && p.weight && p.meta, "linear w4: null pointer");
+  PFB_CHECK_ARG((uintptr_t)p.weight % 16 == 0 && (uintptr_t)p.meta % 16 == 0,
+                "linear w4: weight and meta must be 16-byte aligned");
   Args a = {};
   const int64_t es = p.dtype == PFC_DTYPE_FLOAT32 ? 4 : 2;
   a.x = p.x;
@@ -357,14 +618,13 @@ void launch_linear_w4(const pfk_linear_w4_params& p, cudaStream_t stream) {
   a.y = p.y;
   a.y_st = p.y_st;
   a.weight = (const uint4*)p.weight;
-  a.scales = p.scales;
-  a.scale_dtype = p.scale_dtype;
-  a.zeros = p.zeros;
+  a.meta = p.meta;
   a.bias = p.bias;
   a.rows = (int)p.rows;
   a.inner = (int)p.inner;
   a.outer = (int)p.outer;
   a.blocks = (int)ceil_div(p.inner, kBlock);
+  a.row_blocks = (int)ceil_div(p.outer, 16);
   a.groups = (int)ceil_div(p.inner, p.group);
   a.group_blocks = (int)std::max<int64_t>(1, p.group / kBlock);
   a.vector = (uintptr_t)p.x % 16 == 0 && a.x_st * es % 16 == 0;

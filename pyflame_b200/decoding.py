@@ -433,7 +433,7 @@ class Linear4bit:
     scales[n, k // group], q from 0 to 15.
 
     packed: uint8 [out_features, (in_features + 1) // 2], column 2i in the low
-    half of byte i; scales: float32, float16 or bfloat16 [out_features,
+    half of byte i; scales: float16 or bfloat16 [out_features,
     ceil(in_features / group_size)]; zeros: uint8 of the same shape, 0 to 15,
     or None for 8; bias: [out_features] of the type of x, or None; group_size:
     32, 64 or a multiple of 128.  The constructor lays the weights out for the
@@ -452,7 +452,8 @@ class Linear4bit:
             raise ValueError("group_size must be 32, 64 or a multiple of 128")
         groups = -(-k // group_size)
         _check("packed", packed, (n, (k + 1) // 2), torch.uint8, device)
-        self.scale_code = _code(scales.dtype)
+        if scales.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"scales: dtype must be float16 or bfloat16, not {scales.dtype}")
         _check("scales", scales, (n, groups), scales.dtype, device)
         if zeros is not None:
             _check("zeros", zeros, (n, groups), torch.uint8, device)
@@ -465,10 +466,15 @@ class Linear4bit:
             bias = bias.contiguous()
         self.in_features, self.out_features, self.group_size = k, n, int(group_size)
         self.device, self.scales, self.zeros, self.bias = device, scales.contiguous(), zeros, bias
-        self.weight = torch.empty((n, -(-k // 128) * 16), dtype=torch.int32, device=device)
+        blocks, row_blocks = -(-k // 128), -(-n // 16)
+        self.weight = torch.empty((row_blocks, blocks, 256), dtype=torch.int32, device=device)
+        self.meta = torch.empty((row_blocks, blocks * (128 // group_size) if group_size < 128 else groups, 16), dtype=torch.int32,
+                                device=device)
         self._plans = _Plans()
         packed = packed.contiguous()
-        _call(N.lib().pfk_w4_arrange, device, packed.data_ptr(), n, k, self.weight.data_ptr())
+        p = N.W4ArrangeParamsC(k, n, self.group_size, packed.data_ptr(), self.scales.data_ptr(), _code(scales.dtype),
+                               None if zeros is None else zeros.data_ptr(), self.weight.data_ptr(), self.meta.data_ptr())
+        _call(N.lib().pfk_w4_arrange, device, C.byref(p))
 
     @classmethod
     def quantize(cls, weight, group_size: int = 128, bias=None, symmetric: bool = False, scale_dtype=None) -> "Linear4bit":
@@ -529,7 +535,6 @@ class Linear4bit:
             _check("out", out, shape, x.dtype, self.device, output=True)
             y_st = (out if len(shape) == 2 else out.view(-1, self.out_features)).stride(0)
         p = N.LinearW4ParamsC(code, rows.shape[0], self.in_features, self.out_features, self.group_size, None,
-                              rows.stride(0), None, y_st, self.weight.data_ptr(), self.scales.data_ptr(), self.scale_code,
-                              None if self.zeros is None else self.zeros.data_ptr(),
+                              rows.stride(0), None, y_st, self.weight.data_ptr(), self.meta.data_ptr(),
                               None if self.bias is None else self.bias.data_ptr())
         return p, shape, len(x.shape) != 2

@@ -55,7 +55,8 @@ def test_nothing_to_do_needs_no_device(native):
     assert L.pfk_paged_attention_workspace(C.byref(t), C.byref(n)) == 0 and n.value == 0
     w = native.LinearW4ParamsC(0, 0, 64, 64, 64)
     assert L.pfk_linear_w4(C.byref(w), None) == 0
-    assert L.pfk_w4_arrange(None, 0, 64, None, None) == 0
+    r = native.W4ArrangeParamsC(64, 0, 64, None, None, 1)
+    assert L.pfk_w4_arrange(C.byref(r), None) == 0
 
 
 @pytest.mark.parametrize("change,word", [
@@ -102,18 +103,28 @@ def test_attention_refusals(native, change, word):
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(dtype=7), "dtype"), (dict(scale_dtype=4), "dtype"), (dict(rows=-1), "rows"), (dict(rows=(1 << 20) + 1), "rows"),
+    (dict(dtype=7), "dtype"), (dict(rows=-1), "rows"), (dict(rows=(1 << 20) + 1), "rows"),
     (dict(inner=0), "inner"), (dict(outer=0), "inner"), (dict(group=16), "group"), (dict(group=96), "group"), (dict(group=192), "group"),
-    (dict(x=None), "null"), (dict(weight=None), "null"), (dict(weight=FAKE + 4), "aligned"), (dict(scales=None), "null"),
+    (dict(x=None), "null"), (dict(weight=None), "null"), (dict(weight=FAKE + 4), "aligned"), (dict(meta=None), "null"),
+    (dict(meta=FAKE + 8), "aligned"),
 ])
 def test_linear_refusals(native, change, word):
-    v = dict(dtype=0, rows=1, inner=256, outer=32, group=128, x=FAKE, x_st=256, y=FAKE, y_st=32, weight=FAKE, scales=FAKE,
-             scale_dtype=1, zeros=None, bias=None)
+    v = dict(dtype=0, rows=1, inner=256, outer=32, group=128, x=FAKE, x_st=256, y=FAKE, y_st=32, weight=FAKE, meta=FAKE,
+             bias=None)
     v.update(change)
     p = native.LinearW4ParamsC(*v.values())
     refused(native, native.lib().pfk_linear_w4(C.byref(p), None), word)
-    refused(native, native.lib().pfk_w4_arrange(None, 4, 64, None, None), "null")
-    refused(native, native.lib().pfk_w4_arrange(FAKE, -4, 64, FAKE, None), "size")
+    refused(native, native.lib().pfk_linear_w4(None, None), "null")
+
+
+@pytest.mark.parametrize("args,word", [
+    ((64, 4, 64, None, FAKE, 1, None, FAKE, FAKE), "null"), ((64, 4, 64, FAKE, FAKE, 1, None, FAKE, None), "null"),
+    ((64, -4, 64, FAKE, FAKE, 1, None, FAKE, FAKE), "size"), ((64, 4, 48, FAKE, FAKE, 1, None, FAKE, FAKE), "group"),
+    ((64, 4, 64, FAKE, FAKE, 0, None, FAKE, FAKE), "scale_dtype")])
+def test_arrange_refusals(native, args, word):
+    p = native.W4ArrangeParamsC(*args)
+    refused(native, native.lib().pfk_w4_arrange(C.byref(p), None), word)
+    refused(native, native.lib().pfk_w4_arrange(None, None), "null")
 
 
 def test_host_tensors_are_refused(native):
