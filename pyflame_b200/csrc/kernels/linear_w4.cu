@@ -20,12 +20,12 @@
 // (with whole rows in turn every load was eight pieces of 64 bytes: 22 us for
 // TIME_UP at 16384 x 4096).
 //
-// Two shapes of CTA, 8 warps each:
-//   few rows of x (8 columns of the instruction): the warps share the columns
-//   of 16 weight rows, or in pairs those of 64; a CTA keeps its part of x and
+// Two shapes of CTA:
+//   few rows of x (8 columns of the instruction): 8 warps share the columns of
+//   16 weight rows, or in pairs those of 64; a CTA keeps its part of x and
 //   walks over row tiles, so x is staged once;
-//   more: 128 weight rows (4 warps of 32, so that a fragment of x read from
-//   shared memory serves two instructions), two warps share the columns, x in
+//   more: 8 warps, 128 weight rows (32 a warp, so that a fragment of x read from
+//   shared memory serves two instructions), in pairs over the columns, x in
 //   chunks through two buffers.
 // Weights, scales and zeros reach a warp through a ring of its own in shared
 // memory, filled by asynchronous copies several steps ahead.  Where the rows
@@ -48,8 +48,6 @@
 namespace pfb {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kBlock = 128;  // columns of a warp's step
 constexpr int kPad = 32;     // values between rows of x in shared memory: rows start 64 bytes apart mod 128
 constexpr int kSmemMost = 220 * 1024;
@@ -154,12 +152,12 @@ __device__ __forceinline__ unsigned word(const uint4& u, int i) { return i == 0 
 // 16-bit parts: part p of row r in row p*rows + r; zeros behind the last
 // column.  16-bit rows that are aligned go by asynchronous copies, to be
 // waited for; width is a multiple of 128.
-template <typename T>
+template <typename T, int W>
 __device__ __noinline__ void stage(const T* x, long long x_st, int inner, int vector, typename Num<T>::N* xs, int pitch,
                                    int rows, int k0, int width) {
   using M = Num<T>;
   const int pieces = (width + 255) / 256;  // a warp takes 256 columns of a row at a time
-  for (int i = threadIdx.x >> 5; i < rows * pieces; i += kWarps) {
+  for (int i = threadIdx.x >> 5; i < rows * pieces; i += W) {
     const int r = i / pieces, c = (i - r * pieces) * 256 + (threadIdx.x & 31) * 8, k = k0 + c;
     if (c >= width) continue;
     const T* src = x + r * x_st + k;
@@ -204,6 +202,8 @@ __device__ __noinline__ void stage(const T* x, long long x_st, int inner, int ve
 // columns.
 template <typename T, int NT, int G, int MT, int RW>
 struct Shape {
+  static constexpr int kWarps = 8;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kAcross = kWarps / RW;       // warps along the columns
   static constexpr int kRows = 16 * MT * RW;        // weight rows of a tile
   static constexpr int kStep = kBlock * kAcross;    // columns of a CTA's step
@@ -211,13 +211,13 @@ struct Shape {
   static constexpr int kWords = kBlock / G;         // meta words of a block's row
   static constexpr int kSlot = MT * (1024 + 64 * kWords);
   static constexpr int kRing = kDepth * kSlot;
-  static constexpr int kPitch = NT * 8 + 1;
+  static constexpr int kPitch = NT * 8 + 4;
   static constexpr size_t ring_bytes = (size_t)kWarps * kRing;
   static constexpr size_t red_bytes = (size_t)kAcross * kRows * kPitch * 4;
 };
 
 template <typename T, int NT, int G, int MT, int RW>
-__global__ void __launch_bounds__(kThreads, MT > 1 ? 1 : 2) linear_kernel(const Args a) {
+__global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), MT > 1 ? 1 : 2) linear_kernel(const Args a) {
   using M = Num<T>;
   using N = typename M::N;
   using N2 = typename M::N2;
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, MT > 1 ? 1 : 2) linear_kernel(const 
     const int k = (b0 + step * S::kAcross) * kBlock;
     const int width = min(a.tile, (b1 - b0) * kBlock - step * S::kStep);
     if (width > 0)
-      stage<T>((const T*)a.x + first * a.x_st, a.x_st, a.inner, a.vector, xs + (a.whole ? 0 : (step / per_buffer & 1) * buffer), pitch, rows, k, width);
+      stage<T, S::kWarps>((const T*)a.x + first * a.x_st, a.x_st, a.inner, a.vector, xs + (a.whole ? 0 : (step / per_buffer & 1) * buffer), pitch, rows, k, width);
   };
   stage_from(0);
   commit();
@@ -352,6 +352,9 @@ __global__ void __launch_bounds__(kThreads, MT > 1 ? 1 : 2) linear_kernel(const 
               meta[mt][h][0] = *m;
             }
           }
+        // With many columns of x the scales are applied every 32 weight columns,
+        // whatever the group: sums of a whole group would not fit the registers.
+        constexpr int GG = MT > 1 ? 32 : G;
         float part[MT][NT][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // 32 columns
@@ -380,12 +383,12 @@ __global__ void __launch_bounds__(kThreads, MT > 1 ? 1 : 2) linear_kernel(const 
             const uint4 b = *reinterpret_cast<const uint4*>(xk + at[nt] + j * 32);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              if (j * 32 % G == 0) M::mma_first(part[mt][nt], f1[mt], b.x, b.y);
+              if (j * 32 % GG == 0) M::mma_first(part[mt][nt], f1[mt], b.x, b.y);
               else M::mma(part[mt][nt], f1[mt], b.x, b.y);
               M::mma(part[mt][nt], f2[mt], b.z, b.w);
             }
           }
-          if ((j + 1) * 32 % G == 0) {
+          if ((j + 1) * 32 % GG == 0) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
               const float ca = scale_of(meta[mt][0][j * 32 / G]), cb = scale_of(meta[mt][1][j * 32 / G]);
@@ -419,36 +422,47 @@ __global__ void __launch_bounds__(kThreads, MT > 1 ? 1 : 2) linear_kernel(const 
         for (int r = 0; r < 4; ++r)
           red[(kw * S::kRows + (rw * MT + mt) * 16 + g + 8 * (r >> 1)) * S::kPitch + nt * 8 + 2 * t + (r & 1)] = acc[mt][nt][r];
     __syncthreads();
-    if (ranks > 1) {
+    int n_first = 0, n_count = S::kRows, sums = S::kAcross;
+    if (ranks > 1) {  // each rank adds up a share of the tile's rows, 16 bytes at a time
+      const int quads = (cols + 3) / 4;
+      auto quad = [&](const float* of, int w, int n, int c) -> float4 {
+        return *reinterpret_cast<const float4*>(of + (w * S::kRows + n) * S::kPitch + c);
+      };
+      auto add = [](float4& x, const float4& y) { x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w; };
       if constexpr (S::kAcross > 1) {
-        for (int j = tid; j < S::kRows * cols; j += kThreads) {
-          const int n = j % S::kRows, c = j / S::kRows;
-          float v = red[n * S::kPitch + c];
+        for (int j = tid; j < S::kRows * quads; j += S::kThreads) {
+          const int n = j % S::kRows, c = j / S::kRows * 4;
+          float4 v = quad(red, 0, n, c);
 #pragma unroll
-          for (int w = 1; w < S::kAcross; ++w) v += red[(w * S::kRows + n) * S::kPitch + c];
-          red[n * S::kPitch + c] = v;  // read and written by this thread alone
+          for (int w = 1; w < S::kAcross; ++w) add(v, quad(red, w, n, c));
+          *reinterpret_cast<float4*>(red + n * S::kPitch + c) = v;  // read and written by this thread alone
         }
       }
       cluster.sync();
+      n_count = S::kRows / ranks;
+      n_first = rank * n_count;
+      sums = 1;
+      for (int j = tid; j < n_count * quads; j += S::kThreads) {
+        const int n = n_first + j % n_count, c = j / n_count * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int r = 0; r < ranks; ++r) add(v, quad(cluster.map_shared_rank(red, r), 0, n, c));
+        *reinterpret_cast<float4*>(red + n * S::kPitch + c) = v;  // only this rank reads this share
+      }
+      cluster.sync();
     }
-    // a rank writes its share of the tile's outputs
-    for (int j = tid + rank * kThreads; j < S::kRows * rows; j += kThreads * ranks) {
-      const int m = j / S::kRows, n = j % S::kRows;
+    for (int j = tid; j < n_count * rows; j += S::kThreads) {
+      const int m = j / n_count, n = n_first + j % n_count;
       if (n0 + n >= a.outer) continue;
       float v = 0.f;
 #pragma unroll
       for (int p = M::kParts - 1; p >= 0; --p) {
-        if (ranks > 1) {
-          for (int r = 0; r < ranks; ++r) v += cluster.map_shared_rank(red, r)[n * S::kPitch + p * rows + m];
-        } else {
-#pragma unroll
-          for (int w = 0; w < S::kAcross; ++w) v += red[(w * S::kRows + n) * S::kPitch + p * rows + m];
-        }
+        const float* of = red + n * S::kPitch + p * rows + m;
+        for (int w = 0; w < sums; ++w) v += of[w * S::kRows * S::kPitch];
       }
       if (a.bias) v += (float)((const T*)a.bias)[n0 + n];
       ((T*)a.y)[(long long)(first + m) * a.y_st + n0 + n] = T(v);
     }
-    if (ranks > 1) cluster.sync();  // the others' reads of this CTA's sums are over
   }
 }
 
@@ -531,7 +545,7 @@ void launch_sized(Args a, cudaStream_t stream) {
   const int64_t across = MT > 1 ? a.tiles : std::min<int64_t>(a.tiles, wave);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(across * ranks), (unsigned)ceil_div(a.rows, a.chunk));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -539,14 +553,14 @@ void launch_sized(Args a, cudaStream_t stream) {
   attr[0].val.clusterDim.x = (unsigned)ranks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
   PFB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const Args&)a));
 }
 
 template <typename T>
 void launch_typed(Args& a, int64_t group, cudaStream_t stream) {
   constexpr int parts = Num<T>::kParts;
-  const int64_t most = 64 / parts;  // rows of x whose parts fit eight column blocks
+  const int64_t most = 48 / parts;  // rows of x whose parts fit six column blocks
   const int64_t chunks = ceil_div(a.rows, most);
   a.chunk = (int)ceil_div(a.rows, chunks);
   const int cols = a.chunk * parts;
@@ -560,8 +574,8 @@ void launch_typed(Args& a, int64_t group, cudaStream_t stream) {
   using I2 = std::integral_constant<int, 2>;
   using I3 = std::integral_constant<int, 3>;
   using I4 = std::integral_constant<int, 4>;
+  using I5 = std::integral_constant<int, 5>;
   using I6 = std::integral_constant<int, 6>;
-  using I8 = std::integral_constant<int, 8>;
   // with enough weight rows for one wave of 64-row tiles the warps take rows
   // of their own and join only in pairs, once a tile; so do they where all of
   // x does not fit beside the ring
@@ -570,8 +584,8 @@ void launch_typed(Args& a, int64_t group, cudaStream_t stream) {
   else if (cols <= 16) grouped(I2(), I2(), I4());
   else if (cols <= 24) grouped(I3(), I2(), I4());
   else if (cols <= 32) grouped(I4(), I2(), I4());
-  else if (cols <= 48) grouped(I6(), I2(), I4());
-  else grouped(I8(), I2(), I4());
+  else if (cols <= 40) grouped(I5(), I2(), I4());
+  else grouped(I6(), I2(), I4());
 }
 
 void check_group(int64_t group) {

@@ -72,23 +72,31 @@ def _cuda(t, name: str):
     return t.device
 
 
-_device = _stream = None
+class _Bound:
+    """torch and the library's entry points, looked up once."""
+    torch = device = stream = rope = append = attend = linear = None
+
+    @classmethod
+    def load(cls):
+        import torch
+        L = N.lib()
+        # what torch.cuda.current_device() and current_stream().cuda_stream read, without their 2 us of Python
+        cls.device, cls.stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        cls.rope, cls.append = L.pfk_rope, L.pfk_paged_append
+        cls.attend, cls.linear = L.pfk_paged_attention, L.pfk_linear_w4
+        cls.torch = torch
 
 
 def _call(fn, device, *args) -> None:
     """One entry point on torch's current stream of `device`."""
-    global _device, _stream
-    if _device is None:
-        import torch
-        # what torch.cuda.current_device() and current_stream().cuda_stream read, without their 2 us of Python
-        _device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
     index = device.index
-    if _device() == index:
-        N.check(fn(*args, _stream(index)))
+    if _Bound.device() == index:
+        rc = fn(*args, _Bound.stream(index))
     else:
-        import torch
-        with torch.cuda.device(device):
-            N.check(fn(*args, _stream(index)))
+        with _Bound.torch.cuda.device(device):
+            rc = fn(*args, _Bound.stream(index))
+    if rc:
+        N.check(rc)
 
 
 class _Plans(dict):
@@ -173,6 +181,7 @@ class RotaryEmbedding:
     def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, layout: str = "half",
                  scaling: Optional[dict] = None, inv_freq=None, factor: float = 1.0, device="cuda"):
         import torch
+        _Bound.load()
         rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
         if not 1 <= head_dim <= 1024:
             raise ValueError("head_dim must be 1 to 1024")
@@ -220,19 +229,18 @@ class RotaryEmbedding:
         return p, x.is_contiguous(), out is not None and tuple(xs) != tuple(ys) and x.numel() > 0
 
     def _run(self, x, positions, out, inverse: int):
-        import torch
         key = (inverse, x.dtype, x.shape, x.stride(), x.device, x.requires_grad, positions.dtype, positions.shape,
                positions.stride(), positions.device)
         if out is not None:
             key += (out.dtype, out.shape, out.stride(), out.device, out.requires_grad)
         plan = self._plans.get(key) or self._plans.keep(key, self._plan(x, positions, out, inverse), x, out)
         if out is None:
-            out = torch.empty_like(x) if plan[1] else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = _Bound.torch.empty_like(x) if plan[1] else x.new_empty(x.shape)
         elif plan[2] and out.data_ptr() == x.data_ptr():
             raise ValueError("out: shares x's memory with other strides")
         p = N.RopeParamsC.from_buffer_copy(plan[0])
         p.positions = positions.data_ptr()
-        _call(N.lib().pfk_rope, self.device, x.data_ptr(), out.data_ptr(), C.byref(p))
+        _call(_Bound.rope, self.device, x.data_ptr(), out.data_ptr(), C.byref(p))
         return out
 
     def apply(self, x, positions, out=None):
@@ -279,6 +287,7 @@ class PagedKVCache:
 
     def _take(self, k, v):
         import torch
+        _Bound.load()
         device = _cuda(k, "k")
         code = _code(k.dtype)
         _check("k", k, (None,) * 4, k.dtype, device, output=True)
@@ -303,7 +312,6 @@ class PagedKVCache:
         head_dim] are rotated by `positions` (int64 [tokens]); returns the
         rotated queries (`q_out`, which may be q, or a new tensor, whose rows
         of skipped tokens are 0).  The slots of one call are distinct."""
-        import torch
         key = ("append", k.dtype, k.shape, k.stride(), k.device, k.requires_grad, v.dtype, v.shape, v.stride(), v.device,
                v.requires_grad, slots.dtype, slots.shape, slots.stride(), slots.device)
         if rotary is not None and positions is not None:
@@ -321,12 +329,12 @@ class PagedKVCache:
             p.positions, p.rotary = positions.data_ptr(), rotary._c
         if q is not None:
             if q_out is None:
-                q_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+                q_out = q.new_zeros(q.shape)
             elif plan[1] and q_out.data_ptr() == q.data_ptr():
                 raise ValueError("q_out: shares q's memory with other strides")
             if p.q_heads:
                 p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
-        _call(N.lib().pfk_paged_append, self.device, C.byref(p))
+        _call(_Bound.append, self.device, C.byref(p))
         return q_out
 
     def _append_plan(self, k, v, slots, positions, rotary, q, q_out):
@@ -368,7 +376,7 @@ class PagedKVCache:
         a sequence's last `window` tokens are seen.  A sequence of length 0
         gives 0.  With return_lse also the natural logarithm of the sum of
         exp(score), float32 [batch, q_heads] (-inf for length 0)."""
-        import torch
+        torch = _Bound.torch
         key = ("attend", scale, window, return_lse, q.dtype, q.shape, q.stride(), q.device, q.requires_grad, block_table.dtype,
                block_table.shape, block_table.stride(), block_table.device, seq_lens.dtype, seq_lens.shape, seq_lens.stride(),
                seq_lens.device)
@@ -377,7 +385,7 @@ class PagedKVCache:
         plan = self._plans.get(key) or self._plans.keep(
             key, self._attend_plan(q, block_table, seq_lens, scale, window, out), q, out)
         if out is None:
-            out = torch.empty_like(q) if plan[1] else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q) if plan[1] else q.new_empty(q.shape)
         p = N.PagedAttentionParamsC.from_buffer_copy(plan[0])
         p.q, p.out, p.block_table, p.seq_lens = q.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
         lse = None
@@ -387,7 +395,7 @@ class PagedKVCache:
         # a workspace per call, from torch's allocator: calls on several streams and captured graphs share none
         work = torch.empty(p.workspace_bytes, dtype=torch.uint8, device=q.device)
         p.workspace = work.data_ptr()
-        _call(N.lib().pfk_paged_attention, self.device, C.byref(p))
+        _call(_Bound.attend, self.device, C.byref(p))
         return (out, lse) if return_lse else out
 
     def _attend_plan(self, q, block_table, seq_lens, scale, window, out):
@@ -443,6 +451,7 @@ class Linear4bit:
 
     def __init__(self, packed, scales, zeros=None, bias=None, in_features: Optional[int] = None, group_size: int = 128):
         import torch
+        _Bound.load()
         device = _cuda(packed, "packed")
         if len(packed.shape) != 2 or 0 in packed.shape:
             raise ValueError("packed must be [out_features, (in_features + 1) // 2]")
@@ -506,7 +515,6 @@ class Linear4bit:
 
     def __call__(self, x, out=None):
         """x: [..., in_features], the rows at any one stride."""
-        import torch
         key = (x.dtype, x.shape, x.stride(), x.device, x.requires_grad)
         if out is not None:
             key += (out.dtype, out.shape, out.stride(), out.device, out.requires_grad)
@@ -514,10 +522,10 @@ class Linear4bit:
         if plan[2]:
             x = x.reshape(-1, self.in_features)
         if out is None:
-            out = torch.empty(plan[1], dtype=x.dtype, device=x.device)
+            out = x.new_empty(plan[1])
         p = N.LinearW4ParamsC.from_buffer_copy(plan[0])
         p.x, p.y = x.data_ptr(), out.data_ptr()
-        _call(N.lib().pfk_linear_w4, self.device, C.byref(p))
+        _call(_Bound.linear, self.device, C.byref(p))
         return out
 
     def _plan(self, x, out):

@@ -461,7 +461,8 @@ def test_linear4_extremes(dtype):
     if dtype != F16:  # fp16 may overflow to an infinity there, as its rounding says
         within(got[1], y[1], tol[1])
     assert layer(x[:0]).shape == (0, 32)
-    assert layer(x.view(2, 2, 256)).shape == (2, 2, 32) and torch.equal(layer(x[0]), got[0])
+    assert torch.equal(layer(x.view(2, 2, 256)).view(4, 32).nan_to_num(), got.nan_to_num())
+    within(layer(x[0]), y[0], tol[0])  # one row alone is added in another order
 
 
 # ---------------------------------------------------------------------------
