@@ -25,6 +25,36 @@ struct FastDiv {
   }
 };
 
+// These kernels follow one another within microseconds, so each is launched
+// as a programmatic dependent: its CTAs come up as the kernel before it in the
+// stream ends, and begin() waits until everything before it is finished and
+// visible.  Nothing is read or written before that, and every thread passes
+// it, so a kernel is done only when all before it are.  In a stream of calls
+// this takes 1 to 3 us off each (one of 8191 tokens appended: 41.0 -> 38.0,
+// 48 sequences attended: 144.8 -> 142.8).  A kernel does not let the next one
+// come up before it ends: CTAs that wait take room from those that work (128
+// sequences attended: 448 us for 425; 2047 tokens rotated: 5.8 for 4.3).
+__device__ __forceinline__ void begin() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename A>
+inline void launch_following(void (*kernel)(A), dim3 grid, int threads, size_t smem, cudaStream_t stream, const A& args,
+                             int cluster = 1) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  PFB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
+}
+
 inline void check_decode_dtype(int dtype) {
   PFB_CHECK_ARG(dtype == PFC_DTYPE_FLOAT32 || dtype == PFC_DTYPE_FLOAT16 || dtype == PFC_DTYPE_BFLOAT16,
                 "dtype must be float32, float16 or bfloat16");

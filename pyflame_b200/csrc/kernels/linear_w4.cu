@@ -217,7 +217,7 @@ struct Shape {
 };
 
 template <typename T, int NT, int G, int MT, int RW>
-__global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), MT > 1 ? 1 : 2) linear_kernel(const Args a) {
+__global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), MT > 1 ? 1 : 2) linear_kernel(Args a) {
   using M = Num<T>;
   using N = typename M::N;
   using N2 = typename M::N2;
@@ -247,6 +247,7 @@ __global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), MT > 1 ? 
     if (width > 0)
       stage<T, S::kWarps>((const T*)a.x + first * a.x_st, a.x_st, a.inner, a.vector, xs + (a.whole ? 0 : (step / per_buffer & 1) * buffer), pitch, rows, k, width);
   };
+  begin();
   stage_from(0);
   commit();
 
@@ -543,18 +544,7 @@ void launch_sized(Args a, cudaStream_t stream) {
   // a CTA walks over row tiles (few rows of x), keeping x
   const int64_t wave = std::max<int64_t>(1, slots / ranks);
   const int64_t across = MT > 1 ? a.tiles : std::min<int64_t>(a.tiles, wave);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(across * ranks), (unsigned)ceil_div(a.rows, a.chunk));
-  cfg.blockDim = dim3(S::kThreads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = ranks > 1 ? 1 : 0;
-  PFB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const Args&)a));
+  launch_following<Args>(kernel, dim3((unsigned)(across * ranks), (unsigned)ceil_div(a.rows, a.chunk)), S::kThreads, (size_t)smem, stream, a, ranks);
 }
 
 template <typename T>

@@ -222,7 +222,7 @@ struct Layout {
 };
 
 template <typename T, int DP, int NT, bool CORES>
-__global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident)) attend_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident)) attend_kernel(Args a) {
   using L = Layout<T, DP, NT, CORES>;
   using Tr = Traits<T>;
   constexpr int VEC = L::kVec, HEADS = L::kHeads;
@@ -239,7 +239,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  asm volatile("griddepcontrol.launch_dependents;");
+  begin();
+  // the join may come up as soon as the last of these CTAs has started
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // the list of tiles: its length, and the row that holds this CTA's first
   const int per_row = a.kv_heads * a.chunks;
@@ -732,12 +734,13 @@ constexpr int kMostCtas = 4096;
 // c of the first kernel and went on, in the order of the list; and writes
 // the outputs of sequence c if it is empty.
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a) {
   using Tr = Traits<T>;
   __shared__ float weights[kMostCtas];
   __shared__ float red[kJoinThreads / 32];
   __shared__ float4 acc[kJoinThreads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c0 = blockIdx.x;
+  begin();
   if (c0 < a.batch && span_of<64>(a, c0).tiles == 0) {
     for (int qh = blockIdx.y; qh < a.q_heads; qh += gridDim.y) {
       for (int d = tid; d < a.head_dim; d += kJoinThreads)
@@ -745,7 +748,6 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Args a) {
       if (tid == 0 && a.lse) a.lse[(long long)c0 * a.q_heads + qh] = -INFINITY;
     }
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (c0 >= a.ctas) return;
   const int4 rec = a.records[c0];
   if (!rec.w) return;
@@ -828,18 +830,8 @@ int wave() {
 
 template <class K>
 void launch_sized(Args& a, cudaStream_t stream) {
-  K::run<<<(unsigned)a.ctas, kThreads, K::L::smem, stream>>>(a);
-  PFB_CUDA(cudaGetLastError());
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::max(a.ctas, a.batch), (unsigned)a.heads);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  PFB_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<typename K::T>, (const Args&)a));
+  launch_following<Args>(K::run, dim3((unsigned)a.ctas), kThreads, K::L::smem, stream, a);
+  launch_following<Args>(join_kernel<typename K::T>, dim3((unsigned)std::max(a.ctas, a.batch), (unsigned)a.heads), kJoinThreads, 0, stream, a);
 }
 
 template <typename T_, int DP, int NT, bool CORES>

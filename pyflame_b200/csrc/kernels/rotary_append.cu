@@ -87,10 +87,11 @@ struct alignas(sizeof(T) * VEC) Chunk {
 // values on, or 2j and 2j + 1), the rest are neighbouring chunks that are
 // copied.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads) rotary_kernel(Args a) {
   extern __shared__ float2 table[];  // [per_cta][rot / 2]
   __shared__ long long place[64];    // of a token's row in the cache; -1: skipped
   using C = Chunk<T, VEC>;
+  begin();
   const long long first = (long long)blockIdx.x * a.per_cta;
   const int mine = (int)min((long long)a.per_cta, a.total - first);
   const int half = a.rot >> 1;
@@ -197,8 +198,7 @@ void launch_vec(Args& a, cudaStream_t stream) {
   if (half) per = std::max<int64_t>(1, std::min<int64_t>(per, kTableMax / half));
   a.per_cta = (int)per;
   const size_t smem = (size_t)per * half * sizeof(float2);
-  rotary_kernel<T, VEC><<<(unsigned)ceil_div(a.total, per), kThreads, smem, stream>>>(a);
-  PFB_CUDA(cudaGetLastError());
+  launch_following<Args>(rotary_kernel<T, VEC>, dim3((unsigned)ceil_div(a.total, per)), kThreads, smem, stream, a);
 }
 
 // The widest access that every pointer, stride and boundary of the rows allows.
