@@ -82,14 +82,14 @@ struct Num {  // 16-bit type of the products, its magic number for 4-bit integer
   static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
   static __device__ __forceinline__ N of(float v) { return __float2bfloat16_rn(v); }
   static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   // c = the product, with nothing added
   static __device__ __forceinline__ void mma_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
@@ -103,14 +103,14 @@ struct Num<__half> {
   static constexpr int kParts = 1;
   static __device__ __forceinline__ N of(float v) { return __float2half_rn(v); }
   static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   // c = the product, with nothing added
   static __device__ __forceinline__ void mma_first(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
@@ -379,16 +379,22 @@ __global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), MT > 1 ? 
               f2[mt][h] = q[2];
               f2[mt][h + 2] = q[3];
             }
+          // two instructions a column block and 16 rows; those of one sum are
+          // kept apart (next to each other each waits for the one before it)
+          uint4 b[NT];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const uint4 b = *reinterpret_cast<const uint4*>(xk + at[nt] + j * 32);
+            b[nt] = *reinterpret_cast<const uint4*>(xk + at[nt] + j * 32);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              if (j * 32 % GG == 0) M::mma_first(part[mt][nt], f1[mt], b.x, b.y);
-              else M::mma(part[mt][nt], f1[mt], b.x, b.y);
-              M::mma(part[mt][nt], f2[mt], b.z, b.w);
+              if (j * 32 % GG == 0) M::mma_first(part[mt][nt], f1[mt], b[nt].x, b[nt].y);
+              else M::mma(part[mt][nt], f1[mt], b[nt].x, b[nt].y);
             }
           }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) M::mma(part[mt][nt], f2[mt], b[nt].z, b[nt].w);
           if ((j + 1) * 32 % GG == 0) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {

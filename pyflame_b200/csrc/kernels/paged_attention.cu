@@ -92,6 +92,8 @@ struct Args {
   int heads;  // of a full unit: min(group, unit_heads)
 };
 
+__device__ const uint4 kZeros[64] = {};  // a row of the widest head
+
 struct Span {
   int begin, end, tiles;  // seen keys, and the tiles that cover them
 };
@@ -211,14 +213,14 @@ struct Layout {
   static constexpr int kHeads = CORES ? NT : NT * 8;
   static constexpr int kPitch = DP + 4;
   // a step's keys in blocks of 8: 16 fp32 rows of 256 do not fit the registers
-  static constexpr int kRows = CORES && DP > 128 ? 1 : 2;
+  static constexpr int kRows = CORES ? 1 : 2;
   static constexpr int kTile = 8 * kRows * kWarps;  // keys of a CTA's step
   static constexpr size_t q_bytes = CORES ? (size_t)NT * DP * 4 : (size_t)kQ * NT * 32 * 16 * (sizeof(T) == 4 ? 2 : 1);
   static constexpr size_t o_bytes = (size_t)kWarps * kHeads * kPitch * 4;
   static constexpr size_t m_bytes = (size_t)2 * kWarps * kHeads * 4;
   static constexpr size_t smem = q_bytes + o_bytes + m_bytes;
   // CTAs that share an SM: as many warps' loads in flight as the registers hold
-  static constexpr int kResident = sizeof(T) == 2 ? (DP <= 64 ? (NT == 1 ? 4 : 3) : DP <= 128 && NT == 1 ? 3 : 2) : DP <= 64 ? 3 : 2;
+  static constexpr int kResident = CORES ? (DP <= 64 ? 4 : DP <= 128 ? 3 : 2) : sizeof(T) == 2 ? (DP <= 64 ? (NT == 1 ? 4 : 3) : DP <= 128 && NT == 1 ? 3 : 2) : DP <= 64 ? 3 : 2;
 };
 
 template <typename T, int DP, int NT, bool CORES>
@@ -346,30 +348,45 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
     }
     return p;
   };
+  // Keys that are not there (masked, or of a bad page) are read from a row of
+  // zeros: what lies in their place may be NaN, which a weight of 0 would not
+  // hide.  Chunks behind head_dim stay the zeros they start as.
   uint4 kr[L::kRows][L::kQ], vr[2 * L::kRows][L::kV];
-  unsigned ku[L::kRows], vu[2 * L::kRows];  // places of the rows that are loaded next
-  const char *kp, *vp;
+#pragma unroll
+  for (int r = 0; r < L::kRows; ++r)
+#pragma unroll
+    for (int c = 0; c < L::kQ; ++c) kr[r][c] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int r = 0; r < 2 * L::kRows; ++r)
+#pragma unroll
+    for (int c = 0; c < L::kV; ++c) vr[r][c] = make_uint4(0, 0, 0, 0);
+  const char *kp[L::kRows], *vp[2 * L::kRows];  // the rows that are loaded next
+  bool seen[L::kRows];                          // whether those keys are there
   auto aim = [&](const Place& p) {
+    const char* k = a.k + p.head * a.head_bytes;
+    const char* v = a.v + p.head * a.head_bytes;
+    const char* none = reinterpret_cast<const char*>(kZeros);
 #pragma unroll
-    for (int r = 0; r < L::kRows; ++r) ku[r] = __shfl_sync(~0u, p.where, g + 8 * r);
+    for (int r = 0; r < L::kRows; ++r) {
+      const unsigned u = __shfl_sync(~0u, p.where, g + 8 * r);
+      seen[r] = u != kNone;
+      kp[r] = (u != kNone ? k + u * a.unit_bytes : none) + t * 16;
+    }
 #pragma unroll
-    for (int r = 0; r < 2 * L::kRows; ++r) vu[r] = __shfl_sync(~0u, p.where, 2 * t + (r & 1) + 8 * (r >> 1));
-    kp = a.k + p.head * a.head_bytes + t * 16;
-    vp = a.v + p.head * a.head_bytes + g * 16;
+    for (int r = 0; r < 2 * L::kRows; ++r) {
+      const unsigned u = __shfl_sync(~0u, p.where, 2 * t + (r & 1) + 8 * (r >> 1));
+      vp[r] = (u != kNone ? v + u * a.unit_bytes : none) + g * 16;
+    }
   };
   auto load_k = [&](int c) {
 #pragma unroll
-    for (int r = 0; r < L::kRows; ++r) {
-      kr[r][c] = make_uint4(0, 0, 0, 0);
-      if (ku[r] != kNone && (c * 4 + t) * VEC < a.head_dim) kr[r][c] = load16(kp + ku[r] * a.unit_bytes + c * 64);
-    }
+    for (int r = 0; r < L::kRows; ++r)
+      if ((c * 4 + t) * VEC < a.head_dim) kr[r][c] = load16(kp[r] + c * 64);
   };
   auto load_v = [&](int c) {
 #pragma unroll
-    for (int r = 0; r < 2 * L::kRows; ++r) {
-      vr[r][c] = make_uint4(0, 0, 0, 0);
-      if (vu[r] != kNone && (c * 8 + g) * VEC < a.head_dim) vr[r][c] = load16(vp + vu[r] * a.unit_bytes + c * 128);
-    }
+    for (int r = 0; r < 2 * L::kRows; ++r)
+      if ((c * 8 + g) * VEC < a.head_dim) vr[r][c] = load16(vp[r] + c * 128);
   };
   aim(place());
 #pragma unroll
@@ -442,29 +459,29 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
     for (int step = 0; step < count; ++step) {
       bool live[L::kRows];
 #pragma unroll
-      for (int r = 0; r < L::kRows; ++r) live[r] = ku[r] != kNone;
+      for (int r = 0; r < L::kRows; ++r) live[r] = seen[r];
       aim(next);
       if constexpr (CORES) {
         float s[NT][L::kRows];  // of keys g (and g + 8), the same in a quad's lanes
 #pragma unroll
         for (int h = 0; h < NT; ++h) {
-          float even[L::kRows], odd[L::kRows];
+          float sum[L::kRows][4];
 #pragma unroll
-          for (int r = 0; r < L::kRows; ++r) even[r] = odd[r] = 0.f;
+          for (int r = 0; r < L::kRows; ++r) sum[r][0] = sum[r][1] = sum[r][2] = sum[r][3] = 0.f;
 #pragma unroll
           for (int c = 0; c < L::kQ; ++c) {
             const float4 q = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(qs) + h * DP + (c * 4 + t) * 4);
 #pragma unroll
             for (int r = 0; r < L::kRows; ++r) {
-              even[r] = fmaf(q.x, __uint_as_float(kr[r][c].x), even[r]);
-              odd[r] = fmaf(q.y, __uint_as_float(kr[r][c].y), odd[r]);
-              even[r] = fmaf(q.z, __uint_as_float(kr[r][c].z), even[r]);
-              odd[r] = fmaf(q.w, __uint_as_float(kr[r][c].w), odd[r]);
+              sum[r][0] = fmaf(q.x, __uint_as_float(kr[r][c].x), sum[r][0]);
+              sum[r][1] = fmaf(q.y, __uint_as_float(kr[r][c].y), sum[r][1]);
+              sum[r][2] = fmaf(q.z, __uint_as_float(kr[r][c].z), sum[r][2]);
+              sum[r][3] = fmaf(q.w, __uint_as_float(kr[r][c].w), sum[r][3]);
             }
             if (h == NT - 1) load_k(c);
           }
 #pragma unroll
-          for (int r = 0; r < L::kRows; ++r) s[h][r] = even[r] + odd[r];
+          for (int r = 0; r < L::kRows; ++r) s[h][r] = (sum[r][0] + sum[r][1]) + (sum[r][2] + sum[r][3]);
         }
         float p[NT][2 * L::kRows];  // of the lane's value rows
 #pragma unroll
@@ -728,7 +745,6 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
 }
 
 constexpr int kJoinThreads = 256;
-constexpr int kMostCtas = 4096;
 
 // CTA (c, h): joins the shares of query head h of the unit that began in CTA
 // c of the first kernel and went on, in the order of the list; and writes
@@ -736,10 +752,9 @@ constexpr int kMostCtas = 4096;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a) {
   using Tr = Traits<T>;
-  __shared__ float weights[kMostCtas];
-  __shared__ float red[kJoinThreads / 32];
   __shared__ float4 acc[kJoinThreads];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c0 = blockIdx.x;
+  __shared__ float2 stats[kJoinThreads / 16];
+  const int tid = threadIdx.x, c0 = blockIdx.x;
   begin();
   if (c0 < a.batch && span_of<64>(a, c0).tiles == 0) {
     for (int qh = blockIdx.y; qh < a.q_heads; qh += gridDim.y) {
@@ -761,50 +776,32 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a) {
   const int across = cols <= 16 ? 16 : cols <= 32 ? 32 : 64;  // threads of a share
   const int groups = kJoinThreads / across, gi = tid / across, col = tid % across;
 
+  // x, of maximum m, joined to (top, sum, v): one pass, each of its loads
+  // independent of the others
   float top = -INFINITY, sum = 0.f;
-  for (int i = tid; i < shares; i += kJoinThreads) top = fmaxf(top, a.stats[share(i)].x);
-#pragma unroll
-  for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, off));
-  if (lane == 0) red[warp] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[w]);
-  __syncthreads();
-  for (int i = tid; i < shares; i += kJoinThreads) {
-    const float2 st = a.stats[share(i)];
-    const float f = st.x == -INFINITY ? (top == -INFINITY ? 1.f : 0.f) : exp2_fast(st.x - top);
-    weights[i] = f;
-    sum += f * st.y;
-  }
-#pragma unroll
-  for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(~0u, sum, off);
-  if (lane == 0) red[warp] = sum;
-  __syncthreads();
-  sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[w];
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto join = [&](float m, float l, float4 x) {
+    const float to = fmaxf(top, m);
+    const float f = top == to ? 1.f : exp2_fast(top - to), g = m == to ? 1.f : exp2_fast(m - to);
+    v.x = v.x * f + x.x * g;
+    v.y = v.y * f + x.y * g;
+    v.z = v.z * f + x.z * g;
+    v.w = v.w * f + x.w * g;
+    sum = sum * f + l * g;
+    top = to;
+  };
   if (col < cols) {
 #pragma unroll 4
     for (int i = gi; i < shares; i += groups) {
-      const float4 x = *reinterpret_cast<const float4*>(a.parts + share(i) * a.head_dim + col * 4);
-      const float f = weights[i];
-      v.x = fmaf(f, x.x, v.x);
-      v.y = fmaf(f, x.y, v.y);
-      v.z = fmaf(f, x.z, v.z);
-      v.w = fmaf(f, x.w, v.w);
+      const float2 st = a.stats[share(i)];
+      join(st.x, st.y, *reinterpret_cast<const float4*>(a.parts + share(i) * a.head_dim + col * 4));
     }
   }
   acc[tid] = v;
+  if (col == 0) stats[gi] = make_float2(top, sum);
   __syncthreads();
   if (gi == 0 && col < cols) {
-    for (int w = 1; w < groups; ++w) {
-      const float4 x = acc[w * across + col];
-      v.x += x.x;
-      v.y += x.y;
-      v.z += x.z;
-      v.w += x.w;
-    }
+    for (int w = 1; w < groups; ++w) join(stats[w].x, stats[w].y, acc[w * across + col]);
     T* out = (T*)a.out + (long long)b * a.o_sb + (long long)qh * a.o_sh + col * 4;
     const float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -823,7 +820,7 @@ int wave() {
     PFB_CUDA(cudaFuncSetAttribute(K::run, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)K::L::smem));
     int per = 0;
     PFB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, K::run, kThreads, K::L::smem));
-    ctas[dev] = std::min(std::max(1, per) * device_sm_count(dev), kMostCtas);
+    ctas[dev] = std::max(1, per) * device_sm_count(dev);
   });
   return ctas[dev];
 }

@@ -10,10 +10,13 @@
 // through sincospif, so cosines and sines are within 2 ulp at any position.
 //
 // The work is bound by memory: every value is read once and written once, in
-// accesses of up to 16 bytes.  A CTA takes a few tokens, computes their r/2
-// cosines and sines once into shared memory (they are shared by all heads),
-// and its threads then turn pairs of chunks, the rows of q, k and v of a
-// token in one list, so that one launch stores keys, values and queries.
+// accesses of up to 16 bytes that are marked as streaming (two prompts of
+// 4096 tokens, 32 heads of 128 in bf16, 134 MB: 21.2 us, 6.3 TB/s, for 23.9
+// without the marks).  A CTA takes a few tokens, computes their r/2 cosines
+// and sines once into shared memory (they are shared by all heads), and its
+// threads then turn pairs of chunks, the rows of q, k and v of a token in one
+// list, so that one launch stores keys, values and queries (8191 tokens with
+// 32 query and 8 key-value heads of 128 in fp16, 201 MB: 34.2 us, 5.9 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,7 +31,8 @@
 namespace pfb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int kTokens = 64;     // a CTA takes at most
 constexpr int kTableMax = 2048;  // cosine-sine pairs a CTA keeps (16 KB)
 
 // One family of rows: `heads` rows a token, read at
@@ -51,8 +55,9 @@ struct Args {
   int per_cta = 1;             // tokens a CTA takes
   int head_dim = 0, rot = 0;   // values of a head, and how many are turned
   int items = 0;               // chunk pairs of a row
-  FastDiv by_items, by_heads, by_tokens, by_page;
+  FastDiv by_tokens, by_page;
   int all_heads = 0;
+  int split = 1;  // CTAs that share a token's rows
   int interleaved = 0;
   int inverse = 0;
   float factor = 1.f;
@@ -64,22 +69,51 @@ struct Args {
   int* err = nullptr;
 };
 
-template <typename T>
-__device__ __forceinline__ float to_f(T v) {
-  return (float)v;
+__device__ __forceinline__ float2 turned(float u1, float u2, float2 cs) {
+  return make_float2(fmaf(u1, cs.x, -(u2 * cs.y)), fmaf(u1, cs.y, u2 * cs.x));
 }
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Chunk {
-  T v[VEC];
+// An access of VEC values as plain words: structs of __half or __nv_bfloat16
+// are copied value by value.
+template <int BYTES> struct Raw;
+template <> struct Raw<16> { using R = uint4; };
+template <> struct Raw<8> { using R = uint2; };
+template <> struct Raw<4> { using R = unsigned; };
+template <> struct Raw<2> { using R = unsigned short; };
+
+// Two values of a chunk, e and e + 1, as floats, and back.
+template <typename T>
+struct Two;
+template <>
+struct Two<float> {
+  static __device__ __forceinline__ float2 get(const unsigned* w, int e) { return make_float2(__uint_as_float(w[e]), __uint_as_float(w[e + 1])); }
+  static __device__ __forceinline__ void put(unsigned* w, int e, float2 f) { w[e] = __float_as_uint(f.x), w[e + 1] = __float_as_uint(f.y); }
+  static __device__ __forceinline__ float one(unsigned r) { return __uint_as_float(r); }
+  static __device__ __forceinline__ unsigned one_of(float f) { return __float_as_uint(f); }
+};
+template <>
+struct Two<__half> {
+  static __device__ __forceinline__ float2 get(const unsigned* w, int e) {
+    return __half22float2(*reinterpret_cast<const __half2*>(w + e / 2));
+  }
+  static __device__ __forceinline__ void put(unsigned* w, int e, float2 f) {
+    const __half2 h = __float22half2_rn(f);
+    w[e / 2] = *reinterpret_cast<const unsigned*>(&h);
+  }
+  static __device__ __forceinline__ float one(unsigned short r) { return __half2float(__ushort_as_half(r)); }
+  static __device__ __forceinline__ unsigned short one_of(float f) { return __half_as_ushort(__float2half_rn(f)); }
+};
+template <>
+struct Two<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 get(const unsigned* w, int e) {
+    return make_float2(__uint_as_float(w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xffff0000u));
+  }
+  static __device__ __forceinline__ void put(unsigned* w, int e, float2 f) {
+    const __nv_bfloat162 h = __float22bfloat162_rn(f);
+    w[e / 2] = *reinterpret_cast<const unsigned*>(&h);
+  }
+  static __device__ __forceinline__ float one(unsigned short r) { return __bfloat162float(__ushort_as_bfloat16(r)); }
+  static __device__ __forceinline__ unsigned short one_of(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 };
 
 // VEC: values of one access.  A row is `items` pairs of chunks: the first
@@ -89,94 +123,111 @@ struct alignas(sizeof(T) * VEC) Chunk {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(Args a) {
   extern __shared__ float2 table[];  // [per_cta][rot / 2]
-  __shared__ long long place[64];    // of a token's row in the cache; -1: skipped
-  using C = Chunk<T, VEC>;
+  // of a token's rows in each family: where they are read (in elements), and
+  // where they are written, -1 for a token that is skipped
+  __shared__ long long from[3][kTokens], to[3][kTokens];
+  using R = typename Raw<sizeof(T) * VEC>::R;
+  using P = Two<T>;
   begin();
   const long long first = (long long)blockIdx.x * a.per_cta;
   const int mine = (int)min((long long)a.per_cta, a.total - first);
   const int half = a.rot >> 1;
+  const int pairs = half / VEC;
 
   for (int i = threadIdx.x; i < mine * half; i += kThreads) {
     const int tok = i / half, p = i - tok * half;
-    const unsigned n = (unsigned)(first + tok);
-    const unsigned b = a.by_tokens.div(n);
+    const unsigned n = (unsigned)(first + tok), b = a.by_tokens.div(n);
     const long long pos = a.positions[(long long)b * a.p_sb + (long long)(n - b * a.tokens) * a.p_st];
     const double turns = (double)pos * a.inv_freq[p] * 0.15915494309189533577;  // 1 / (2 pi)
     float s, c;
     sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    table[i] = make_float2(c * a.factor, (a.inverse ? -s : s) * a.factor);
+    // angle j*VEC + e at [e][j]: neighbouring lanes, with neighbouring j, read neighbouring places
+    table[tok * half + p % VEC * pairs + p / VEC] = make_float2(c * a.factor, (a.inverse ? -s : s) * a.factor);
   }
-  if (a.slots) {
-    for (int i = threadIdx.x; i < mine; i += kThreads) {
-      const long long slot = a.slots[first + i];
-      long long at = -1;
+  for (int tok = threadIdx.x; tok < mine; tok += kThreads) {
+    const unsigned n = (unsigned)(first + tok), b = a.by_tokens.div(n);
+    const long long t = n - b * a.tokens;
+    long long place = 0;
+    if (a.slots) {
+      const long long slot = a.slots[n];
+      place = -1;
       if (slot >= a.num_slots) {
         if (a.err) *a.err = PFC_ERR_INVALID_ARGUMENT;
       } else if (slot >= 0) {
         const unsigned page = a.by_page.div((unsigned)slot);
-        at = (long long)page * a.page_stride + (slot - (long long)page * a.by_page.d) * a.token_stride;
+        place = (long long)page * a.page_stride + (slot - (long long)page * a.by_page.d) * a.token_stride;
       }
-      place[i] = at;
+    }
+    for (int f = 0; f < a.families; ++f) {
+      const Rows& r = a.rows[f];
+      from[f][tok] = b * r.sb + t * r.st;
+      to[f][tok] = place < 0 ? -1 : r.paged ? place : b * r.db + t * r.dt;
     }
   }
   __syncthreads();
 
-  const int pairs = half / VEC;
+  // a thread keeps its place j in the rows and walks over them; rows wider
+  // than the CTA take several passes
   const int chunks = a.head_dim / VEC;
-  const unsigned count = (unsigned)mine * a.all_heads * a.items;
-  for (unsigned it = threadIdx.x; it < count; it += kThreads) {
-    const unsigned row = a.by_items.div(it);
-    const int j = (int)(it - row * a.items);
-    const unsigned tok = a.by_heads.div(row);
-    int h = (int)(row - tok * a.all_heads);
-    int f = 0;
-    while (h >= a.rows[f].heads) h -= a.rows[f++].heads;
-    const Rows& r = a.rows[f];
-    if (a.slots && place[tok] < 0) continue;
-    const unsigned n = (unsigned)(first + tok);
-    const unsigned b = a.by_tokens.div(n);
-    const long long t = n - b * a.tokens;
-    const T* src = (const T*)r.src + b * r.sb + t * r.st + h * r.sh;
-    T* dst = (T*)r.dst + b * r.db + (r.paged ? place[tok] : t * r.dt) + h * r.dh;
-    const bool turn = r.rotate && j < pairs;
-    int c1, c2;  // the item's chunks
-    if (turn) {
-      c1 = a.interleaved ? 2 * j : j;
-      c2 = a.interleaved ? 2 * j + 1 : j + pairs;
-    } else {
-      c1 = r.rotate ? 2 * pairs + 2 * (j - pairs) : 2 * j;
-      c2 = c1 + 1;
+  const int head_first = a.all_heads * blockIdx.y / a.split, head_last = a.all_heads * (blockIdx.y + 1) / a.split;
+  const int wide = min(a.items, kThreads), stride = kThreads / wide;
+  const int start = threadIdx.x / wide;
+  if (start >= stride) return;
+  for (int j = threadIdx.x - start * wide; j < a.items; j += wide) {
+    int tok = 0, head = head_first + start;
+    for (;; head += stride) {
+      while (head >= head_last) {
+        head -= head_last - head_first;
+        ++tok;
+      }
+      if (tok >= mine) break;
+      int h = head, f = 0;
+      while (h >= a.rows[f].heads) h -= a.rows[f++].heads;
+      const Rows& r = a.rows[f];
+      const long long at = to[f][tok];
+      if (at < 0) continue;
+      const T* src = (const T*)r.src + from[f][tok] + h * r.sh;
+      T* dst = (T*)r.dst + at + h * r.dh;
+      const bool turn = r.rotate && j < pairs;
+      int c1 = 2 * j, c2 = 2 * j + 1;  // the item's chunks; 2 * pairs is the first behind the turned ones
+      if (turn && !a.interleaved) {
+        c1 = j;
+        c2 = j + pairs;
+      }
       if (c1 >= chunks) continue;
-    }
-    const bool two = c2 < chunks;
-    C x1 = *reinterpret_cast<const C*>(src + c1 * VEC), x2{};
-    if (two) x2 = *reinterpret_cast<const C*>(src + c2 * VEC);
+      const bool two = c2 < chunks;
+    R r1 = __ldcs(reinterpret_cast<const R*>(src + c1 * VEC)), r2{};
+    if (two) r2 = __ldcs(reinterpret_cast<const R*>(src + c2 * VEC));
     if (turn) {
-      const float2* cs = table + tok * half;
-      if (a.interleaved && VEC > 1) {
-        // pairs are neighbours: chunk c1 holds angles j*VEC ... , c2 the rest
-#pragma unroll
-        for (int e = 0; e < VEC; e += 2) {
-          const float2 p = cs[j * VEC + e / 2], q = cs[j * VEC + VEC / 2 + e / 2];
-          const float u1 = to_f(x1.v[e]), u2 = to_f(x1.v[(e + 1) % VEC]);
-          const float w1 = to_f(x2.v[e]), w2 = to_f(x2.v[(e + 1) % VEC]);
-          x1.v[e] = from_f<T>(fmaf(u1, p.x, -(u2 * p.y)));
-          x1.v[(e + 1) % VEC] = from_f<T>(fmaf(u1, p.y, u2 * p.x));
-          x2.v[e] = from_f<T>(fmaf(w1, q.x, -(w2 * q.y)));
-          x2.v[(e + 1) % VEC] = from_f<T>(fmaf(w1, q.y, w2 * q.x));
-        }
+      const float2* cs = table + tok * half + j;
+      if constexpr (VEC == 1) {
+        const float2 y = turned(P::one(r1), P::one(r2), cs[0]);
+        r1 = P::one_of(y.x);
+        r2 = P::one_of(y.y);
       } else {
+        unsigned* x1 = reinterpret_cast<unsigned*>(&r1);
+        unsigned* x2 = reinterpret_cast<unsigned*>(&r2);
+        if (a.interleaved) {  // chunk c1 holds the pairs of angles j*VEC ... , c2 those of the VEC/2 behind
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float2 p = cs[j * VEC + e];
-          const float u1 = to_f(x1.v[e]), u2 = to_f(x2.v[e]);
-          x1.v[e] = from_f<T>(fmaf(u1, p.x, -(u2 * p.y)));
-          x2.v[e] = from_f<T>(fmaf(u1, p.y, u2 * p.x));
+          for (int e = 0; e < VEC; e += 2) {
+            const float2 u = P::get(x1, e), w = P::get(x2, e);
+            P::put(x1, e, turned(u.x, u.y, cs[(e / 2) * pairs]));
+            P::put(x2, e, turned(w.x, w.y, cs[(VEC / 2 + e / 2) * pairs]));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; e += 2) {
+            const float2 u = P::get(x1, e), w = P::get(x2, e);
+            const float2 y = turned(u.x, w.x, cs[(e) * pairs]), z = turned(u.y, w.y, cs[(e + 1) * pairs]);
+            P::put(x1, e, make_float2(y.x, z.x));
+            P::put(x2, e, make_float2(y.y, z.y));
+          }
         }
       }
     }
-    *reinterpret_cast<C*>(dst + c1 * VEC) = x1;
-    if (two) *reinterpret_cast<C*>(dst + c2 * VEC) = x2;
+    __stcs(reinterpret_cast<R*>(dst + c1 * VEC), r1);
+    if (two) __stcs(reinterpret_cast<R*>(dst + c2 * VEC), r2);
+    }
   }
 }
 
@@ -188,17 +239,21 @@ void launch_vec(Args& a, cudaStream_t stream) {
   bool copies = false;
   for (int f = 0; f < a.families; ++f) copies |= !a.rows[f].rotate;
   if (copies) a.items = std::max(a.items, (int)ceil_div(a.head_dim / VEC, 2));
-  a.by_items = FastDiv((unsigned)a.items);
-  a.by_heads = FastDiv((unsigned)a.all_heads);
   a.by_tokens = FastDiv((unsigned)a.tokens);
-  // about four items a thread, as long as the table fits
+  // about four items a thread, as long as the table fits (two: 22.5 us, eight:
+  // 21.4, sixteen: 27 for the prompts' 21.2), fewer where that would leave
+  // less than four CTAs an SM
   const int64_t per_token = (int64_t)a.all_heads * a.items;
-  int64_t per = std::max<int64_t>(1, 4 * kThreads / per_token);
-  per = std::min<int64_t>({per, 64, a.total});
+  const int64_t filled = a.total / (4 * (int64_t)device_sm_count(current_device()));
+  int64_t per = std::max<int64_t>(1, std::min<int64_t>(4 * kThreads / per_token, filled));
+  per = std::min<int64_t>({per, kTokens, a.total});
   if (half) per = std::max<int64_t>(1, std::min<int64_t>(per, kTableMax / half));
   a.per_cta = (int)per;
   const size_t smem = (size_t)per * half * sizeof(float2);
-  launch_following<Args>(rotary_kernel<T, VEC>, dim3((unsigned)ceil_div(a.total, per)), kThreads, smem, stream, a);
+  // with few tokens several CTAs share one's rows, an item a thread
+  const int64_t sms = device_sm_count(current_device());
+  a.split = (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div(per_token, kThreads), 2 * sms / a.total, a.all_heads}));
+  launch_following<Args>(rotary_kernel<T, VEC>, dim3((unsigned)ceil_div(a.total, per), (unsigned)a.split), kThreads, smem, stream, a);
 }
 
 // The widest access that every pointer, stride and boundary of the rows allows.
