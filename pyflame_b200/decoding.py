@@ -17,6 +17,9 @@ are checked on the host; a wrong one raises ValueError or TypeError.  Page
 numbers, slots and lengths are device data: a kernel that meets a bad one skips
 it and sets the cache's error flag, which `PagedKVCache.check()` raises.
 
+A handle (rotation, cache, layer) owns tables that its kernels read: keep it as
+long as graphs that captured its calls.
+
 The calls take part in no autograd graph of torch and refuse tensors that
 require a gradient; RotaryEmbedding.backward is the rotation's gradient.  They
 have no counterpart in PyFlame.
@@ -97,6 +100,13 @@ def _call(fn, device, *args) -> None:
             rc = fn(*args, _Bound.stream(index))
     if rc:
         N.check(rc)
+
+
+def _model(t, shape, dtype):
+    """A tensor that outputs of a small call are made like: torch.empty_like
+    takes half the time of torch.empty.  None where it would hold much memory
+    (a large call does not notice the difference)."""
+    return t.new_empty(shape, dtype=dtype) if math.prod(shape) <= 1 << 16 else None
 
 
 class _Plans(dict):
@@ -204,6 +214,7 @@ class RotaryEmbedding:
         self.device = self.inv_freq.device
         self._c = N.RotaryC(self.inv_freq.data_ptr(), rotary_dim, int(layout == "interleaved"), self.factor)
         self._plans = _Plans()
+        self._kind = (self.head_dim, self.device.index)
 
     def _plan(self, x, positions, out, inverse: int):
         import torch
@@ -229,10 +240,10 @@ class RotaryEmbedding:
         return p, x.is_contiguous(), out is not None and tuple(xs) != tuple(ys) and x.numel() > 0
 
     def _run(self, x, positions, out, inverse: int):
-        key = (inverse, x.dtype, x.shape, x.stride(), x.device, x.requires_grad, positions.dtype, positions.shape,
-               positions.stride(), positions.device)
+        key = (inverse, x.dtype, x.shape, x.stride(), x.get_device(), x.requires_grad, positions.dtype, positions.shape,
+               positions.stride(), positions.get_device())
         if out is not None:
-            key += (out.dtype, out.shape, out.stride(), out.device, out.requires_grad)
+            key += (out.dtype, out.shape, out.stride(), out.get_device(), out.requires_grad)
         plan = self._plans.get(key) or self._plans.keep(key, self._plan(x, positions, out, inverse), x, out)
         if out is None:
             out = _Bound.torch.empty_like(x) if plan[1] else x.new_empty(x.shape)
@@ -312,15 +323,12 @@ class PagedKVCache:
         head_dim] are rotated by `positions` (int64 [tokens]); returns the
         rotated queries (`q_out`, which may be q, or a new tensor, whose rows
         of skipped tokens are 0).  The slots of one call are distinct."""
-        key = ("append", k.dtype, k.shape, k.stride(), k.device, k.requires_grad, v.dtype, v.shape, v.stride(), v.device,
-               v.requires_grad, slots.dtype, slots.shape, slots.stride(), slots.device)
-        if rotary is not None and positions is not None:
-            key += (rotary.head_dim, rotary.device, positions.dtype, positions.shape, positions.stride(), positions.device)
-        if q is not None:
-            key += (q.dtype, q.shape, q.stride(), q.device, q.requires_grad)
-        if q_out is not None:
-            key += (q_out.dtype, q_out.shape, q_out.stride(), q_out.device, q_out.requires_grad)
-        key += (rotary is None, positions is None, q is None, q_out is None)
+        key = (k.dtype, k.shape, k.stride(), k.get_device(), k.requires_grad, v.dtype, v.shape, v.stride(), v.get_device(),
+               v.requires_grad, slots.dtype, slots.shape, slots.stride(), slots.get_device(),
+               None if rotary is None else rotary._kind,
+               None if positions is None else (positions.dtype, positions.shape, positions.stride(), positions.get_device()),
+               None if q is None else (q.dtype, q.shape, q.stride(), q.get_device(), q.requires_grad),
+               None if q_out is None else (q_out.dtype, q_out.shape, q_out.stride(), q_out.get_device(), q_out.requires_grad))
         plan = self._plans.get(key) or self._plans.keep(
             key, self._append_plan(k, v, slots, positions, rotary, q, q_out), k, v, q, q_out)
         p = N.PagedAppendParamsC.from_buffer_copy(plan[0])
@@ -377,28 +385,29 @@ class PagedKVCache:
         gives 0.  With return_lse also the natural logarithm of the sum of
         exp(score), float32 [batch, q_heads] (-inf for length 0)."""
         torch = _Bound.torch
-        key = ("attend", scale, window, return_lse, q.dtype, q.shape, q.stride(), q.device, q.requires_grad, block_table.dtype,
-               block_table.shape, block_table.stride(), block_table.device, seq_lens.dtype, seq_lens.shape, seq_lens.stride(),
-               seq_lens.device)
+        scale, window = None if scale is None else float(scale), int(window)
+        key = (scale, window, return_lse, q.dtype, q.shape, q.stride(), q.get_device(), q.requires_grad, block_table.dtype,
+               block_table.shape, block_table.stride(), block_table.get_device(), seq_lens.dtype, seq_lens.shape,
+               seq_lens.stride(), seq_lens.get_device())
         if out is not None:
-            key += (out.dtype, out.shape, out.stride(), out.device, out.requires_grad)
+            key += (out.dtype, out.shape, out.stride(), out.get_device(), out.requires_grad)
         plan = self._plans.get(key) or self._plans.keep(
-            key, self._attend_plan(q, block_table, seq_lens, scale, window, out), q, out)
+            key, self._attend_plan(q, block_table, seq_lens, scale, window, out, return_lse), q, out)
         if out is None:
             out = torch.empty_like(q) if plan[1] else q.new_empty(q.shape)
         p = N.PagedAttentionParamsC.from_buffer_copy(plan[0])
         p.q, p.out, p.block_table, p.seq_lens = q.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
         lse = None
         if return_lse:
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+            lse = torch.empty_like(plan[3]) if plan[3] is not None else q.new_empty(q.shape[:2], dtype=torch.float32)
             p.lse = lse.data_ptr()
         # a workspace per call, from torch's allocator: calls on several streams and captured graphs share none
-        work = torch.empty(p.workspace_bytes, dtype=torch.uint8, device=q.device)
+        work = torch.empty(plan[2], dtype=torch.uint8, device=self.device)
         p.workspace = work.data_ptr()
         _call(_Bound.attend, self.device, C.byref(p))
         return (out, lse) if return_lse else out
 
-    def _attend_plan(self, q, block_table, seq_lens, scale, window, out):
+    def _attend_plan(self, q, block_table, seq_lens, scale, window, out, return_lse):
         import torch
         if len(q.shape) != 3:
             raise ValueError("q must be [batch, q_heads, head_dim]")
@@ -410,22 +419,23 @@ class PagedKVCache:
         _check("seq_lens", seq_lens, (batch,), torch.int32, self.device)
         if window < 0:
             raise ValueError("window must not be negative")
-        scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+        scale = 1.0 / math.sqrt(d) if scale is None else scale
         if out is not None:
             _check("out", out, (batch, heads, d), self.dtype, self.device, output=True)
         qs = q.stride()
         os = torch.empty(q.shape, device="meta").stride() if out is None else out.stride()
         p = N.PagedAttentionParamsC(self._c, batch, heads, None, qs[0], qs[1], None, os[0], os[1], None, None,
-                                    block_table.stride(0), block_table.shape[1], None, int(window), scale)
+                                    block_table.stride(0), block_table.shape[1], None, window, scale)
         size = C.c_size_t(0)
         with torch.cuda.device(self.device):
             N.check(N.lib().pfk_paged_attention_workspace(C.byref(p), C.byref(size)))
         p.workspace_bytes = size.value
-        return p, q.is_contiguous()
+        return p, q.is_contiguous(), size.value, _model(q, (batch, heads), torch.float32) if return_lse else None
 
     def check(self) -> None:
         """Wait for the device and raise PfcError if a call met a slot, page
         or length outside the cache since the last check."""
+        _Bound.torch.cuda.synchronize(self.device)
         code = int(self._err.item())
         if code:
             self._err.zero_()
@@ -457,8 +467,8 @@ class Linear4bit:
             raise ValueError("packed must be [out_features, (in_features + 1) // 2]")
         n = packed.shape[0]
         k = 2 * packed.shape[1] if in_features is None else int(in_features)
-        if group_size not in (32, 64) and (group_size < 128 or group_size % 128):
-            raise ValueError("group_size must be 32, 64 or a multiple of 128")
+        if k < 1 or group_size not in (32, 64) and (group_size < 128 or group_size % 128):
+            raise ValueError("group_size must be 32, 64 or a multiple of 128, in_features positive")
         groups = -(-k // group_size)
         _check("packed", packed, (n, (k + 1) // 2), torch.uint8, device)
         if scales.dtype not in (torch.float16, torch.bfloat16):
@@ -489,9 +499,17 @@ class Linear4bit:
     def quantize(cls, weight, group_size: int = 128, bias=None, symmetric: bool = False, scale_dtype=None) -> "Linear4bit":
         """Weights [out_features, in_features] rounded to 4 bits: the nearest
         of 16 evenly spaced values that cover each group's range and 0
-        (symmetric: 15 steps around 8)."""
+        (symmetric: 15 steps around 8).  Scales are float16, or bfloat16 where
+        one is outside float16's normal range."""
         import torch
         _cuda(weight, "weight")
+        if len(weight.shape) != 2 or 0 in weight.shape:
+            raise ValueError("weight must be [out_features, in_features]")
+        if group_size not in (32, 64) and (group_size < 128 or group_size % 128):
+            raise ValueError("group_size must be 32, 64 or a multiple of 128")
+        weight = weight.detach().float()
+        if not bool(torch.isfinite(weight).all()):
+            raise ValueError("weight: holds an infinity or NaN")
         n, k = weight.shape
         groups = -(-k // group_size)
         w = torch.zeros((n, groups * group_size), dtype=torch.float32, device=weight.device)
@@ -501,8 +519,13 @@ class Linear4bit:
             scale = w.abs().amax(-1) / 7.0
         else:
             low, high = w.amin(-1).clamp(max=0.0), w.amax(-1).clamp(min=0.0)
-            scale = (high - low) / 15.0
-        scales = scale.to(torch.float16 if scale_dtype is None else scale_dtype)
+            scale = high / 15.0 - low / 15.0
+        if scale_dtype is None:
+            normal = (scale == 0) | ((scale >= 2.0 ** -14) & (scale <= 65504.0))
+            scale_dtype = torch.float16 if bool(normal.all()) else torch.bfloat16
+        scales = scale.to(scale_dtype)
+        if not bool(torch.isfinite(scales).all()):
+            raise ValueError(f"weight: too large for scales of {scale_dtype}")
         s = scales.float()
         step = torch.where(s > 0, s, torch.ones_like(s))
         zeros = None if symmetric else (-low / step).round().clamp(0, 15)
@@ -514,15 +537,18 @@ class Linear4bit:
         return cls(packed, scales, None if symmetric else zeros.to(torch.uint8), bias, k, group_size)
 
     def __call__(self, x, out=None):
-        """x: [..., in_features], the rows at any one stride."""
-        key = (x.dtype, x.shape, x.stride(), x.device, x.requires_grad)
+        """x: [..., in_features]; `out`, [..., out_features], may not overlap
+        it.  Rows at one stride are read where they are."""
+        key = (x.dtype, x.shape, x.stride(), x.get_device(), x.requires_grad)
         if out is not None:
-            key += (out.dtype, out.shape, out.stride(), out.device, out.requires_grad)
+            key += (out.dtype, out.shape, out.stride(), out.get_device(), out.requires_grad)
         plan = self._plans.get(key) or self._plans.keep(key, self._plan(x, out), x, out)
         if plan[2]:
             x = x.reshape(-1, self.in_features)
+        if out is not None and out.data_ptr() == x.data_ptr() and x.numel():
+            raise ValueError("out: may not be x")
         if out is None:
-            out = x.new_empty(plan[1])
+            out = _Bound.torch.empty_like(plan[3]) if plan[3] is not None else x.new_empty(plan[1])
         p = N.LinearW4ParamsC.from_buffer_copy(plan[0])
         p.x, p.y = x.data_ptr(), out.data_ptr()
         _call(_Bound.linear, self.device, C.byref(p))
@@ -541,8 +567,11 @@ class Linear4bit:
         y_st = self.out_features
         if out is not None:
             _check("out", out, shape, x.dtype, self.device, output=True)
-            y_st = (out if len(shape) == 2 else out.view(-1, self.out_features)).stride(0)
+            try:
+                y_st = (out if len(shape) == 2 else out.view(-1, self.out_features)).stride(0)
+            except RuntimeError:
+                raise ValueError("out: its rows must be at one stride") from None
         p = N.LinearW4ParamsC(code, rows.shape[0], self.in_features, self.out_features, self.group_size, None,
                               rows.stride(0), None, y_st, self.weight.data_ptr(), self.meta.data_ptr(),
                               None if self.bias is None else self.bias.data_ptr())
-        return p, shape, len(x.shape) != 2
+        return p, shape, len(x.shape) != 2, _model(x, shape, x.dtype) if out is None else None

@@ -406,7 +406,8 @@ def linear_tol(x, w, y, t, k, group):
     (5, 127, 17, 128, True, True), (7, 129, 100, 64, True, False), (8, 1000, 33, 32, True, True), (9, 1024, 48, 256, True, False),
     (16, 2049, 31, 128, False, False), (17, 640, 40, 4096, True, True), (21, 5000, 24, 32, True, False),
     (22, 384, 20, 64, False, True), (33, 4096, 37, 64, True, False), (64, 1536, 16, 128, True, True), (65, 200, 50, 32, True, False),
-    (200, 700, 19, 128, False, True)])
+    (200, 700, 19, 128, False, True), (1, 16384, 200, 256, True, False), (8, 16384, 70, 128, True, True), (5, 9000, 130, 32, True, False),
+    (2, 512, 10000, 64, True, False), (48, 9000, 300, 64, True, True), (40, 16384, 129, 512, False, False), (13, 3000, 2000, 32, True, False)])
 def test_linear4(dtype, rows, inner, outer, group, zeros, bias):
     g = gen(rows + inner)
     packed, scales, z, w = weights(g, outer, inner, group, zeros)
@@ -442,6 +443,22 @@ def test_linear4_quantize(scale_dtype, symmetric, inner, group):
     # half a step, and what the scale's own rounding moves: up to 15 steps at eps/2 each
     assert bool(((back - w).abs() <= step * (0.5 + 15 * HALF[scale_dtype] + 2.0 ** -20) + 1e-30).all())
     assert bool((back[3] == 0).all())
+
+
+def test_linear4_quantize_ranges():
+    g = gen(13)
+    for size in (1e-9, 1e6):  # scales outside float16's range
+        w = randn(g, 20, 100) * size
+        layer = pf.Linear4bit.quantize(w, 32)
+        assert layer.scales.dtype == BF16
+        back = layer(torch.eye(100, device="cuda")).T
+        step = layer.scales.float().repeat_interleave(32, 1)[:, :100]
+        assert bool(((back - w).abs() <= step * (0.5 + 15 * HALF[BF16] + 2.0 ** -20)).all())
+    w[1, 1] = math.inf
+    for bad in (lambda: pf.Linear4bit.quantize(w, 32), lambda: pf.Linear4bit.quantize(w[0], 32), lambda: pf.Linear4bit.quantize(w, 48),
+                lambda: pf.Linear4bit.quantize(randn(g, 4, 64) * 1e8, 32, scale_dtype=F16)):
+        with pytest.raises(ValueError):
+            bad()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -562,6 +579,83 @@ def test_captured_steps_replay():
             assert torch.equal(out, want), step
 
 
+def test_first_call_captured_after_a_fork():
+    """Calls of shapes not seen before, captured where two streams join, after a copy, and followed by another library's
+    kernel; replayed on new data."""
+    g = gen(45)
+    layer = Layer(g, F16, q_heads=6, dim=40)
+    x = randn(g, 5, 256, dtype=F16)
+    source = torch.zeros_like(x)
+    pos, slots = torch.arange(5, device="cuda"), torch.arange(5, device="cuda") * 9
+    table, lens = torch.arange(5, dtype=torch.int32, device="cuda")[:, None].contiguous(), torch.ones(5, dtype=torch.int32, device="cuda")
+    slots = torch.arange(5, device="cuda") * 8
+    other = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            moved = x * 2
+        x.copy_(source)
+        torch.cuda.current_stream().wait_stream(other)
+        got = layer.step(x, pos, slots, table, lens) + moved.sum() * 0
+    for _ in range(3):
+        source.copy_(randn(g, 5, 256, dtype=F16))
+        graph.replay()
+        want = layer.step(source, pos, slots, table, lens)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_calls_from_two_threads():
+    import threading
+    g = gen(46)
+    cache, q, table, n = make_batch(g, [700, 90], 16, 2, 8, 64, F16)
+    r = pf.RotaryEmbedding(64)
+    layer = pf.Linear4bit(*weights(g, 96, 512, 64, True)[:3], in_features=512, group_size=64)
+    pos = torch.arange(2, device="cuda")
+    xs = [randn(g, i + 1, 512, dtype=F16) for i in range(12)]
+    want = [layer(x) for x in xs], cache.attend(q, table, n), r.apply(q, pos)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(stream):
+        with torch.cuda.stream(stream):
+            for i in range(60):
+                ok = (torch.equal(layer(xs[i % 12]), want[0][i % 12]) and torch.equal(cache.attend(q, table, n), want[1])
+                      and torch.equal(r.apply(q, pos), want[2]))
+                if not ok:
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(torch.cuda.Stream(),)) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    cache.check()
+
+
+def test_plans_follow_their_arguments():
+    """Calls that differ in one argument are not taken for one another."""
+    g = gen(47)
+    cache, q, table, n = make_batch(g, [300, 200], 16, 2, 8, 64, F32)
+    for scale, window in ((None, 0), (0.5, 0), (0.5, 7), (None, 7), (torch.tensor(0.25), 7), (1, 1)):
+        out, _, tol, _ = attention(cache, q, table, n, window, None if scale is None else float(scale))
+        within(cache.attend(q, table, n, scale=scale, window=window), out, tol)
+    scale = torch.tensor(0.25)
+    first = cache.attend(q, table, n, scale=scale)
+    scale.fill_(0.75)
+    out, _, tol, _ = attention(cache, q, table, n, 0, 0.75)
+    within(cache.attend(q, table, n, scale=scale), out, tol)
+    assert not torch.equal(first, cache.attend(q, table, n, scale=scale))
+    x = randn(g, 4, 64, 8, 64)  # the same shape in other strides
+    r, pos = pf.RotaryEmbedding(64), torch.arange(64, device="cuda")
+    for v in (x, x.transpose(0, 1).contiguous().transpose(0, 1), x.transpose(1, 2).contiguous().transpose(1, 2)):
+        y, mag = turn(v, pos, r)
+        within(r.apply(v, pos), y, turn_tol(y, mag, F32))
+        within(r.backward(v, pos), turn(v, pos, r, -1)[0], turn_tol(y.abs() + mag, mag, F32))
+
+
 def test_two_streams_at_once():
     g = gen(50)
     cache, q, table, n = make_batch(g, [4000, 3000], 16, 2, 16, 128, BF16)
@@ -600,7 +694,8 @@ def test_refusals():
         lambda: cache.append(x, x, i64, q_out=x), lambda: cache.append(x, x, i64, q=x[:2]),
         lambda: cache.attend(x[:, :1], table, lens), lambda: cache.attend(x, table[:2], lens), lambda: cache.attend(x, table, lens[:1]),
         lambda: cache.attend(x, table, lens, window=-1), lambda: cache.attend(x[0], table, lens),
-        lambda: layer(torch.zeros(2, 63, device="cuda")), lambda: layer(torch.zeros(2, 64)),
+        lambda: layer(torch.zeros(2, 63, device="cuda")), lambda: layer(x[0].view(2, 64), out=x[0].view(16, 8)[:2]),
+        lambda: layer(torch.zeros(2, 3, 64, device="cuda"), out=torch.zeros(3, 2, 8, device="cuda").transpose(0, 1)), lambda: layer(torch.zeros(2, 64)),
         lambda: pf.Linear4bit(torch.zeros(8, 32, dtype=torch.uint8, device="cuda"), torch.ones(8, 2, device="cuda", dtype=F16), group_size=64),
         lambda: pf.Linear4bit(torch.zeros(8, 32, dtype=torch.uint8, device="cuda"), torch.ones(8, 1, device="cuda", dtype=F16), group_size=48),
         lambda: pf.Linear4bit(torch.zeros(8, 32, dtype=torch.uint8, device="cuda"), torch.ones(8, 1, device="cuda", dtype=F16),
