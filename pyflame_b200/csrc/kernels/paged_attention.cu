@@ -37,6 +37,7 @@
 // fp32, more: both operands are split into tf32 high and low parts, three
 // products (the dropped low-low term is below 2^-22 of the product).  Scores,
 // maxima, sums and outputs are held in fp32.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -55,6 +56,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kMostRanks = 8;  // CTAs of a cluster
 constexpr unsigned kNone = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -223,7 +225,9 @@ struct Layout {
   static constexpr int kResident = CORES ? (DP <= 64 ? 4 : DP <= 128 ? 3 : 2) : sizeof(T) == 2 ? (DP <= 64 ? (NT == 1 ? 4 : 3) : DP <= 128 && NT == 1 ? 3 : 2) : DP <= 64 ? 3 : 2;
 };
 
-template <typename T, int DP, int NT, bool CORES>
+// CLUSTER: a cluster of CTAs for each unit, each an equal part of its tiles;
+// otherwise runs of the list of all tiles.
+template <typename T, int DP, int NT, bool CORES, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident)) attend_kernel(Args a) {
   using L = Layout<T, DP, NT, CORES>;
   using Tr = Traits<T>;
@@ -242,11 +246,28 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   begin();
+  const int per_row = a.kv_heads * a.chunks;
+  int row, unit, tile;  // unit: of the row
+  Span sp;
+  long long t0, t1, list_total = 0;
+  int list_ctas = 0;
+  namespace cg = cooperative_groups;
+  __shared__ float2 part[HEADS];  // of a cluster's CTA: each head's maximum and sum
+  if constexpr (CLUSTER) {
+    const int ranks = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
+    const int u = blockIdx.x / ranks;
+    row = u / per_row;
+    unit = u - row * per_row;
+    sp = span_of<L::kTile>(a, row);
+    t0 = (long long)sp.tiles * rank / ranks;
+    t1 = (long long)sp.tiles * (rank + 1) / ranks;
+    tile = (int)t0;
+    if (t0 == t1 && tid < HEADS) part[tid] = make_float2(-INFINITY, 0.f);
+  } else {
   // the join may come up as soon as the last of these CTAs has started
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // the list of tiles: its length, and the row that holds this CTA's first
-  const int per_row = a.kv_heads * a.chunks;
   Span mine = {0, 0, 0};
   auto scan_rows = [&](int b) -> long long {  // tiles of the rows before b in its block of rows; scan: warps' sums
     mine = b < a.batch ? span_of<L::kTile>(a, b) : Span{0, 0, 0};
@@ -281,8 +302,8 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
   // CTAs share an SM: 505 us for 487 with the longer runs first)
   const int ctas = (int)min((long long)a.ctas, total);
   const long long c = min((int)blockIdx.x, ctas);
-  const long long t0 = ctas ? (long long)divide(total * c, ctas) : 0;
-  const long long t1 = c < ctas ? (long long)divide(total * (c + 1), ctas) : t0;
+  t0 = ctas ? (long long)divide(total * c, ctas) : 0;
+  t1 = c < ctas ? (long long)divide(total * (c + 1), ctas) : t0;
   if (t0 >= t1) {
     if (tid == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
@@ -302,10 +323,13 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
     if (before > t0) break;  // total > t0: some block of rows gets there
   }
   __syncthreads();
-  int row = found_row;
-  Span sp = found_span;
-  int unit = (int)divide(t0 - found_before, sp.tiles);  // of the row
-  int tile = (int)((t0 - found_before) - (long long)unit * sp.tiles);
+  row = found_row;
+  sp = found_span;
+  unit = (int)divide(t0 - found_before, sp.tiles);
+  tile = (int)((t0 - found_before) - (long long)unit * sp.tiles);
+  list_total = total;
+  list_ctas = ctas;
+  }
   int4 record = make_int4(0, 0, 0, 0);
 
   const float scale2 = a.scale * kLog2e;
@@ -720,7 +744,10 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
         v += f * os[(size_t)(w * HEADS + h) * L::kPitch + d];
         sum += f * ls[w * HEADS + h];
       }
-      if (whole) {
+      if constexpr (CLUSTER) {
+        os[(size_t)h * L::kPitch + d] = v;  // read and written by this thread alone
+        if (d == 0) part[h] = make_float2(top, sum);
+      } else if (whole) {
         ((T*)a.out)[(long long)row * a.o_sb + (long long)(first_q + h) * a.o_sh + d] = Tr::from(sum == 0.f ? 0.f : v / sum);
         if (d == 0 && a.lse)
           a.lse[(long long)row * a.q_heads + first_q + h] = sum == 0.f ? -INFINITY : (top + log2f(sum) - Tr::kShift) * kLn2;
@@ -729,9 +756,10 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
         if (d == 0) a.stats[share + h] = make_float2(top, sum);
       }
     }
+    if (CLUSTER) break;
     if (tile == 0 && !whole) {  // the CTA that has the unit's last tile
       // tile x is in the last CTA c with floor(total c / ctas) <= x
-      record = make_int4(row, unit, (int)divide((at + sp.tiles) * ctas + total - 1, total) - 1, 1);
+      record = make_int4(row, unit, (int)divide((at + sp.tiles) * list_ctas + list_total - 1, list_total) - 1, 1);
     }
     at += count;
     tile = 0;
@@ -741,7 +769,43 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
       if (at < t1) sp = span_of<L::kTile>(a, ++row);
     }
   }
-  if (tid == 0) a.records[blockIdx.x] = record;
+  if constexpr (CLUSTER) {  // each CTA joins a part of the outputs, in the order of the ranks
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int ranks = (int)cluster.num_blocks();
+    const int head = unit / a.chunks, first_q = head * a.group + (unit - head * a.chunks) * a.unit_heads;
+    const int heads = min(a.unit_heads, (head + 1) * a.group - first_q);
+    for (int i = (int)cluster.block_rank() * kThreads + tid; i < heads * a.head_dim; i += kThreads * ranks) {
+      const int h = i / a.head_dim, d = i - h * a.head_dim;
+      float2 st[kMostRanks];
+      float o[kMostRanks];
+#pragma unroll
+      for (int r = 0; r < kMostRanks; ++r) {
+        st[r] = make_float2(-INFINITY, 0.f);
+        o[r] = 0.f;
+        if (r < ranks) {
+          st[r] = cluster.map_shared_rank(part, r)[h];
+          o[r] = cluster.map_shared_rank(os, r)[(size_t)h * L::kPitch + d];
+        }
+      }
+      float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+      for (int r = 0; r < kMostRanks; ++r) top = fmaxf(top, st[r].x);
+#pragma unroll
+      for (int r = 0; r < kMostRanks; ++r) {
+        if (st[r].x == -INFINITY && st[r].y == 0.f) continue;  // no keys: its outputs were never written
+        const float f = st[r].x == top ? 1.f : exp2_fast(st[r].x - top);
+        v += f * o[r];
+        sum += f * st[r].y;
+      }
+      ((T*)a.out)[(long long)row * a.o_sb + (long long)(first_q + h) * a.o_sh + d] = Tr::from(sum == 0.f ? 0.f : v / sum);
+      if (d == 0 && a.lse)
+        a.lse[(long long)row * a.q_heads + first_q + h] = sum == 0.f ? -INFINITY : (top + log2f(sum) - Tr::kShift) * kLn2;
+    }
+    cluster.sync();  // the others' reads of this CTA's part are over
+  } else if (tid == 0) {
+    a.records[blockIdx.x] = record;
+  }
 }
 
 constexpr int kJoinThreads = 256;
@@ -818,6 +882,7 @@ int wave() {
   const int dev = current_device();
   std::call_once(once[dev], [dev] {
     PFB_CUDA(cudaFuncSetAttribute(K::run, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)K::L::smem));
+    PFB_CUDA(cudaFuncSetAttribute(K::run_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)K::L::smem));
     int per = 0;
     PFB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, K::run, kThreads, K::L::smem));
     ctas[dev] = std::max(1, per) * device_sm_count(dev);
@@ -826,7 +891,12 @@ int wave() {
 }
 
 template <class K>
-void launch_sized(Args& a, cudaStream_t stream) {
+void launch_sized(Args& a, int ranks, cudaStream_t stream) {
+  if (ranks) {
+    const int64_t ctas = (int64_t)a.batch * a.kv_heads * a.chunks * ranks;
+    launch_following<Args>(K::run_cluster, dim3((unsigned)ctas), kThreads, K::L::smem, stream, a, ranks);
+    return;
+  }
   launch_following<Args>(K::run, dim3((unsigned)a.ctas), kThreads, K::L::smem, stream, a);
   launch_following<Args>(join_kernel<typename K::T>, dim3((unsigned)std::max(a.ctas, a.batch), (unsigned)a.heads), kJoinThreads, 0, stream, a);
 }
@@ -835,7 +905,8 @@ template <typename T_, int DP, int NT, bool CORES>
 struct Kernel {
   using T = T_;
   using L = Layout<T, DP, NT, CORES>;
-  static constexpr auto run = attend_kernel<T, DP, NT, CORES>;
+  static constexpr auto run = attend_kernel<T, DP, NT, CORES, false>;
+  static constexpr auto run_cluster = attend_kernel<T, DP, NT, CORES, true>;
 };
 
 // Query heads of a unit, as many as the registers hold: on the tensor cores
@@ -901,8 +972,11 @@ void check(const pfk_paged_attention_params& p) {
   PFB_CHECK_ARG(std::isfinite(p.scale), "paged attention: scale is not finite");
 }
 
+constexpr int64_t kClusterTiles = 64;
+
 struct Plan {
   int ctas, heads;
+  int ranks;  // CTAs of a unit's cluster; 0: runs of the list of all tiles
   int64_t stats_at, parts_at, bytes;
 };
 
@@ -911,6 +985,18 @@ Plan plan_of(const pfk_paged_attention_params& p) {
   const int64_t group = p.q_heads / p.cache.heads;
   w.heads = (int)std::min<int64_t>(group, unit_heads(p));
   dispatch(p, [&](auto k) { w.ctas = wave<decltype(k)>(); });
+  // With tables for short sequences a cluster takes each unit: no list, no
+  // workspace, no second launch.
+  int64_t seen = p.table_width * p.cache.page_size;
+  if (p.window) seen = std::min<int64_t>(seen, p.window + 64);
+  const int64_t units = p.batch * p.cache.heads * ceil_div(group, unit_heads(p)), tiles = ceil_div(seen, 64);
+  w.ranks = 0;
+  w.stats_at = w.parts_at = w.bytes = 0;
+  if (tiles <= kClusterTiles && units <= INT32_MAX / kMostRanks) {
+    w.ranks = 1;
+    while (w.ranks < kMostRanks && w.ranks < tiles && units * w.ranks * 2 <= 2 * (int64_t)w.ctas) w.ranks *= 2;
+    return w;
+  }
   w.stats_at = (int64_t)w.ctas * 16;
   w.parts_at = round_up(w.stats_at + (int64_t)w.ctas * 2 * w.heads * 8, 16);
   w.bytes = w.parts_at + (int64_t)w.ctas * 2 * w.heads * p.cache.head_dim * 4;
@@ -947,7 +1033,7 @@ void launch_paged_attention(const pfk_paged_attention_params& p, cudaStream_t st
   const int64_t span = (c.num_pages - 1) * (page_bytes / unit) + (c.page_size - 1) * (token_bytes / unit);
   PFB_CHECK_ARG(span < 0xffffffffll, "paged attention: the cache spans more than 2^32 - 1 of its strides' common divisor");
   const Plan w = plan_of(p);
-  PFB_CHECK_ARG(p.workspace && p.workspace_bytes >= (size_t)w.bytes && (uintptr_t)p.workspace % 16 == 0,
+  PFB_CHECK_ARG(w.bytes == 0 || (p.workspace && p.workspace_bytes >= (size_t)w.bytes && (uintptr_t)p.workspace % 16 == 0),
                 "paged attention: workspace missing, too small or not 16-byte aligned");
   a.k = (const char*)c.k;
   a.v = (const char*)c.v;
@@ -984,7 +1070,7 @@ void launch_paged_attention(const pfk_paged_attention_params& p, cudaStream_t st
   a.parts = (float*)(ws + w.parts_at);
   a.ctas = w.ctas;
   a.heads = w.heads;
-  dispatch(p, [&](auto k) { launch_sized<decltype(k)>(a, stream); });
+  dispatch(p, [&](auto k) { launch_sized<decltype(k)>(a, w.ranks, stream); });
 }
 
 }  // namespace pfb

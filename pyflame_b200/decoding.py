@@ -402,8 +402,9 @@ class PagedKVCache:
             lse = torch.empty_like(plan[3]) if plan[3] is not None else q.new_empty(q.shape[:2], dtype=torch.float32)
             p.lse = lse.data_ptr()
         # a workspace per call, from torch's allocator: calls on several streams and captured graphs share none
-        work = torch.empty(plan[2], dtype=torch.uint8, device=self.device)
-        p.workspace = work.data_ptr()
+        if plan[2]:
+            work = torch.empty(plan[2], dtype=torch.uint8, device=self.device)
+            p.workspace = work.data_ptr()
         _call(_Bound.attend, self.device, C.byref(p))
         return (out, lse) if return_lse else out
 

@@ -257,6 +257,13 @@ def attention(cache, q, table, lens, window=0, scale=None):
     return out, lse, tol, lse_tol
 
 
+def tables(table, page):
+    """The table as it is, and one with room for long sequences: the kernels share their work in another way."""
+    wide = torch.full((table.shape[0], table.shape[1] + 100000 // page), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    return table, wide
+
+
 LENS = {
     "one": [1], "edges": [15, 16, 17, 63, 64, 65, 128, 0, 1], "empty": [0], "empties": [0, 0, 5, 0], "long": [5000],
     "ragged": [3, 700, 0, 129, 2048, 64, 1], "many": [(i * 37) % 90 for i in range(300)],
@@ -274,11 +281,12 @@ def test_attend(dtype, lens, page, heads, q_heads, dim, window):
     g = gen(page + dim)
     cache, q, table, n = make_batch(g, LENS[lens], page, heads, q_heads, dim, dtype)
     out, lse, tol, lse_tol = attention(cache, q, table, n, window)
-    got, got_lse = cache.attend(q, table, n, window=window, return_lse=True)
-    within(got, out, tol, "out")
-    within(got_lse, lse, lse_tol, "lse")
-    again = cache.attend(q, table, n, window=window)
-    assert torch.equal(again, got)  # shares are joined in one order
+    for t in tables(table, page):
+        got, got_lse = cache.attend(q, t, n, window=window, return_lse=True)
+        within(got, out, tol, "out")
+        within(got_lse, lse, lse_tol, "lse")
+        again = cache.attend(q, t, n, window=window)
+        assert torch.equal(again, got)  # shares are joined in one order
     cache.check()
 
 
@@ -290,11 +298,12 @@ def test_attend_strides_and_layouts(dtype):
     view = wide[:, 1, 2:10, 3:67]  # no 16-byte alignment, two strides
     view.copy_(q)
     out, _, tol, _ = attention(cache, q, table, n, scale=0.3)
-    target = torch.full((9, 10, 70), 5.0, device="cuda", dtype=dtype)
-    got = cache.attend(view, table[:, :-1], n, scale=0.3, out=target[1:8, 1:9, 5:69])
-    within(got, out, tol)
-    target[1:8, 1:9, 5:69] = 5.0
-    assert bool((target == 5).all())  # nothing around it was touched
+    for t in tables(table[:, :-1], 16):
+        target = torch.full((9, 10, 70), 5.0, device="cuda", dtype=dtype)
+        got = cache.attend(view, t, n, scale=0.3, out=target[1:8, 1:9, 5:69])
+        within(got, out, tol)
+        target[1:8, 1:9, 5:69] = 5.0
+        assert bool((target == 5).all())  # nothing around it was touched
     # a table inside a larger one
     big = torch.full((7, table.shape[1] + 5), -1, dtype=torch.int32, device="cuda")
     big[:, 2:-3] = table
@@ -314,9 +323,10 @@ def test_attend_bad_pages_and_lengths(dtype):
         k, v = (x[table[1, keep // 16].long(), keep % 16, 0].double() for x in (cache.k, cache.v))
         out[1] = torch.softmax(q[1].double() @ k.T / 8, -1) @ v
         tol[1] = tol[1].amax() * 4  # of the same magnitudes, fewer keys
-        within(cache.attend(q, t, n), out, tol)
-        with pytest.raises(pf._native.PfcError):
-            cache.check()
+        for tt in tables(t, 16):
+            within(cache.attend(q, tt, n), out, tol)
+            with pytest.raises(pf._native.PfcError):
+                cache.check()
     for bad, means in ((-5, 0), (1000, 48), (2 ** 31 - 1, 48)):
         m = n.clone()
         m[2] = bad
@@ -337,11 +347,12 @@ def test_attend_extremes(dtype):
     cache.v[table[2, 1].long(), 2, 0, 7] = math.nan
     cache.k[table[3, 0].long(), 0, 0, 0] = math.inf
     out, _, tol, _ = attention(cache, q, table, n)
-    got = cache.attend(q, table, n)
-    within(got[:2], out[:2], tol[:2])
-    assert bool(got[2, :, 7].isnan().all()) and bool(got[2, :, :7].isfinite().all())
-    within(got[2, :, :7], out[2, :, :7], tol[2, :, :7].nan_to_num(1e-2))
-    assert bool(got[0].isfinite().all())
+    for t in tables(table, 16):
+        got = cache.attend(q, t, n)
+        within(got[:2], out[:2], tol[:2])
+        assert bool(got[2, :, 7].isnan().all()) and bool(got[2, :, :7].isfinite().all())
+        within(got[2, :, :7], out[2, :, :7], tol[2, :, :7].nan_to_num(1e-2))
+        assert bool(got[0].isfinite().all())
 
 
 def test_attend_small_weights_in_fp16():
@@ -353,9 +364,10 @@ def test_attend_small_weights_in_fp16():
     cache.k[0, 0, 0, 0] = 20.0
     cache.v[0, 1:] = 1.0
     one = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
-    got = cache.attend(q, one, torch.tensor([n], dtype=torch.int32, device="cuda"), scale=math.log(2.0))
     want = 4000 * 2.0 ** -20 / (1 + 4000 * 2.0 ** -20)
-    within(got, torch.full((1, 1, 64), want, dtype=torch.float64, device="cuda"), want * (HALF[F16] + 2.0 ** -16))
+    for t in tables(one, n):
+        got = cache.attend(q, t, torch.tensor([n], dtype=torch.int32, device="cuda"), scale=math.log(2.0))
+        within(got, torch.full((1, 1, 64), want, dtype=torch.float64, device="cuda"), want * (HALF[F16] + 2.0 ** -16))
 
 
 def test_attend_offsets_past_32_bits():
@@ -375,7 +387,8 @@ def test_attend_offsets_past_32_bits():
     assert torch.equal(k[chosen].flatten(0, 1), new_k) and torch.equal(v[chosen].flatten(0, 1), new_v)
     q = randn(g, 1, 16, dim, dtype=BF16)
     out, _, tol, _ = attention(cache, q, table, n)
-    within(cache.attend(q, table, n), out, tol)
+    for t in tables(table, page):
+        within(cache.attend(q, t, n), out, tol)
     cache.check()
 
 
@@ -543,7 +556,7 @@ def test_captured_steps_replay():
     """A captured step follows its inputs; two captured graphs replayed at once on two streams do not meet."""
     dtype = BF16
     layers = [Layer(gen(30 + i), dtype) for i in range(2)]
-    table = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    table = tables(torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4), 8)[1]
     state, graphs, outs = [], [], []
     side = torch.cuda.Stream()
     for layer in layers:
@@ -660,6 +673,7 @@ def test_two_streams_at_once():
     g = gen(50)
     cache, q, table, n = make_batch(g, [4000, 3000], 16, 2, 16, 128, BF16)
     q2 = randn(g, 2, 16, 128, dtype=BF16)
+    table = tables(table, 16)[1]
     want, want2 = cache.attend(q, table, n), cache.attend(q2, table, n)
     torch.cuda.synchronize()
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
@@ -726,6 +740,7 @@ def test_refusals():
 
 def test_workspace_is_checked(native):
     cache, q, table, n = make_batch(gen(60), [40], 16, 1, 4, 64, F32)
+    table = tables(table, 16)[1]
     out = torch.zeros_like(q)
     work = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
     p = native.PagedAttentionParamsC(cache._c, 1, 4, q.data_ptr(), 256, 64, out.data_ptr(), 256, 64, None, table.data_ptr(),
