@@ -300,7 +300,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
   }
   // runs of total / ctas tiles, the longer ones spread evenly (neighbouring
   // CTAs share an SM: 505 us for 487 with the longer runs first)
-  const int ctas = (int)min((long long)a.ctas, total);
+  // at least four tiles each: more shares cost more than they save (one
+  // sequence of 4096 keys and 8 units: 21.4 us with one, 16.0 two, 14.3 four)
+  const int ctas = (int)min((long long)a.ctas, (total + 3) / 4);
   const long long c = min((int)blockIdx.x, ctas);
   t0 = ctas ? (long long)divide(total * c, ctas) : 0;
   t1 = c < ctas ? (long long)divide(total * (c + 1), ctas) : t0;
@@ -412,6 +414,43 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
     for (int r = 0; r < 2 * L::kRows; ++r)
       if ((c * 8 + g) * VEC < a.head_dim) vr[r][c] = load16(vp[r] + c * 128);
   };
+  // Q in the order of the second operand's registers
+  auto stage_q = [&](int row, int first_q, int heads) {
+          const T* qp = (const T*)a.q + (long long)row * a.q_sb + (long long)first_q * a.q_sh;
+          if constexpr (CORES) {
+            for (int i = tid; i < NT * DP; i += kThreads) {
+              const int h = i / DP, d = i - h * DP;
+              reinterpret_cast<float*>(qs)[i] = h < heads && d < a.head_dim ? qp[h * a.q_sh + d] : 0.f;
+            }
+          } else {
+            for (int i = tid; i < NT * L::kQ * 32; i += kThreads) {
+              const int l = i & 31, c = (i >> 5) % L::kQ, nt = (i >> 5) / L::kQ;
+              const int h = nt * 8 + (l >> 2), d0 = (c * 4 + (l & 3)) * VEC;
+              if constexpr (k32) {
+                uint4 hi = {}, lo = {};
+                float x[4];
+    #pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : 0.f;
+                split(x[0], hi.x, lo.x);
+                split(x[1], hi.y, lo.y);
+                split(x[2], hi.z, lo.z);
+                split(x[3], hi.w, lo.w);
+                qs[i] = hi;
+                qs[NT * L::kQ * 32 + i] = lo;
+              } else {
+                alignas(16) T x[8];
+    #pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : Tr::from(0.f);
+                qs[i] = *reinterpret_cast<uint4*>(x);
+              }
+            }
+          }
+  };
+  // the first unit's before the chain of loads that leads to its first keys
+  if (t0 < t1) {
+    const int head = unit / a.chunks, first_q = head * a.group + (unit - head * a.chunks) * a.unit_heads;
+    stage_q(row, first_q, min(a.unit_heads, (head + 1) * a.group - first_q));
+  }
   aim(place());
 #pragma unroll
   for (int c = 0; c < L::kQ; ++c) load_k(c);
@@ -426,38 +465,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
     const int first_q = head * a.group + (unit - head * a.chunks) * a.unit_heads;
     const int heads = min(a.unit_heads, (head + 1) * a.group - first_q);
 
-    // Q in the order of the second operand's registers
-    __syncthreads();  // the previous piece's reads of shared memory are over
-    {
-      const T* qp = (const T*)a.q + (long long)row * a.q_sb + (long long)first_q * a.q_sh;
-      if constexpr (CORES) {
-        for (int i = tid; i < NT * DP; i += kThreads) {
-          const int h = i / DP, d = i - h * DP;
-          reinterpret_cast<float*>(qs)[i] = h < heads && d < a.head_dim ? qp[h * a.q_sh + d] : 0.f;
-        }
-      } else {
-        for (int i = tid; i < NT * L::kQ * 32; i += kThreads) {
-          const int l = i & 31, c = (i >> 5) % L::kQ, nt = (i >> 5) / L::kQ;
-          const int h = nt * 8 + (l >> 2), d0 = (c * 4 + (l & 3)) * VEC;
-          if constexpr (k32) {
-            uint4 hi = {}, lo = {};
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : 0.f;
-            split(x[0], hi.x, lo.x);
-            split(x[1], hi.y, lo.y);
-            split(x[2], hi.z, lo.z);
-            split(x[3], hi.w, lo.w);
-            qs[i] = hi;
-            qs[NT * L::kQ * 32 + i] = lo;
-          } else {
-            alignas(16) T x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : Tr::from(0.f);
-            qs[i] = *reinterpret_cast<uint4*>(x);
-          }
-        }
-      }
+    if (at != t0) {
+      __syncthreads();  // the previous piece's reads of shared memory are over
+      stage_q(row, first_q, heads);
     }
     __syncthreads();
 
@@ -972,7 +982,7 @@ void check(const pfk_paged_attention_params& p) {
   PFB_CHECK_ARG(std::isfinite(p.scale), "paged attention: scale is not finite");
 }
 
-constexpr int64_t kClusterTiles = 64;
+constexpr int64_t kClusterTiles = 64;  // of 64 keys: the longest sequences that clusters take
 
 struct Plan {
   int ctas, heads;
@@ -985,16 +995,19 @@ Plan plan_of(const pfk_paged_attention_params& p) {
   const int64_t group = p.q_heads / p.cache.heads;
   w.heads = (int)std::min<int64_t>(group, unit_heads(p));
   dispatch(p, [&](auto k) { w.ctas = wave<decltype(k)>(); });
-  // With tables for short sequences a cluster takes each unit: no list, no
-  // workspace, no second launch.
+  // Few units with tables for short sequences: a cluster takes each, with no
+  // list, no workspace and no second launch (one sequence, 8 units, list /
+  // cluster: 100 keys 9.4 / 7.3 us, 1000 keys 11.3 / 8.0, 4096 keys 14.3 /
+  // 13.6, 16384 keys 28 / 47; 8 sequences of up to 1000 keys, 64 units: 15.4
+  // / 20.4).
   int64_t seen = p.table_width * p.cache.page_size;
   if (p.window) seen = std::min<int64_t>(seen, p.window + 64);
   const int64_t units = p.batch * p.cache.heads * ceil_div(group, unit_heads(p)), tiles = ceil_div(seen, 64);
   w.ranks = 0;
   w.stats_at = w.parts_at = w.bytes = 0;
-  if (tiles <= kClusterTiles && units <= INT32_MAX / kMostRanks) {
+  if (tiles <= kClusterTiles && units * kMostRanks <= device_sm_count(current_device())) {
     w.ranks = 1;
-    while (w.ranks < kMostRanks && w.ranks < tiles && units * w.ranks * 2 <= 2 * (int64_t)w.ctas) w.ranks *= 2;
+    while (w.ranks < kMostRanks && w.ranks < tiles) w.ranks *= 2;
     return w;
   }
   w.stats_at = (int64_t)w.ctas * 16;
