@@ -567,20 +567,17 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
         float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          // fp32 has 48 instructions on a score and keeps three accumulators,
-          // so as not to wait for each; 16-bit types have 8 (two accumulators
-          // measured 505 us for 423 at 128 sequences of 5000 keys)
-          constexpr int CH = k32 ? 3 : 1;
-          float acc[CH][4];
+          // one accumulator for the 8 instructions of 16-bit types (two measured
+          // 505 us for 423 at 128 sequences of 5000 keys); in fp32 one for each
+          // chunk's six, added up in fp32: the instruction truncates its sums
 #pragma unroll
-          for (int i = 0; i < CH; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][r] = 0.f;
+          for (int r = 0; r < 4; ++r) s[nt][r] = 0.f;
 #pragma unroll
           for (int c = 0; c < L::kQ; ++c) {
             const uint4 b = qs[(nt * L::kQ + c) * 32 + lane];
             if constexpr (k32) {
               const uint4 bl = qs[(NT * L::kQ + nt * L::kQ + c) * 32 + lane];
+              float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 unsigned h0, h1, h2, h3, l0, l1, l2, l3;
@@ -588,18 +585,18 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
                 split(__uint_as_float(word(kr[1][c], 2 * e)), h1, l1);
                 split(__uint_as_float(word(kr[0][c], 2 * e + 1)), h2, l2);
                 split(__uint_as_float(word(kr[1][c], 2 * e + 1)), h3, l3);
-                mma_tf32(acc[CH / 2], l0, l1, l2, l3, word(b, 2 * e), word(b, 2 * e + 1));
-                mma_tf32(acc[CH - 1], h0, h1, h2, h3, word(bl, 2 * e), word(bl, 2 * e + 1));
-                mma_tf32(acc[0], h0, h1, h2, h3, word(b, 2 * e), word(b, 2 * e + 1));
+                mma_tf32(part, l0, l1, l2, l3, word(b, 2 * e), word(b, 2 * e + 1));
+                mma_tf32(part, h0, h1, h2, h3, word(bl, 2 * e), word(bl, 2 * e + 1));
+                mma_tf32(part, h0, h1, h2, h3, word(b, 2 * e), word(b, 2 * e + 1));
               }
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[nt][r] += part[r];
             } else {
-              Tr::mma(acc[0], kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, b.x, b.y);
-              Tr::mma(acc[0], kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, b.z, b.w);
+              Tr::mma(s[nt], kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, b.x, b.y);
+              Tr::mma(s[nt], kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, b.z, b.w);
             }
             if (nt == NT - 1) load_k(c);
           }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[nt][r] = k32 ? acc[0][r] + (acc[CH / 2][r] + acc[CH - 1][r]) : acc[0][r];
         }
 
         unsigned pt[NT][4];  // P as the second operand: 16-bit hi, lo of keys 0-7 and 8-15; fp32 its four values
@@ -663,6 +660,16 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
 #pragma unroll
         for (int c = 0; c < L::kV; ++c) {
           if constexpr (k32) {
+            // a step's products in accumulators of their own, added to the
+            // running output in fp32: with the truncating instruction adding
+            // to it directly, 16 steps lost 3e-6 of it
+            float sum[NT][2][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum[nt][j][r] = 0.f;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {  // keys 8i ... 8i + 7
               unsigned bh[NT][2], bl[NT][2];
@@ -680,12 +687,18 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
                 split(__uint_as_float(word(vr[2 * i + 1][c], 2 * j + 1)), h3, l3);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                  mma_tf32(o[nt][c][j], l0, l1, l2, l3, bh[nt][0], bh[nt][1]);
-                  mma_tf32(o[nt][c][j], h0, h1, h2, h3, bl[nt][0], bl[nt][1]);
-                  mma_tf32(o[nt][c][j], h0, h1, h2, h3, bh[nt][0], bh[nt][1]);
+                  mma_tf32(sum[nt][j], l0, l1, l2, l3, bh[nt][0], bh[nt][1]);
+                  mma_tf32(sum[nt][j], h0, h1, h2, h3, bl[nt][0], bl[nt][1]);
+                  mma_tf32(sum[nt][j], h0, h1, h2, h3, bh[nt][0], bh[nt][1]);
                 }
               }
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[nt][c][j][r] += sum[nt][j][r];
           } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {

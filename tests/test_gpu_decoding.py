@@ -355,6 +355,19 @@ def test_attend_extremes(dtype):
         assert bool(got[0].isfinite().all())
 
 
+@pytest.mark.parametrize("q_heads", [12, 24, 48, 96])
+def test_attend_fp32_keeps_its_precision(q_heads):
+    """Long runs of keys in one accumulator, which a truncating one would lose systematically. In the norm over independent
+    keys the relative errors of a weight add in quadrature, rounding errors with their rms (their bound by the square root
+    of 3): the argument of its exponential (2^-24 of about 7), exp2 (2^-22), the products of its score (3 2^-22 of about 1),
+    its own and the value's splitting (3 2^-23), and 100 additions of 2^-24: 6.3e-7, below 2^-20."""
+    g = gen(14)
+    cache, q, table, n = make_batch(g, [6000] * 6, 64, 12, q_heads, 64, F32, spoil=False)
+    out = attention(cache, q, table, n)[0]
+    got = cache.attend(q, table, n).double()
+    assert float((got - out).norm() / out.norm()) < 2.0 ** -20
+
+
 def test_attend_small_weights_in_fp16():
     """A weight below fp16's range still counts: 4000 keys of weight 2^-20 next to one of weight 1."""
     n = 4001
