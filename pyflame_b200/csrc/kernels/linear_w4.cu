@@ -202,12 +202,13 @@ __device__ __noinline__ void stage(const T* x, long long x_st, int inner, int ve
 // columns.
 template <typename T, int NT, int G, int MT, int RW>
 struct Shape {
+  static constexpr bool kMany = NT > 1;             // rows of x: one tile a CTA, x in chunks
   static constexpr int kWarps = 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kAcross = kWarps / RW;       // warps along the columns
   static constexpr int kRows = 16 * MT * RW;        // weight rows of a tile
   static constexpr int kStep = kBlock * kAcross;    // columns of a CTA's step
-  static constexpr int kDepth = MT > 1 ? 4 : 6;     // slots of a warp's ring; all but one are on their way
+  static constexpr int kDepth = kMany ? 4 : 6;     // slots of a warp's ring; all but one are on their way
   static constexpr int kWords = kBlock / G;         // meta words of a block's row
   static constexpr int kSlot = MT * (1024 + 64 * kWords);
   static constexpr int kRing = kDepth * kSlot;
@@ -217,7 +218,7 @@ struct Shape {
 };
 
 template <typename T, int NT, int G, int MT, int RW>
-__global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), MT > 1 ? 1 : 2) linear_kernel(Args a) {
+__global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), (Shape<T, NT, G, MT, RW>::kMany ? 1 : 2)) linear_kernel(Args a) {
   using M = Num<T>;
   using N = typename M::N;
   using N2 = typename M::N2;
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), MT > 1 ? 
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   char* ring = smem + warp * S::kRing;
-  N* xs = reinterpret_cast<N*>(smem + S::ring_bytes + (MT > 1 ? 0 : S::red_bytes));
+  N* xs = reinterpret_cast<N*>(smem + S::ring_bytes + (S::kMany ? 0 : S::red_bytes));
   float* red = reinterpret_cast<float*>(smem + S::ring_bytes);  // [across][rows][kPitch]; of a single tile in x's place
   const int rw = warp % RW, kw = warp / RW;
   cg::cluster_group cluster = cg::this_cluster();
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), MT > 1 ? 
           }
         // With many columns of x the scales are applied every 32 weight columns,
         // whatever the group: sums of a whole group would not fit the registers.
-        constexpr int GG = MT > 1 ? 32 : G;
+        constexpr int GG = S::kMany ? 32 : G;
         float part[MT][NT][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // 32 columns
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), MT > 1 ? 
     // column 2t or 2t + 1), then the cluster's
     const int n0 = tile * S::kRows;
     __syncthreads();  // the previous tile's sums have been read, and all of x
-    if (MT == 1 && !a.whole && tile + stride < a.tiles) {
+    if (!S::kMany && !a.whole && tile + stride < a.tiles) {
       stage_from(0);
       commit();
     }
@@ -515,6 +516,14 @@ __global__ void arrange_kernel(const ArrangeArgs a) {
   }
 }
 
+// CTAs of a cluster: the columns are shared as long as that fills the device
+// and leaves each CTA two steps.
+int ranks_of(int64_t tiles, int64_t slots, int64_t blocks, int across) {
+  int ranks = 1;
+  while (ranks < 8 && tiles * ranks * 2 <= slots && blocks >= ranks * 2 * 2 * across) ranks *= 2;
+  return ranks;
+}
+
 template <typename T, int NT, int G, int MT, int RW>
 void launch_sized(Args a, cudaStream_t stream) {
   using S = Shape<T, NT, G, MT, RW>;
@@ -525,18 +534,15 @@ void launch_sized(Args a, cudaStream_t stream) {
     PFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
   });
   a.tiles = (int)ceil_div(a.outer, S::kRows);
-  const int64_t slots = (MT > 1 ? 1 : 2) * (int64_t)sms;
-  // the columns are shared as long as that fills the device and leaves each
-  // CTA two steps
-  int ranks = 1;
-  while (ranks < 8 && (int64_t)a.tiles * ranks * 2 <= slots && a.blocks >= ranks * 2 * 2 * S::kAcross) ranks *= 2;
+  const int64_t slots = (S::kMany ? 1 : 2) * (int64_t)sms;
+  const int ranks = ranks_of(a.tiles, slots, a.blocks, S::kAcross);
   a.part_blocks = (int)ceil_div(a.blocks, ranks);
   const int cols = a.chunk * Num<T>::kParts;
   const int64_t mine = round_up((int64_t)a.part_blocks * kBlock, S::kStep);
   auto bytes = [&](int64_t width) { return (int64_t)cols * (width + kPad) * 2; };
   // a CTA's part of x in one buffer, where as many CTAs still fit an SM
-  constexpr int64_t fixed = (int64_t)S::ring_bytes + (MT > 1 ? 0 : (int64_t)S::red_bytes);
-  constexpr int64_t room = (MT > 1 ? (int64_t)kSmemMost : kSmemHalf) - fixed;
+  constexpr int64_t fixed = (int64_t)S::ring_bytes + (S::kMany ? 0 : (int64_t)S::red_bytes);
+  constexpr int64_t room = (S::kMany ? (int64_t)kSmemMost : kSmemHalf) - fixed;
   a.whole = bytes(mine) <= room;
   int64_t width = mine;
   if (!a.whole) {
@@ -545,11 +551,11 @@ void launch_sized(Args a, cudaStream_t stream) {
   }
   a.tile = (int)width;
   const int64_t x_bytes = (a.whole ? 1 : 2) * bytes(width);
-  const int64_t smem = fixed + (MT > 1 ? std::max<int64_t>(x_bytes, S::red_bytes) : x_bytes);
+  const int64_t smem = fixed + (S::kMany ? std::max<int64_t>(x_bytes, S::red_bytes) : x_bytes);
   PFB_CHECK_ARG(smem <= kSmemMost, "linear w4: tile does not fit");
   // a CTA walks over row tiles (few rows of x), keeping x
   const int64_t wave = std::max<int64_t>(1, slots / ranks);
-  const int64_t across = MT > 1 ? a.tiles : std::min<int64_t>(a.tiles, wave);
+  const int64_t across = S::kMany ? a.tiles : std::min<int64_t>(a.tiles, wave);
   launch_following<Args>(kernel, dim3((unsigned)(across * ranks), (unsigned)ceil_div(a.rows, a.chunk)), S::kThreads, (size_t)smem, stream, a, ranks);
 }
 
@@ -572,16 +578,26 @@ void launch_typed(Args& a, int64_t group, cudaStream_t stream) {
   using I4 = std::integral_constant<int, 4>;
   using I5 = std::integral_constant<int, 5>;
   using I6 = std::integral_constant<int, 6>;
-  // with enough weight rows for one wave of 64-row tiles the warps take rows
-  // of their own and join only in pairs, once a tile; so do they where all of
-  // x does not fit beside the ring
-  const bool tall = ceil_div(a.outer, 64) >= device_sm_count(current_device()) || (int64_t)cols * a.blocks * kBlock * 2 > 40 * 1024;
-  if (cols <= 8) tall ? grouped(I1(), I1(), I4()) : grouped(I1(), I1(), I1());
-  else if (cols <= 16) grouped(I2(), I2(), I4());
-  else if (cols <= 24) grouped(I3(), I2(), I4());
-  else if (cols <= 32) grouped(I4(), I2(), I4());
-  else if (cols <= 40) grouped(I5(), I2(), I4());
-  else grouped(I6(), I2(), I4());
+  const int64_t sms = device_sm_count(current_device());
+  if (cols <= 8) {
+    // with enough weight rows for one wave of 64-row tiles the warps take rows
+    // of their own and join only in pairs, once a tile; so do they where all
+    // of x does not fit beside the ring
+    const bool tall = ceil_div(a.outer, 64) >= sms || (int64_t)cols * a.blocks * kBlock * 2 > 40 * 1024;
+    tall ? grouped(I1(), I1(), I4()) : grouped(I1(), I1(), I1());
+    return;
+  }
+  // 128-row tiles, or 32-row ones where those would leave half of the device
+  // idle (40 rows of x in fp16, 128- / 32-row tiles: 200 x 12000 weights 16.1
+  // / 9.4 us, 4000 x 1000 11.2 / 9.0, 4000 x 12000 29.7 / 51.7)
+  const int64_t tiles = ceil_div(a.outer, 128);
+  const bool low = tiles * ranks_of(tiles, sms, a.blocks, 2) * 2 < sms;
+  auto many = [&](auto nt) { low ? grouped(nt, I1(), I2()) : grouped(nt, I2(), I4()); };
+  if (cols <= 16) many(I2());
+  else if (cols <= 24) many(I3());
+  else if (cols <= 32) many(I4());
+  else if (cols <= 40) many(I5());
+  else many(I6());
 }
 
 void check_group(int64_t group) {
