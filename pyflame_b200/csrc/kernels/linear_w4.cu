@@ -17,21 +17,29 @@
 // A lane holds 16 bytes of each of two weight rows in a block of 128 columns:
 // the arranged layout gives it 8 columns of each of the four 32-column groups,
 // so that no instruction mixes two groups, and puts a warp's 1 KB together
-// (with whole rows in turn every load was eight pieces of 64 bytes: 22 us for
-// TIME_UP at 16384 x 4096).
+// (with whole rows in turn every load was eight pieces of 64 bytes: one fp32
+// row times 16384 x 4096 weights 22.3 us for 19.7 at that stage).
 //
-// Two shapes of CTA:
-//   few rows of x (8 columns of the instruction): 8 warps share the columns of
-//   16 weight rows, or in pairs those of 64; a CTA keeps its part of x and
+// Three shapes of CTA, 8 warps each:
+//   few rows of x (8 columns of the instruction): the warps share the columns
+//   of 16 weight rows, or in pairs those of 64; a CTA keeps its part of x and
 //   walks over row tiles, so x is staged once;
-//   more: 8 warps, 128 weight rows (32 a warp, so that a fragment of x read from
-//   shared memory serves two instructions), in pairs over the columns, x in
-//   chunks through two buffers.
+//   more, and weight rows that fill the device: 128 weight rows (32 a warp, so
+//   that a fragment of x read from shared memory serves two instructions), in
+//   pairs over the columns, x in chunks through two buffers;
+//   more, and fewer weight rows: 32 weight rows, four warps over the columns.
 // Weights, scales and zeros reach a warp through a ring of its own in shared
 // memory, filled by asynchronous copies several steps ahead.  Where the rows
 // alone do not fill the device, the CTAs of a cluster share the columns and
 // add their sums through distributed shared memory, in the order of their
 // ranks: results do not depend on timing and nothing needs a workspace.
+//
+// Measured (device time in a stream of calls; the bytes at 6.4 TB/s in
+// brackets): one bf16 row, 4096 x 4096, groups of 128: 4.7 us (1.4); one fp32
+// row, 16384 x 4096, groups of 64: 14.1 us (5.8), 7.4 M instructions, which
+// bound it at 56% of the issue slots; 33 fp16 rows, 4096 x 16384, groups of 32:
+// 32.8 us (6.4), the tensor pipe 34% busy, the rest latency between the
+// instructions of two warps a scheduler (16 narrower warps measured the same).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -598,16 +606,19 @@ void launch_typed(Args& a, int64_t group, cudaStream_t stream) {
   using I6 = std::integral_constant<int, 6>;
   const int64_t sms = device_sm_count(current_device());
   if (cols <= 8) {
-    // with enough weight rows for one wave of 64-row tiles the warps take rows
-    // of their own and join only in pairs, once a tile; so do they where all
-    // of x does not fit beside the ring
-    const bool tall = ceil_div(a.outer, 64) >= sms || (int64_t)cols * a.blocks * kBlock * 2 > 40 * 1024;
+    // With long rows of weights, enough of them for one wave of 64-row tiles,
+    // the warps take rows of their own and join only in pairs, once a tile
+    // (one fp32 row, 16384 x 4096: 14.1 us for 14.9; 12000 x 2000 in fp16: 7.4
+    // for 6.8, 4096 x 4096 in bf16 5.8 for 4.7); so do they where all of x does
+    // not fit beside the ring.
+    const bool tall = (ceil_div(a.outer, 64) >= sms && a.blocks >= 32) || (int64_t)cols * a.blocks * kBlock * 2 > 40 * 1024;
     tall ? grouped(I1(), I1(), I4()) : grouped(I1(), I1(), I1());
     return;
   }
   // 128-row tiles, or 32-row ones where those would leave half of the device
-  // idle (40 rows of x in fp16, 128- / 32-row tiles: 200 x 12000 weights 16.1
-  // / 9.4 us, 4000 x 1000 11.2 / 9.0, 4000 x 12000 29.7 / 51.7)
+  // idle (40 rows of x in fp16, 128- / 32-row tiles: 200 x 12000 weights 14.4
+  // / 7.6 us, 1000 x 8000 11.9 / 8.8, 4000 x 1000 10.9 / 6.5, 4000 x 12000 26.7
+  // / 37.1)
   const int64_t tiles = ceil_div(a.outer, 128);
   const bool low = tiles * ranks_of(tiles, sms, a.blocks, 2) * 2 < sms;
   auto many = [&](auto nt) { low ? grouped(nt, I1(), I2()) : grouped(nt, I2(), I4()); };
