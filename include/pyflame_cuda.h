@@ -469,7 +469,7 @@ PFC_API int pfk_w4_arrange(const pfk_w4_arrange_params* p, void* stream);
 
 typedef struct pfk_linear_w4_params {
     int dtype; /* of x, y and bias */
-    int64_t rows, inner, outer;
+    int64_t rows, inner, outer; /* rows at most 1048560 */
     int64_t group;
     const void* x; /* [rows][inner] */
     int64_t x_st;

@@ -657,7 +657,8 @@ void launch_w4_arrange(const pfk_w4_arrange_params& p, cudaStream_t stream) {
 
 void launch_linear_w4(const pfk_linear_w4_params& p, cudaStream_t stream) {
   check_decode_dtype(p.dtype);
-  PFB_CHECK_ARG(p.rows >= 0 && p.rows <= (1 << 20), "linear w4: rows must be 0 to 2^20");
+  // a grid has up to 65535 chunks of rows, of 16 in float32
+  PFB_CHECK_ARG(p.rows >= 0 && p.rows <= 65535 * 16, "linear w4: rows must be 0 to 1048560");
   PFB_CHECK_ARG(p.inner >= 1 && p.inner <= (1 << 28) && p.outer >= 1 && p.outer <= (1 << 28),
                 "linear w4: inner and outer must be 1 to 2^28");
   check_group(p.group);

@@ -117,6 +117,12 @@ def test_linear_refusals(native, change, word):
     refused(native, native.lib().pfk_linear_w4(None, None), "null")
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_linear_rows_of_one_grid(native, dtype):
+    p = native.LinearW4ParamsC(dtype, 65535 * 16 + 1, 256, 32, 128, FAKE, 256, FAKE, 32, FAKE, FAKE, None)
+    refused(native, native.lib().pfk_linear_w4(C.byref(p), None), "rows")
+
+
 @pytest.mark.parametrize("args,word", [
     ((64, 4, 64, None, FAKE, 1, None, FAKE, FAKE), "null"), ((64, 4, 64, FAKE, FAKE, 1, None, FAKE, None), "null"),
     ((64, -4, 64, FAKE, FAKE, 1, None, FAKE, FAKE), "size"), ((64, 4, 48, FAKE, FAKE, 1, None, FAKE, FAKE), "group"),

@@ -455,6 +455,17 @@ def test_linear4(dtype, rows, inner, outer, group, zeros, bias):
     assert bool((big == 3).all())
 
 
+def test_linear4_most_rows():
+    g = gen(12)
+    packed, scales, z, w = weights(g, 8, 32, 32, True)
+    layer = pf.Linear4bit(packed, scales, z, group_size=32)
+    x = randn(g, 65535 * 16, 32)
+    y = x.double() @ w.T
+    within(layer(x), y, linear_tol(x, w, y, F32, 32, 32))
+    with pytest.raises(pf._native.PfcError, match="rows"):
+        layer(x[:1].expand(65535 * 16 + 1, 32))
+
+
 @pytest.mark.parametrize("scale_dtype", [F16, BF16])
 @pytest.mark.parametrize("symmetric", [False, True])
 @pytest.mark.parametrize("inner,group", [(256, 64), (301, 32), (130, 128)])
