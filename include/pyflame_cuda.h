@@ -427,7 +427,7 @@ typedef struct pfk_paged_attention_params {
     int64_t batch, q_heads; /* q_heads a multiple of the cache's heads */
     const void* q;          /* [batch][q_heads][head_dim] */
     int64_t q_sb, q_sh;
-    void* out; /* [batch][q_heads][head_dim] */
+    void* out; /* [batch][q_heads][head_dim]; may be q itself (same pointer and strides), not overlap it otherwise */
     int64_t o_sb, o_sh;
     float* lse; /* [batch][q_heads] dense: natural log of the sum of exp(score), or NULL */
     const int32_t* block_table; /* page of tokens [i*page_size, (i+1)*page_size) of sequence b at [b*table_stride + i] */
@@ -441,9 +441,10 @@ typedef struct pfk_paged_attention_params {
 } pfk_paged_attention_params;
 PFC_API int pfk_paged_attention_workspace(const pfk_paged_attention_params* p, size_t* bytes);
 /* out[b,h] = sum_j softmax_j(scale * q[b,h].k[j]) v[j] over the tokens j of
- * sequence b, with key-value head h / (q_heads / heads).  Infinite or NaN
- * values in a seen row make that sequence's result NaN; what lies in a page
- * outside the seen tokens has no effect. */
+ * sequence b, with key-value head h / (q_heads / heads).  Queries and seen
+ * rows are finite: where one holds an infinity or NaN, the results that depend
+ * on it may be NaN.  What lies in a page outside the seen tokens has no
+ * effect. */
 PFC_API int pfk_paged_attention(const pfk_paged_attention_params* p, void* stream);
 
 /* Lays 4-bit weights out for pfk_linear_w4, once.

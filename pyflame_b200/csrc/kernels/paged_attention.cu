@@ -1025,7 +1025,7 @@ Plan plan_of(const pfk_paged_attention_params& p) {
   // 13.6, 16384 keys 28 / 47; 8 sequences of up to 1000 keys, 64 units: 15.4
   // / 20.4).
   int64_t seen = p.table_width * p.cache.page_size;
-  if (p.window) seen = std::min<int64_t>(seen, p.window + 64);
+  if (p.window) seen = std::min<int64_t>(seen, std::min<int64_t>(p.window, INT32_MAX) + 64);
   const int64_t units = p.batch * p.cache.heads * ceil_div(group, unit_heads(p)), tiles = ceil_div(seen, 64);
   w.ranks = 0;
   w.stats_at = w.parts_at = w.bytes = 0;
@@ -1061,6 +1061,10 @@ void launch_paged_attention(const pfk_paged_attention_params& p, cudaStream_t st
   check(p);
   if (p.batch == 0) return;
   PFB_CHECK_ARG(p.q && p.out && p.seq_lens && (p.block_table || p.table_width == 0), "paged attention: null pointer");
+  // a CTA reads its unit's queries before any of the unit's outputs are
+  // written, so the output may take the queries' place, row for row
+  PFB_CHECK_ARG(p.out != p.q || ((p.batch == 1 || p.q_sb == p.o_sb) && (p.q_heads == 1 || p.q_sh == p.o_sh)),
+                "paged attention: out shares q's memory with other strides");
   const pfk_paged_cache& c = p.cache;
   const int64_t es = c.dtype == PFC_DTYPE_FLOAT32 ? 4 : 2;
   Args a = {};

@@ -13,9 +13,10 @@ They are hand-written kernels of libpyflame_cuda.so (the pfk_* entry points of
 include/pyflame_cuda.h).  Every call runs on torch's current stream of its
 tensors' device, does not synchronise, and may be captured into a CUDA graph
 (each captured call has its own workspace, from torch's allocator).  Arguments
-are checked on the host; a wrong one raises ValueError or TypeError.  Page
-numbers, slots and lengths are device data: a kernel that meets a bad one skips
-it and sets the cache's error flag, which `PagedKVCache.check()` raises.
+are checked on the host; a wrong one raises ValueError or TypeError, a size or
+layout that the kernels do not take PfcError.  Page numbers, slots and lengths
+are device data: a kernel that meets a bad one skips it and sets the cache's
+error flag, which `PagedKVCache.check()` raises.
 
 A handle (rotation, cache, layer) owns tables that its kernels read: keep it as
 long as graphs that captured its calls.
@@ -378,14 +379,16 @@ class PagedKVCache:
                return_lse: bool = False):
         """Attention of one new token per sequence, its own key among the
         cached: q [batch, q_heads, head_dim] (q_heads a multiple of num_heads;
-        query head h reads key-value head h // (q_heads / num_heads)),
-        block_table int32 [batch, pages], seq_lens int32 [batch].  `scale`
-        (1/sqrt(head_dim) by default) multiplies the scores; `window` > 0: only
-        a sequence's last `window` tokens are seen.  A sequence of length 0
-        gives 0.  With return_lse also the natural logarithm of the sum of
-        exp(score), float32 [batch, q_heads] (-inf for length 0)."""
+        query head h reads key-value head h // (q_heads / num_heads); head_dim
+        a multiple of 8, at most 256), block_table int32 [batch, pages],
+        seq_lens int32 [batch].  `scale` (1/sqrt(head_dim) by default)
+        multiplies the scores; `window` > 0: only a sequence's last `window`
+        tokens are seen.  A sequence of length 0 gives 0.  With return_lse also
+        the natural logarithm of the sum of exp(score), float32 [batch,
+        q_heads] (-inf for length 0).  `out` may be q.  An infinity or NaN in q
+        or in a seen row may make the results that depend on it NaN."""
         torch = _Bound.torch
-        scale, window = None if scale is None else float(scale), int(window)
+        scale, window = None if scale is None else float(scale), min(int(window), 0x7FFFFFFF)
         key = (scale, window, return_lse, q.dtype, q.shape, q.stride(), q.get_device(), q.requires_grad, block_table.dtype,
                block_table.shape, block_table.stride(), block_table.get_device(), seq_lens.dtype, seq_lens.shape,
                seq_lens.stride(), seq_lens.get_device())
@@ -395,6 +398,8 @@ class PagedKVCache:
             key, self._attend_plan(q, block_table, seq_lens, scale, window, out, return_lse), q, out)
         if out is None:
             out = torch.empty_like(q) if plan[1] else q.new_empty(q.shape)
+        elif plan[4] and out.data_ptr() == q.data_ptr():
+            raise ValueError("out: shares q's memory with other strides")
         p = N.PagedAttentionParamsC.from_buffer_copy(plan[0])
         p.q, p.out, p.block_table, p.seq_lens = q.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
         lse = None
@@ -431,7 +436,8 @@ class PagedKVCache:
         with torch.cuda.device(self.device):
             N.check(N.lib().pfk_paged_attention_workspace(C.byref(p), C.byref(size)))
         p.workspace_bytes = size.value
-        return p, q.is_contiguous(), size.value, _model(q, (batch, heads), torch.float32) if return_lse else None
+        return (p, q.is_contiguous(), size.value, _model(q, (batch, heads), torch.float32) if return_lse else None,
+                tuple(qs) != tuple(os) and q.numel() > 0)
 
     def check(self) -> None:
         """Wait for the device and raise PfcError if a call met a slot, page
@@ -532,8 +538,6 @@ class Linear4bit:
         zeros = None if symmetric else (-low / step).round().clamp(0, 15)
         z = 8.0 if symmetric else zeros[..., None]
         q = ((w / step[..., None]).round() + z).clamp(0, 15).to(torch.uint8).view(n, -1)[:, :(k + 1) // 2 * 2]
-        if q.shape[1] % 2:
-            q = torch.nn.functional.pad(q, (0, 1))
         packed = q[:, 0::2] | (q[:, 1::2] << 4)
         return cls(packed, scales, None if symmetric else zeros.to(torch.uint8), bias, k, group_size)
 

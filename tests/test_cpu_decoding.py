@@ -102,6 +102,12 @@ def test_attention_refusals(native, change, word):
     refused(native, native.lib().pfk_paged_attention(None, None), "null")
 
 
+@pytest.mark.parametrize("strides", [(128, 64), (256, 128)])
+def test_attention_into_queries_with_other_strides(native, strides):
+    p = native.PagedAttentionParamsC(cache(native), 2, 4, FAKE, 256, 64, FAKE, *strides, None, FAKE, 4, 4, FAKE, 0, 0.125)
+    refused(native, native.lib().pfk_paged_attention(C.byref(p), None), "strides")
+
+
 @pytest.mark.parametrize("change,word", [
     (dict(dtype=7), "dtype"), (dict(rows=-1), "rows"), (dict(rows=(1 << 20) + 1), "rows"),
     (dict(inner=0), "inner"), (dict(outer=0), "inner"), (dict(group=16), "group"), (dict(group=96), "group"), (dict(group=192), "group"),

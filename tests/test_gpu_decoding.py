@@ -311,6 +311,40 @@ def test_attend_strides_and_layouts(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,heads,q_heads", [("ragged", 2, 8), ("one", 1, 20), ("edges", 2, 2), ("many", 1, 12), ("long", 2, 6)])
+def test_attend_into_the_queries(dtype, lens, heads, q_heads):
+    g = gen(13)
+    cache, q, table, n = make_batch(g, LENS[lens], 16, heads, q_heads, 64, dtype)
+    for t in tables(table, 16):
+        want = cache.attend(q, t, n)
+        wide = torch.full((len(q), q_heads + 2, 70), 5.0, device="cuda", dtype=dtype)
+        view = wide[:, 1:-1, 3:67]
+        view.copy_(q)
+        assert cache.attend(view, t, n, out=view) is view and torch.equal(view, want)
+        view[:] = 5.0
+        assert bool((wide == 5).all())
+    cache.check()
+
+
+def test_attend_refuses_queries_with_other_strides():
+    cache = pf.PagedKVCache(4, 16, 2, 64)
+    q = torch.zeros(2, 2, 64, device="cuda")
+    table, n = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    for _ in range(2):  # checked for the first time, and as a known call
+        with pytest.raises(ValueError, match="strides"):
+            cache.attend(q, table, n, out=q.transpose(0, 1))
+
+
+@pytest.mark.parametrize("window", [300, 2 ** 31 - 1, 2 ** 31, 2 ** 63 - 1, 2 ** 64, 2 ** 80])
+def test_attend_windows_beyond_all_keys(window):
+    g = gen(14)
+    cache, q, table, n = make_batch(g, [300, 0, 17], 16, 1, 2, 64, F32)
+    out, _, tol, _ = attention(cache, q, table, n)
+    for t in tables(table, 16):  # a window may change how the work is shared, and so the order of the sums
+        within(cache.attend(q, t, n, window=window), out, tol)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attend_bad_pages_and_lengths(dtype):
     g = gen(9)
     cache, q, table, n = make_batch(g, [40, 40, 40], 16, 1, 4, 64, dtype, spoil=False)
