@@ -367,8 +367,8 @@ PFC_API int pfk_check_bounded_wait(int* err, int64_t limit_us, void* stream);
  * skip a bad one and set the cache's `err`. */
 
 /* Rotary positions: pair i of a head's first rotary_dim values is turned by
- * the angle positions * inv_freq[i], taken in 64 bits, and its cosine and
- * sine are multiplied by `factor`.  The values behind rotary_dim are copied. */
+ * the angle positions * inv_freq[i], taken in two 64-bit numbers (positions
+ * below 2^53), and its cosine and sine are multiplied by `factor`.  The values behind rotary_dim are copied. */
 typedef struct pfk_rotary {
     const double* inv_freq; /* device, rotary_dim / 2 angles per position */
     int64_t rotary_dim;     /* even, at most head_dim; 0: no rotation */

@@ -5,9 +5,12 @@
 //   (y1, y2) = (x1 cos a - x2 sin a, x1 sin a + x2 cos a),
 // cosine and sine multiplied by a factor (1 unless the frequencies were
 // rescaled).  The gradient is the same kernel with -a.  The angle is formed
-// and reduced in 64 bits: at position 10^6 an angle in 32 bits is off by up
-// to 0.03 radian.  What is left of it, in half-turns within [-1, 1], goes
-// through sincospif, so cosines and sines are within 2 ulp at any position.
+// and reduced in two 64-bit numbers: at position 10^6 an angle in 32 bits is
+// off by up to 0.03 radian, and the nearer a quarter turn's multiple, the more
+// a single 64-bit number loses of the small sine or cosine there.  What is
+// left, at most an eighth of a turn, goes through sincospif in fp32: cosines
+// and sines, however small, are within 2 ulp of those of position * w_i at
+// positions below 2^53.
 //
 // The work is bound by memory: every value is read once and written once, in
 // accesses of up to 16 bytes that are marked as streaming (two prompts of
@@ -68,6 +71,26 @@ struct Args {
   long long num_slots = 0, page_stride = 0, token_stride = 0;
   int* err = nullptr;
 };
+
+// Cosine and sine of pos * w.  pos * w is a + b exactly (b the product's
+// rounding error, by fma), 2 / pi is kHigh + kLow, and the quarter turns
+// n + r, |r| <= 1/2, come from their products with the leading one, a * kHigh,
+// rounded only after n is subtracted.
+__device__ __forceinline__ float2 cos_sin(long long pos, double w) {
+  constexpr double kHigh = 0x1.45f306dc9c883p-1, kLow = -0x1.6b01ec5417056p-55;
+  const double p = (double)pos, a = p * w, b = fma(p, w, -a);
+  const double n = rint(a * kHigh);
+  const double r = fma(a, kHigh, -n) + fma(b, kHigh, a * kLow);
+  float s, c;
+  sincospif((float)(0.5 * r), &s, &c);
+  const int quarter = (int)((long long)n & 3);
+  if (quarter & 1) {
+    const float t = c;
+    c = -s;
+    s = t;
+  }
+  return quarter & 2 ? make_float2(-c, -s) : make_float2(c, s);
+}
 
 __device__ __forceinline__ float2 turned(float u1, float u2, float2 cs) {
   return make_float2(fmaf(u1, cs.x, -(u2 * cs.y)), fmaf(u1, cs.y, u2 * cs.x));
@@ -138,11 +161,9 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(Args a) {
     const int tok = i / half, p = i - tok * half;
     const unsigned n = (unsigned)(first + tok), b = a.by_tokens.div(n);
     const long long pos = a.positions[(long long)b * a.p_sb + (long long)(n - b * a.tokens) * a.p_st];
-    const double turns = (double)pos * a.inv_freq[p] * 0.15915494309189533577;  // 1 / (2 pi)
-    float s, c;
-    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+    const float2 cs = cos_sin(pos, a.inv_freq[p]);
     // angle j*VEC + e at [e][j]: neighbouring lanes, with neighbouring j, read neighbouring places
-    table[tok * half + p % VEC * pairs + p / VEC] = make_float2(c * a.factor, (a.inverse ? -s : s) * a.factor);
+    table[tok * half + p % VEC * pairs + p / VEC] = make_float2(cs.x * a.factor, (a.inverse ? -cs.y : cs.y) * a.factor);
   }
   for (int tok = threadIdx.x; tok < mine; tok += kThreads) {
     const unsigned n = (unsigned)(first + tok), b = a.by_tokens.div(n);

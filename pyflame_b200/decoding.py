@@ -185,7 +185,8 @@ class RotaryEmbedding:
 
     layout "half" turns the pairs (i, i + rotary_dim/2), "interleaved" the
     pairs (2i, 2i + 1), by position * inv_freq[i].  Angles are formed and
-    reduced in 64 bits, so far positions lose nothing.  `inv_freq` (a sequence
+    reduced in two 64-bit numbers, so far positions (below 2^53) and small
+    cosines lose nothing.  `inv_freq` (a sequence
     of rotary_dim / 2 numbers) replaces base and scaling (rotary_frequencies).
     """
 
