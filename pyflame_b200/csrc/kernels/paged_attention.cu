@@ -38,8 +38,13 @@
 // fp32, up to 4 query heads a key-value head, and heads above 128: fp32 FMAs
 // on the CUDA cores.  fp32, more: both operands are split into tf32 high and
 // low parts, three products (the dropped low-low term is below 2^-22 of the
-// product), summed a step at a time.  Scores, maxima, sums and outputs are
-// held in fp32.
+// product).  Scores, maxima, sums and outputs are held in fp32.  The tensor
+// cores truncate what they add, so nothing runs on in their accumulators: a
+// step's products of weights and values have one of their own, which is added
+// to the running output in fp32, rounded to nearest (added to it by the
+// instruction, 131072 keys of a 16-bit type lost up to 3e-5 of the values'
+// size; the addition costs 1% of the time: one sequence of 131071 103 us for
+// 102, 48 of 0 to 8192 151 for 149.5).
 //
 // Measured (device time in a stream of calls; the bytes at 6.4 TB/s in
 // brackets): 128 sequences of 2048 to 8192 keys, bf16, 32/8 heads of 128, 2.69
@@ -145,6 +150,14 @@ struct Traits<__nv_bfloat16> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
+  // c = the product, with nothing added
+  static __device__ __forceinline__ void mma_first(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3,
+                                                   unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  }
   static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
 };
 template <>
@@ -164,6 +177,14 @@ struct Traits<__half> {
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  // c = the product, with nothing added
+  static __device__ __forceinline__ void mma_first(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3,
+                                                   unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
   }
   static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
 };
@@ -578,9 +599,10 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
         float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          // one accumulator for the 8 instructions of 16-bit types (two measured
-          // 505 us for 423 at 128 sequences of 5000 keys); in fp32 one for each
-          // chunk's six, added up in fp32: the instruction truncates its sums
+          // one accumulator for a score's 4 to 16 instructions of 16-bit types,
+          // which truncate less than 2^-19 of its terms in all (two accumulators
+          // measured 505 us for 423 at 128 sequences of 5000 keys); in fp32 one
+          // for each chunk's six, added up in fp32
 #pragma unroll
           for (int r = 0; r < 4; ++r) s[nt][r] = 0.f;
 #pragma unroll
@@ -671,9 +693,8 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
 #pragma unroll
         for (int c = 0; c < L::kV; ++c) {
           if constexpr (k32) {
-            // a step's products in accumulators of their own, added to the
-            // running output in fp32: with the truncating instruction adding
-            // to it directly, 16 steps lost 3e-6 of it
+            // with the instruction adding to the running output, 16 steps
+            // lost 3e-6 of it
             float sum[NT][2][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -717,11 +738,15 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
               const unsigned a1 = __byte_perm(word(vr[0][c], j), word(vr[1][c], j), 0x7632);
               const unsigned a2 = __byte_perm(word(vr[2][c], j), word(vr[3][c], j), 0x5410);
               const unsigned a3 = __byte_perm(word(vr[2][c], j), word(vr[3][c], j), 0x7632);
+              float sum[NT][4];  // the step's
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                Tr::mma(o[nt][c][j], a0, a1, a2, a3, pt[nt][1], pt[nt][3]);
-                Tr::mma(o[nt][c][j], a0, a1, a2, a3, pt[nt][0], pt[nt][2]);
-              }
+              for (int nt = 0; nt < NT; ++nt) Tr::mma_first(sum[nt], a0, a1, a2, a3, pt[nt][1], pt[nt][3]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) Tr::mma(sum[nt], a0, a1, a2, a3, pt[nt][0], pt[nt][2]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[nt][c][j][r] += sum[nt][r];
             }
           }
           load_v(c);

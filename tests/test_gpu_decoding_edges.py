@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import pyflame_b200 as pf
-from tests.test_gpu_decoding import within
+from tests.test_gpu_decoding import BF16, F16, HALF, gen, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,30 @@ def test_rope_cosines_next_to_quarter_turns(w):
     for got, sign in ((r.apply(x, pos), 1), (r.backward(x, pos), -1)):
         want = torch.stack((torch.stack((c, sign * s), -1), torch.stack((-sign * s, c), -1)), 1)
         within(got, want, 2.0 ** -22 * want.abs())
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("q_heads,dim", [(1, 64), (8, 128), (16, 128), (8, 256)])
+def test_attend_long_rows_keep_their_precision(dtype, q_heads, dim):
+    """Values around 1 in the first half of a row and around -1 in the second: the running output climbs to half of the
+    weights' sum and comes back, so what each addition loses shows beside a small result. 131072 keys make 2048 additions
+    in each of four warps, to a running output of half the sum at most. Rounded to nearest, an addition is off by an ulp
+    / sqrt(12) in the root mean square, so a warp by sqrt(2048) 2^-23 / 2 / sqrt(12) = 7.8e-7 and the mean of four by
+    3.9e-7; a step's own sum of 16 products, which the instruction truncates, adds at most 2^-22. Six times the first
+    and the second are below 2^-18. Cut off instead, the additions would lose about 6e-5."""
+    g = gen(70)
+    page, n, rows = 64, 131072, 300  # rows for every CTA of one wave; they share the pages
+    cache = pf.PagedKVCache.from_tensors(*(randn(g, n // page, page, 1, dim, dtype=dtype) for _ in range(2)))
+    cache.v.copy_(torch.rand(cache.v.shape, generator=g, device="cuda") + 0.5)
+    cache.v[n // page // 2:].neg_()
+    q = randn(g, rows, q_heads, dim, dtype=dtype)
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").expand(rows, -1)
+    got = cache.attend(q, table, torch.full((rows,), n, dtype=torch.int32, device="cuda"))
+    k, v = (x.view(n, dim).double() for x in (cache.k, cache.v))
+    for i in range(0, rows, 37):
+        want = torch.softmax(q[i].double() @ k.T * dim ** -0.5, -1) @ v
+        within(got[i], want, HALF[dtype] * want.abs() + 2.0 ** -18, f"row {i}")
