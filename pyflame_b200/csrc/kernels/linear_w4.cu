@@ -11,8 +11,9 @@
 // is ever rounded.  fp32 x enters as three bf16 parts (8 bits each, 24 in
 // all), which take three columns of the instruction instead of three
 // instructions.  Two weights cost one logic operation and one subtraction:
-// a nibble pair OR-ed into the mantissas of two 16-bit numbers is 2^7 + q
-// (2^10 + q in fp16), from which 2^7 + z is subtracted exactly.
+// a nibble pair OR-ed into the mantissas of two 16-bit numbers of value 2^10 is
+// 2^10 + q in fp16, from which 2^10 + z is subtracted exactly; in bf16 it is
+// 2^-4 + 2^-11 q, and the result is multiplied by 2^11.
 //
 // A lane holds 16 bytes of each of two weight rows in a block of 128 columns:
 // the arranged layout gives it 8 columns of each of the four 32-column groups,
@@ -83,10 +84,16 @@ struct Args {
 };
 
 template <typename T>
-struct Num {  // 16-bit type of the products, its magic number for 4-bit integers, and the parts of x
+struct Num {  // 16-bit type of the products, its magic number for 4-bit integers, what a unit of them stands for, and the parts of x
   using N = __nv_bfloat16;
   using N2 = __nv_bfloat162;
-  static constexpr unsigned kMagic = 0x43004300u;  // 128
+  // 2^-4, in whose mantissa a unit is 2^-11: q - z enters as its 2^-11th, and a
+  // sum of 128 columns, at most 15 * 128 of the largest x, stays in fp32's
+  // range whatever x is.  Nothing is lost at the other end: with x in steps of
+  // bf16's smallest, 2^-133, the products are in steps of 2^-144, and fp32's
+  // smallest is 2^-149.  (Results below 2^-115 come in steps of 2^-138.)
+  static constexpr unsigned kMagic = 0x3d803d80u;
+  static constexpr float kUnit = 2048.f;
   static constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
   static __device__ __forceinline__ N of(float v) { return __float2bfloat16_rn(v); }
   static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
@@ -107,7 +114,8 @@ template <>
 struct Num<__half> {
   using N = __half;
   using N2 = __half2;
-  static constexpr unsigned kMagic = 0x64006400u;  // 1024
+  static constexpr unsigned kMagic = 0x64006400u;  // 1024; sums of fp16 products are far inside fp32's range
+  static constexpr float kUnit = 1.f;
   static constexpr int kParts = 1;
   static __device__ __forceinline__ N of(float v) { return __float2half_rn(v); }
   static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
@@ -494,6 +502,7 @@ __global__ void __launch_bounds__((Shape<T, NT, G, MT, RW>::kThreads), (Shape<T,
         const float* of = red + n * S::kPitch + p * rows + m;
         for (int w = 0; w < sums; ++w) v += of[w * S::kRows * S::kPitch];
       }
+      v *= M::kUnit;
       if (a.bias) v += (float)((const T*)a.bias)[n0 + n];
       ((T*)a.y)[(long long)(first + m) * a.y_st + n0 + n] = T(v);
     }

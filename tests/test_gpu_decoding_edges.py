@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import pyflame_b200 as pf
-from tests.test_gpu_decoding import BF16, F16, HALF, gen, randn, within
+from tests.test_gpu_decoding import BF16, F16, F32, HALF, gen, linear_tol, randn, weights, within
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,38 @@ def test_attend_long_rows_keep_their_precision(dtype, q_heads, dim):
     for i in range(0, rows, 37):
         want = torch.softmax(q[i].double() @ k.T * dim ** -0.5, -1) @ v
         within(got[i], want, HALF[dtype] * want.abs() + 2.0 ** -18, f"row {i}")
+
+
+# ---------------------------------------------------------------------------
+# 4-bit weights
+# ---------------------------------------------------------------------------
+
+SHAPES = [(1, 256, 32, 32), (1, 512, 40, 64), (2, 384, 17, 128), (3, 4096, 10000, 128), (20, 512, 40, 32), (40, 256, 300, 256)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,inner,outer,group", SHAPES)
+def test_linear4_sums_beyond_the_largest_number(dtype, rows, inner, outer, group):
+    """Groups whose sum of x (q - z) is above the type's largest number, and comes back with the scale."""
+    g = gen(81)
+    packed, scales, z, w = weights(g, outer, inner, group, True, BF16, 2.0 ** -16)
+    x = (torch.rand(rows, inner, generator=g, device="cuda") * 1e38 + 2e38).to(dtype)
+    y = x.double() @ w.T
+    assert float(y.abs().max()) < 1e38
+    layer = pf.Linear4bit(packed, scales, z, in_features=inner, group_size=group)
+    within(layer(x), y, linear_tol(x, w, y, dtype, inner, group))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,inner,outer,group", SHAPES)
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -118])
+def test_linear4_smallest_numbers(dtype, rows, inner, outer, group, size):
+    """Rows of tiny numbers, of which no bit may be lost where scales bring the result back to the middle. (fp32 values above
+    2^-110 split into three normal bf16 numbers; smaller ones lose what is below 2^-134, half of bf16's smallest step.)"""
+    g = gen(82)
+    packed, scales, z, w = weights(g, outer, inner, group, True, BF16, 2.0 ** 40)
+    x = (randn(g, rows, inner) * size).to(dtype)
+    y = x.double() @ w.T
+    layer = pf.Linear4bit(packed, scales, z, in_features=inner, group_size=group)
+    lost = 2.0 ** -134 * w.abs().sum(1) if dtype == F32 else 0.0
+    within(layer(x), y, linear_tol(x, w, y, dtype, inner, group) + lost)
