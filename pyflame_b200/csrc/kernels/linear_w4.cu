@@ -173,14 +173,18 @@ __device__ __forceinline__ void store_parts(typename Num<T>::N* dst, int between
   } else {
     float rest[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) rest[e] = v[e];
+    for (int e = 0; e < 8; ++e) rest[e] = v[e] + 0.f;  // a NaN has its highest bit set, and stays one when cut off
 #pragma unroll
     for (int p = 0; p < M::kParts; ++p) {
       unsigned w[4];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(rest[e], rest[e + 1]);
-        w[e / 2] = *reinterpret_cast<const unsigned*>(&h);
+        if (p == 0) {  // cut off: fp32 has finite numbers that bf16 would round to an infinity
+          w[e / 2] = __byte_perm(__float_as_uint(rest[e]), __float_as_uint(rest[e + 1]), 0x7632);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(rest[e], rest[e + 1]);
+          w[e / 2] = *reinterpret_cast<const unsigned*>(&h);
+        }
         const float x = rest[e] - __uint_as_float(w[e / 2] << 16), y = rest[e + 1] - __uint_as_float(w[e / 2] & 0xffff0000u);
         rest[e] = isfinite(x) ? x : 0.f;  // an infinity or NaN is the first part
         rest[e + 1] = isfinite(y) ? y : 0.f;

@@ -66,6 +66,22 @@ def test_attend_long_rows_keep_their_precision(dtype, q_heads, dim):
 SHAPES = [(1, 256, 32, 32), (1, 512, 40, 64), (2, 384, 17, 128), (3, 4096, 10000, 128), (20, 512, 40, 32), (40, 256, 300, 256)]
 
 
+@pytest.mark.parametrize("rows,inner,outer,group", SHAPES)
+def test_linear4_largest_numbers_in_fp32(rows, inner, outer, group):
+    """Single values of a row at fp32's largest, which is above bf16's largest."""
+    g = gen(80)
+    packed, scales, z, w = weights(g, outer, inner, group, True, BF16, 2.0 ** -8)
+    x = torch.zeros(rows, inner, device="cuda")
+    most = torch.finfo(F32).max
+    x[:, 7] = most
+    x[0, inner - 1] = -most
+    x[rows - 1, 20] = 3.395e38  # between the two largest
+    w = w.clone()
+    y = x.double() @ w.T
+    layer = pf.Linear4bit(packed, scales, z, in_features=inner, group_size=group)
+    within(layer(x), y, linear_tol(x, w, y, F32, inner, group))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,inner,outer,group", SHAPES)
 def test_linear4_sums_beyond_the_largest_number(dtype, rows, inner, outer, group):
@@ -92,3 +108,17 @@ def test_linear4_smallest_numbers(dtype, rows, inner, outer, group, size):
     layer = pf.Linear4bit(packed, scales, z, in_features=inner, group_size=group)
     lost = 2.0 ** -134 * w.abs().sum(1) if dtype == F32 else 0.0
     within(layer(x), y, linear_tol(x, w, y, dtype, inner, group) + lost)
+
+
+@pytest.mark.parametrize("bits", [0x7f800001, 0x7f80ffff, 0x7fc00000, 0x7fffffff])
+@pytest.mark.parametrize("rows,inner,outer,group", SHAPES[:5:2])
+def test_linear4_any_nan_in_fp32(rows, inner, outer, group, bits):
+    """Also a NaN whose only bits are below bf16's, of either sign, makes its row NaN and no other."""
+    g = gen(83)
+    packed, scales, z, w = weights(g, outer, inner, group, True, BF16)
+    x = torch.cat((randn(g, rows, inner), randn(g, 2, inner)))
+    x.view(torch.int32)[:2, 9] = torch.tensor([bits, bits - 2 ** 31], dtype=torch.int64, device="cuda").to(torch.int32)
+    got = pf.Linear4bit(packed, scales, z, in_features=inner, group_size=group)(x)
+    assert bool(got[:2].isnan().all())
+    y = x[2:].double() @ w.T
+    within(got[2:], y, linear_tol(x[2:], w, y, F32, inner, group))
