@@ -22,8 +22,8 @@ A handle (rotation, cache, layer) owns tables that its kernels read: keep it as
 long as graphs that captured its calls.
 
 The calls take part in no autograd graph of torch and refuse tensors that
-require a gradient; RotaryEmbedding.backward is the rotation's gradient.  They
-have no counterpart in PyFlame.
+require a gradient or carry a forward-mode tangent; RotaryEmbedding.backward is
+the rotation's gradient.  They have no counterpart in PyFlame.
 """
 from __future__ import annotations
 
@@ -70,6 +70,14 @@ def _check(name: str, t, shape, dtype, device, last_contiguous: bool = True, out
         raise ValueError(f"{name}: an output may not have elements that share memory")
 
 
+def _no_tangents(**tensors) -> None:
+    """Refuses dual tensors of forward-mode differentiation.  Not a matter of a
+    call's kept checks: a tensor has a tangent or not, whatever its shape."""
+    for name, t in tensors.items():
+        if t is not None and _Bound.forward.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name}: carries a tangent, which this call does not (detach it)")
+
+
 def _cuda(t, name: str):
     if t.device.type != "cuda":
         raise ValueError(f"{name}: must be on a CUDA device, not on {t.device}")
@@ -78,17 +86,18 @@ def _cuda(t, name: str):
 
 class _Bound:
     """torch and the library's entry points, looked up once."""
-    torch = device = stream = rope = append = attend = linear = None
+    torch = forward = device = stream = rope = append = attend = linear = None
 
     @classmethod
     def load(cls):
         import torch
+        import torch.autograd.forward_ad as forward
         L = N.lib()
         # what torch.cuda.current_device() and current_stream().cuda_stream read, without their 2 us of Python
         cls.device, cls.stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
         cls.rope, cls.append = L.pfk_rope, L.pfk_paged_append
         cls.attend, cls.linear = L.pfk_paged_attention, L.pfk_linear_w4
-        cls.torch = torch
+        cls.torch, cls.forward = torch, forward
 
 
 def _call(fn, device, *args) -> None:
@@ -242,6 +251,8 @@ class RotaryEmbedding:
         return p, x.is_contiguous(), out is not None and tuple(xs) != tuple(ys) and x.numel() > 0
 
     def _run(self, x, positions, out, inverse: int):
+        if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
+            _no_tangents(x=x, out=out)
         key = (inverse, x.dtype, x.shape, x.stride(), x.get_device(), x.requires_grad, positions.dtype, positions.shape,
                positions.stride(), positions.get_device())
         if out is not None:
@@ -301,6 +312,7 @@ class PagedKVCache:
     def _take(self, k, v):
         import torch
         _Bound.load()
+        _no_tangents(k=k, v=v)
         device = _cuda(k, "k")
         code = _code(k.dtype)
         _check("k", k, (None,) * 4, k.dtype, device, output=True)
@@ -325,6 +337,8 @@ class PagedKVCache:
         head_dim] are rotated by `positions` (int64 [tokens]); returns the
         rotated queries (`q_out`, which may be q, or a new tensor, whose rows
         of skipped tokens are 0).  The slots of one call are distinct."""
+        if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
+            _no_tangents(k=k, v=v, q=q, q_out=q_out)
         key = (k.dtype, k.shape, k.stride(), k.get_device(), k.requires_grad, v.dtype, v.shape, v.stride(), v.get_device(),
                v.requires_grad, slots.dtype, slots.shape, slots.stride(), slots.get_device(),
                None if rotary is None else rotary._kind,
@@ -388,6 +402,8 @@ class PagedKVCache:
         the natural logarithm of the sum of exp(score), float32 [batch,
         q_heads] (-inf for length 0).  `out` may be q.  An infinity or NaN in q
         or in a seen row may make the results that depend on it NaN."""
+        if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
+            _no_tangents(q=q, out=out)
         torch = _Bound.torch
         scale, window = None if scale is None else float(scale), min(int(window), 0x7FFFFFFF)
         key = (scale, window, return_lse, q.dtype, q.shape, q.stride(), q.get_device(), q.requires_grad, block_table.dtype,
@@ -470,6 +486,7 @@ class Linear4bit:
     def __init__(self, packed, scales, zeros=None, bias=None, in_features: Optional[int] = None, group_size: int = 128):
         import torch
         _Bound.load()
+        _no_tangents(scales=scales, bias=bias)
         device = _cuda(packed, "packed")
         if len(packed.shape) != 2 or 0 in packed.shape:
             raise ValueError("packed must be [out_features, (in_features + 1) // 2]")
@@ -545,6 +562,8 @@ class Linear4bit:
     def __call__(self, x, out=None):
         """x: [..., in_features]; `out`, [..., out_features], may not overlap
         it.  Rows at one stride are read where they are."""
+        if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
+            _no_tangents(x=x, out=out)
         key = (x.dtype, x.shape, x.stride(), x.get_device(), x.requires_grad)
         if out is not None:
             key += (out.dtype, out.shape, out.stride(), out.get_device(), out.requires_grad)

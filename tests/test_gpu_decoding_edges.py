@@ -122,3 +122,44 @@ def test_linear4_any_nan_in_fp32(rows, inner, outer, group, bits):
     assert bool(got[:2].isnan().all())
     y = x[2:].double() @ w.T
     within(got[2:], y, linear_tol(x[2:], w, y, F32, inner, group))
+
+
+# ---------------------------------------------------------------------------
+# what a call may not be given
+# ---------------------------------------------------------------------------
+
+def _calls(dtype=F32):
+    """One call of each kind: (name of the tensor, the call with that tensor, the tensor)."""
+    cache, r = pf.PagedKVCache(4, 16, 2, 64, dtype), pf.RotaryEmbedding(64)
+    layer = pf.Linear4bit(*weights(gen(95), 64, 64, 64, True)[:3], group_size=64)
+    x, pos = randn(gen(96), 3, 2, 64, dtype=dtype), torch.arange(3, device="cuda")
+    table, lens = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(x)
+    return x, [
+        ("x", lambda t: r.apply(t, pos)), ("x", lambda t: r.backward(t, pos)), ("out", lambda t: r.apply(x, pos, out=t)),
+        ("k", lambda t: cache.append(t, x, pos)), ("v", lambda t: cache.append(x, t, pos)),
+        ("q", lambda t: cache.append(x, x, pos, q=t)), ("q_out", lambda t: cache.append(out, out, pos, q=x, q_out=t)),
+        ("q", lambda t: cache.attend(t, table, lens)), ("out", lambda t: cache.attend(x, table, lens, out=t)),
+        ("x", lambda t: layer(t)), ("x", lambda t: layer(t.flatten(0, 1)[:2])), ("out", lambda t: layer(x, out=t))]
+
+
+def test_tangents_are_refused():
+    """A forward-mode tangent would be lost in silence: refused at the first call and at a known one."""
+    import torch.autograd.forward_ad as forward
+    x, calls = _calls()
+    for known in (False, True):
+        for name, call in calls:
+            t = torch.empty_like(x)
+            if known:
+                call(t.copy_(x))
+            with forward.dual_level():
+                dual = forward.make_dual(t, torch.ones_like(t))
+                with pytest.raises(RuntimeError, match="tangent"):
+                    call(dual)
+                call(t)  # without a tangent it runs there too
+    r, pos = pf.RotaryEmbedding(64), torch.arange(3, device="cuda")
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: r.apply(t, pos), (x,), (torch.ones_like(x),))
+    bias = torch.zeros(64, device="cuda")
+    with forward.dual_level(), pytest.raises(RuntimeError, match="tangent"):
+        pf.Linear4bit(*weights(gen(95), 64, 64, 64, True)[:3], bias=forward.make_dual(bias, torch.ones_like(bias)), group_size=64)
