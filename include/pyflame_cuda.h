@@ -411,8 +411,8 @@ typedef struct pfk_paged_append_params {
     int64_t k_st, k_sh;
     const void* v;
     int64_t v_st, v_sh;
-    const void* q; /* [tokens][q_heads][head_dim], rotated into q_out (which may be q); NULL: none */
-    void* q_out;
+    const void* q; /* [tokens][q_heads][head_dim], rotated into q_out; NULL: none */
+    void* q_out;   /* may be q (same pointer and strides), not overlap it, k or v otherwise */
     int64_t q_heads, q_st, q_sh, qo_st, qo_sh;
     const int64_t* slots;     /* [tokens]; negative: the token is skipped, its q_out row left as it was */
     const int64_t* positions; /* [tokens]; may be NULL without rotation */
@@ -475,7 +475,7 @@ typedef struct pfk_linear_w4_params {
     int64_t group;
     const void* x; /* [rows][inner] */
     int64_t x_st;
-    void* y; /* [rows][outer] */
+    void* y; /* [rows][outer], not overlapping x or bias */
     int64_t y_st;
     const uint32_t* weight; /* pfk_w4_arrange's, 16-byte aligned */
     const uint32_t* meta;

@@ -347,6 +347,9 @@ void launch_rope(const void* x, void* y, const pfk_rope_params& p, cudaStream_t 
   take_rotary(a, p.rotary, p.head_dim);
   if (p.batch * p.tokens * p.heads == 0) return;
   PFB_CHECK_ARG(x && y, "rope: null pointer");
+  // in place a row is read and written by the same threads
+  PFB_CHECK_ARG(x != y || ((p.batch == 1 || p.x_sb == p.y_sb) && (p.tokens == 1 || p.x_st == p.y_st) && (p.heads == 1 || p.x_sh == p.y_sh)),
+                "rope: y shares x's memory with other strides");
   PFB_CHECK_ARG(p.rotary.rotary_dim == 0 || p.positions, "rope: null positions");
   Rows& r = a.rows[0];
   r.src = x;
@@ -376,6 +379,8 @@ void launch_paged_append(const pfk_paged_append_params& p, cudaStream_t stream) 
   take_rotary(a, p.rotary, p.cache.head_dim);
   if (p.tokens == 0) return;
   PFB_CHECK_ARG(p.k && p.v && p.slots, "paged append: null pointer");
+  PFB_CHECK_ARG(!p.q || p.q != p.q_out || ((p.tokens == 1 || p.q_st == p.qo_st) && (p.q_heads <= 1 || p.q_sh == p.qo_sh)),
+                "paged append: q_out shares q's memory with other strides");
   PFB_CHECK_ARG(p.rotary.rotary_dim == 0 || p.positions, "paged append: null positions");
   Rows& k = a.rows[0];
   k.src = p.k;

@@ -70,6 +70,39 @@ def _check(name: str, t, shape, dtype, device, last_contiguous: bool = True, out
         raise ValueError(f"{name}: an output may not have elements that share memory")
 
 
+def _extent(t) -> int:
+    """Bytes from a tensor's first element to behind its last."""
+    return (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else 0
+
+
+class _Place:
+    """The places of a tensor's elements, for numpy (which reads none of them)."""
+
+    def __init__(self, t):
+        size = t.element_size()
+        self.__array_interface__ = {"version": 3, "typestr": f"|V{size}", "data": (t.data_ptr(), False), "shape": tuple(t.shape),
+                                    "strides": tuple(st * size for st in t.stride())}
+
+
+def _share(a, b) -> bool:
+    """Whether two tensors have memory in common: exactly, also where rows of
+    one lie between rows of the other."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    try:
+        return np.shares_memory(np.asarray(_Place(a)), np.asarray(_Place(b)), max_work=1 << 20)
+    except np.exceptions.TooHardError:  # strides that no slicing gives
+        return True
+
+
+def _apart(name: str, out, **others) -> None:
+    """Refuses an output that shares memory with one of the others.  Callers
+    ask where the extents of the two meet, which is not often."""
+    for other, t in others.items():
+        if _share(out, t):
+            raise ValueError(f"{name}: shares memory with {other.replace('_', ' ')}")
+
+
 def _no_tangents(**tensors) -> None:
     """Refuses dual tensors of forward-mode differentiation.  Not a matter of a
     call's kept checks: a tensor has a tangent or not, whatever its shape."""
@@ -110,6 +143,11 @@ def _call(fn, device, *args) -> None:
             rc = fn(*args, _Bound.stream(index))
     if rc:
         N.check(rc)
+
+
+def _other_strides(a, b) -> bool:
+    """Of two tensors of one shape: whether the same start means other places."""
+    return any(n > 1 and s != r for n, s, r in zip(a.shape, a.stride(), b.stride())) and a.numel() > 0
 
 
 def _model(t, shape, dtype):
@@ -248,7 +286,9 @@ class RotaryEmbedding:
         ys = torch.empty(x.shape, device="meta").stride() if out is None else out.stride()
         p = N.RopeParamsC(code, inverse, batch, tokens, heads, self.head_dim, xs[0] if dims == 4 else 0, xs[-3], xs[-2],
                           ys[0] if dims == 4 else 0, ys[-3], ys[-2], None, p_sb, p_st, self._c)
-        return p, x.is_contiguous(), out is not None and tuple(xs) != tuple(ys) and x.numel() > 0
+        if out is None:  # a new one meets nothing
+            return p, x.is_contiguous(), 0, False
+        return p, _extent(out), _extent(x), _other_strides(x, out)
 
     def _run(self, x, positions, out, inverse: int):
         if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
@@ -260,17 +300,22 @@ class RotaryEmbedding:
         plan = self._plans.get(key) or self._plans.keep(key, self._plan(x, positions, out, inverse), x, out)
         if out is None:
             out = _Bound.torch.empty_like(x) if plan[1] else x.new_empty(x.shape)
-        elif plan[2] and out.data_ptr() == x.data_ptr():
-            raise ValueError("out: shares x's memory with other strides")
+        at, to = x.data_ptr(), out.data_ptr()
+        if at == to:
+            if plan[3]:
+                raise ValueError("out: shares x's memory with other strides")
+        elif plan[2] and to < at + plan[2] and at < to + plan[1]:
+            _apart("out", out, x=x)
         p = N.RopeParamsC.from_buffer_copy(plan[0])
         p.positions = positions.data_ptr()
-        _call(_Bound.rope, self.device, x.data_ptr(), out.data_ptr(), C.byref(p))
+        _call(_Bound.rope, self.device, at, to, C.byref(p))
         return out
 
     def apply(self, x, positions, out=None):
         """x rotated.  x: [tokens, heads, head_dim] or [batch, tokens, heads,
         head_dim], any strides with a contiguous head; positions: int64
-        [tokens] (shared by a batch) or [batch, tokens].  `out` may be x."""
+        [tokens] (shared by a batch) or [batch, tokens].  `out` may be x, or
+        shares no memory with it."""
         return self._run(x, positions, out, 0)
 
     def backward(self, dy, positions, out=None):
@@ -304,7 +349,8 @@ class PagedKVCache:
     def from_tensors(cls, k, v) -> "PagedKVCache":
         """A cache in the caller's tensors, [num_pages, page_size, num_heads,
         head_dim] with the same strides and a contiguous head (heads stored
-        before tokens: the permuted view)."""
+        before tokens: the permuted view).  Where they share memory, the cache
+        can be attended to, not appended to."""
         self = cls.__new__(cls)
         self._take(k, v)
         return self
@@ -327,6 +373,9 @@ class PagedKVCache:
         self.num_pages, self.page_size, self.num_heads, self.head_dim = k.shape
         self._err = torch.zeros(1, dtype=torch.int32, device=device)
         self._c = N.PagedCacheC(code, k.data_ptr(), v.data_ptr(), *k.shape, *k.stride()[:3], self._err.data_ptr())
+        # keys, values and what may lie between them
+        self._start, self._end = min(k.data_ptr(), v.data_ptr()), max(t.data_ptr() + _extent(t) for t in (k, v))
+        self._one_memory = _share(k, v)
         self._plans = _Plans()
         self._no_rotary = N.RotaryC(None, 0, 0, 1.0)
 
@@ -335,8 +384,10 @@ class PagedKVCache:
         (int64 [tokens], page * page_size + offset; negative: the token is
         skipped).  With `rotary`, keys and queries q [tokens, q_heads,
         head_dim] are rotated by `positions` (int64 [tokens]); returns the
-        rotated queries (`q_out`, which may be q, or a new tensor, whose rows
-        of skipped tokens are 0).  The slots of one call are distinct."""
+        rotated queries (`q_out`, which may be q and otherwise shares no memory
+        with the inputs, or a new tensor, whose rows of skipped tokens are 0).
+        The slots of one call are distinct; k, v and q may be rows of the
+        cache, if the call's slots are not among them."""
         if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
             _no_tangents(k=k, v=v, q=q, q_out=q_out)
         key = (k.dtype, k.shape, k.stride(), k.get_device(), k.requires_grad, v.dtype, v.shape, v.stride(), v.get_device(),
@@ -348,14 +399,24 @@ class PagedKVCache:
         plan = self._plans.get(key) or self._plans.keep(
             key, self._append_plan(k, v, slots, positions, rotary, q, q_out), k, v, q, q_out)
         p = N.PagedAppendParamsC.from_buffer_copy(plan[0])
-        p.k, p.v, p.slots = k.data_ptr(), v.data_ptr(), slots.data_ptr()
+        p.k, p.v, p.slots = at_k, at_v, _ = k.data_ptr(), v.data_ptr(), slots.data_ptr()
         if rotary is not None:
             p.positions, p.rotary = positions.data_ptr(), rotary._c
         if q is not None:
             if q_out is None:
                 q_out = q.new_zeros(q.shape)
-            elif plan[1] and q_out.data_ptr() == q.data_ptr():
-                raise ValueError("q_out: shares q's memory with other strides")
+            else:
+                size_q, size_k, size_v, size, other = plan[1]
+                at, to = q.data_ptr(), q_out.data_ptr()
+                end = to + size
+                if at == to:
+                    if other:
+                        raise ValueError("q_out: shares q's memory with other strides")
+                elif to < at + size_q and at < end:
+                    _apart("q_out", q_out, q=q)
+                if (to < at_k + size_k and at_k < end or to < at_v + size_v and at_v < end
+                        or to < self._end and self._start < end):
+                    _apart("q_out", q_out, k=k, v=v, the_keys=self.k, the_values=self.v)
             if p.q_heads:
                 p.q, p.q_out = q.data_ptr(), q_out.data_ptr()
         _call(_Bound.append, self.device, C.byref(p))
@@ -364,6 +425,8 @@ class PagedKVCache:
     def _append_plan(self, k, v, slots, positions, rotary, q, q_out):
         import torch
         n, h, d = len(k), self.num_heads, self.head_dim
+        if self._one_memory:
+            raise ValueError("the cache's keys share memory with its values")
         _check("k", k, (n, h, d), self.dtype, self.device)
         _check("v", v, (n, h, d), self.dtype, self.device)
         _check("slots", slots, (n,), torch.int64, self.device)
@@ -373,7 +436,7 @@ class PagedKVCache:
             if rotary.head_dim != d or rotary.device != self.device:
                 raise ValueError("rotary: is for another head_dim or device")
             _check("positions", positions, (n,), torch.int64, self.device)
-        ks, vs, other = k.stride(), v.stride(), False
+        ks, vs, outputs = k.stride(), v.stride(), None
         p = N.PagedAppendParamsC(self._c, n, None, ks[0], ks[1], None, vs[0], vs[1])
         p.rotary = self._no_rotary
         if q is not None:
@@ -382,13 +445,13 @@ class PagedKVCache:
             if q_out is not None:
                 _check("q_out", q_out, q.shape, self.dtype, self.device, output=True)
                 os = q_out.stride()
-                other = tuple(qs) != tuple(os) and q.numel() > 0
+                outputs = _extent(q), _extent(k), _extent(v), _extent(q_out), _other_strides(q, q_out)
             else:
                 os = torch.empty(q.shape, device="meta").stride()
             p.q_heads, p.q_st, p.q_sh, p.qo_st, p.qo_sh = q.shape[1], qs[0], qs[1], os[0], os[1]
         elif q_out is not None:
             raise ValueError("q_out without q")
-        return p, other
+        return p, outputs
 
     def attend(self, q, block_table, seq_lens, scale: Optional[float] = None, window: int = 0, out=None,
                return_lse: bool = False):
@@ -400,7 +463,8 @@ class PagedKVCache:
         multiplies the scores; `window` > 0: only a sequence's last `window`
         tokens are seen.  A sequence of length 0 gives 0.  With return_lse also
         the natural logarithm of the sum of exp(score), float32 [batch,
-        q_heads] (-inf for length 0).  `out` may be q.  An infinity or NaN in q
+        q_heads] (-inf for length 0).  `out` may be q and otherwise shares no
+        memory with it or the cache.  An infinity or NaN in q
         or in a seen row may make the results that depend on it NaN."""
         if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
             _no_tangents(q=q, out=out)
@@ -415,10 +479,18 @@ class PagedKVCache:
             key, self._attend_plan(q, block_table, seq_lens, scale, window, out, return_lse), q, out)
         if out is None:
             out = torch.empty_like(q) if plan[1] else q.new_empty(q.shape)
-        elif plan[4] and out.data_ptr() == q.data_ptr():
-            raise ValueError("out: shares q's memory with other strides")
+        at, to = q.data_ptr(), out.data_ptr()
+        if plan[4] is not None:
+            size_q, size, other = plan[4]
+            if at == to:
+                if other:
+                    raise ValueError("out: shares q's memory with other strides")
+            elif to < at + size_q and at < to + size:
+                _apart("out", out, q=q)
+            if to < self._end and self._start < to + size:
+                _apart("out", out, the_keys=self.k, the_values=self.v)
         p = N.PagedAttentionParamsC.from_buffer_copy(plan[0])
-        p.q, p.out, p.block_table, p.seq_lens = q.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
+        p.q, p.out, p.block_table, p.seq_lens = at, to, block_table.data_ptr(), seq_lens.data_ptr()
         lse = None
         if return_lse:
             lse = torch.empty_like(plan[3]) if plan[3] is not None else q.new_empty(q.shape[:2], dtype=torch.float32)
@@ -454,7 +526,7 @@ class PagedKVCache:
             N.check(N.lib().pfk_paged_attention_workspace(C.byref(p), C.byref(size)))
         p.workspace_bytes = size.value
         return (p, q.is_contiguous(), size.value, _model(q, (batch, heads), torch.float32) if return_lse else None,
-                tuple(qs) != tuple(os) and q.numel() > 0)
+                None if out is None else (_extent(q), _extent(out), _other_strides(q, out)))
 
     def check(self) -> None:
         """Wait for the device and raise PfcError if a call met a slot, page
@@ -510,6 +582,7 @@ class Linear4bit:
             bias = bias.contiguous()
         self.in_features, self.out_features, self.group_size = k, n, int(group_size)
         self.device, self.scales, self.zeros, self.bias = device, scales.contiguous(), zeros, bias
+        self._bias_size = 0 if bias is None else _extent(bias)
         blocks, row_blocks = -(-k // 128), -(-n // 16)
         self.weight = torch.empty((row_blocks, blocks, 256), dtype=torch.int32, device=device)
         self.meta = torch.empty((row_blocks, blocks * (128 // group_size) if group_size < 128 else groups, 16), dtype=torch.int32,
@@ -560,8 +633,8 @@ class Linear4bit:
         return cls(packed, scales, None if symmetric else zeros.to(torch.uint8), bias, k, group_size)
 
     def __call__(self, x, out=None):
-        """x: [..., in_features]; `out`, [..., out_features], may not overlap
-        it.  Rows at one stride are read where they are."""
+        """x: [..., in_features]; `out`, [..., out_features], shares no memory
+        with it.  Rows at one stride are read where they are."""
         if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
             _no_tangents(x=x, out=out)
         key = (x.dtype, x.shape, x.stride(), x.get_device(), x.requires_grad)
@@ -570,12 +643,14 @@ class Linear4bit:
         plan = self._plans.get(key) or self._plans.keep(key, self._plan(x, out), x, out)
         if plan[2]:
             x = x.reshape(-1, self.in_features)
-        if out is not None and out.data_ptr() == x.data_ptr() and x.numel():
-            raise ValueError("out: may not be x")
         if out is None:
             out = _Bound.torch.empty_like(plan[3]) if plan[3] is not None else x.new_empty(plan[1])
+        elif x.data_ptr() < out.data_ptr() + plan[4] and out.data_ptr() < x.data_ptr() + plan[5]:
+            _apart("out", out, x=x)
         p = N.LinearW4ParamsC.from_buffer_copy(plan[0])
         p.x, p.y = x.data_ptr(), out.data_ptr()
+        if self.bias is not None and p.y < p.bias + self._bias_size and p.bias < p.y + plan[4]:
+            _apart("out", out, the_bias=self.bias)
         _call(_Bound.linear, self.device, C.byref(p))
         return out
 
@@ -599,4 +674,5 @@ class Linear4bit:
         p = N.LinearW4ParamsC(code, rows.shape[0], self.in_features, self.out_features, self.group_size, None,
                               rows.stride(0), None, y_st, self.weight.data_ptr(), self.meta.data_ptr(),
                               None if self.bias is None else self.bias.data_ptr())
-        return p, shape, len(x.shape) != 2, _model(x, shape, x.dtype) if out is None else None
+        return (p, shape, len(x.shape) != 2, _model(x, shape, x.dtype) if out is None else None,
+                0 if out is None else _extent(out), _extent(rows))

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import pyflame_b200 as pf
-from tests.test_gpu_decoding import BF16, F16, F32, HALF, gen, linear_tol, randn, weights, within
+from tests.test_gpu_decoding import BF16, F16, F32, HALF, gen, linear_tol, make_batch, randn, weights, within
 
 pytestmark = pytest.mark.gpu
 
@@ -163,3 +163,63 @@ def test_tangents_are_refused():
     bias = torch.zeros(64, device="cuda")
     with forward.dual_level(), pytest.raises(RuntimeError, match="tangent"):
         pf.Linear4bit(*weights(gen(95), 64, 64, 64, True)[:3], bias=forward.make_dual(bias, torch.ones_like(bias)), group_size=64)
+
+
+def test_overlapping_outputs_are_refused():
+    cache, r = pf.PagedKVCache(4, 16, 2, 64), pf.RotaryEmbedding(64)
+    layer = pf.Linear4bit(*weights(gen(95), 64, 64, 64, True)[:3], group_size=64)
+    pos = torch.arange(3, device="cuda")
+    table, lens = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    buf = torch.zeros(1000, device="cuda")
+    at = lambda o: buf[o:o + 384].view(3, 2, 64)
+    wide = torch.zeros(3, 6, 64, device="cuda")  # heads of one projection, interleaved in memory with their neighbours
+    other = torch.zeros(3, 2, 64, device="cuda")
+    for _ in range(2):  # checked for the first time, and as a known call
+        for call in (
+                lambda: r.apply(at(0), pos, out=at(4)), lambda: r.backward(at(64), pos, out=at(0)),
+                lambda: r.apply(wide[:, 0:2], pos, out=wide[:, 1:3]),
+                lambda: cache.append(other, other, pos, q=at(0), q_out=at(383)),
+                lambda: cache.append(at(0), other, pos, q=other, q_out=at(0)),
+                lambda: cache.append(other, at(0), pos, q=other, q_out=at(128)),
+                lambda: cache.append(wide[:, 2:4], other, pos, q=wide[:, :2], q_out=wide[:, 1:3]),
+                lambda: cache.attend(at(0), table, lens, out=at(64)), lambda: cache.attend(wide[:, 2:4], table, lens, out=wide[:, 3:5]),
+                lambda: cache.attend(other, table, lens, out=cache.v[:3, 0]), lambda: cache.attend(other, table, lens, out=cache.k[1:, 3]),
+                lambda: layer(buf[:128].view(2, 64), out=buf[127:255].view(2, 64)),
+                lambda: layer(buf[64:192].view(2, 64), out=buf[:128].view(2, 64))):
+            with pytest.raises(ValueError, match="memory"):
+                call()
+    for shared in (pf.PagedKVCache.from_tensors(cache.k, cache.k), pf.PagedKVCache.from_tensors(cache.k[:3], cache.k[1:])):
+        shared.attend(other, table, lens)
+        with pytest.raises(ValueError, match="memory"):
+            shared.append(other, other, pos)
+    bias = torch.zeros(64, device="cuda")
+    biased = pf.Linear4bit(*weights(gen(95), 64, 64, 64, True)[:3], bias=bias, group_size=64)
+    with pytest.raises(ValueError, match="memory"):
+        biased(torch.zeros(1, 64, device="cuda"), out=bias[None])
+
+
+def test_neighbouring_outputs_are_taken():
+    """Outputs between the inputs' rows in one buffer, and in place of an input, are no overlap."""
+    g = gen(97)
+    r, pos = pf.RotaryEmbedding(64), torch.arange(3, device="cuda")
+    layer = pf.Linear4bit(*weights(g, 64, 64, 64, True)[:3], group_size=64)
+    cache, q, table, lens = make_batch(g, [20, 0, 33], 16, 2, 2, 64, F32)
+    wide = torch.zeros(3, 8, 64, device="cuda")
+    for run in (lambda x, out: r.apply(x, pos, out=out), lambda x, out: cache.attend(x, table, lens, out=out),
+                lambda x, out: cache.append(wide[:, 4:6], wide[:, 6:8], torch.full((3,), -1, device="cuda"), q=x, q_out=out)):
+        for x, out in ((wide[:, 0:2], wide[:, 2:4]), (wide[:, 2:4], wide[:, 0:2]), (wide[:, 1:3], wide[:, 1:3]), (wide[:, 0:4:2], wide[:, 1:4:2])):
+            x.copy_(q)
+            out_of = run(q.clone(), None)
+            keep = out.clone()
+            run(x, out)
+            want = out_of if bool((out_of != 0).any()) else keep  # skipped tokens: the rows stay
+            assert torch.equal(out, want)
+    both = torch.zeros(2, 4, 16, 2, 64, device="cuda").transpose(0, 1)  # keys and values of a page next to each other
+    k = randn(g, 3, 2, 64)
+    pf.PagedKVCache.from_tensors(both[:, 0], both[:, 1]).append(k, -k, torch.arange(3, device="cuda") * 20)
+    for i in range(3):
+        assert torch.equal(both[i * 20 // 16, 0, i * 20 % 16], k[i]) and torch.equal(both[i * 20 // 16, 1, i * 20 % 16], -k[i])
+    rows = torch.zeros(5, 192, device="cuda")
+    rows[:, :64] = randn(g, 5, 64)
+    want = layer(rows[:, :64].clone())
+    assert torch.equal(layer(rows[:, :64], out=rows[:, 64:128]), want) and torch.equal(layer(rows[::2, :64], out=rows[::2, 128:]), want[::2])
