@@ -65,3 +65,13 @@ def test_which_tensors_share_memory():
                 decoding._apart("out", a, the_other=b)
         else:
             decoding._apart("out", a, the_other=b)
+
+
+@pytest.mark.parametrize("shape", [(5,), (1, 7), (7, 1), (4, 1, 5), (0, 9), (2, 3, 1, 8), (1, 1, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_outputs_like_one_element(shape, dtype):
+    memory = torch.zeros((2, 3), dtype=torch.int32)
+    model = decoding._model(memory, shape, dtype)
+    out = torch.empty_like(model)
+    assert model.data_ptr() == memory.data_ptr() and out.shape == shape and out.dtype == dtype and out.is_contiguous()
+    assert out.untyped_storage().nbytes() == out.numel() * out.element_size()

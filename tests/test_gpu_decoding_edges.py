@@ -223,3 +223,23 @@ def test_neighbouring_outputs_are_taken():
     rows[:, :64] = randn(g, 5, 64)
     want = layer(rows[:, :64].clone())
     assert torch.equal(layer(rows[:, :64], out=rows[:, 64:128]), want) and torch.equal(layer(rows[::2, :64], out=rows[::2, 128:]), want[::2])
+
+
+def test_known_calls_hold_no_memory():
+    """What a handle keeps of the calls it knows is of no consequence beside them: no memory for each shape."""
+    g = gen(98)
+    layer = pf.Linear4bit(*weights(g, 1024, 64, 64, True)[:3], group_size=64)
+    cache, q, table, lens = make_batch(g, [1] * 60, 16, 2, 64, 64, F32)
+    r = pf.RotaryEmbedding(64)
+
+    def calls():
+        for n in range(1, 60):
+            layer(torch.zeros(n, 64, device="cuda"))
+            cache.attend(q[:n], table[:n], lens[:n], return_lse=True)
+            r.apply(q[:n], lens[:n].long())
+
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    calls()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() <= before
