@@ -535,6 +535,8 @@ class PagedKVCache:
         code = int(self._err.item())
         if code:
             self._err.zero_()
+            # finished here: later, it would clear the flag of a call on another stream
+            _Bound.torch.cuda.synchronize(self.device)
             raise N.PfcError(code, "a call met a slot, page or length outside the paged cache")
 
 

@@ -1,10 +1,11 @@
 """Token generation without a GPU: tangents, which tensors share memory and are
-refused for it, and what handles keep."""
+refused for it, what handles keep, and the order of a cache's check."""
 import ctypes as C
 
 import pytest
 import torch
 
+import pyflame_b200 as pf
 from pyflame_b200 import decoding
 from tests.test_cpu_decoding import FAKE, cache, refused, rotary
 
@@ -75,3 +76,27 @@ def test_outputs_like_one_element(shape, dtype):
     out = torch.empty_like(model)
     assert model.untyped_storage().data_ptr() == memory.untyped_storage().data_ptr() and out.shape == shape and out.dtype == dtype and out.is_contiguous()
     assert out.untyped_storage().nbytes() == out.numel() * out.element_size()
+
+
+def test_check_leaves_no_write_in_flight(monkeypatch):
+    """The flag is cleared before check() returns: cleared later, it would take the error of a call on another stream."""
+    did = []
+
+    class Flag:
+        def item(self):
+            did.append("read")
+            return -1
+
+        def zero_(self):
+            did.append("clear")
+
+    class Torch:
+        class cuda:
+            synchronize = staticmethod(lambda device: did.append("wait"))
+
+    monkeypatch.setattr(decoding._Bound, "torch", Torch)
+    c = pf.PagedKVCache.__new__(pf.PagedKVCache)
+    c._err, c.device = Flag(), "cuda:0"
+    with pytest.raises(pf._native.PfcError):
+        c.check()
+    assert did == ["wait", "read", "clear", "wait"]
