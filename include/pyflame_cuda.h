@@ -214,8 +214,10 @@ PFC_API int pfc_executor_execute(pfc_executor* ex, pfc_graph* g, const uint64_t*
 /* Device-resident variant: the data of the INPUT/CONSTANT nodes listed in
  * `input_ids` is read from device pointers `in_dev` (dense row-major) instead
  * of host payloads, and outputs are written to device pointers `out_dev`.
- * Work is issued on `stream` (a cudaStream_t; NULL = the executor's stream)
- * and the call returns without synchronising. */
+ * Work is issued on `stream` (a cudaStream_t; NULL = the executor's stream,
+ * which is not ordered with the default one; cudaStreamLegacy names that)
+ * and the call returns without synchronising.  Calls of one executor share
+ * its working memory: those on several streams are ordered by the caller. */
 PFC_API int pfc_executor_execute_device(pfc_executor* ex, pfc_graph* g, const uint64_t* input_ids,
                                 int n_inputs, const void* const* in_dev,
                                 const uint64_t* output_ids, int n_outputs,

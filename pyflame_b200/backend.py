@@ -294,11 +294,20 @@ class CudaExecutor:
         return res
 
     def execute_device(self, graph: Graph, inputs: Dict[int, int], output_ids: Sequence[int],
-                       outputs: Sequence[int], stream: int = 0) -> ExecutionResult:
+                       outputs: Sequence[int], stream=0) -> ExecutionResult:
         """Device-resident execution: `inputs` maps leaf node id -> device
         pointer (dense row-major); `outputs` are device pointers for
-        `output_ids`.  Issued on `stream` (0 = the executor's own stream) and
-        not synchronised.  Raises on failure."""
+        `output_ids`.  Issued on `stream` and not synchronised.  Raises on
+        failure.
+
+        `stream` is a torch stream or a CUDA stream's handle.  0 is the
+        executor's own stream, which is ordered with no other: torch's default
+        stream, whose handle is 0 too, is torch.cuda.current_stream() itself
+        (or 1, its name for CUDA).  An executor's calls share its working
+        memory: those on several streams have to be ordered by the caller, and
+        finished before close()."""
+        if hasattr(stream, "cuda_stream"):
+            stream = stream.cuda_stream or 1
         # a loop of calls with the same arguments (serving, the bench) reuses
         # the ctypes argument block of the previous call
         key = (id(graph), graph.version, tuple(inputs.items()), tuple(output_ids), tuple(outputs), stream)

@@ -682,15 +682,17 @@ int64_t CudaExecutor::run_steps(PlanEntry& pe, const std::vector<void*>& ptrs, c
     }
     cudaGraphExec_t gexec = nullptr;
     cudaGraph_t graph;
-    PFB_CUDA(cudaStreamBeginCapture(s, cudaStreamCaptureModeThreadLocal));
+    // the legacy default stream cannot be captured; its calls' graph is taken on the executor's stream
+    const cudaStream_t on = s == cudaStreamLegacy ? stream_ : s;
+    PFB_CUDA(cudaStreamBeginCapture(on, cudaStreamCaptureModeThreadLocal));
     try {
       for (size_t i = 0; i < P.steps.size(); ++i)
-        if (!P.steps[i].once) launch_step(pe, i, ptrs, s);
+        if (!P.steps[i].once) launch_step(pe, i, ptrs, on);
     } catch (...) {
-      cudaStreamEndCapture(s, &graph);
+      cudaStreamEndCapture(on, &graph);
       throw;
     }
-    PFB_CUDA(cudaStreamEndCapture(s, &graph));
+    PFB_CUDA(cudaStreamEndCapture(on, &graph));
     cudaError_t e = cudaGraphInstantiate(&gexec, graph, 0);
     cudaGraphDestroy(graph);
     if (e != cudaSuccess) {

@@ -1,8 +1,7 @@
 """Token generation over a paged key-value cache.
 
-The steps of a decoder layer for new tokens, on CUDA tensors of torch (the
-memory that `CudaExecutor.execute_device` also takes), in float32, float16 or
-bfloat16:
+The steps of a decoder layer for new tokens, on CUDA tensors of torch, in
+float32, float16 or bfloat16:
 
   Linear4bit        x W^T (+ bias) with 4-bit weights and group scales
   RotaryEmbedding   rotary positions of queries and keys, and their gradient
@@ -17,6 +16,10 @@ are checked on the host; a wrong one raises ValueError or TypeError, a size or
 layout that the kernels do not take PfcError.  Page numbers, slots and lengths
 are device data: a kernel that meets a bad one skips it and sets the cache's
 error flag, which `PagedKVCache.check()` raises.
+
+A graph between them runs on the same memory by `CudaExecutor.execute_device`,
+in their order if its `stream` is torch.cuda.current_stream() (without one it
+runs on the executor's own stream, which waits for no other).
 
 A handle (rotation, cache, layer) owns tables that its kernels read: keep it as
 long as graphs that captured its calls.

@@ -1,5 +1,5 @@
 """Token-generation operators on the GPU where precision, ranges and memory
-come to an edge.
+come to an edge, and next to the graph executor.
 """
 import numpy as np
 import pytest
@@ -243,3 +243,38 @@ def test_known_calls_hold_no_memory():
     calls()
     torch.cuda.synchronize()
     assert torch.cuda.memory_allocated() <= before
+
+
+# ---------------------------------------------------------------------------
+# next to the graph executor
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["default", "side"])
+def test_executor_on_torchs_stream(kind):
+    """A graph between two of these calls, all in the order of torch's current stream (its default one has the handle 0,
+    which names the executor's own stream). Long work goes before each, so that what does not wait reads old data."""
+    g = gen(99)
+    layer = pf.Linear4bit(*weights(g, 64, 256, 64, True, size=0.1)[:3], group_size=64)
+    rotary, pos = pf.RotaryEmbedding(64), torch.arange(8, device="cuda")
+    pf.reset_graph()
+    shape = [8, 1, 64]
+    a = pf.from_numpy(np.random.default_rng(0).standard_normal(shape, np.float32))
+    y = pf.relu(a) * pf.from_numpy(np.full(shape, 2.0, np.float32))
+    graph, ids, leaf = y.graph(), [y.node().id()], a.node().id()
+    ex = pf.CudaExecutor(pf.CudaExecutor.Config())
+    stream = torch.cuda.current_stream() if kind == "default" else torch.cuda.Stream()
+    hidden, doubled = torch.zeros(8, 64, device="cuda"), torch.zeros(8, 1, 64, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for i in range(5):  # the first as a plan is made, the later ones as a replayed graph
+            x = randn(g, 8, 256)
+            want = rotary.apply(torch.relu(layer(x)).view(8, 1, 64) * 2, pos)
+            hidden.zero_()
+            doubled.zero_()
+            torch.cuda._sleep(20_000_000)
+            layer(x, out=hidden)
+            ex.execute_device(graph, {leaf: hidden.data_ptr()}, ids, [doubled.data_ptr()], stream=torch.cuda.current_stream())
+            got = rotary.apply(doubled, pos)
+            assert torch.equal(got, want), i
+    torch.cuda.synchronize()
+    ex.close()
