@@ -302,6 +302,8 @@ CudaExecutor::PlanEntry& CudaExecutor::prepare(Graph& g, const std::vector<uint6
       pe.tail = pool_->allocate(tail_ws_bytes() + kTailCounters * sizeof(unsigned), stream_);
       PFB_CUDA(cudaMemsetAsync((char*)pe.tail + tail_ws_bytes(), 0, kTailCounters * sizeof(unsigned), stream_));
     }
+    // the plan may run on a caller's stream: its memory is there, and its counters are 0, before any launch
+    PFB_CUDA(cudaStreamSynchronize(stream_));
     it = plans_.emplace(key, std::move(pe)).first;
   } else {
     // refresh the splat values seen by this call (the structure is unchanged)
