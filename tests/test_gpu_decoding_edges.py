@@ -6,7 +6,8 @@ import pytest
 import torch
 
 import pyflame_b200 as pf
-from tests.test_gpu_decoding import BF16, F16, F32, HALF, gen, linear_tol, make_batch, randn, weights, within
+from tests.test_gpu_decoding import (BF16, F16, F32, HALF, TYPES, attention, gen, linear_tol, make_batch, randn, weights,
+                                     within)
 
 pytestmark = pytest.mark.gpu
 
@@ -57,6 +58,22 @@ def test_attend_long_rows_keep_their_precision(dtype, q_heads, dim):
     for i in range(0, rows, 37):
         want = torch.softmax(q[i].double() @ k.T * dim ** -0.5, -1) @ v
         within(got[i], want, HALF[dtype] * want.abs() + 2.0 ** -18, f"row {i}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,heads,q_heads,dim,page,window", [
+    (24, 1, 4, 64, 16, 777), (24, 2, 8, 128, 13, 1500), (10, 2, 32, 128, 32, 4999), (20, 1, 1, 256, 16, 333), (24, 2, 10, 80, 1, 601)])
+def test_attend_windows_shared_by_ctas(dtype, rows, heads, q_heads, dim, page, window):
+    """Windows of many tiles, that begin inside a tile and inside a page, with more units than clusters take: the work list,
+    whose units several CTAs share."""
+    g = gen(71)
+    lens = [(i * 1397) % 6001 for i in range(rows)]
+    cache, q, table, n = make_batch(g, lens, page, heads, q_heads, dim, dtype)
+    out, lse, tol, lse_tol = attention(cache, q, table, n, window)
+    got, got_lse = cache.attend(q, table, n, window=window, return_lse=True)
+    within(got, out, tol, "out")
+    within(got_lse, lse, lse_tol, "lse")
+    cache.check()
 
 
 # ---------------------------------------------------------------------------
