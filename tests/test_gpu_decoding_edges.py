@@ -6,8 +6,8 @@ import pytest
 import torch
 
 import pyflame_b200 as pf
-from tests.test_gpu_decoding import (BF16, F16, F32, HALF, TYPES, attention, gen, linear_tol, make_batch, randn, weights,
-                                     within)
+from tests.test_gpu_decoding import (BF16, F16, F32, HALF, TYPES, Layer, attention, gen, linear_tol, make_batch, randn, turn,
+                                     turn_tol, weights, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -31,6 +31,7 @@ def test_rope_cosines_next_to_quarter_turns(w):
     for got, sign in ((r.apply(x, pos), 1), (r.backward(x, pos), -1)):
         want = torch.stack((torch.stack((c, sign * s), -1), torch.stack((-sign * s, c), -1)), 1)
         within(got, want, 2.0 ** -22 * want.abs())
+    assert torch.equal(r.apply(x, -pos), r.backward(x, pos))
 
 
 # ---------------------------------------------------------------------------
@@ -139,6 +140,62 @@ def test_linear4_any_nan_in_fp32(rows, inner, outer, group, bits):
     assert bool(got[:2].isnan().all())
     y = x[2:].double() @ w.T
     within(got[2:], y, linear_tol(x[2:], w, y, F32, inner, group))
+
+
+# ---------------------------------------------------------------------------
+# a layer's calls, each against 64 bits
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_decoding_steps_call_by_call(dtype):
+    """Three sequences over 20 steps, one of them joining late: every call of a step against 64 bits from what the call
+    before it gave, and tolerances that a swapped row or a wrong slot, page, length or position cannot pass."""
+    g = gen(90)
+    layer = Layer(g, dtype)
+    cache, rotary = layer.cache, layer.rotary
+    table = torch.randperm(39, generator=g, device="cuda")[:12].view(3, 4).to(torch.int32)
+    stored = [[] for _ in range(3)]  # the keys and values that each sequence's calls were given, rotated in 64 bits
+
+    def close(got, want, tol, what):
+        within(got, want, tol, what)
+        if bool((want != 0).any()):
+            assert float(tol.double().mean()) < 0.02 * float(want.abs().mean()), (what, "a loose tolerance")
+
+    for step in range(20):
+        x = randn(g, 3, 256, dtype=dtype)
+        pos = torch.tensor([step, step, step - 10], device="cuda")
+        live = pos >= 0
+        at = pos.clamp(min=0)
+        slots = torch.where(live, table[torch.arange(3), at // 8].long() * 8 + at % 8, -1)
+        lens = (pos + 1).clamp(min=0).to(torch.int32)
+        qkv = layer.qkv(x)
+        w = layer.qkv_w[3]
+        y = x.double() @ w.T
+        close(qkv, y, linear_tol(x, w, y, dtype, 256, 64), f"step {step}: qkv")
+        q, k, v = qkv.unflatten(1, (-1, 32)).split([8, 2, 2], 1)
+        turned = cache.append(k, v, slots, positions=pos, rotary=rotary, q=q)
+        for got, of, heads in ((turned, q, 8), (cache.k.flatten(0, 1)[slots.clamp(min=0)], k, 2)):
+            want, mag = turn(of, pos, rotary)
+            close(got[live], want[live], turn_tol(want, mag, dtype)[live], f"step {step}: rotated")
+        assert torch.equal(cache.v.flatten(0, 1)[slots[live]], v[live]) and bool((turned[~live] == 0).all())
+        out = cache.attend(turned, table, lens)
+        want, _, tol, _ = attention(cache, turned, table, lens)
+        close(out, want, tol, f"step {step}: attention")
+        # the cache itself holds what the calls were given, in the order of the positions
+        kk = turn(k, pos, rotary)[0]
+        for b in range(3):
+            if bool(live[b]):
+                stored[b].append((kk[b], v[b].double()))
+                n = len(stored[b])
+                place = table[b, torch.arange(n, device="cuda") // 8].long() * 8 + torch.arange(n, device="cuda") % 8
+                want = torch.stack([c[0] for c in stored[b]])
+                within(cache.k.flatten(0, 1)[place], want, (HALF[dtype] + 2.0 ** -20) * (want.abs() + want.abs().amax()), "keys")
+                assert torch.equal(cache.v.flatten(0, 1)[place].double(), torch.stack([c[1] for c in stored[b]]))
+        got = layer.out(out.flatten(1))
+        w = layer.out_w[3]
+        y = out.flatten(1).double() @ w.T
+        close(got, y, linear_tol(out.flatten(1), w, y, dtype, 256, 32), f"step {step}: out")
+    cache.check()
 
 
 # ---------------------------------------------------------------------------
