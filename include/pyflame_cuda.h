@@ -421,8 +421,9 @@ typedef struct pfk_paged_append_params {
     pfk_rotary rotary;        /* of k and q; rotary_dim 0: copied as they are */
 } pfk_paged_append_params;
 /* Stores rotated keys, values as they are, and rotated queries in one pass.
- * The slots of one call are distinct; of tokens that name the same slot, any
- * one's values may remain. */
+ * The slots of one call are distinct: of tokens that name the same slot, parts
+ * of each may remain.  k, v and q may lie in the cache, outside the call's
+ * slots. */
 PFC_API int pfk_paged_append(const pfk_paged_append_params* p, void* stream);
 
 typedef struct pfk_paged_attention_params {
@@ -444,7 +445,8 @@ typedef struct pfk_paged_attention_params {
 } pfk_paged_attention_params;
 PFC_API int pfk_paged_attention_workspace(const pfk_paged_attention_params* p, size_t* bytes);
 /* out[b,h] = sum_j softmax_j(scale * q[b,h].k[j]) v[j] over the tokens j of
- * sequence b, with key-value head h / (q_heads / heads).  Queries and seen
+ * sequence b, with key-value head h / (q_heads / heads).  `out` overlaps
+ * neither k nor v.  Queries and seen
  * rows are finite: where one holds an infinity or NaN, the results that depend
  * on it may be NaN.  What lies in a page outside the seen tokens has no
  * effect. */

@@ -3,8 +3,10 @@
 //
 //   y[m,n] = sum_g s[n,g] sum_{k in g} x[m,k] (q[n,k] - z[n,g])  (+ bias[n])
 //
-// The weights are read once, at half a byte each; with few rows of x that
-// read bounds the product, so the arithmetic must cost little per weight.  It
+// The weights are read once for up to 48 rows of x (16 in fp32; more rows read
+// and unpack them again for each such chunk), at half a byte each; with few
+// rows that read bounds the product, so the arithmetic must cost little per
+// weight.  It
 // runs on mma.sync: q - z is an integer of at most 5 bits, exact in fp16 and
 // bf16, and so are 16-bit values of x; the products accumulate in fp32 over a
 // group and the group's sum is multiplied by its scale in fp32, so no weight
@@ -36,11 +38,14 @@
 // ranks: results do not depend on timing and nothing needs a workspace.
 //
 // Measured (device time in a stream of calls; the bytes at 6.4 TB/s in
-// brackets): one bf16 row, 4096 x 4096, groups of 128: 4.7 us (1.4); one fp32
-// row, 16384 x 4096, groups of 64: 14.1 us (5.8), 7.4 M instructions, which
-// bound it at 56% of the issue slots; 33 fp16 rows, 4096 x 16384, groups of 32:
-// 32.8 us (6.4), the tensor pipe 34% busy, the rest latency between the
-// instructions of two warps a scheduler (16 narrower warps measured the same).
+// brackets): one bf16 row, 4096 x 4096, groups of 128: 4.7 us (1.4), latency:
+// no load is on its way before the kernel in front has ended; one fp32 row,
+// 16384 x 4096, groups of 64: 14.2 us (5.8), of which its 7.4 M instructions
+// would take 6.6 at full issue, but 256 tiles leave 40 SMs with one CTA and
+// give 108 two, and the 13 warps of an SM that are there on average issue in
+// 56% of the cycles; 33 fp16 rows, 4096 x 16384, groups of 32: 32.7 us (6.4),
+// the tensor pipe 34% busy, the rest latency between the instructions of two
+// warps a scheduler (16 narrower warps measured the same).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

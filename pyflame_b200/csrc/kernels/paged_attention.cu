@@ -3,12 +3,16 @@
 //
 //   s_j = scale q.k_j,  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
 //
-// Every key and value is read once: 2 * D values for 4 * D * G operations (G
-// query heads share a key-value head), so memory bounds it as long as the
-// products run on the tensor cores and the loads never pause.
+// Keys and values are read once for every unit of work: 2 * D values for
+// 4 * D * G operations (G query heads of the unit), so memory bounds it as long
+// as the products run on the tensor cores and the loads never pause.
 //
-// Work.  A unit is one sequence, one key-value head and up to 16 of its query
-// heads; its keys are cut into tiles, a step of a CTA's 4 warps each.  The
+// Work.  A unit is one sequence, one key-value head and some of its query
+// heads: in 16-bit types up to 16, of heads above 128 values up to 8; in fp32
+// up to 8, of heads above 128 up to 2 (what the registers hold).  Wider groups
+// are several units, each of which reads all of the keys again: 40 query heads
+// on one key-value head three times in 16 bits.  A unit's keys are cut into
+// tiles, a step of a CTA's 4 warps each.  The
 // tiles of all units form one list, and each of a fixed number of CTAs (one
 // wave) takes an equal run of it, whatever the sequences' lengths: lengths are
 // device data, so the host could not balance them.  A CTA that has a whole
@@ -33,8 +37,11 @@
 // soon as this step's scores are done, its values as soon as the products are.
 //
 // Types.  16-bit: Q, K, V enter exactly; P is split into a high and a low
-// part, so its rounding (2^-16 and less) stays below that of the output. fp16
-// P is scaled by 2^14 to keep small weights out of its subnormal range.
+// part, so its rounding (2^-18 in bf16, less in fp16) stays far below that of
+// the output, 2^-8 and 2^-11.  fp16 P is scaled by 2^14 to keep small weights
+// out of its subnormal range.  Exponentials are one ex2.approx.ftz in all
+// types: its error, 2^-22 of a weight, is what rounding an fp32 score of size 4
+// does to it, and a weight below 2^-126 of the largest may count as 0.
 // fp32, up to 4 query heads a key-value head, and heads above 128: fp32 FMAs
 // on the CUDA cores.  fp32, more: both operands are split into tf32 high and
 // low parts, three products (the dropped low-low term is below 2^-22 of the
@@ -46,13 +53,15 @@
 // size; the addition costs 1% of the time: one sequence of 131071 103 us for
 // 102, 48 of 0 to 8192 151 for 149.5).
 //
-// Measured (device time in a stream of calls; the bytes at 6.4 TB/s in
+// Measured (device time, replayed from a graph; the bytes at 6.4 TB/s in
 // brackets): 128 sequences of 2048 to 8192 keys, bf16, 32/8 heads of 128, 2.69
-// GB: 407 to 440 us, by the machine (420); 48 of 0 to 8192, fp16: 140 us
-// (126); one of 131071, 64/8 heads: 98 us (84); 7 with a window of 1000, fp32,
-// 20 heads of 80: 23 us (11.7), latency of 5 steps a warp; one of 333, fp32, 12
-// heads of 64: 5.5 us, latency alone: lengths, page numbers, keys and the join
-// follow one another.
+// GB: 407 to 440 us, by the machine (420); 48 of 0 to 8192, fp16: 137 to 140
+// us (126); one of 131071, 64/8 heads: 97 us (84); 7 with a window of 1000,
+// fp32, 20 heads of 80: 23 us (11.7), of which a warp spends most on 8 to 9
+// dependent steps of 8 keys, over registers laid out for heads of 128 (three
+// CTAs an SM), and the join's launch the rest; one of 333, fp32, 12 heads of
+// 64: 5.4 us, latency alone: lengths, page numbers, keys and the join follow
+// one another.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -557,7 +557,7 @@ class Linear4bit:
     or None for 8; bias: [out_features] of the type of x, or None; group_size:
     32, 64 or a multiple of 128.  The constructor lays the weights out for the
     kernel once.  For single tokens and batches of up to some tens of rows;
-    more rows read the weights again for every 48 (16 in float32).
+    more rows read and unpack the weights again for every 48 (16 in float32).
     """
 
     def __init__(self, packed, scales, zeros=None, bias=None, in_features: Optional[int] = None, group_size: int = 128):
