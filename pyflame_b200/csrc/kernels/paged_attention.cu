@@ -305,73 +305,73 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
     tile = (int)t0;
     if (t0 == t1 && tid < HEADS) part[tid] = make_float2(-INFINITY, 0.f);
   } else {
-  // the join may come up as soon as the last of these CTAs has started
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // the join may come up as soon as the last of these CTAs has started
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // the list of tiles: its length, and the row that holds this CTA's first
-  Span mine = {0, 0, 0};
-  auto scan_rows = [&](int b) -> long long {  // tiles of the rows before b in its block of rows; scan: warps' sums
-    mine = b < a.batch ? span_of<L::kTile>(a, b) : Span{0, 0, 0};
-    const long long own = (long long)mine.tiles * per_row;
-    long long sum = own;
+    // the list of tiles: its length, and the row that holds this CTA's first
+    Span mine = {0, 0, 0};
+    auto scan_rows = [&](int b) -> long long {  // tiles of the rows before b in its block of rows; scan: warps' sums
+      mine = b < a.batch ? span_of<L::kTile>(a, b) : Span{0, 0, 0};
+      const long long own = (long long)mine.tiles * per_row;
+      long long sum = own;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(~0u, sum, o);
-      if (lane >= o) sum += up;
-    }
-    if (lane == 31) scan[warp] = sum;
-    __syncthreads();
-    long long start = sum - own;
-    for (int w = 0; w < warp; ++w) start += scan[w];
-    return start;
-  };
-  auto scanned = [&]() -> long long { return scan[0] + scan[1] + scan[2] + scan[3]; };
-  static_assert(kWarps == 4, "scanned() adds four warps' sums");
-  long long total = 0, start = 0;
-  if (a.batch > kThreads) {
-    for (int b = tid; b < a.batch; b += kThreads) total += (long long)span_of<L::kTile>(a, b).tiles * per_row;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-    if (lane == 0) scan[warp] = total;
-    __syncthreads();
-    total = scanned();
-  } else {
-    start = scan_rows(tid);
-    total = scanned();
-  }
-  // runs of total / ctas tiles, the longer ones spread evenly (neighbouring
-  // CTAs share an SM: 505 us for 487 with the longer runs first)
-  // at least four tiles each: more shares cost more than they save (one
-  // sequence of 4096 keys and 8 units: 21.4 us with one, 16.0 two, 14.3 four)
-  const int ctas = (int)min((long long)a.ctas, (total + 3) / 4);
-  const long long c = min((int)blockIdx.x, ctas);
-  t0 = ctas ? (long long)divide(total * c, ctas) : 0;
-  t1 = c < ctas ? (long long)divide(total * (c + 1), ctas) : t0;
-  if (t0 >= t1) {
-    if (tid == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, 0);
-    return;
-  }
-  long long before = 0;
-  for (int base = 0;; base += kThreads) {
-    if (a.batch > kThreads) {
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(~0u, sum, o);
+        if (lane >= o) sum += up;
+      }
+      if (lane == 31) scan[warp] = sum;
       __syncthreads();
-      start = scan_rows(base + tid);
+      long long start = sum - own;
+      for (int w = 0; w < warp; ++w) start += scan[w];
+      return start;
+    };
+    auto scanned = [&]() -> long long { return scan[0] + scan[1] + scan[2] + scan[3]; };
+    static_assert(kWarps == 4, "scanned() adds four warps' sums");
+    long long total = 0, start = 0;
+    if (a.batch > kThreads) {
+      for (int b = tid; b < a.batch; b += kThreads) total += (long long)span_of<L::kTile>(a, b).tiles * per_row;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+      if (lane == 0) scan[warp] = total;
+      __syncthreads();
+      total = scanned();
+    } else {
+      start = scan_rows(tid);
+      total = scanned();
     }
-    if (t0 >= before + start && t0 < before + start + (long long)mine.tiles * per_row) {
-      found_row = base + tid;
-      found_before = before + start;
-      found_span = mine;
+    // runs of total / ctas tiles, the longer ones spread evenly (neighbouring
+    // CTAs share an SM: 505 us for 487 with the longer runs first)
+    // at least four tiles each: more shares cost more than they save (one
+    // sequence of 4096 keys and 8 units: 21.4 us with one, 16.0 two, 14.3 four)
+    const int ctas = (int)min((long long)a.ctas, (total + 3) / 4);
+    const long long c = min((int)blockIdx.x, ctas);
+    t0 = ctas ? (long long)divide(total * c, ctas) : 0;
+    t1 = c < ctas ? (long long)divide(total * (c + 1), ctas) : t0;
+    if (t0 >= t1) {
+      if (tid == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, 0);
+      return;
     }
-    before += scanned();
-    if (before > t0) break;  // total > t0: some block of rows gets there
-  }
-  __syncthreads();
-  row = found_row;
-  sp = found_span;
-  unit = (int)divide(t0 - found_before, sp.tiles);
-  tile = (int)((t0 - found_before) - (long long)unit * sp.tiles);
-  list_total = total;
-  list_ctas = ctas;
+    long long before = 0;
+    for (int base = 0;; base += kThreads) {
+      if (a.batch > kThreads) {
+        __syncthreads();
+        start = scan_rows(base + tid);
+      }
+      if (t0 >= before + start && t0 < before + start + (long long)mine.tiles * per_row) {
+        found_row = base + tid;
+        found_before = before + start;
+        found_span = mine;
+      }
+      before += scanned();
+      if (before > t0) break;  // total > t0: some block of rows gets there
+    }
+    __syncthreads();
+    row = found_row;
+    sp = found_span;
+    unit = (int)divide(t0 - found_before, sp.tiles);
+    tile = (int)((t0 - found_before) - (long long)unit * sp.tiles);
+    list_total = total;
+    list_ctas = ctas;
   }
   int4 record = make_int4(0, 0, 0, 0);
 
@@ -457,35 +457,35 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, DP, NT, CORES>::kResident
   };
   // Q in the order of the second operand's registers
   auto stage_q = [&](int row, int first_q, int heads) {
-          const T* qp = (const T*)a.q + (long long)row * a.q_sb + (long long)first_q * a.q_sh;
-          if constexpr (CORES) {
-            for (int i = tid; i < NT * DP; i += kThreads) {
-              const int h = i / DP, d = i - h * DP;
-              reinterpret_cast<float*>(qs)[i] = h < heads && d < a.head_dim ? qp[h * a.q_sh + d] : 0.f;
-            }
-          } else {
-            for (int i = tid; i < NT * L::kQ * 32; i += kThreads) {
-              const int l = i & 31, c = (i >> 5) % L::kQ, nt = (i >> 5) / L::kQ;
-              const int h = nt * 8 + (l >> 2), d0 = (c * 4 + (l & 3)) * VEC;
-              if constexpr (k32) {
-                uint4 hi = {}, lo = {};
-                float x[4];
-    #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : 0.f;
-                split(x[0], hi.x, lo.x);
-                split(x[1], hi.y, lo.y);
-                split(x[2], hi.z, lo.z);
-                split(x[3], hi.w, lo.w);
-                qs[i] = hi;
-                qs[NT * L::kQ * 32 + i] = lo;
-              } else {
-                alignas(16) T x[8];
-    #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : Tr::from(0.f);
-                qs[i] = *reinterpret_cast<uint4*>(x);
-              }
-            }
-          }
+    const T* qp = (const T*)a.q + (long long)row * a.q_sb + (long long)first_q * a.q_sh;
+    if constexpr (CORES) {
+      for (int i = tid; i < NT * DP; i += kThreads) {
+        const int h = i / DP, d = i - h * DP;
+        reinterpret_cast<float*>(qs)[i] = h < heads && d < a.head_dim ? qp[h * a.q_sh + d] : 0.f;
+      }
+    } else {
+      for (int i = tid; i < NT * L::kQ * 32; i += kThreads) {
+        const int l = i & 31, c = (i >> 5) % L::kQ, nt = (i >> 5) / L::kQ;
+        const int h = nt * 8 + (l >> 2), d0 = (c * 4 + (l & 3)) * VEC;
+        if constexpr (k32) {
+          uint4 hi = {}, lo = {};
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : 0.f;
+          split(x[0], hi.x, lo.x);
+          split(x[1], hi.y, lo.y);
+          split(x[2], hi.z, lo.z);
+          split(x[3], hi.w, lo.w);
+          qs[i] = hi;
+          qs[NT * L::kQ * 32 + i] = lo;
+        } else {
+          alignas(16) T x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = h < heads && d0 + e < a.head_dim ? qp[h * a.q_sh + d0 + e] : Tr::from(0.f);
+          qs[i] = *reinterpret_cast<uint4*>(x);
+        }
+      }
+    }
   };
   // the first unit's before the chain of loads that leads to its first keys
   if (t0 < t1) {

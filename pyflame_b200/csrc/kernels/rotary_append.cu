@@ -217,37 +217,37 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(Args a) {
       }
       if (c1 >= chunks) continue;
       const bool two = c2 < chunks;
-    R r1 = __ldcs(reinterpret_cast<const R*>(src + c1 * VEC)), r2{};
-    if (two) r2 = __ldcs(reinterpret_cast<const R*>(src + c2 * VEC));
-    if (turn) {
-      const float2* cs = table + tok * half + j;
-      if constexpr (VEC == 1) {
-        const float2 y = turned(P::one(r1), P::one(r2), cs[0]);
-        r1 = P::one_of(y.x);
-        r2 = P::one_of(y.y);
-      } else {
-        unsigned* x1 = reinterpret_cast<unsigned*>(&r1);
-        unsigned* x2 = reinterpret_cast<unsigned*>(&r2);
-        if (a.interleaved) {  // chunk c1 holds the pairs of angles j*VEC ... , c2 those of the VEC/2 behind
-#pragma unroll
-          for (int e = 0; e < VEC; e += 2) {
-            const float2 u = P::get(x1, e), w = P::get(x2, e);
-            P::put(x1, e, turned(u.x, u.y, cs[(e / 2) * pairs]));
-            P::put(x2, e, turned(w.x, w.y, cs[(VEC / 2 + e / 2) * pairs]));
-          }
+      R r1 = __ldcs(reinterpret_cast<const R*>(src + c1 * VEC)), r2{};
+      if (two) r2 = __ldcs(reinterpret_cast<const R*>(src + c2 * VEC));
+      if (turn) {
+        const float2* cs = table + tok * half + j;
+        if constexpr (VEC == 1) {
+          const float2 y = turned(P::one(r1), P::one(r2), cs[0]);
+          r1 = P::one_of(y.x);
+          r2 = P::one_of(y.y);
         } else {
+          unsigned* x1 = reinterpret_cast<unsigned*>(&r1);
+          unsigned* x2 = reinterpret_cast<unsigned*>(&r2);
+          if (a.interleaved) {  // chunk c1 holds the pairs of angles j*VEC ... , c2 those of the VEC/2 behind
 #pragma unroll
-          for (int e = 0; e < VEC; e += 2) {
-            const float2 u = P::get(x1, e), w = P::get(x2, e);
-            const float2 y = turned(u.x, w.x, cs[(e) * pairs]), z = turned(u.y, w.y, cs[(e + 1) * pairs]);
-            P::put(x1, e, make_float2(y.x, z.x));
-            P::put(x2, e, make_float2(y.y, z.y));
+            for (int e = 0; e < VEC; e += 2) {
+              const float2 u = P::get(x1, e), w = P::get(x2, e);
+              P::put(x1, e, turned(u.x, u.y, cs[(e / 2) * pairs]));
+              P::put(x2, e, turned(w.x, w.y, cs[(VEC / 2 + e / 2) * pairs]));
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+              const float2 u = P::get(x1, e), w = P::get(x2, e);
+              const float2 y = turned(u.x, w.x, cs[(e) * pairs]), z = turned(u.y, w.y, cs[(e + 1) * pairs]);
+              P::put(x1, e, make_float2(y.x, z.x));
+              P::put(x2, e, make_float2(y.y, z.y));
+            }
           }
         }
       }
-    }
-    __stcs(reinterpret_cast<R*>(dst + c1 * VEC), r1);
-    if (two) __stcs(reinterpret_cast<R*>(dst + c2 * VEC), r2);
+      __stcs(reinterpret_cast<R*>(dst + c1 * VEC), r1);
+      if (two) __stcs(reinterpret_cast<R*>(dst + c2 * VEC), r2);
     }
   }
 }
