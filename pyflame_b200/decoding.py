@@ -236,8 +236,8 @@ class RotaryEmbedding:
     layout "half" turns the pairs (i, i + rotary_dim/2), "interleaved" the
     pairs (2i, 2i + 1), by position * inv_freq[i].  Angles are formed and
     reduced in two 64-bit numbers, so far positions (below 2^53) and small
-    cosines lose nothing.  `inv_freq` (a sequence
-    of rotary_dim / 2 numbers) replaces base and scaling (rotary_frequencies).
+    cosines lose nothing.  `inv_freq` (a sequence of rotary_dim / 2 numbers)
+    replaces base and scaling (rotary_frequencies).
     """
 
     def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, layout: str = "half",
@@ -467,8 +467,8 @@ class PagedKVCache:
         tokens are seen.  A sequence of length 0 gives 0.  With return_lse also
         the natural logarithm of the sum of exp(score), float32 [batch,
         q_heads] (-inf for length 0).  `out` may be q and otherwise shares no
-        memory with it or the cache.  An infinity or NaN in q
-        or in a seen row may make the results that depend on it NaN."""
+        memory with it or the cache.  An infinity or NaN in q or in a seen row
+        may make the results that depend on it NaN."""
         if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
             _no_tangents(q=q, out=out)
         torch = _Bound.torch
@@ -587,7 +587,7 @@ class Linear4bit:
             bias = bias.contiguous()
         self.in_features, self.out_features, self.group_size = k, n, int(group_size)
         self.device, self.scales, self.zeros, self.bias = device, scales.contiguous(), zeros, bias
-        self._bias_size = 0 if bias is None else _extent(bias)
+        self._bias_start, self._bias_end = (0, 0) if bias is None else (bias.data_ptr(), bias.data_ptr() + _extent(bias))
         blocks, row_blocks = -(-k // 128), -(-n // 16)
         self.weight = torch.empty((row_blocks, blocks, 256), dtype=torch.int32, device=device)
         self.meta = torch.empty((row_blocks, blocks * (128 // group_size) if group_size < 128 else groups, 16), dtype=torch.int32,
@@ -650,12 +650,14 @@ class Linear4bit:
             x = x.reshape(-1, self.in_features)
         if out is None:
             out = _Bound.torch.empty_like(plan[2])
-        elif x.data_ptr() < out.data_ptr() + plan[3] and out.data_ptr() < x.data_ptr() + plan[4]:
-            _apart("out", out, x=x)
+        else:
+            at, to = x.data_ptr(), out.data_ptr()
+            if at < to + plan[3] and to < at + plan[4]:
+                _apart("out", out, x=x)
+            if to < self._bias_end and self._bias_start < to + plan[3]:
+                _apart("out", out, the_bias=self.bias)
         p = N.LinearW4ParamsC.from_buffer_copy(plan[0])
         p.x, p.y = x.data_ptr(), out.data_ptr()
-        if self.bias is not None and p.y < p.bias + self._bias_size and p.bias < p.y + plan[3]:
-            _apart("out", out, the_bias=self.bias)
         _call(_Bound.linear, self.device, C.byref(p))
         return out
 

@@ -299,6 +299,25 @@ def test_neighbouring_outputs_are_taken():
     assert torch.equal(layer(rows[:, :64], out=rows[:, 64:128]), want) and torch.equal(layer(rows[::2, :64], out=rows[::2, 128:]), want[::2])
 
 
+def test_calls_of_no_rows():
+    """Nothing to do, with and without a bias, a given output, queries: the first time and as a known call."""
+    cache, r = pf.PagedKVCache(4, 16, 2, 64), pf.RotaryEmbedding(64)
+    bias = torch.ones(64, device="cuda")
+    none, pos = torch.zeros(0, 2, 64, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
+    table, lens = torch.zeros(0, 3, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    for b in (None, bias):
+        layer = pf.Linear4bit(*weights(gen(95), 64, 64, 64, True)[:3], bias=b, group_size=64)
+        for out in (None, torch.empty_like(none), none):
+            for _ in range(2):
+                assert layer(none, out=out).shape == (0, 2, 64) and layer(none[:, 0]).shape == (0, 64)
+                assert r.apply(none, pos, out=out).shape == r.backward(none, pos, out=out).shape == (0, 2, 64)
+                assert cache.attend(none, table, lens, out=out).shape == (0, 2, 64)
+                assert cache.attend(none, table, lens, out=out, return_lse=True)[1].shape == (0, 2)
+                assert cache.append(none, none, pos, q=none, q_out=out).shape == (0, 2, 64)
+                assert cache.append(none, none, pos, positions=pos, rotary=r) is None
+    cache.check()
+
+
 def test_known_calls_hold_no_memory():
     """What a handle keeps of the calls it knows is of no consequence beside them: no memory for each shape."""
     g = gen(98)
