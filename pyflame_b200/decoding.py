@@ -374,7 +374,8 @@ class PagedKVCache:
             raise ValueError("a cache holds fewer than 2^31 tokens")
         self.k, self.v, self.device, self.dtype = k, v, device, k.dtype
         self.num_pages, self.page_size, self.num_heads, self.head_dim = k.shape
-        self._err = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # a tensor made in that mode could not be cleared outside it
+            self._err = torch.zeros(1, dtype=torch.int32, device=device)
         self._c = N.PagedCacheC(code, k.data_ptr(), v.data_ptr(), *k.shape, *k.stride()[:3], self._err.data_ptr())
         # keys, values and what may lie between them
         self._start, self._end = min(k.data_ptr(), v.data_ptr()), max(t.data_ptr() + _extent(t) for t in (k, v))

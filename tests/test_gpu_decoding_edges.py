@@ -142,6 +142,21 @@ def test_linear4_any_nan_in_fp32(rows, inner, outer, group, bits):
     within(got[2:], y, linear_tol(x[2:], w, y, F32, inner, group))
 
 
+@pytest.mark.parametrize("dtype,rows,inner,outer,group", [
+    (F32, 2, 9000, 19999, 64), (BF16, 5, 9000, 19999, 128), (F16, 7, 8200, 19000, 32), (F32, 1, 16384, 30000, 32), (F16, 1, 4100, 19999, 64)])
+def test_linear4_more_row_tiles_than_ctas(dtype, rows, inner, outer, group):
+    """CTAs that walk over several tiles of weight rows, with rows of x that are staged again for each, or kept."""
+    g = gen(84)
+    packed, scales, z, w = weights(g, outer, inner, group, True)
+    b = randn(g, outer, dtype=dtype)
+    layer = pf.Linear4bit(packed, scales, z, b, in_features=inner, group_size=group)
+    x = randn(g, rows, inner, dtype=dtype)
+    y = x.double() @ w.T + b.double()
+    tol = linear_tol(x, w, y, dtype, inner, group)
+    for _ in range(2):
+        within(layer(x), y, tol)
+
+
 # ---------------------------------------------------------------------------
 # a layer's calls, each against 64 bits
 # ---------------------------------------------------------------------------
@@ -297,6 +312,40 @@ def test_neighbouring_outputs_are_taken():
     rows[:, :64] = randn(g, 5, 64)
     want = layer(rows[:, :64].clone())
     assert torch.equal(layer(rows[:, :64], out=rows[:, 64:128]), want) and torch.equal(layer(rows[::2, :64], out=rows[::2, 128:]), want[::2])
+
+
+def test_handles_made_in_inference_mode():
+    """Made in torch's inference mode and used outside, made outside and used inside."""
+    def make():
+        cache, r = pf.PagedKVCache(4, 16, 2, 64), pf.RotaryEmbedding(64)
+        return cache, r, pf.Linear4bit(*weights(gen(95), 64, 64, 64, True)[:3], group_size=64)
+
+    def use(cache, r, layer):
+        x, pos = randn(gen(96), 3, 2, 64), torch.arange(3, device="cuda")
+        table, lens = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+        outs = []
+        for _ in range(2):
+            q = cache.append(x, x, pos, positions=pos, rotary=r, q=x)
+            out, lse = cache.attend(q, table, lens, return_lse=True)
+            outs.append((layer(out), lse, r.backward(q, pos)))
+        cache.check()
+        cache.append(x, x, pos + 1000)
+        with pytest.raises(pf._native.PfcError):
+            cache.check()
+        cache.check()
+        return outs
+
+    want = use(*make())
+    with torch.inference_mode():
+        made = make()
+        inside = use(*make())
+    outside = use(*made)
+    made = make()
+    with torch.inference_mode():
+        mixed = use(*made)
+    for got in (inside, outside, mixed):
+        for a, b in zip(sum(got, ()), sum(want, ())):
+            assert torch.equal(a, b)
 
 
 def test_calls_of_no_rows():
