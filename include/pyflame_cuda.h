@@ -446,10 +446,9 @@ typedef struct pfk_paged_attention_params {
 PFC_API int pfk_paged_attention_workspace(const pfk_paged_attention_params* p, size_t* bytes);
 /* out[b,h] = sum_j softmax_j(scale * q[b,h].k[j]) v[j] over the tokens j of
  * sequence b, with key-value head h / (q_heads / heads).  `out` overlaps
- * neither k nor v.  Queries and seen
- * rows are finite: where one holds an infinity or NaN, the results that depend
- * on it may be NaN.  What lies in a page outside the seen tokens has no
- * effect. */
+ * neither k nor v.  Queries and seen rows are finite: where one holds an
+ * infinity or NaN, the results that depend on it may be NaN.  What lies in a
+ * page outside the seen tokens has no effect. */
 PFC_API int pfk_paged_attention(const pfk_paged_attention_params* p, void* stream);
 
 /* Lays 4-bit weights out for pfk_linear_w4, once.

@@ -3,19 +3,19 @@
 //
 //   y[m,n] = sum_g s[n,g] sum_{k in g} x[m,k] (q[n,k] - z[n,g])  (+ bias[n])
 //
-// The weights are read once for up to 48 rows of x (16 in fp32; more rows read
-// and unpack them again for each such chunk), at half a byte each; with few
-// rows that read bounds the product, so the arithmetic must cost little per
-// weight.  It
-// runs on mma.sync: q - z is an integer of at most 5 bits, exact in fp16 and
-// bf16, and so are 16-bit values of x; the products accumulate in fp32 over a
-// group and the group's sum is multiplied by its scale in fp32, so no weight
-// is ever rounded.  fp32 x enters as three bf16 parts (8 bits each, 24 in
-// all), which take three columns of the instruction instead of three
-// instructions.  Two weights cost one logic operation and one subtraction:
-// a nibble pair OR-ed into the mantissas of two 16-bit numbers of value 2^10 is
-// 2^10 + q in fp16, from which 2^10 + z is subtracted exactly; in bf16 it is
-// 2^-4 + 2^-11 q, and the result is multiplied by 2^11.
+// The weights are read once for up to 48 rows of x (16 in fp32; more rows
+// read and unpack them again for each such chunk), at half a byte each; with
+// few rows that read bounds the product, so the arithmetic must cost little
+// per weight.  It runs on mma.sync: q - z is an integer of at most 5 bits,
+// exact in fp16 and bf16, and so are 16-bit values of x; the products
+// accumulate in fp32 over a group and the group's sum is multiplied by its
+// scale in fp32, so no weight is ever rounded.  fp32 x enters as three bf16
+// parts (8 bits each, 24 in all), which take three columns of the instruction
+// instead of three instructions.  Two weights cost one logic operation and
+// one subtraction: a nibble pair OR-ed into the mantissas of two 16-bit
+// numbers of value 2^10 is 2^10 + q in fp16, from which 2^10 + z is
+// subtracted exactly; in bf16 it is 2^-4 + 2^-11 q, and the result is
+// multiplied by 2^11.
 //
 // A lane holds 16 bytes of each of two weight rows in a block of 128 columns:
 // the arranged layout gives it 8 columns of each of the four 32-column groups,
@@ -25,8 +25,9 @@
 //
 // Three shapes of CTA, 8 warps each:
 //   few rows of x (8 columns of the instruction): the warps share the columns
-//   of 16 weight rows, or in pairs those of 64; a CTA keeps its part of x and
-//   walks over row tiles, so x is staged once;
+//   of 16 weight rows, or in pairs those of 64; a CTA walks over row tiles and
+//   keeps its part of x, which is staged once (again for each tile, through
+//   two buffers, where it does not fit);
 //   more, and weight rows that fill the device: 128 weight rows (32 a warp, so
 //   that a fragment of x read from shared memory serves two instructions), in
 //   pairs over the columns, x in chunks through two buffers;
@@ -89,7 +90,7 @@ struct Args {
 };
 
 template <typename T>
-struct Num {  // 16-bit type of the products, its magic number for 4-bit integers, what a unit of them stands for, and the parts of x
+struct Num {  // 16-bit type of the products, its magic number for 4-bit integers and their unit, and the parts of x
   using N = __nv_bfloat16;
   using N2 = __nv_bfloat162;
   // 2^-4, in whose mantissa a unit is 2^-11: q - z enters as its 2^-11th, and a

@@ -9,18 +9,18 @@
 //
 // Work.  A unit is one sequence, one key-value head and some of its query
 // heads: in 16-bit types up to 16, of heads above 128 values up to 8; in fp32
-// up to 8, of heads above 128 up to 2 (what the registers hold).  Wider groups
-// are several units, each of which reads all of the keys again: 40 query heads
-// on one key-value head three times in 16 bits.  A unit's keys are cut into
-// tiles, a step of a CTA's 4 warps each.  The
-// tiles of all units form one list, and each of a fixed number of CTAs (one
-// wave) takes an equal run of it, whatever the sequences' lengths: lengths are
-// device data, so the host could not balance them.  A CTA that has a whole
-// unit writes its output; a unit that is shared leaves (m, sum, o) of each
-// share in the workspace, and a second small kernel joins the shares in the
-// order of the list, so that results do not depend on timing and nothing has
-// to be zero beforehand.  Few units of short sequences have a cluster of CTAs
-// each instead, which joins its shares through distributed shared memory.
+// up to 8, of heads above 128 up to 2 (what the registers hold).  Wider
+// groups are several units, each of which reads all of the keys again: 40
+// query heads on one key-value head three times in 16 bits.  A unit's keys
+// are cut into tiles, a step of a CTA's 4 warps each.  The tiles of all units
+// form one list, and each of a fixed number of CTAs (one wave) takes an equal
+// run of it, whatever the sequences' lengths: lengths are device data, so the
+// host could not balance them.  A CTA that has a whole unit writes its
+// output; a unit that is shared leaves (m, sum, o) of each share in the
+// workspace, and a second small kernel joins the shares in the order of the
+// list, so that results do not depend on timing and nothing has to be zero
+// beforehand.  Few units of short sequences have a cluster of CTAs each
+// instead, which joins its shares through distributed shared memory.
 //
 // Step.  A warp takes 16 keys at a time (8 on the CUDA cores), straight from
 // global memory into registers, without shared memory: lane (g, t) = (lane /
