@@ -490,6 +490,132 @@ typedef struct pfk_linear_w4_params {
  * bfloat16 calls below 2^-115 come in steps of 2^-138. */
 PFC_API int pfk_linear_w4(const pfk_linear_w4_params* p, void* stream);
 
+/* ---- a decoder layer's step, continued -------------------------------------- */
+/* A paged cache in 4 bits, low-rank adapters beside a shared projection, and a
+ * mixture-of-experts layer: for new tokens, on the terms of the section above. */
+
+/* Keys and values in 4 bits.  A head's values are cut into groups of `group`
+ * (the last may be shorter); value = low + step * code, with
+ *   low  = bfloat16(the group's least value),
+ *   step = bfloat16((its greatest value - low) * fp32(1 / 15)), 0 where that is below 2^-126,
+ *   code = the nearest whole number (ties to even) to (value - low) * (1 / step), from 0 to 15,
+ * every operation in fp32.  Groups that hold an infinity, a NaN or a value
+ * above 2^126 in size are kept as NaN.
+ * Both are held by [num_pages][heads][page_size]: codes in W / 8 words each
+ * (W: head_dim rounded up to 64, 96, 128 or 256; in the order of the
+ * attention's operands, pfk_cache4_read gives the values), scales in a word
+ * for each group (their number rounded up to a power of two), step's bits in
+ * the high half and low's in the low one.  Slot numbers are page * page_size +
+ * offset. */
+typedef struct pfk_cache4 {
+  uint32_t *k, *v;               /* codes, 16-byte aligned */
+  uint32_t *k_scales, *v_scales; /* 16-byte aligned */
+  int64_t num_pages, page_size, heads, head_dim; /* head_dim a multiple of 8, at most 256; fewer than 2^31
+                                                    tokens, and than 2^32 - 1 heads of them */
+  int64_t group;                /* 32, 64 or 128 */
+  int* err; /* device int or NULL: as in pfk_paged_cache */
+} pfk_cache4;
+/* Words of a head's codes, and of its scales. */
+PFC_API int pfk_cache4_words(int64_t head_dim, int64_t group, int64_t* codes, int64_t* scales);
+
+typedef struct pfk_cache4_append_params {
+  pfk_cache4 cache;
+  int dtype; /* of k, v and q */
+  int64_t tokens;
+  const void* k; /* [tokens][heads][head_dim] */
+  int64_t k_st, k_sh;
+  const void* v;
+  int64_t v_st, v_sh;
+  const void* q; /* [tokens][q_heads][head_dim], rotated into q_out; NULL: none */
+  void* q_out;   /* may be q (same pointer and strides), not overlap it, k or v otherwise */
+  int64_t q_heads, q_st, q_sh, qo_st, qo_sh;
+  const int64_t* slots;     /* [tokens]; negative: the token is skipped, its q_out row left as it was */
+  const int64_t* positions; /* [tokens]; may be NULL without rotation */
+  pfk_rotary rotary;        /* of k, in 64 bits and rounded to fp32 once, and of q */
+} pfk_cache4_append_params;
+/* The slots of one call are distinct: of tokens that name the same slot, parts
+ * of each may remain. */
+PFC_API int pfk_cache4_append(const pfk_cache4_append_params* p, void* stream);
+
+typedef struct pfk_cache4_read_params {
+  pfk_cache4 cache;
+  int dtype; /* of k and v */
+  int64_t tokens;
+  const int64_t* slots; /* [tokens]; negative: zeros */
+  void *k, *v;          /* [tokens][heads][head_dim] dense */
+} pfk_cache4_read_params;
+/* What the cache holds at the slots, rounded to dtype. */
+PFC_API int pfk_cache4_read(const pfk_cache4_read_params* p, void* stream);
+
+typedef struct pfk_cache4_attention_params {
+  pfk_cache4 cache;
+  int dtype; /* of q and out */
+  int64_t batch, q_heads; /* q_heads a multiple of the cache's heads */
+  const void* q;          /* [batch][q_heads][head_dim] */
+  int64_t q_sb, q_sh;
+  void* out; /* [batch][q_heads][head_dim]; may be q itself (same pointer and strides), not overlap it otherwise */
+  int64_t o_sb, o_sh;
+  float* lse;
+  const int32_t* block_table;
+  int64_t table_stride, table_width;
+  const int32_t* seq_lens;
+  int64_t window;
+  float scale;
+  void* workspace; /* pfk_cache4_attention_workspace bytes, as in pfk_paged_attention_params */
+  size_t workspace_bytes;
+} pfk_cache4_attention_params;
+PFC_API int pfk_cache4_attention_workspace(const pfk_cache4_attention_params* p, size_t* bytes);
+/* pfk_paged_attention over the values that the 4-bit cache holds. */
+PFC_API int pfk_cache4_attention(const pfk_cache4_attention_params* p, void* stream);
+
+typedef struct pfk_adapters_params {
+  int dtype; /* of x, base, out, a and b */
+  int64_t rows, inner, outer, adapters;
+  int64_t rank;    /* of a and b: a multiple of 16, at most 256; unused ranks are 0 */
+  const void* x;   /* [rows][inner] */
+  int64_t x_st;
+  const int32_t* index; /* [rows]: the row's adapter; negative: none */
+  const void* base;     /* [rows][outer], or NULL: 0 */
+  int64_t base_st;
+  void* out; /* [rows][outer]; may be base (same pointer and stride), not overlap base or x otherwise */
+  int64_t out_st;
+  const void* a; /* [adapters][rank][a_st], zeros behind inner; 16-byte aligned rows */
+  int64_t a_st;
+  const void* b; /* [adapters][outer][rank], 16-byte aligned */
+  const float* scales; /* [adapters] */
+  int* err;            /* device int or NULL: set to PFC_ERR_INVALID_ARGUMENT where an index names no adapter (its row is base) */
+} pfk_adapters_params;
+/* out[m] = base[m] + scales[i] * b[i] (a[i] x[m]) with i = index[m]: sums in
+ * fp32, the result rounded once. */
+PFC_API int pfk_adapters(const pfk_adapters_params* p, void* stream);
+
+typedef struct pfk_experts_params {
+  int dtype;       /* of x, gate_up, down and y */
+  int activation;  /* of the gate: 0 SiLU, 1 GELU (tanh form) */
+  int renormalize; /* 1: the chosen experts' weights add up to 1; 0: they are parts of the softmax over all */
+  int64_t tokens, width, inner; /* width and inner at most 65536 */
+  int64_t experts, top;         /* experts at most 1024, top at most 32 */
+  const void* x; /* [tokens][width] */
+  int64_t x_st;
+  const float* router; /* [experts][router_st], zeros behind width; rows of multiples of 16 bytes, as all weights */
+  int64_t router_st;
+  const void* gate_up; /* [experts][2 * inner][gate_up_st]: the gate's rows, then the other factor's; zeros behind width */
+  int64_t gate_up_st;
+  const void* down; /* [experts][width][down_st], zeros behind inner */
+  int64_t down_st;
+  void* y; /* [tokens][width]; may be x (same pointer and stride), not overlap it otherwise */
+  int64_t y_st;
+  int32_t* chosen; /* [tokens][top] dense, best first, ties to the lower expert; NULL: not wanted */
+  float* weights;  /* [tokens][top] dense, or NULL */
+  void* workspace; /* pfk_experts_workspace bytes, 16-byte aligned, not shared by calls that may overlap */
+  size_t workspace_bytes;
+} pfk_experts_params;
+PFC_API int pfk_experts_workspace(const pfk_experts_params* p, size_t* bytes);
+/* y = sum over the `top` experts with the largest router logits (taken in 64
+ * bits) of weight * down (act(gate x) * (up x)).  A NaN among the logits
+ * counts as the lowest.  The weights are read once for every 128 tokens. */
+PFC_API int pfk_experts(const pfk_experts_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,11 +6,14 @@ tensors, graph nodes, ops, nn modules, device selection and `eval`, with
 libpyflame_cuda.so (include/pyflame_cuda.h); there is no CPU evaluation path.
 """
 from . import autograd, decoding, ir, nn, serving
+from .adapters import LowRankAdapters
 from .backend import (Backend, CudaExecutor, DeviceInfo, ExecutionResult, Executor, ExecutorConfig, MemoryStats,
                       cuda_device_count, cuda_get_device, cuda_get_device_info, cuda_is_available, cuda_set_device,
                       cuda_synchronize)
+from .cache4bit import PagedKVCache4bit
 from .decoding import Linear4bit, PagedKVCache, RotaryEmbedding, rotary_frequencies
 from .device import device_info, eval, get_device, set_device, set_precision, synchronize
+from .experts import MixtureOfExperts
 from .ir import DType, Graph, Node, NodeType, OpType, TensorSpec, dtype_name, dtype_size
 from .tensor import (Tensor, abs, arange, broadcast_to, cat, clamp, cos, exp, from_numpy, full, gelu,
                      get_current_graph, log, log_softmax, manual_seed, matmul, maximum, minimum, ones, pow, rand,

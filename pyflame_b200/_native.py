@@ -103,6 +103,43 @@ class LinearW4ParamsC(C.Structure):
         ("x", _P), ("x_st", _I64), ("y", _P), ("y_st", _I64), ("weight", _P), ("meta", _P), ("bias", _P)]
 
 
+class Cache4C(C.Structure):
+    _fields_ = [(n, _P) for n in ("k", "v", "k_scales", "v_scales")] + [(n, _I64) for n in (
+        "num_pages", "page_size", "heads", "head_dim", "group")] + [("err", _P)]
+
+
+class Cache4AppendParamsC(C.Structure):
+    _fields_ = [("cache", Cache4C), ("dtype", C.c_int), ("tokens", _I64), ("k", _P), ("k_st", _I64), ("k_sh", _I64), ("v", _P),
+                ("v_st", _I64), ("v_sh", _I64), ("q", _P), ("q_out", _P)] + [(n, _I64) for n in (
+                    "q_heads", "q_st", "q_sh", "qo_st", "qo_sh")] + [
+        ("slots", _P), ("positions", _P), ("rotary", RotaryC)]
+
+
+class Cache4ReadParamsC(C.Structure):
+    _fields_ = [("cache", Cache4C), ("dtype", C.c_int), ("tokens", _I64), ("slots", _P), ("k", _P), ("v", _P)]
+
+
+class Cache4AttentionParamsC(C.Structure):
+    _fields_ = [("cache", Cache4C), ("dtype", C.c_int), ("batch", _I64), ("q_heads", _I64), ("q", _P), ("q_sb", _I64),
+                ("q_sh", _I64), ("out", _P), ("o_sb", _I64), ("o_sh", _I64), ("lse", _P), ("block_table", _P),
+                ("table_stride", _I64), ("table_width", _I64), ("seq_lens", _P), ("window", _I64),
+                ("scale", C.c_float), ("workspace", _P), ("workspace_bytes", C.c_size_t)]
+
+
+class AdaptersParamsC(C.Structure):
+    _fields_ = [("dtype", C.c_int)] + [(n, _I64) for n in ("rows", "inner", "outer", "adapters", "rank")] + [
+        ("x", _P), ("x_st", _I64), ("index", _P), ("base", _P), ("base_st", _I64), ("out", _P), ("out_st", _I64),
+        ("a", _P), ("a_st", _I64), ("b", _P), ("scales", _P), ("err", _P)]
+
+
+class ExpertsParamsC(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("activation", C.c_int), ("renormalize", C.c_int)] + [(n, _I64) for n in (
+        "tokens", "width", "inner", "experts", "top")] + [
+        ("x", _P), ("x_st", _I64), ("router", _P), ("router_st", _I64), ("gate_up", _P), ("gate_up_st", _I64),
+        ("down", _P), ("down_st", _I64), ("y", _P), ("y_st", _I64), ("chosen", _P), ("weights", _P),
+        ("workspace", _P), ("workspace_bytes", C.c_size_t)]
+
+
 # name -> (restype, argtypes); the list is the C-ABI of include/pyflame_cuda.h
 SIGNATURES = {
     "pfc_cuda_is_available": (C.c_int, []),
@@ -153,6 +190,14 @@ SIGNATURES = {
     "pfk_paged_attention": (C.c_int, [C.POINTER(PagedAttentionParamsC), _P]),
     "pfk_w4_arrange": (C.c_int, [C.POINTER(W4ArrangeParamsC), _P]),
     "pfk_linear_w4": (C.c_int, [C.POINTER(LinearW4ParamsC), _P]),
+    "pfk_cache4_words": (C.c_int, [_I64, _I64, C.POINTER(_I64), C.POINTER(_I64)]),
+    "pfk_cache4_append": (C.c_int, [C.POINTER(Cache4AppendParamsC), _P]),
+    "pfk_cache4_read": (C.c_int, [C.POINTER(Cache4ReadParamsC), _P]),
+    "pfk_cache4_attention_workspace": (C.c_int, [C.POINTER(Cache4AttentionParamsC), C.POINTER(C.c_size_t)]),
+    "pfk_cache4_attention": (C.c_int, [C.POINTER(Cache4AttentionParamsC), _P]),
+    "pfk_adapters": (C.c_int, [C.POINTER(AdaptersParamsC), _P]),
+    "pfk_experts_workspace": (C.c_int, [C.POINTER(ExpertsParamsC), C.POINTER(C.c_size_t)]),
+    "pfk_experts": (C.c_int, [C.POINTER(ExpertsParamsC), _P]),
 }
 
 _lib = None

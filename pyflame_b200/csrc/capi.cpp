@@ -547,4 +547,57 @@ int pfk_linear_w4(const pfk_linear_w4_params* p, void* stream) {
   });
 }
 
+int pfk_cache4_words(int64_t head_dim, int64_t group, int64_t* codes, int64_t* scales) {
+  return guarded([&] { pfb::cache4_words(head_dim, group, codes, scales); });
+}
+
+int pfk_cache4_append(const pfk_cache4_append_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_cache4_append(*p, as_stream(stream));
+  });
+}
+
+int pfk_cache4_read(const pfk_cache4_read_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_cache4_read(*p, as_stream(stream));
+  });
+}
+
+int pfk_cache4_attention_workspace(const pfk_cache4_attention_params* p, size_t* bytes) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p && bytes, "null argument");
+    *bytes = pfb::cache4_attention_workspace(*p);
+  });
+}
+
+int pfk_cache4_attention(const pfk_cache4_attention_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_cache4_attention(*p, as_stream(stream));
+  });
+}
+
+int pfk_adapters(const pfk_adapters_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_adapters(*p, as_stream(stream));
+  });
+}
+
+int pfk_experts_workspace(const pfk_experts_params* p, size_t* bytes) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p && bytes, "null argument");
+    *bytes = pfb::experts_workspace(*p);
+  });
+}
+
+int pfk_experts(const pfk_experts_params* p, void* stream) {
+  return guarded([&] {
+    PFB_CHECK_ARG(p, "null parameters");
+    pfb::launch_experts(*p, as_stream(stream));
+  });
+}
+
 }  // extern "C"

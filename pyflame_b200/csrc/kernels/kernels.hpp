@@ -264,5 +264,13 @@ size_t paged_attention_workspace(const pfk_paged_attention_params& p);
 void launch_paged_attention(const pfk_paged_attention_params& p, cudaStream_t stream);
 void launch_w4_arrange(const pfk_w4_arrange_params& p, cudaStream_t stream);
 void launch_linear_w4(const pfk_linear_w4_params& p, cudaStream_t stream);
+void cache4_words(int64_t head_dim, int64_t group, int64_t* codes, int64_t* scales);
+void launch_cache4_append(const pfk_cache4_append_params& p, cudaStream_t stream);
+void launch_cache4_read(const pfk_cache4_read_params& p, cudaStream_t stream);
+size_t cache4_attention_workspace(const pfk_cache4_attention_params& p);
+void launch_cache4_attention(const pfk_cache4_attention_params& p, cudaStream_t stream);
+void launch_adapters(const pfk_adapters_params& p, cudaStream_t stream);
+size_t experts_workspace(const pfk_experts_params& p);
+void launch_experts(const pfk_experts_params& p, cudaStream_t stream);
 
 }  // namespace pfb
