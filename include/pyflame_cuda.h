@@ -501,9 +501,11 @@ PFC_API int pfk_linear_w4(const pfk_linear_w4_params* p, void* stream);
  *   code = the nearest whole number (ties to even) to (value - low) * (1 / step), from 0 to 15,
  * every operation in fp32.  Groups that hold an infinity, a NaN or a value
  * above 2^126 in size are kept as NaN.
- * Both are held by [num_pages][heads][page_size]: codes in W / 8 words each
- * (W: head_dim rounded up to 64, 96, 128 or 256; in the order of the
- * attention's operands, pfk_cache4_read gives the values), scales in a word
+ * Both are held by [num_pages][heads]: of each of the page's tokens a key's
+ * codes in W / 8 words (W: head_dim rounded up to 64, 96, 128 or 256), of each
+ * two of them the values' codes in W / 4 words (an odd page's last two are one
+ * token and room for another), in the order of the attention's operands
+ * (pfk_cache4_read gives the values); scales of each token in a word
  * for each group (their number rounded up to a power of two), step's bits in
  * the high half and low's in the low one.  Slot numbers are page * page_size +
  * offset. */
@@ -515,7 +517,7 @@ typedef struct pfk_cache4 {
   int64_t group;                /* 32, 64 or 128 */
   int* err; /* device int or NULL: as in pfk_paged_cache */
 } pfk_cache4;
-/* Words of a head's codes, and of its scales. */
+/* Words of a key's codes (of two tokens' values: twice as many), and of a token's scales. */
 PFC_API int pfk_cache4_words(int64_t head_dim, int64_t group, int64_t* codes, int64_t* scales);
 
 typedef struct pfk_cache4_append_params {

@@ -33,8 +33,9 @@ class PagedKVCache4bit:
     NaN.  head_dim: a multiple of 8, at most 256.
 
     `k`, `v` (codes, in an order of their own) and `k_scales`, `v_scales` are
-    int32 [num_pages, num_heads, page_size, ...]: a page is moved by copying
-    its rows of all four.  Which pages a sequence owns is the caller's
+    int32 [num_pages, num_heads, ...]: a page is moved by copying its rows of
+    all four.  Values of two tokens share words, so a page of an odd size has
+    room for one more.  Which pages a sequence owns is the caller's
     bookkeeping.  Keys, values and queries of a call are float32, float16 or
     bfloat16; the cache itself has no type.
     """
@@ -52,15 +53,17 @@ class PagedKVCache4bit:
             raise ValueError(f"device: must be a CUDA device, not {device}")
         codes, scales = C.c_int64(0), C.c_int64(0)
         N.check(N.lib().pfk_cache4_words(dim, group, C.byref(codes), C.byref(scales)))
-        records = pages * heads * size
+        records, pairs = pages * heads * size, pages * heads * ((size + 1) // 2)
         with torch.inference_mode(False):  # a tensor made in that mode could not be written outside it
             # one memory for all, so that an output that lies in it is found by one comparison
-            memory = torch.zeros(records * 2 * (codes.value + scales.value) + 4 * 4, dtype=torch.int32, device=device)
+            memory = torch.zeros(records * (codes.value + 2 * scales.value) + pairs * 2 * codes.value + 4 * 4, dtype=torch.int32,
+                                 device=device)
             self._err = torch.zeros(1, dtype=torch.int32, device=device)
         parts, at = [], 0
-        for words in (codes.value, codes.value, scales.value, scales.value):
-            parts.append(memory[at:at + records * words].view(pages, heads, size, words))
-            at += -(-records * words // 4) * 4  # the next begins at a multiple of 16 bytes
+        for rows, words in ((size, codes.value), ((size + 1) // 2, 2 * codes.value), (size, scales.value), (size, scales.value)):
+            count = pages * heads * rows * words
+            parts.append(memory[at:at + count].view(pages, heads, rows, words))
+            at += -(-count // 4) * 4  # the next begins at a multiple of 16 bytes
         self.k, self.v, self.k_scales, self.v_scales = parts
         self.device = memory.device
         self.num_pages, self.page_size, self.num_heads, self.head_dim, self.group_size = pages, size, heads, dim, group

@@ -194,6 +194,25 @@ __device__ __forceinline__ unsigned quantize(const float (&x)[16], int in, bool 
   return !some ? 0 : fine ? word : 0x7fc07fc0u;
 }
 
+// A slot's token: head 0 of its page, and its offset there; page -1: none.
+struct Place {
+  int page, offset;
+};
+__device__ __forceinline__ Place place_of(const Args& a, long long slot) {
+  if (slot >= a.num_slots && a.err) *a.err = PFC_ERR_INVALID_ARGUMENT;
+  if (slot < 0 || slot >= a.num_slots) return {-1, 0};
+  const unsigned page = a.by_page.div((unsigned)slot);
+  return {(int)page, (int)((unsigned)slot - page * a.by_page.d)};
+}
+__device__ __forceinline__ long long record_of(const Args& a, const Place& p, int head) {
+  return ((long long)p.page * a.heads + head) * a.by_page.d + p.offset;
+}
+// The place of 16 bits `half` of a token's values.
+__device__ __forceinline__ long long value_at(const Args& a, const Place& p, int head, int blocks, int half) {
+  const long long pair = ((long long)p.page * a.heads + head) * ((a.by_page.d + 1) >> 1) + (p.offset >> 1);
+  return (pair * (8 * blocks) + half) * 2 + (p.offset & 1);
+}
+
 // Where the angle of pair p lies among a token's half: lanes that turn chunks
 // of 8 values next to each other read places next to each other.  (In the order
 // of the pairs, 16 lanes' reads met in one bank: 99 us for a prompt of 8191
@@ -202,14 +221,14 @@ __device__ __forceinline__ int spread_of(int half, int interleaved) {
   const int angles = interleaved ? 4 : 8;  // of a chunk
   return half % angles == 0 ? angles : 1;
 }
-__device__ __forceinline__ int place_of(int p, int half, int spread) { return p % spread * (half / spread) + p / spread; }
+__device__ __forceinline__ int angle_at(int p, int half, int spread) { return p % spread * (half / spread) + p / spread; }
 
 // Lanes of a row of BLOCKS blocks of 32 values, 16 each.
 constexpr int lanes_of(int blocks) { return blocks <= 2 ? 4 : blocks <= 4 ? 8 : 16; }
 
 // Keys and values.
 template <typename T, int BLOCKS, bool KEYS, bool WIDE>
-__device__ __forceinline__ void store_rows(const Args& a, const double2* turns, const long long* records, int first, int mine,
+__device__ __forceinline__ void store_rows(const Args& a, const double2* turns, const Place* places, int first, int mine,
                                            int head_first, int head_last) {
   constexpr int LANES = lanes_of(BLOCKS), ROWS = 32 / LANES;  // rows of a warp at a time
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -222,11 +241,11 @@ __device__ __forceinline__ void store_rows(const Args& a, const double2* turns, 
   const long long st = a.st[KEYS ? 0 : 1], sh = a.sh[KEYS ? 0 : 1];
   int i = warp * ROWS + lane / LANES, tok = i / heads, head = head_first + i - tok * heads;
   for (int i0 = warp * ROWS; i0 < rows; i0 += kWarps * ROWS, i += kWarps * ROWS) {
-    const long long record = i < rows ? records[tok] : -1;
+    const Place place = i < rows ? places[tok] : Place{-1, 0};
     float x[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] = 0.f;
-    if (record >= 0) {
+    if (place.page >= 0) {
       const T* src = (const T*)a.src[KEYS ? 0 : 1] + (long long)(first + tok) * st + head * sh;
       const double2* cs = turns + tok * half;
 #pragma unroll
@@ -276,15 +295,15 @@ __device__ __forceinline__ void store_rows(const Args& a, const double2* turns, 
     }
     unsigned codes[2];
     const unsigned scales = quantize(x, in, some, lanes, codes);
-    if (record >= 0 && part < 2 * BLOCKS) {
-      const long long at = record + (long long)head * a.by_page.d;
+    if (place.page >= 0 && part < 2 * BLOCKS) {
+      const long long at = record_of(a, place, head);
       if constexpr (KEYS) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) a.k[at * (4 * BLOCKS) + cache4_key_word(2 * part + s, BLOCKS)] = codes[s];
       } else {
-        unsigned short* v = reinterpret_cast<unsigned short*>(a.v + at * (4 * BLOCKS));
+        unsigned short* v = reinterpret_cast<unsigned short*>(a.v) + value_at(a, place, head, BLOCKS, 0);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) v[cache4_value_half(4 * part + s, BLOCKS)] = (unsigned short)(codes[s >> 1] >> (16 * (s & 1)));
+        for (int s = 0; s < 4; ++s) v[2 * cache4_value_half(4 * part + s, BLOCKS)] = (unsigned short)(codes[s >> 1] >> (16 * (s & 1)));
       }
       if (part % lanes == 0) (KEYS ? a.k_scales : a.v_scales)[at * a.groups + group] = scales;
     }
@@ -295,7 +314,7 @@ __device__ __forceinline__ void store_rows(const Args& a, const double2* turns, 
 // Queries: a thread turns two chunks of 8 values that turn together, or
 // copies two.  Both are read before either is written: q_out may be q.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void turn_queries(const Args& a, const float2* turns, const long long* records, int first, int mine,
+__device__ __forceinline__ void turn_queries(const Args& a, const float2* turns, const Place* places, int first, int mine,
                                              int head_first, int head_last) {
   const int half = a.rot >> 1, chunks = a.head_dim / 8;
   const bool by_chunk = a.interleaved || half % 8 == 0;  // a turned chunk's partner is a chunk, or itself
@@ -304,7 +323,7 @@ __device__ __forceinline__ void turn_queries(const Args& a, const float2* turns,
     const int items = half + (a.head_dim - a.rot);
     for (int i = threadIdx.x; i < mine * heads * items; i += kThreads) {
       const int row = i / items, p = i - row * items, tok = row / heads, head = head_first + row - tok * heads;
-      if (records[tok] < 0) continue;
+      if (places[tok].page < 0) continue;
       const T* src = (const T*)a.src[2] + (long long)(first + tok) * a.st[2] + head * a.sh[2];
       T* to = (T*)a.q_out + (long long)(first + tok) * a.qo_st + head * a.qo_sh;
       if (p < half) {
@@ -327,7 +346,7 @@ __device__ __forceinline__ void turn_queries(const Args& a, const float2* turns,
   const int c1 = turn ? j : 2 * pairs + 2 * (j - pairs), c2 = turn ? j + pairs : c1 + 1;
   int tok = row_first / heads, head = head_first + row_first - tok * heads;
   for (int i = row_first; i < mine * heads; i += step) {
-    if (records[tok] >= 0) {
+    if (places[tok].page >= 0) {
       const T* src = (const T*)a.src[2] + (long long)(first + tok) * a.st[2] + head * a.sh[2];
       T* to = (T*)a.q_out + (long long)(first + tok) * a.qo_st + head * a.qo_sh;
       float x[8], y[8];
@@ -367,33 +386,25 @@ __device__ __forceinline__ void turn_queries(const Args& a, const float2* turns,
   }
 }
 
-// The first record of a slot's token (that of head 0), -1 where there is none.
-__device__ __forceinline__ long long record_of(const Args& a, long long slot) {
-  if (slot >= a.num_slots && a.err) *a.err = PFC_ERR_INVALID_ARGUMENT;
-  if (slot < 0 || slot >= a.num_slots) return -1;
-  const unsigned page = a.by_page.div((unsigned)slot);
-  return (long long)page * a.heads * a.by_page.d + (slot - (long long)page * a.by_page.d);
-}
-
 // CTA (i, j): tokens i * per_cta on, and the j-th part of their heads
 template <typename T, int BLOCKS, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 8) append_kernel(Args a) {
   extern __shared__ double2 turns[];  // [per_cta][rot / 2], then the same as float2
-  __shared__ long long records[kTokens];
+  __shared__ Place places[kTokens];
   const int tid = threadIdx.x, half = a.rot >> 1;
   begin();
   const int first = blockIdx.x * a.per_cta, mine = min(a.per_cta, a.tokens - first);
   float2* turns32 = reinterpret_cast<float2*>(turns + a.per_cta * half);
   const int spread = spread_of(half, a.interleaved);
   for (int i = tid; i < mine * half; i += kThreads) {
-    const int tok = i / half, p = i - tok * half, at = tok * half + place_of(p, half, spread);
+    const int tok = i / half, p = i - tok * half, at = tok * half + angle_at(p, half, spread);
     double2 cs = cos_sin(a.positions[first + tok], a.inv_freq[p]);
     cs.x *= a.factor;
     cs.y *= a.factor;
     turns[at] = cs;
     turns32[at] = make_float2((float)cs.x, (float)cs.y);
   }
-  if (tid < mine) records[tid] = record_of(a, a.slots[first + tid]);
+  if (tid < mine) places[tid] = place_of(a, a.slots[first + tid]);
   __syncthreads();
   const int part = blockIdx.y;
   const int h0 = a.heads * part / a.split, h1 = a.heads * (part + 1) / a.split;
@@ -401,12 +412,12 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(Args a) {
   // queries are bound by memory, keys and values by their instructions: every
   // other CTA begins with the latter
   const bool late = blockIdx.x & 1;
-  if (!late && q0 < q1) turn_queries<T, WIDE>(a, turns32, records, first, mine, q0, q1);
+  if (!late && q0 < q1) turn_queries<T, WIDE>(a, turns32, places, first, mine, q0, q1);
   if (h0 < h1) {
-    store_rows<T, BLOCKS, true, WIDE>(a, turns, records, first, mine, h0, h1);
-    store_rows<T, BLOCKS, false, WIDE>(a, turns, records, first, mine, h0, h1);
+    store_rows<T, BLOCKS, true, WIDE>(a, turns, places, first, mine, h0, h1);
+    store_rows<T, BLOCKS, false, WIDE>(a, turns, places, first, mine, h0, h1);
   }
-  if (late && q0 < q1) turn_queries<T, WIDE>(a, turns32, records, first, mine, q0, q1);
+  if (late && q0 < q1) turn_queries<T, WIDE>(a, turns32, places, first, mine, q0, q1);
 }
 
 // CTA (i, j): tokens i * per_cta on, and the j-th part of their keys' and
@@ -416,10 +427,10 @@ constexpr int kReadTokens = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(kReadThreads) read_kernel(Args a) {
-  __shared__ long long firsts[kReadTokens];  // records of the tokens' first heads, -1: none
+  __shared__ Place places[kReadTokens];
   begin();
   const int tid = threadIdx.x, first = blockIdx.x * a.per_cta, mine = min(a.per_cta, a.tokens - first);
-  if (tid < mine) firsts[tid] = record_of(a, a.slots[first + tid]);
+  if (tid < mine) places[tid] = place_of(a, a.slots[first + tid]);
   __syncthreads();
   const int chunks = a.head_dim / 8, items = 2 * a.heads * chunks, each = items / a.split, rest = items % a.split;
   const int part = blockIdx.y, from = each * part + min(part, rest), to = from + each + (part < rest);
@@ -430,19 +441,20 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(Args a) {
     // words of the codes, or halves of them, and of the scales
     const uint32_t* codes = value ? a.v : a.k;
     const uint32_t* scales = (value ? a.v_scales : a.k_scales) + chunk * 8 / a.group;
-    const int place = value ? cache4_value_half(2 * chunk, a.blocks) : cache4_key_word(chunk, a.blocks);
+    const int at = value ? cache4_value_half(2 * chunk, a.blocks) : cache4_key_word(chunk, a.blocks);
     const int next = value ? cache4_value_half(2 * chunk + 1, a.blocks) : 0;
     T* out = (T*)a.out[value] + (((long long)first * a.heads + head) * chunks + chunk) * 8;
 #pragma unroll 4
     for (int tok = 0; tok < mine; ++tok) {
-      const bool there = firsts[tok] >= 0;
-      const long long record = there ? firsts[tok] + (long long)head * a.by_page.d : 0;
+      const bool there = places[tok].page >= 0;
+      const Place place = there ? places[tok] : Place{0, 0};
+      const long long record = record_of(a, place, head);
       unsigned c;
       if (value) {
-        const unsigned short* v = reinterpret_cast<const unsigned short*>(codes + record * (4 * a.blocks));
-        c = v[place] | (unsigned)v[next] << 16;
+        const unsigned short* v = reinterpret_cast<const unsigned short*>(codes) + value_at(a, place, head, a.blocks, 0);
+        c = v[2 * at] | (unsigned)v[2 * next] << 16;
       } else {
-        c = codes[record * (4 * a.blocks) + place];
+        c = codes[record * (4 * a.blocks) + at];
       }
       const unsigned word = scales[record * a.groups];
       const float step = __uint_as_float(word & 0xffff0000u), low = __uint_as_float(word << 16);

@@ -8,11 +8,14 @@
 //     up), for lane t of four and block j; a lane's words of an even number of
 //     blocks lie together, those of a last odd block (W = 96) behind;
 //   values: 16 bits hold the 4 values 32j + 4g ... + 3, for lane g of eight
-//     and block j; again a lane's even number of blocks lie together.
+//     and block j; again a lane's even number of blocks lie together.  Two
+//     tokens of a page next to each other share words, the even one's 16 bits
+//     in the low halves: the operand's registers pair keys.
 // A head's scales are a word for each group: step's bfloat16 bits in the high
 // half, low's in the low half; their number is rounded up to a power of two.
 // Token o of page p of head h is record (p * heads + h) * page_size + o of the
-// codes and of the scales: a head's tokens of a page lie together.
+// keys and of both scales, and in pair (p * heads + h) * pairs + o / 2 of the
+// values, pairs = (page_size + 1) / 2: a head's tokens of a page lie together.
 #pragma once
 
 #include <cuda_bf16.h>
