@@ -5,27 +5,31 @@
 //
 // The weights of the chosen experts are the work: 3 * width * inner values
 // each, read once for all the tokens that chose the expert, and with a few
-// tokens memory is the bound.  Three kernels, each launched as a programmatic
+// tokens memory is the bound.  Kernels, each launched as a programmatic
 // dependent of the one before:
 //
-// 1. route: a cluster of 8 CTAs for each token, or for four of many: each CTA
-//    an eighth of the experts' logits, in 64 bits, since which expert a token
-//    takes is a decision that no rounding should make; the first CTA gathers
-//    them through distributed shared memory and picks.  Copies x, aligned and
-//    padded, for the next kernel.
-// 2. up: a CTA of 4 warps for 8 gate rows and their 8 up rows of an expert,
+// 1. route: a cluster of 8 CTAs for up to 4 tokens: each CTA an eighth of the
+//    experts' logits, in 64 bits, since which expert a token takes is a
+//    decision that no rounding should make (mma.sync in 64 bits takes 500
+//    cycles an instruction on this device); the first CTA gathers them through
+//    distributed shared memory and picks.  It copies x, aligned and padded,
+//    for the next kernel, and lists the (token, choice) pairs by expert.  With
+//    more than 4 tokens a kernel of one CTA lists them.
+// 2. up: a CTA of 4 warps takes 8 gate rows and their 8 up rows of an expert,
 //    which share the 16 rows of a matrix instruction, so that a lane ends with
 //    a gate and its up value.  The warps share the summed axis, 64 bytes of a
 //    row at a time (256 consecutive bytes a CTA).  What leaves is w act(g) u
 //    in two 16-bit parts (one fp32 value): a single one would round as
 //    coarsely as the output does.
-// 3. down: a cluster for 16 rows of the output.  All (used expert, 64 bytes)
-//    pieces of those rows form one list, of which each warp of the cluster
-//    takes an equal run; at an expert's end it adds what it has to its own
-//    table of tokens in shared memory.  The tables are added in the order of
-//    warps and ranks: no atomics, the same bits each time.
+// 3. down: a cluster for 16 rows of the output.  All (expert, 64 bytes) pieces
+//    of those rows form one list, of which each warp of the cluster takes an
+//    equal run; at an expert's end it adds what it has to its own table of
+//    tokens in shared memory.  The tables are added in the order of warps and
+//    ranks: no atomics, the same bits each time.
 //
-// Rows come straight from memory into operand registers (streamed.cuh).
+// The rows come through a ring of asynchronous copies in shared memory for
+// each warp, whose lanes read what they copied, as operand registers
+// (streamed.cuh): the copies run ahead over the borders of rows and experts.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -52,9 +56,10 @@ constexpr int kMostExperts = 1024;
 constexpr int kMostTop = 32;
 constexpr int kRouteRanks = 8;
 constexpr int kRouteThreads = 256;
+constexpr int kRouteTokens = 4;  // of a cluster
+constexpr int kRouteBlock = 2048;  // values of x that it holds of a token at a time
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRouteBlock = 1024;  // values of x that the router's kernel holds of a token at a time
 
 struct Args {
   int tokens, width, inner, experts, top;
@@ -76,362 +81,515 @@ struct Args {
   long long x_row;
   char* h;  // [parts][tokens * top][h_row bytes], zeros behind inner
   long long h_row, h_part;
-  int4* used;  // how many, then of each: expert, first of its pairs, their number
+  // parts of experts' pairs: how many, then of each: expert, first of its pairs, their number (at most 8 NT)
+  int4* parts;
   int* pairs;  // [tokens * top] by expert
+  int most_parts;
 };
 
 // ---------------------------------------------------------------------------
 // route
 // ---------------------------------------------------------------------------
 
-// TB tokens a cluster
-template <typename T, int TB>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(Args a) {
-  extern __shared__ double shared[];
-  double* xd = shared;                               // [TB][kRouteBlock]
-  double* logits = shared + TB * kRouteBlock;        // [TB][experts of a rank]
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank();
-  const int share = (a.experts + kRouteRanks - 1) / kRouteRanks;
-  double* all = logits + TB * share;                 // rank 0: [TB][experts]
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int first = (int)(blockIdx.x / kRouteRanks) * TB;
-  const int mine = min(TB, a.tokens - first);
-  const int e0 = rank * share, e1 = min(a.experts, e0 + share);
-  begin();
-
-  // x for the next kernel: the cluster's CTAs share the row
-  const int padded = (int)(a.x_row / (int)sizeof(T));
-  for (int i = rank * kRouteThreads + tid; i < mine * padded; i += kRouteRanks * kRouteThreads) {
-    const int n = i / padded, d = i - n * padded;
-    reinterpret_cast<T*>(a.xs + (first + n) * a.x_row)[d] =
-        d < a.width ? ((const T*)a.x)[(first + n) * a.x_st + d] : from_float<T>(0.f);
-  }
-
-  for (int i = tid; i < TB * share; i += kRouteThreads) logits[i] = 0.0;
-  for (int base = 0; base < a.width; base += kRouteBlock) {
-    const int len = min(kRouteBlock, a.width - base);
-    const int len4 = (len + 3) & ~3;  // rows of the router are padded with zeros to a multiple of 4
-    __syncthreads();
-    for (int i = tid; i < TB * len4; i += kRouteThreads) {
-      const int n = i / len4, d = i - n * len4;
-      xd[n * kRouteBlock + d] =
-          n < mine && d < len ? (double)to_float<T>(((const T*)a.x)[(first + n) * a.x_st + base + d]) : 0.0;
-    }
-    __syncthreads();
-    for (int e = e0 + warp; e < e1; e += kRouteThreads / 32) {
-      const float4* row = reinterpret_cast<const float4*>(a.router + e * a.router_st + base);
-      double sum[TB];
+// Lists the pairs by expert, in parts of at most `most`: threads of one CTA;
+// shared: [experts + pairs] ints.  The order of an expert's pairs, of which a
+// token has one at most, has no effect: their sums are apart.
+__device__ void list_pairs(const Args& a, const int* chosen, int* shared, int most) {
+  int *hist = shared, *place = shared + a.experts;
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, pairs = a.tokens * a.top;
+  for (int e = tid; e < a.experts; e += threads) hist[e] = 0;
+  __syncthreads();
+  for (int p = tid; p < pairs; p += threads) place[p] = atomicAdd(&hist[chosen[p]], 1);
+  __syncthreads();
+  if (tid < 32) {
+    int start = 0, parts = 0;
+    for (int base = 0; base < a.experts; base += 32) {
+      const int e = base + lane, n = e < a.experts ? hist[e] : 0, own = (n + most - 1) / most;
+      int sum = n, before = own;
 #pragma unroll
-      for (int n = 0; n < TB; ++n) sum[n] = 0.0;
-#pragma unroll 4
-      for (int d = lane; d < len4 / 4; d += 32) {
-        const float4 r = row[d];
-        const double r0 = r.x, r1 = r.y, r2 = r.z, r3 = r.w;
-#pragma unroll
-        for (int n = 0; n < TB; ++n) {
-          const double2 u = *reinterpret_cast<const double2*>(xd + n * kRouteBlock + 4 * d);
-          const double2 v = *reinterpret_cast<const double2*>(xd + n * kRouteBlock + 4 * d + 2);
-          sum[n] = fma(r0, u.x, fma(r1, u.y, fma(r2, v.x, fma(r3, v.y, sum[n]))));
+      for (int o = 1; o < 32; o <<= 1) {
+        const int s = __shfl_up_sync(~0u, sum, o), b = __shfl_up_sync(~0u, before, o);
+        if (lane >= o) {
+          sum += s;
+          before += b;
         }
+      }
+      const int first = start + sum - n;
+      for (int k = 0; k < own; ++k) a.parts[1 + parts + before - own + k] = make_int4(e, first + k * most, min(most, n - k * most), 0);
+      if (e < a.experts) hist[e] = first;
+      start += __shfl_sync(~0u, sum, 31);
+      parts += __shfl_sync(~0u, before, 31);
+    }
+    if (lane == 0) a.parts[0] = make_int4(parts, 0, 0, 0);
+  }
+  __syncthreads();
+  for (int p = tid; p < pairs; p += threads) a.pairs[hist[chosen[p]] + place[p]] = p;
+}
+
+// Parts of the logits of EP experts and TB tokens, over `len` values (a
+// multiple of 4) of the router's rows and of x in shared memory: a warp, whose
+// lanes share the summed axis; sum[e][n] is whole in every lane.
+template <int TB, int EP>
+__device__ __forceinline__ void logits_of(double (&sum)[EP][TB], const float* const (&rows)[EP], const float* xs, int len) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int e = 0; e < EP; ++e)
+#pragma unroll
+    for (int n = 0; n < TB; ++n) sum[e][n] = 0.;
+  constexpr int UNROLL = TB == 1 ? 16 : 4;  // loads on their way
+  for (int d0 = 4 * lane; d0 < len; d0 += 128 * UNROLL) {
+    float4 r[UNROLL][EP];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int e = 0; e < EP; ++e)
+        r[u][e] = d0 + 128 * u < len ? __ldg(reinterpret_cast<const float4*>(rows[e] + d0 + 128 * u)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (d0 + 128 * u >= len) break;
+      double w[EP][4];
+#pragma unroll
+      for (int e = 0; e < EP; ++e) {
+        w[e][0] = r[u][e].x;
+        w[e][1] = r[u][e].y;
+        w[e][2] = r[u][e].z;
+        w[e][3] = r[u][e].w;
       }
 #pragma unroll
       for (int n = 0; n < TB; ++n) {
+        const float4 v = *reinterpret_cast<const float4*>(xs + n * kRouteBlock + d0 + 128 * u);
+        const double y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int o = 16; o; o >>= 1) sum[n] += __shfl_xor_sync(~0u, sum[n], o);
-        if (lane == 0) logits[n * share + e - e0] += sum[n];
+        for (int e = 0; e < EP; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[e][n] = fma(w[e][i], y[i], sum[e][n]);
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < EP; ++e)
+#pragma unroll
+    for (int n = 0; n < TB; ++n)
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum[e][n] += __shfl_xor_sync(~0u, sum[e][n], o);
+}
+
+// Numbers in the order of their values; NaN as the lowest.
+__device__ __forceinline__ unsigned long long ordered(double v) {
+  if (!(v >= -1.7976931348623157e308)) v = -INFINITY;
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+  return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double value_of(unsigned long long o) {
+  return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o));
+}
+
+// TB tokens a cluster
+template <typename T, int TB>
+__global__ void __launch_bounds__(kRouteThreads) route_kernel(Args a) {
+  extern __shared__ __align__(16) double shared[];
+  __shared__ int choice[TB * kMostTop];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int first = (int)(blockIdx.x / kRouteRanks) * TB, mine = min(TB, a.tokens - first);
+  const int share = (a.experts + kRouteRanks - 1) / kRouteRanks, e0 = rank * share, e1 = min(a.experts, e0 + share);
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(shared);  // rank 0: [tokens][experts]
+  double* logits = shared + TB * a.experts;                                  // [tokens][share]
+  float* xs = reinterpret_cast<float*>(logits + TB * share + (TB * (a.experts + share) & 1));  // [tokens][kRouteBlock]
+  // rank 0 has started, and its memory can be written
+  cluster.sync();
+  begin();
+
+  const T* x = (const T*)a.x + first * a.x_st;
+  const int padded = (int)(a.x_row / (int)sizeof(T));
+  constexpr int kWarpsHere = kRouteThreads / 32;
+  auto row = [&](int e, int base) { return a.router + (long long)min(e, a.experts - 1) * a.router_st + base; };
+  for (int base = 0; base < padded; base += kRouteBlock) {
+    if (base) __syncthreads();
+    // x in fp32 for this kernel, and as it is, a part by each rank, for the next
+#pragma unroll
+    for (int n = 0; n < TB; ++n) {
+      T v[kRouteBlock / kRouteThreads];
+#pragma unroll
+      for (int i = 0; i < kRouteBlock / kRouteThreads; ++i) {
+        const int d = base + i * kRouteThreads + tid;
+        v[i] = n < mine && d < a.width ? x[n * a.x_st + d] : from_float<T>(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < kRouteBlock / kRouteThreads; ++i) {
+        const int d = base + i * kRouteThreads + tid;
+        xs[n * kRouteBlock + d - base] = to_float<T>(v[i]);
+        if (i % kRouteRanks == rank && n < mine && d < padded) reinterpret_cast<T*>(a.xs + (first + n) * a.x_row)[d] = v[i];
+      }
+    }
+    __syncthreads();
+    const int len = (int)min((long long)kRouteBlock, a.router_st - base);
+    auto put = [&](int e, int n, double s) {
+      double* to = logits + n * share + e - e0;
+      *to = base ? *to + s : s;
+    };
+    if (TB > 1 && share > kWarpsHere) {  // x is read and converted once for two experts
+      for (int e = e0 + 2 * warp; e < e1; e += 2 * kWarpsHere) {
+        double sum[2][TB];
+        const float* rows[2] = {row(e, base), row(e + 1, base)};
+        logits_of<TB, 2>(sum, rows, xs, len);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int n = 0; n < TB; ++n)
+            if (lane == 0 && e + k < e1) put(e + k, n, sum[k][n]);
+      }
+    } else {
+      for (int e = e0 + warp; e < e1; e += kWarpsHere) {
+        double sum[1][TB];
+        const float* rows[1] = {row(e, base)};
+        logits_of<TB, 1>(sum, rows, xs, len);
+#pragma unroll
+        for (int n = 0; n < TB; ++n)
+          if (lane == 0) put(e, n, sum[0][n]);
       }
     }
   }
   __syncthreads();
-  cluster.sync();  // rank 0 has started, and its memory can be written
-  double* to = cluster.map_shared_rank(all, 0);
-  for (int i = tid; i < TB * (e1 - e0); i += kRouteThreads) {
+  unsigned long long* to = cluster.map_shared_rank(keys, 0);
+  for (int i = tid; i < mine * (e1 - e0); i += kRouteThreads) {
     const int n = i / (e1 - e0), e = i - n * (e1 - e0);
-    to[n * a.experts + e0 + e] = logits[n * share + e];
+    to[n * a.experts + e0 + e] = ordered(logits[n * share + e]);
   }
   cluster.sync();
-  if (rank != 0 || warp >= mine) return;
+  if (rank != 0) return;
 
-  // a warp picks for a token; NaN counts as the lowest
-  const int n = warp;
-  double* l = all + n * a.experts;
-  double best = -INFINITY;
-  for (int e = lane; e < a.experts; e += 32) {
-    if (!(l[e] >= -1.7976931348623157e308)) l[e] = -INFINITY;
-    best = fmax(best, l[e]);
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) best = fmax(best, __shfl_xor_sync(~0u, best, o));
-  float total = 0.f;
-  if (!a.renormalize) {
-    for (int e = lane; e < a.experts; e += 32) total += expf((float)(l[e] - best));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-  }
-  unsigned taken = 0;  // of the lane's experts lane + 32 i
-  float part = 0.f;    // of the choice that the lane keeps: the lane-th
-  int kept = 0;
-  for (int j = 0; j < a.top; ++j) {
-    double m = -INFINITY;
-    int at = INT_MAX;
-    for (int e = lane, i = 0; e < a.experts; e += 32, ++i) {
-      if (!(taken >> i & 1) && (at == INT_MAX || l[e] > m)) {
-        m = l[e];
-        at = e;
+  if (warp < mine) {  // a warp picks for a token
+    const unsigned long long* l = keys + warp * a.experts;
+    unsigned taken = 0;  // of the lane's experts lane + 32 i
+    unsigned long long best = 0;
+    int at = INT_MAX;  // the lane's best that is not taken
+    auto look = [&]() {
+      best = 0;
+      at = INT_MAX;
+      for (int e = lane, i = 0; e < a.experts; e += 32, ++i)
+        if (!(taken >> i & 1) && (at == INT_MAX || l[e] > best)) {
+          best = l[e];
+          at = e;
+        }
+    };
+    look();
+    double top = 0.;
+    float total = 0.f, own_part = 0.f;
+    int kept = 0;
+    for (int j = 0; j < a.top; ++j) {
+      const unsigned high = __reduce_max_sync(~0u, (unsigned)(best >> 32));
+      const unsigned low = __reduce_max_sync(~0u, (unsigned)(best >> 32) == high ? (unsigned)best : 0u);
+      const unsigned long long won = (unsigned long long)high << 32 | low;
+      const int e = (int)__reduce_min_sync(~0u, best == won ? (unsigned)at : (unsigned)INT_MAX);
+      const double v = value_of(won);
+      if (j == 0) top = v;
+      const float w = expf((float)(v - top));
+      total += w;
+      if (lane == j) {
+        own_part = w;
+        kept = e;
+      }
+      if (at == e) {
+        taken |= 1u << (e >> 5);
+        look();
       }
     }
+    if (!a.renormalize) {
+      total = 0.f;
+      for (int e = lane; e < a.experts; e += 32) total += expf((float)(value_of(l[e]) - top));
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const double om = __shfl_xor_sync(~0u, m, o);
-      const int oat = __shfl_xor_sync(~0u, at, o);
-      if (oat != INT_MAX && (at == INT_MAX || om > m || (om == m && oat < at))) {
-        m = om;
-        at = oat;
-      }
+      for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
     }
-    if ((at & 31) == lane) taken |= 1u << (at >> 5);
-    const float w = expf((float)(m - best));
-    if (a.renormalize) total += w;
-    if (lane == j) {
-      part = w;
-      kept = at;
+    if (lane < a.top) {
+      a.chosen[(long long)(first + warp) * a.top + lane] = kept;
+      a.weights[(long long)(first + warp) * a.top + lane] = own_part / total;
+      choice[warp * a.top + lane] = kept;
     }
   }
-  if (lane < a.top) {
-    a.chosen[(long long)(first + n) * a.top + lane] = kept;
-    a.weights[(long long)(first + n) * a.top + lane] = part / total;
+  if (a.tokens <= TB) {
+    __syncthreads();
+    list_pairs(a, choice, reinterpret_cast<int*>(shared), 8);
   }
 }
 
-// ---------------------------------------------------------------------------
-// up
-// ---------------------------------------------------------------------------
-
-// acc[n] += 16 rows of this warp x its vectors, over the rows' pieces of 64
-// bytes c = first, first + step, ... below `pieces`.  Bytes from `bytes` on
-// belong to no row.  PARTS: of the vectors, which add up.
-// UNROLL pieces are in flight, and share accumulators that are added to acc in
-// fp32, rounded to nearest: the tensor cores truncate what they add.
-template <typename T, int NT, int PARTS, int UNROLL>
-__device__ __forceinline__ void stream_rows(float (&acc)[NT][4], const char* row0, const char* row1, const char* const (&vec)[NT],
-                                            long long part, int first, int step, int pieces, int bytes, int t) {
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int c0 = first; c0 < pieces; c0 += step * UNROLL) {
-    uint4 a0[UNROLL], a1[UNROLL], b[UNROLL][PARTS][NT];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int at = (c0 + u * step) * 64 + t * 16;
-      const bool in = c0 + u * step < pieces && at < bytes;
-      a0[u] = in && row0 ? load_stream(row0 + at) : zero;
-      a1[u] = in && row1 ? load_stream(row1 + at) : zero;
-#pragma unroll
-      for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          b[u][p][n] = in && vec[n] ? *reinterpret_cast<const uint4*>(vec[n] + p * part + at) : zero;
-    }
-    float sum[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-#pragma unroll
-      for (int p = PARTS - 1; p >= 0; --p) chunk_product<T, NT>(sum, a0[u], a1[u], b[u][p]);
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[n][r] += sum[n][r];
-  }
+__global__ void __launch_bounds__(kRouteThreads) list_kernel(Args a) {
+  extern __shared__ double shared[];
+  begin();
+  list_pairs(a, a.chosen, reinterpret_cast<int*>(shared), a.tokens <= 8 ? 8 : 16);
 }
+
+// ---------------------------------------------------------------------------
+// up and down
+// ---------------------------------------------------------------------------
 
 template <typename T>
 struct Parts {
   static constexpr int kH = sizeof(T) == 2 ? 2 : 1;  // of an intermediate value
 };
 
-template <typename T, int NT, int UNROLL>
-__device__ __forceinline__ void up_block(const Args& a, int expert, int row, const int* list, int count, float4* red) {
+// A warp's ring: stages of a piece of 16 rows and of the vectors, NB blocks of 8.
+template <int NB, int DEPTH>
+struct Ring {
+  static constexpr int kStage = (2 + NB) * 512, kBytes = kStage * DEPTH;
+  uint32_t base;  // of the lane
+  __device__ __forceinline__ Ring(char* warp_memory) : base((uint32_t)__cvta_generic_to_shared(warp_memory) + (threadIdx.x & 31) * 16) {}
+  __device__ __forceinline__ uint32_t stage(int s) const { return base + s * kStage; }
+  static __device__ __forceinline__ uint4 read(uint32_t at) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+    return r;
+  }
+};
+
+// What the vectors of a piece add up to with its rows, added to acc in fp32,
+// rounded to nearest: the tensor cores truncate what they add.
+template <typename T, int NT, int PARTS, class R>
+__device__ __forceinline__ void take_piece(float (&acc)[NT][4], uint32_t at, bool second) {
+  const uint4 a0 = R::read(at), a1 = R::read(at + 512);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (n && !second) continue;  // the same in all lanes
+    float sum[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int p = PARTS - 1; p >= 0; --p) {
+      const uint4 b[1] = {R::read(at + 1024 + (p * NT + n) * 512)};
+      chunk_product<T, 1>(sum, a0, a1, b);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[n][r] += sum[0][r];
+  }
+}
+
+template <typename T, int NT>
+struct Up {
+  static constexpr int kDepth = NT == 1 ? 8 : 6;
+  using R = Ring<NT, kDepth>;
+  static constexpr int kResident = 4;  // CTAs an SM
+  static size_t smem(int parts, int pairs) { return (size_t)kWarps * R::kBytes + (size_t)parts * 16 + (size_t)round_up(pairs, 4) * 4; }
+};
+
+// Units are 8 rows of a part of an expert's pairs; CTAs take them in turn.
+template <typename T, int NT>
+__global__ void __launch_bounds__(kThreads, (Up<T, NT>::kResident)) up_kernel(Args a) {
+  using U = Up<T, NT>;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float4 red[2][kWarps][NT][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const char* base = a.gate_up + expert * a.up_expert;
-  const int f = row + g;
-  const char* gate = f < a.inner ? base + f * a.up_row : nullptr;
-  const char* up = f < a.inner ? base + (a.inner + (long long)f) * a.up_row : nullptr;
-  const char* vec[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) vec[n] = n * 8 + g < count ? a.xs + (long long)(list[n * 8 + g] / a.top) * a.x_row : nullptr;
-  float acc[NT][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-  const int bytes = (int)min(a.x_row, a.up_row);
-  stream_rows<T, NT, 1, UNROLL>(acc, gate, up, vec, 0, warp, kWarps, (bytes + 63) / 64, bytes, t);
-#pragma unroll
-  for (int n = 0; n < NT; ++n) red[(warp * NT + n) * 32 + lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-  __syncthreads();
-  static_assert(NT <= kWarps, "a warp finishes a block of vectors");
-  if (warp < NT) {
-    float4 s = red[warp * 32 + lane];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) {
-      const float4 v = red[(w * NT + warp) * 32 + lane];
-      s.x += v.x;
-      s.y += v.y;
-      s.z += v.z;
-      s.w += v.w;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int slot = warp * 8 + 2 * t + i;
-      if (slot >= count) continue;
-      const int pair = list[slot];
-      const float gv = i ? s.y : s.x, uv = i ? s.w : s.z;
-      const float act = a.act ? act_apply<2>(gv) : act_apply<5>(gv);
-      // rows behind the last are zeros (their sums are)
-      const float v = act * uv * a.weights[pair];
-      T* to = reinterpret_cast<T*>(a.h + pair * a.h_row) + f;
-      if constexpr (sizeof(T) == 4) {
-        *to = v;
-      } else {
-        T hi, lo;
-        two_parts(v, hi, lo);
-        *to = hi;
-        *reinterpret_cast<T*>(reinterpret_cast<char*>(to) + a.h_part) = lo;
-      }
-    }
-  }
-  __syncthreads();
-}
-
-// grid: (blocks of 8 rows + 1, experts or pairs).  The extra block of the
-// first row lists the pairs by expert for the next kernel.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) up_kernel(Args a) {
-  __shared__ float4 red[kWarps * 4 * 32];
-  extern __shared__ int list[];  // [pairs]
-  __shared__ int counts[kWarps];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int4* parts = reinterpret_cast<int4*>(smem + kWarps * U::R::kBytes);
+  int* pairs = reinterpret_cast<int*>(parts + a.most_parts);
+  typename U::R ring(smem + warp * U::R::kBytes);
   begin();
-  const int pairs = a.tokens * a.top;
+  for (int i = tid; i < a.most_parts; i += kThreads) parts[i] = a.parts[1 + i];  // those behind the last are not looked at
+  for (int i = tid; i < a.tokens * a.top; i += kThreads) pairs[i] = a.pairs[i];
+  const int blocks = (a.inner + 7) / 8, units = a.parts[0].x * blocks;
+  const int bytes = (int)min(a.x_row, a.up_row), pieces = (bytes + 63) / 64;
+  __syncthreads();
+  if ((int)blockIdx.x >= units) return;
 
-  if (blockIdx.x == gridDim.x - 1) {
-    if (blockIdx.y) return;
-    __shared__ int hist[kMostExperts];
-    for (int e = tid; e < a.experts; e += kThreads) hist[e] = 0;
-    __syncthreads();
-    // the order of an expert's pairs has no effect: a token has one of them
-    // at most, and their sums are apart
-    for (int p = tid; p < pairs; p += kThreads) list[p] = atomicAdd(&hist[a.chosen[p]], 1);
-    __syncthreads();
-    if (warp == 0) {  // starts of the used experts
-      int start = 0, used = 0;
-      for (int base = 0; base < a.experts; base += 32) {
-        const int e = base + lane, n = e < a.experts ? hist[e] : 0;
-        int sum = n;
+  // what the copies stand at
+  struct {
+    int unit, piece;
+    const char *gate, *up, *vec[NT];
+    bool second;
+  } ahead = {};
+  auto aim = [&]() {  // at the unit's rows
+    const int i = ahead.unit / blocks, f = (ahead.unit - i * blocks) * 8 + g;
+    const int4 p = parts[i];
+    const char* base = a.gate_up + p.x * a.up_expert;
+    ahead.gate = f < a.inner ? base + f * a.up_row : nullptr;
+    ahead.up = f < a.inner ? base + (a.inner + (long long)f) * a.up_row : nullptr;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int up = __shfl_up_sync(~0u, sum, o);
-          if (lane >= o) sum += up;
+    for (int n = 0; n < NT; ++n) ahead.vec[n] = n * 8 + g < p.z ? a.xs + (long long)(pairs[p.y + n * 8 + g] / a.top) * a.x_row : nullptr;
+    ahead.second = p.z > 8;
+  };
+  auto copy = [&](int s) {
+    if (ahead.unit < units) {
+      const uint32_t to = ring.stage(s);
+      const int at = ahead.piece * 64 + t * 16;
+      const bool in = at < bytes;
+      copy_async(to, in && ahead.gate ? ahead.gate + at : nullptr, a.xs);
+      copy_async(to + 512, in && ahead.up ? ahead.up + at : nullptr, a.xs);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (n == 0 || ahead.second) copy_async(to + 1024 + n * 512, in && ahead.vec[n] ? ahead.vec[n] + at : nullptr, a.xs);
+      ahead.piece += kWarps;
+      if (ahead.piece >= pieces) {
+        ahead.piece = warp;
+        ahead.unit += gridDim.x;
+        if (ahead.unit < units) aim();
+      }
+    }
+    copy_commit();
+  };
+  ahead.unit = warp < pieces ? (int)blockIdx.x : units;  // a warp without pieces has nothing to copy
+  ahead.piece = warp;
+  if (ahead.unit < units) aim();
+#pragma unroll
+  for (int s = 0; s < U::kDepth; ++s) copy(s);
+
+  int stage = 0, turn = 0;
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
+    const int i = unit / blocks, f = (unit - i * blocks) * 8 + g;
+    const int4 p = parts[i];
+    // of the block of vectors that this warp finishes
+    int pair[2] = {-1, -1};
+    float weight[2];
+    if (warp < NT) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int slot = warp * 8 + 2 * t + k;
+        if (slot < p.z) {
+          pair[k] = pairs[p.y + slot];
+          weight[k] = a.weights[pair[k]];
         }
-        const unsigned some = __ballot_sync(~0u, n > 0);
-        if (n) a.used[1 + used + __popc(some & ((1u << lane) - 1))] = make_int4(e, start + sum - n, n, 0);
-        if (e < a.experts) hist[e] = start + sum - n;
-        start += __shfl_sync(~0u, sum, 31);
-        used += __popc(some);
       }
-      if (lane == 0) a.used[0] = make_int4(used, 0, 0, 0);
     }
+    float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    for (int c = warp; c < pieces; c += kWarps) {
+      copy_wait<U::kDepth - 1>();
+      take_piece<T, NT, 1, typename U::R>(acc, ring.stage(stage), p.z > 8);
+      copy(stage);
+      if (++stage == U::kDepth) stage = 0;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) red[turn][warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
     __syncthreads();
-    for (int p = tid; p < pairs; p += kThreads) a.pairs[hist[a.chosen[p]] + list[p]] = p;
-    return;
-  }
-
-  // the block's expert and the pairs that chose it: with fewer pairs than
-  // experts, the expert of pair y where that is the first of its pairs
-  const bool by_pair = pairs < a.experts;
-  const int expert = by_pair ? a.chosen[blockIdx.y] : (int)blockIdx.y;
-  int count = 0;
-  for (int base = 0; base < pairs; base += kThreads) {
-    const int p = base + tid;
-    const bool match = p < pairs && a.chosen[p] == expert;
-    const unsigned some = __ballot_sync(~0u, match);
-    if (lane == 0) counts[warp] = __popc(some);
-    __syncthreads();
-    int at = count;
-    for (int w = 0; w < warp; ++w) at += counts[w];
-    if (match) list[at + __popc(some & ((1u << lane) - 1))] = p;
-    for (int w = 0; w < kWarps; ++w) count += counts[w];
-    __syncthreads();
-  }
-  if (count == 0 || (by_pair && list[0] != (int)blockIdx.y)) return;
-  const int row = blockIdx.x * 8;
-  for (int at = 0; at < count; at += 32) {
-    const int some = min(32, count - at);
-    if (some <= 8) up_block<T, 1, 8>(a, expert, row, list + at, some, red);
-    else if (some <= 16) up_block<T, 2, 4>(a, expert, row, list + at, some, red);
-    else up_block<T, 4, 2>(a, expert, row, list + at, some, red);
+    static_assert(NT <= kWarps, "a warp finishes a block of vectors");
+    if (warp < NT) {
+      float4 s = red[turn][0][warp][lane];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) {
+        const float4 v = red[turn][w][warp][lane];
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (pair[k] < 0) continue;
+        const float gv = k ? s.y : s.x, uv = k ? s.w : s.z;
+        const float act = a.act ? act_apply<2>(gv) : act_apply<5>(gv);
+        // rows behind the last are zeros (their sums are)
+        const float v = f < a.inner ? act * uv * weight[k] : 0.f;
+        T* to = reinterpret_cast<T*>(a.h + pair[k] * a.h_row) + f;
+        if constexpr (sizeof(T) == 4) {
+          *to = v;
+        } else {
+          T hi, lo;
+          two_parts(v, hi, lo);
+          *to = hi;
+          *reinterpret_cast<T*>(reinterpret_cast<char*>(to) + a.h_part) = lo;
+        }
+      }
+    }
   }
 }
 
-// ---------------------------------------------------------------------------
-// down
-// ---------------------------------------------------------------------------
+template <typename T, int NT>
+struct Down {
+  static constexpr int kDepth = NT == 1 ? 6 : 4;
+  using R = Ring<NT * Parts<T>::kH, kDepth>;
+  static constexpr int kResident = NT == 1 ? 4 : 3;
+  static size_t smem(int parts, int pairs, int tokens) {
+    return (size_t)kWarps * (R::kBytes + tokens * 64) + (size_t)parts * 16 + (size_t)round_up(pairs, 4) * 4;
+  }
+};
 
-// One expert's pieces [c0, c1) for some of its pairs, added to the warp's table.
-template <typename T, int NT, int UNROLL>
-__device__ __forceinline__ void down_run(const Args& a, const char* row0, const char* row1, int bytes, int first, int count, int c0,
-                                         int c1, float* table) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const char* vec[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) vec[n] = n * 8 + g < count ? a.h + (long long)a.pairs[first + n * 8 + g] * a.h_row : nullptr;
-  float acc[NT][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-  stream_rows<T, NT, Parts<T>::kH, UNROLL>(acc, row0, row1, vec, a.h_part, c0, 1, c1, bytes, t);
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int slot = n * 8 + 2 * t + i;
-      if (slot < count) {
-        float* to = table + a.pairs[first + slot] / a.top * 16;
-        to[g] += acc[n][i];
-        to[g + 8] += acc[n][i + 2];
-      }
-    }
-  __syncwarp();
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) down_kernel(Args a) {
-  extern __shared__ float tables[];  // [warps][tokens][16]
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
+template <typename T, int NT>
+__global__ void __launch_bounds__(kThreads, (Down<T, NT>::kResident)) down_kernel(Args a) {
+  using D = Down<T, NT>;
+  constexpr int PARTS = Parts<T>::kH;
+  extern __shared__ __align__(16) char smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int row = (int)(blockIdx.x / ranks) * 16;
-  const int cells = a.tokens * 16;
+  const int row = (int)(blockIdx.x / ranks) * 16, cells = a.tokens * 16;
+  float* tables = reinterpret_cast<float*>(smem + kWarps * D::R::kBytes);  // [warps][tokens][16]
+  int4* parts = reinterpret_cast<int4*>(tables + kWarps * cells);
+  int* pairs = reinterpret_cast<int*>(parts + a.most_parts);
+  typename D::R ring(smem + warp * D::R::kBytes);
   for (int i = tid; i < kWarps * cells; i += kThreads) tables[i] = 0.f;
   begin();
+  for (int i = tid; i < a.most_parts; i += kThreads) parts[i] = a.parts[1 + i];
+  for (int i = tid; i < a.tokens * a.top; i += kThreads) pairs[i] = a.pairs[i];
   const int bytes = (int)min(a.h_row, a.down_row), pieces = (bytes + 63) / 64;
-  const int used = a.used[0].x;
-  const int total = used * pieces, q = rank * kWarps + warp, of = ranks * kWarps;
+  const int total = a.parts[0].x * pieces, q = rank * kWarps + warp, of = ranks * kWarps;
   const int p0 = (int)((long long)total * q / of), p1 = (int)((long long)total * (q + 1) / of);
   __syncthreads();
-  float* table = tables + warp * cells;
-  for (int p = p0; p < p1;) {
-    const int i = p / pieces, c0 = p - i * pieces, c1 = min(pieces, c0 + p1 - p);
-    const int4 u = a.used[1 + i];
-    const char* base = a.down + u.x * a.down_expert;
-    const char* row0 = row + g < a.width ? base + (row + g) * a.down_row : nullptr;
-    const char* row1 = row + g + 8 < a.width ? base + (row + g + 8) * a.down_row : nullptr;
-    for (int at = 0; at < u.z; at += 32) {
-      const int some = min(32, u.z - at);
-      if (some <= 8) down_run<T, 1, sizeof(T) == 2 ? 4 : 8>(a, row0, row1, bytes, u.y + at, some, c0, c1, table);
-      else if (some <= 16) down_run<T, 2, 4>(a, row0, row1, bytes, u.y + at, some, c0, c1, table);
-      else down_run<T, 4, 2>(a, row0, row1, bytes, u.y + at, some, c0, c1, table);
+
+  struct {
+    int at, part, piece;
+    const char *row0, *row1, *vec[NT];
+    bool second;
+  } ahead = {p0, pieces ? p0 / pieces : 0, 0, nullptr, nullptr, {}, false};
+  ahead.piece = p0 - ahead.part * pieces;
+  auto aim = [&]() {
+    const int4 p = parts[ahead.part];
+    const char* base = a.down + p.x * a.down_expert;
+    ahead.row0 = row + g < a.width ? base + (row + g) * a.down_row : nullptr;
+    ahead.row1 = row + g + 8 < a.width ? base + (row + g + 8) * a.down_row : nullptr;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) ahead.vec[n] = n * 8 + g < p.z ? a.h + (long long)pairs[p.y + n * 8 + g] * a.h_row : nullptr;
+    ahead.second = p.z > 8;
+  };
+  auto copy = [&](int s) {
+    if (ahead.at < p1) {
+      const uint32_t to = ring.stage(s);
+      const int at = ahead.piece * 64 + t * 16;
+      const bool in = at < bytes;
+      copy_async(to, in && ahead.row0 ? ahead.row0 + at : nullptr, a.h);
+      copy_async(to + 512, in && ahead.row1 ? ahead.row1 + at : nullptr, a.h);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (n == 0 || ahead.second) {
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p)
+            copy_async(to + 1024 + (p * NT + n) * 512, in && ahead.vec[n] ? ahead.vec[n] + p * a.h_part + at : nullptr, a.h);
+        }
+      if (++ahead.piece == pieces) {
+        ahead.piece = 0;
+        ++ahead.part;
+        if (ahead.at + 1 < p1) aim();
+      }
+      ++ahead.at;
     }
-    p += c1 - c0;
+    copy_commit();
+  };
+  if (p0 < p1) aim();
+#pragma unroll
+  for (int s = 0; s < D::kDepth; ++s) copy(s);
+
+  float* table = tables + warp * cells;
+  int stage = 0;
+  for (int p = p0; p < p1;) {
+    const int i = p / pieces, end = min(p1, (i + 1) * pieces);
+    const int4 e = parts[i];
+    float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    for (; p < end; ++p) {
+      copy_wait<D::kDepth - 1>();
+      take_piece<T, NT, PARTS, typename D::R>(acc, ring.stage(stage), e.z > 8);
+      copy(stage);
+      if (++stage == D::kDepth) stage = 0;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int slot = n * 8 + 2 * t + k;
+        if (slot < e.z) {
+          float* to = table + pairs[e.y + slot] / a.top * 16;
+          to[g] += acc[n][k];
+          to[g + 8] += acc[n][k + 2];
+        }
+      }
+    __syncwarp();
   }
   __syncthreads();
   for (int i = tid; i < cells; i += kThreads) {
@@ -440,14 +598,15 @@ __global__ void __launch_bounds__(kThreads) down_kernel(Args a) {
     for (int w = 1; w < kWarps; ++w) s += tables[w * cells + i];
     tables[i] = s;
   }
-  cluster.sync();
+  if (ranks > 1) cluster.sync();
+  else __syncthreads();
   for (int i = rank * kThreads + tid; i < cells; i += kThreads * ranks) {
     float s = 0.f;
     for (int r = 0; r < ranks; ++r) s += cluster.map_shared_rank(tables, r)[i];
     const int n = i >> 4, d = row + (i & 15);
     if (d < a.width) ((T*)a.y)[n * a.y_st + d] = from_float<T>(s);
   }
-  cluster.sync();  // the others' reads of this CTA's table are over
+  if (ranks > 1) cluster.sync();  // the others' reads of this CTA's table are over
 }
 
 // ---------------------------------------------------------------------------
@@ -471,40 +630,85 @@ void check(const pfk_experts_params& p) {
 
 struct Plan {
   int64_t block, x_row, h_row, h_part;  // of a pass
-  int64_t h_at, used_at, pairs_at, chosen_at, weights_at, bytes;
+  int64_t most_parts, h_at, parts_at, pairs_at, chosen_at, weights_at, bytes;
 };
+
+// At most so many parts of experts' pairs.
+int64_t parts_of(const pfk_experts_params& p, int64_t tokens) {
+  const int64_t pairs = tokens * p.top;
+  return std::min(pairs, p.experts) + (tokens > 8 ? pairs / 16 : 0);
+}
 
 Plan plan_of(const pfk_experts_params& p) {
   Plan w;
   const int64_t es = size_of(p.dtype);
   w.block = std::min<int64_t>(p.tokens, kBlockTokens);
   const int64_t pairs = w.block * p.top;
+  w.most_parts = parts_of(p, w.block);
   w.x_row = round_up(p.width * es, 16);
   w.h_row = round_up(round_up(p.inner, 8) * es, 16);
   w.h_part = pairs * w.h_row;
   w.h_at = round_up(w.block * w.x_row, 128);
-  w.used_at = round_up(w.h_at + w.h_part * (es == 2 ? 2 : 1), 128);
-  w.pairs_at = round_up(w.used_at + (std::min(pairs, p.experts) + 1) * (int64_t)sizeof(int4), 128);
+  w.parts_at = round_up(w.h_at + w.h_part * (es == 2 ? 2 : 1), 128);
+  w.pairs_at = round_up(w.parts_at + (w.most_parts + 1) * (int64_t)sizeof(int4), 128);
   w.chosen_at = round_up(w.pairs_at + pairs * 4, 128);
   w.weights_at = round_up(w.chosen_at + pairs * 4, 128);
   w.bytes = w.weights_at + pairs * 4;
   return w;
 }
 
+// Sets what a kernel may take of shared memory, once per device, and asks how
+// many of its CTAs share an SM (with the usual amount).
+template <typename F>
+int resident(F kernel, size_t most, size_t usual, std::once_flag* once, int* per) {
+  const int dev = current_device();
+  std::call_once(once[dev], [&] {
+    PFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    PFB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per[dev], kernel, kThreads, usual));
+    per[dev] = std::max(1, per[dev]);
+  });
+  return per[dev];
+}
+
+constexpr size_t kSharedOfSm = 228 * 1024;
+constexpr int kMostPairs = kBlockTokens * kMostTop, kMostParts = kMostExperts + kMostPairs / 16;
+
+template <typename T, int NT>
+void launch_products(const Args& a, cudaStream_t stream) {
+  using U = Up<T, NT>;
+  using D = Down<T, NT>;
+  const int sms = device_sm_count(current_device()), pairs = a.tokens * a.top;
+  static std::once_flag once_up[64], once_down[64];
+  static int per_up[64], per_down[64];
+  const int per = resident(up_kernel<T, NT>, U::smem(kMostParts, kMostPairs), U::smem(64, 64), once_up, per_up);
+  const int64_t units = (int64_t)a.most_parts * ceil_div(a.inner, 8);
+  launch_following<Args>(up_kernel<T, NT>, dim3((unsigned)std::min<int64_t>(units, (int64_t)per * sms)), kThreads, U::smem(a.most_parts, pairs),
+                         stream, a);
+  resident(down_kernel<T, NT>, D::smem(kMostParts, kMostPairs, kBlockTokens), D::smem(64, 64, 8 * NT), once_down, per_down);
+  // as many CTAs as the device holds at once (a second round of few would take as
+  // long as the first), but runs of at least 8 pieces for a warp
+  const size_t smem = D::smem(a.most_parts, pairs, a.tokens);
+  const int64_t blocks = ceil_div(a.width, 16), pieces = a.most_parts * ceil_div(a.h_row, 64);
+  const int64_t slots = std::min<int64_t>(D::kResident, (int64_t)(kSharedOfSm / (smem + 1024))) * sms;
+  int ranks = 1;
+  while (ranks < 8 && blocks * (ranks + 1) <= slots && pieces >= 8 * kWarps * (ranks + 1)) ++ranks;
+  launch_following<Args>(down_kernel<T, NT>, dim3((unsigned)(blocks * ranks)), kThreads, smem, stream, a, ranks);
+}
+
 template <int TB>
 size_t route_smem(int64_t experts) {
-  return (size_t)TB * (kRouteBlock + ceil_div(experts, kRouteRanks) + experts) * sizeof(double);
+  const int64_t doubles = TB * (experts + ceil_div(experts, kRouteRanks));
+  return (size_t)((doubles + (doubles & 1)) * 8 + TB * kRouteBlock * 4);
 }
 
 template <typename T, int TB>
-void launch_route(const Args& a, cudaStream_t stream) {
+void launch_route(const Args& a, size_t list, cudaStream_t stream) {
   static std::once_flag once[64];
   std::call_once(once[current_device()], [] {
     PFB_CUDA(cudaFuncSetAttribute(route_kernel<T, TB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)route_smem<TB>(kMostExperts)));
   });
-  const size_t smem = route_smem<TB>(a.experts);
-  launch_following<Args>(route_kernel<T, TB>, dim3((unsigned)(ceil_div(a.tokens, TB) * kRouteRanks)), kRouteThreads, smem, stream, a,
-                         kRouteRanks);
+  launch_following<Args>(route_kernel<T, TB>, dim3((unsigned)(ceil_div(a.tokens, TB) * kRouteRanks)), kRouteThreads,
+                         std::max(route_smem<TB>(a.experts), list), stream, a, kRouteRanks);
 }
 
 template <typename T>
@@ -517,17 +721,11 @@ void launch_typed(const pfk_experts_params& p, const Plan& w, Args a, cudaStream
     if (p.weights) a.weights = p.weights + first * p.top;
     const int pairs = a.tokens * a.top;
     a.h_part = pairs * w.h_row;
-    a.tokens <= 16 ? launch_route<T, 1>(a, stream) : launch_route<T, 4>(a, stream);
-    const size_t list = (size_t)pairs * 4;
-    launch_following<Args>(up_kernel<T>, dim3((unsigned)(ceil_div(p.inner, 8) + 1), (unsigned)std::min<int64_t>(pairs, p.experts)),
-                           kThreads, list, stream, a);
-    // enough CTAs for the device, but runs of at least 8 pieces for a warp
-    const int64_t blocks = ceil_div(p.width, 16), pieces = std::min<int64_t>(pairs, p.experts) * ceil_div(w.h_row, 64);
-    const int sms = device_sm_count(current_device());
-    int ranks = 1;
-    while (ranks < 8 && blocks * ranks < 4 * sms && pieces >= 8 * kWarps * 2 * ranks) ranks *= 2;
-    const size_t tables = (size_t)kWarps * a.tokens * 16 * sizeof(float);
-    launch_following<Args>(down_kernel<T>, dim3((unsigned)(blocks * ranks)), kThreads, tables, stream, a, ranks);
+    a.most_parts = (int)parts_of(p, a.tokens);
+    const size_t list = (size_t)(a.experts + pairs) * sizeof(int);
+    a.tokens == 1 ? launch_route<T, 1>(a, list, stream) : launch_route<T, kRouteTokens>(a, list, stream);
+    if (a.tokens > kRouteTokens) launch_following<Args>(list_kernel, dim3(1), kRouteThreads, list, stream, a);
+    a.tokens <= 8 ? launch_products<T, 1>(a, stream) : launch_products<T, 2>(a, stream);
   }
 }
 
@@ -570,7 +768,7 @@ void launch_experts(const pfk_experts_params& p, cudaStream_t stream) {
   a.x_row = w.x_row;
   a.h = ws + w.h_at;
   a.h_row = w.h_row;
-  a.used = (int4*)(ws + w.used_at);
+  a.parts = (int4*)(ws + w.parts_at);
   a.pairs = (int*)(ws + w.pairs_at);
   a.chosen = (int*)(ws + w.chosen_at);
   a.weights = (float*)(ws + w.weights_at);

@@ -58,6 +58,18 @@ __device__ __forceinline__ void split_tf32(unsigned x, unsigned& hi, unsigned& l
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(__uint_as_float(x) - __uint_as_float(hi)));
 }
 
+// Asynchronous copies of 16 bytes into shared memory, zeros where `from` is
+// null.  A lane reads only what it copied itself, so that waiting for its own
+// copies is enough.
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, const void* any) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from ? from : any), "r"(from ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
 // c[n] += 16 rows x 8 vectors of one chunk, for NT blocks of vectors
 template <typename T, int NT>
 __device__ __forceinline__ void chunk_product(float (&c)[NT][4], const uint4& a0, const uint4& a1, const uint4 (&b)[NT]) {
