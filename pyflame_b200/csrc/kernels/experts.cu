@@ -87,6 +87,11 @@ struct Args {
   int most_parts;
 };
 
+// Lets the next kernel come up while this one works: the kernels in front of
+// another leave room for its CTAs, or their own are all there already.  The
+// next one's wait in begin() is the same.
+__device__ __forceinline__ void let_next_come() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------
 // route
 // ---------------------------------------------------------------------------
@@ -197,6 +202,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(Args a) {
   unsigned long long* keys = reinterpret_cast<unsigned long long*>(shared);  // rank 0: [tokens][experts]
   double* logits = shared + TB * a.experts;                                  // [tokens][share]
   float* xs = reinterpret_cast<float*>(logits + TB * share + (TB * (a.experts + share) & 1));  // [tokens][kRouteBlock]
+  if (gridDim.x == kRouteRanks) let_next_come();  // the others' SMs are free
   // rank 0 has started, and its memory can be written
   cluster.sync();
   begin();
@@ -316,6 +322,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(Args a) {
 
 __global__ void __launch_bounds__(kRouteThreads) list_kernel(Args a) {
   extern __shared__ double shared[];
+  let_next_come();
   begin();
   list_pairs(a, a.chosen, reinterpret_cast<int*>(shared), a.tokens <= 8 ? 8 : 16);
 }
@@ -335,7 +342,6 @@ struct Ring {
   static constexpr int kStage = (2 + NB) * 512, kBytes = kStage * DEPTH;
   uint32_t base;  // of the lane
   __device__ __forceinline__ Ring(char* warp_memory) : base((uint32_t)__cvta_generic_to_shared(warp_memory) + (threadIdx.x & 31) * 16) {}
-  __device__ __forceinline__ uint32_t stage(int s) const { return base + s * kStage; }
   static __device__ __forceinline__ uint4 read(uint32_t at) {
     uint4 r;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
@@ -388,35 +394,46 @@ __global__ void __launch_bounds__(kThreads, (Up<T, NT>::kResident)) up_kernel(Ar
   __syncthreads();
   if ((int)blockIdx.x >= units) return;
 
-  // what the copies stand at
+  // What the copies stand at.  Rows and vectors that are not there are read
+  // nowhere: their size is 0, their place some other's.
   struct {
-    int unit, piece;
+    int unit, at;
     const char *gate, *up, *vec[NT];
+    int rows, vecs[NT];  // sizes
     bool second;
   } ahead = {};
   auto aim = [&]() {  // at the unit's rows
     const int i = ahead.unit / blocks, f = (ahead.unit - i * blocks) * 8 + g;
     const int4 p = parts[i];
-    const char* base = a.gate_up + p.x * a.up_expert;
-    ahead.gate = f < a.inner ? base + f * a.up_row : nullptr;
-    ahead.up = f < a.inner ? base + (a.inner + (long long)f) * a.up_row : nullptr;
+    ahead.at = warp * 64 + t * 16;
+    ahead.rows = f < a.inner ? 16 : 0;
+    ahead.gate = a.gate_up + p.x * a.up_expert + min(f, a.inner - 1) * a.up_row + ahead.at;
+    ahead.up = ahead.gate + a.inner * a.up_row;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) ahead.vec[n] = n * 8 + g < p.z ? a.xs + (long long)(pairs[p.y + n * 8 + g] / a.top) * a.x_row : nullptr;
+    for (int n = 0; n < NT; ++n) {
+      const int slot = n * 8 + g;
+      ahead.vecs[n] = slot < p.z ? 16 : 0;
+      ahead.vec[n] = a.xs + (long long)(pairs[p.y + min(slot, p.z - 1)] / a.top) * a.x_row + ahead.at;
+    }
     ahead.second = p.z > 8;
   };
-  auto copy = [&](int s) {
+  auto copy = [&](uint32_t to) {
     if (ahead.unit < units) {
-      const uint32_t to = ring.stage(s);
-      const int at = ahead.piece * 64 + t * 16;
-      const bool in = at < bytes;
-      copy_async(to, in && ahead.gate ? ahead.gate + at : nullptr, a.xs);
-      copy_async(to + 512, in && ahead.up ? ahead.up + at : nullptr, a.xs);
+      const bool in = ahead.at < bytes;
+      copy_async(to, ahead.gate, in ? ahead.rows : 0);
+      copy_async(to + 512, ahead.up, in ? ahead.rows : 0);
+      copy_async(to + 1024, ahead.vec[0], in ? ahead.vecs[0] : 0);
+      if (NT > 1 && ahead.second) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        if (n == 0 || ahead.second) copy_async(to + 1024 + n * 512, in && ahead.vec[n] ? ahead.vec[n] + at : nullptr, a.xs);
-      ahead.piece += kWarps;
-      if (ahead.piece >= pieces) {
-        ahead.piece = warp;
+        for (int n = 1; n < NT; ++n) copy_async(to + 1024 + n * 512, ahead.vec[n], in ? ahead.vecs[n] : 0);
+      }
+      constexpr int kStep = kWarps * 64;
+      ahead.at += kStep;
+      ahead.gate += kStep;
+      ahead.up += kStep;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) ahead.vec[n] += kStep;
+      if (ahead.at - t * 16 >= bytes) {
         ahead.unit += gridDim.x;
         if (ahead.unit < units) aim();
       }
@@ -424,12 +441,12 @@ __global__ void __launch_bounds__(kThreads, (Up<T, NT>::kResident)) up_kernel(Ar
     copy_commit();
   };
   ahead.unit = warp < pieces ? (int)blockIdx.x : units;  // a warp without pieces has nothing to copy
-  ahead.piece = warp;
   if (ahead.unit < units) aim();
+  uint32_t at = ring.base;
 #pragma unroll
-  for (int s = 0; s < U::kDepth; ++s) copy(s);
+  for (int s = 0; s < U::kDepth; ++s) copy(at + s * U::R::kStage);
 
-  int stage = 0, turn = 0;
+  int turn = 0;
   for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
     const int i = unit / blocks, f = (unit - i * blocks) * 8 + g;
     const int4 p = parts[i];
@@ -451,9 +468,9 @@ __global__ void __launch_bounds__(kThreads, (Up<T, NT>::kResident)) up_kernel(Ar
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     for (int c = warp; c < pieces; c += kWarps) {
       copy_wait<U::kDepth - 1>();
-      take_piece<T, NT, 1, typename U::R>(acc, ring.stage(stage), p.z > 8);
-      copy(stage);
-      if (++stage == U::kDepth) stage = 0;
+      take_piece<T, NT, 1, typename U::R>(acc, at, p.z > 8);
+      copy(at);
+      at = at == ring.base + (U::kDepth - 1) * U::R::kStage ? ring.base : at + U::R::kStage;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) red[turn][warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
@@ -523,49 +540,61 @@ __global__ void __launch_bounds__(kThreads, (Down<T, NT>::kResident)) down_kerne
   __syncthreads();
 
   struct {
-    int at, part, piece;
+    int left, part, at;
     const char *row0, *row1, *vec[NT];
+    int rows0, rows1, vecs[NT];  // sizes, as above
     bool second;
-  } ahead = {p0, pieces ? p0 / pieces : 0, 0, nullptr, nullptr, {}, false};
-  ahead.piece = p0 - ahead.part * pieces;
-  auto aim = [&]() {
+  } ahead = {};
+  auto aim = [&](int piece) {
     const int4 p = parts[ahead.part];
-    const char* base = a.down + p.x * a.down_expert;
-    ahead.row0 = row + g < a.width ? base + (row + g) * a.down_row : nullptr;
-    ahead.row1 = row + g + 8 < a.width ? base + (row + g + 8) * a.down_row : nullptr;
+    ahead.at = piece * 64 + t * 16;
+    ahead.rows0 = row + g < a.width ? 16 : 0;
+    ahead.rows1 = row + g + 8 < a.width ? 16 : 0;
+    const char* base = a.down + p.x * a.down_expert + ahead.at;
+    ahead.row0 = base + min(row + g, a.width - 1) * a.down_row;
+    ahead.row1 = base + min(row + g + 8, a.width - 1) * a.down_row;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) ahead.vec[n] = n * 8 + g < p.z ? a.h + (long long)pairs[p.y + n * 8 + g] * a.h_row : nullptr;
+    for (int n = 0; n < NT; ++n) {
+      const int slot = n * 8 + g;
+      ahead.vecs[n] = slot < p.z ? 16 : 0;
+      ahead.vec[n] = a.h + (long long)pairs[p.y + min(slot, p.z - 1)] * a.h_row + ahead.at;
+    }
     ahead.second = p.z > 8;
   };
-  auto copy = [&](int s) {
-    if (ahead.at < p1) {
-      const uint32_t to = ring.stage(s);
-      const int at = ahead.piece * 64 + t * 16;
-      const bool in = at < bytes;
-      copy_async(to, in && ahead.row0 ? ahead.row0 + at : nullptr, a.h);
-      copy_async(to + 512, in && ahead.row1 ? ahead.row1 + at : nullptr, a.h);
+  auto copy = [&](uint32_t to) {
+    if (ahead.left) {
+      const bool in = ahead.at < bytes;
+      copy_async(to, ahead.row0, in ? ahead.rows0 : 0);
+      copy_async(to + 512, ahead.row1, in ? ahead.rows1 : 0);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
         if (n == 0 || ahead.second) {
 #pragma unroll
-          for (int p = 0; p < PARTS; ++p)
-            copy_async(to + 1024 + (p * NT + n) * 512, in && ahead.vec[n] ? ahead.vec[n] + p * a.h_part + at : nullptr, a.h);
+          for (int p = 0; p < PARTS; ++p) copy_async(to + 1024 + (p * NT + n) * 512, ahead.vec[n] + p * a.h_part, in ? ahead.vecs[n] : 0);
         }
-      if (++ahead.piece == pieces) {
-        ahead.piece = 0;
+      ahead.at += 64;
+      ahead.row0 += 64;
+      ahead.row1 += 64;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) ahead.vec[n] += 64;
+      --ahead.left;
+      if (ahead.at - t * 16 >= bytes) {
         ++ahead.part;
-        if (ahead.at + 1 < p1) aim();
+        if (ahead.left) aim(0);
       }
-      ++ahead.at;
     }
     copy_commit();
   };
-  if (p0 < p1) aim();
+  ahead.left = p1 - p0;
+  if (p0 < p1) {
+    ahead.part = p0 / pieces;
+    aim(p0 - ahead.part * pieces);
+  }
+  uint32_t at = ring.base;
 #pragma unroll
-  for (int s = 0; s < D::kDepth; ++s) copy(s);
+  for (int s = 0; s < D::kDepth; ++s) copy(at + s * D::R::kStage);
 
   float* table = tables + warp * cells;
-  int stage = 0;
   for (int p = p0; p < p1;) {
     const int i = p / pieces, end = min(p1, (i + 1) * pieces);
     const int4 e = parts[i];
@@ -574,9 +603,9 @@ __global__ void __launch_bounds__(kThreads, (Down<T, NT>::kResident)) down_kerne
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     for (; p < end; ++p) {
       copy_wait<D::kDepth - 1>();
-      take_piece<T, NT, PARTS, typename D::R>(acc, ring.stage(stage), e.z > 8);
-      copy(stage);
-      if (++stage == D::kDepth) stage = 0;
+      take_piece<T, NT, PARTS, typename D::R>(acc, at, e.z > 8);
+      copy(at);
+      at = at == ring.base + (D::kDepth - 1) * D::R::kStage ? ring.base : at + D::R::kStage;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)

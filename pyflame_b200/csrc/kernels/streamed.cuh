@@ -51,18 +51,21 @@ __device__ __forceinline__ void mma8_tf32(float (&c)[4], unsigned a0, unsigned a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo, both tf32, hi the nearest: lo is at most 2^-11 of x and loses
-// 2^-11 of itself.  An infinity has a low part of NaN, so its products are NaN.
+// x = hi + lo: hi has the sign, the exponent and 10 bits of the mantissa, lo
+// the other 13 exactly, of which the tensor cores take the first 11: what is
+// lost is below 2^-21 of x.  (Both parts rounded to the nearest cost three
+// instructions more for each value.)  An infinity has a low part of NaN, so
+// its products are NaN.
 __device__ __forceinline__ void split_tf32(unsigned x, unsigned& hi, unsigned& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(x)));
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(__uint_as_float(x) - __uint_as_float(hi)));
+  hi = x & 0xffffe000u;
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
 }
 
-// Asynchronous copies of 16 bytes into shared memory, zeros where `from` is
-// null.  A lane reads only what it copied itself, so that waiting for its own
-// copies is enough.
-__device__ __forceinline__ void copy_async(uint32_t to, const void* from, const void* any) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from ? from : any), "r"(from ? 16 : 0) : "memory");
+// Asynchronous copies of 16 bytes into shared memory; of size 0: zeros, and
+// nothing is read.  A lane reads only what it copied itself, so that waiting
+// for its own copies is enough.
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int size) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(size) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
