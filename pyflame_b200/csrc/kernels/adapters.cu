@@ -12,10 +12,16 @@
 // the vectors of A's products (streamed.cuh).  A cluster of CTAs takes a
 // group, few rows several CTAs: each a part of x's axis in the first product,
 // whose sums meet through distributed shared memory in the order of the
-// ranks, and a part of the outputs in the second.  There the group's rows are
-// the 16 rows of a matrix instruction, and what lies between the products
-// enters as two 16-bit parts (fp32: split tf32), so that it rounds far less
-// than the output.  A lane ends with 8 neighbouring outputs of a row.
+// ranks, and a part of the outputs in the second.  What lies between the
+// products enters the second as two 16-bit parts (fp32: split tf32), so that
+// it rounds far less than the output.
+//
+// Groups of up to 8 rows read A and B, which are most of their bytes, through
+// a ring of asynchronous copies for each warp: B's copies are on their way
+// before the first product's sums have met.  In larger groups x, base and out
+// are most of the bytes: x comes through the ring, and in the second product
+// the rows are the 16 rows of a matrix instruction, so that a lane ends with 8
+// neighbouring outputs of a row.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -57,110 +63,274 @@ struct Args {
   const float* scales;
   int* err;
   int x_wide, out_wide;  // rows may be accessed 16 bytes at a time
-  int most_slots;        // 8, 16 or 32: of a group at most
+  int most_slots;        // 8 or 32: of a group at most
   int per_tile;          // clusters that share a tile's groups
 };
 
+constexpr int kRing = 10752;  // bytes of a warp's ring: 7 stages of few rows, 3 of many
+
 // 16 bytes of a row of x from byte `at` on, zeros behind the row's end
 template <typename T>
-__device__ __forceinline__ uint4 load_row(const T* row, int at, int inner, bool wide) {
+__device__ __forceinline__ uint4 load_row(const T* row, int at, int inner) {
   constexpr int VEC = 16 / sizeof(T);
   const int first = at / (int)sizeof(T);
-  if (wide && first + VEC <= inner) return *reinterpret_cast<const uint4*>(row + first);
   alignas(16) T v[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) v[e] = first + e < inner ? row[first + e] : from_float<T>(0.f);
   return *reinterpret_cast<const uint4*>(v);
 }
 
-// The first product over the CTA's pieces of x's axis, for RT blocks of 16
-// ranks from r0 on: sums[rank][slots], NT * 8 slots.
-template <typename T, int RT, int NT, int UNROLL>
-__device__ __forceinline__ void shrink(const Args& a, int adapter, int r0, const T* const (&rows)[4], int q, int of, float4* red,
-                                       float* sums) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const char* weights = a.a + ((long long)adapter * a.rank + r0 + g) * a.a_row;
-  const int bytes = (int)a.a_row, pieces = (bytes + 63) / 64;
-  float acc[RT][NT][4];
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.f;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int c0 = q; c0 < pieces; c0 += of * UNROLL) {
-    uint4 w[UNROLL][RT][2], v[UNROLL][NT];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int at = (c0 + u * of) * 64 + t * 16;
-      const bool in = at < bytes;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) v[u][n] = in && rows[n] ? load_row<T>(rows[n], at, a.inner, a.x_wide) : zero;
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        w[u][r][0] = in ? *reinterpret_cast<const uint4*>(weights + (r * 16) * a.a_row + at) : zero;
-        w[u][r][1] = in ? *reinterpret_cast<const uint4*>(weights + (r * 16 + 8) * a.a_row + at) : zero;
-      }
-    }
-    // a step's sums are added in fp32, rounded to nearest: the tensor cores truncate
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      float sum[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) chunk_product<T, NT>(sum, w[u][r][0], w[u][r][1], v[u]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[r][n][i] += sum[n][i];
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      red[((warp * RT + r) * NT + n) * 32 + lane] = make_float4(acc[r][n][0], acc[r][n][1], acc[r][n][2], acc[r][n][3]);
-  __syncthreads();
-  for (int i = tid; i < RT * NT * 32; i += kThreads) {
+__device__ __forceinline__ uint4 read_shared(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at) : "memory");
+  return r;
+}
+
+// Adds up what the warps left of `blocks` blocks of 16 ranks x 8 vectors, at
+// red + warp * pitch (in float4), to sums[rank][slots].
+__device__ __forceinline__ void add_warps(const float4* red, int pitch, int blocks, int nt, int r0, int slots, float* sums) {
+  for (int i = threadIdx.x; i < blocks * 32; i += kThreads) {
     float4 s = red[i];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) {
-      const float4 v = red[w * RT * NT * 32 + i];
+      const float4 v = red[w * pitch + i];
       s.x += v.x;
       s.y += v.y;
       s.z += v.z;
       s.w += v.w;
     }
-    const int l = i & 31, n = (i >> 5) % NT, r = (i >> 5) / NT;
-    float* to = sums + (r0 + r * 16 + (l >> 2)) * (NT * 8) + n * 8 + 2 * (l & 3);
+    const int l = i & 31, b = i >> 5, n = b % nt, r = b / nt;
+    float* to = sums + (r0 + r * 16 + (l >> 2)) * slots + n * 8 + 2 * (l & 3);
     to[0] = s.x;
     to[1] = s.y;
-    to[8 * NT * 8] = s.z;
-    to[8 * NT * 8 + 1] = s.w;
+    to[8 * slots] = s.z;
+    to[8 * slots + 1] = s.w;
   }
-  __syncthreads();
 }
 
-template <typename T, int NT>
-__device__ __forceinline__ void shrink_all(const Args& a, int adapter, const T* const (&rows)[4], int q, int of, float4* red,
-                                           float* sums) {
-  int r0 = 0;
-  if constexpr (NT == 1)
-    for (; r0 + 64 <= a.rank; r0 += 64) shrink<T, 4, NT, 2>(a, adapter, r0, rows, q, of, red, sums);
-  for (; r0 + 32 <= a.rank; r0 += 32) shrink<T, 2, NT, NT == 4 ? 2 : 4>(a, adapter, r0, rows, q, of, red, sums);
-  for (; r0 < a.rank; r0 += 16) shrink<T, 1, NT, NT == 4 ? 2 : 4>(a, adapter, r0, rows, q, of, red, sums);
+// Shared memory: the warps' rings, then (a group of few rows) the warps' sums
+// of up to two blocks of ranks and h, then the sums that the cluster reads.  A
+// group of many rows has its warps' sums and h in the rings' place.
+template <typename T>
+struct Layout {
+  static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
+  // of a row of h: the ranks, rounded up to whole pieces of 64 bytes, and rows in other banks
+  static __host__ __device__ int pitch(int rank) { return (rank * (int)sizeof(T) + 63) / 64 * (64 / (int)sizeof(T)) + 16 / (int)sizeof(T); }
+  static constexpr int kRed = kWarps * 2 * 512;
+  static __host__ __device__ int h_bytes(int rank, int slots) { return kParts * slots * pitch(rank) * (int)sizeof(T); }
+  static __host__ __device__ int sums_at(int rank) { return kWarps * kRing + kRed + h_bytes(rank, 8); }
+  static int bytes(int rank, int slots) { return sums_at(rank) + rank * slots * 4; }
+};
+
+// h [slots][pitch], the cluster's sums times the adapter's scale, in parts;
+// zeros behind the ranks.
+template <typename T>
+__device__ __forceinline__ void make_h(const Args& a, cg::cluster_group& cluster, int ranks, float scale, float* sums, int slots, T* h, int part) {
+  const int pitch = Layout<T>::pitch(a.rank), wide = pitch - 16 / (int)sizeof(T);
+  for (int j = threadIdx.x; j < slots * wide; j += kThreads) {
+    const int s = j / wide, r = j - s * wide;
+    float v = 0.f;
+    if (r < a.rank) {
+      const int at = r * slots + s;
+      if (ranks > 1) {
+#pragma unroll
+        for (int c = 0; c < kMostRanks; ++c)
+          if (c < ranks) v += cluster.map_shared_rank(sums, c)[at];
+      } else {
+        v = sums[at];
+      }
+      v *= scale;
+    }
+    if constexpr (sizeof(T) == 4) {
+      h[s * pitch + r] = v;
+    } else {
+      T hi, lo;
+      two_parts(v, hi, lo);
+      h[s * pitch + r] = hi;
+      h[part + s * pitch + r] = lo;
+    }
+  }
 }
 
-// The second product: h [slots][pitch] in shared memory (16-bit: the high
-// parts, then the low ones), the group's rows of 16, MT blocks of them; the
+// A group of up to 8 rows.
+template <typename T>
+__device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& cluster, int ranks, int adapter, const int* slots, int count,
+                                         int row0, int q, int of, char* smem) {
+  using L = Layout<T>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  constexpr int kStage = 1536, kDepth = kRing / kStage;
+  float4* red = reinterpret_cast<float4*>(smem + kWarps * kRing);
+  T* h = reinterpret_cast<T*>(smem + kWarps * kRing + L::kRed);
+  float* sums = reinterpret_cast<float*>(smem + L::sums_at(a.rank));
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * kRing) + lane * 16;
+
+  const int a_bytes = (int)a.a_row, b_bytes = a.rank * (int)sizeof(T);
+  const int a_pieces = (a_bytes + 63) / 64, b_pieces = (b_bytes + 63) / 64;
+  const T* row = g < count ? (const T*)a.x + (long long)(row0 + slots[g]) * a.x_st : nullptr;
+  const int x_size = row && a.x_wide ? 16 : 0;
+  const char* a_first = a.a + ((long long)adapter * a.rank + g) * a.a_row;
+  const char* b_first = (const char*)a.b + (long long)adapter * a.outer * b_bytes;
+  const int blocks = (a.outer + 15) / 16;
+
+  // What the copies stand at: pieces q, q + of, ... of A's blocks of 16 rows,
+  // one block after the other, then all pieces of B's blocks q, q + of, ...
+  int r_ahead = q < a_pieces ? 0 : a.rank, c_ahead = q, u_ahead = q, k_ahead = 0;
+  auto copy = [&](uint32_t to) {
+    if (r_ahead < a.rank) {
+      const int at = c_ahead * 64 + t * 16;
+      const int size = at < a_bytes ? 16 : 0;
+      const char* from = a_first + r_ahead * a.a_row + at;
+      copy_async(to, from, size);
+      copy_async(to + 512, from + 8 * a.a_row, size);
+      // rows of x end where their values do: a last piece that is not whole is read by elements
+      copy_async(to + 1024, row ? (const char*)row + at : a.a, at + 16 <= a.inner * (int)sizeof(T) ? x_size : 0);
+      c_ahead += of;
+      if (c_ahead >= a_pieces) {
+        c_ahead = q;
+        r_ahead += 16;
+      }
+    } else if (u_ahead < blocks) {
+      const int at = k_ahead * 64 + t * 16, n = u_ahead * 16 + g;
+      const int size = at < b_bytes ? 16 : 0;
+      const char* from = b_first + (long long)min(n, a.outer - 1) * b_bytes + at;
+      copy_async(to, from, n < a.outer ? size : 0);
+      copy_async(to + 512, n + 8 < a.outer ? from + 8 * b_bytes : from, n + 8 < a.outer ? size : 0);
+      if (++k_ahead == b_pieces) {
+        k_ahead = 0;
+        u_ahead += of;
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kDepth; ++s) copy(ring + s * kStage);
+  uint32_t at = ring;
+  auto next = [&]() { at = at == ring + (kDepth - 1) * kStage ? ring : at + kStage; };
+
+  for (int r0 = 0; r0 < a.rank; r0 += 32) {
+    const int some = min(2, (a.rank - r0) / 16);
+    for (int r = 0; r < some; ++r) {
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int c = q; c < a_pieces; c += of) {
+        copy_wait<kDepth - 1>();
+        uint4 v[1] = {read_shared(at + 1024)};
+        const int byte = c * 64 + t * 16;
+        if (row && (!a.x_wide || byte + 16 > a.inner * (int)sizeof(T))) v[0] = load_row<T>(row, byte, a.inner);
+        float sum[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+        chunk_product<T, 1>(sum, read_shared(at), read_shared(at + 512), v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] += sum[0][i];
+        copy(at);
+        next();
+      }
+      red[(warp * 2 + r) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    }
+    __syncthreads();
+    add_warps(red, 64, some, 1, r0, 8, sums);
+    __syncthreads();
+  }
+  if (ranks > 1) cluster.sync();
+  const int pitch = L::pitch(a.rank), part = 8 * pitch;
+  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 8, h, part);
+  // the others have read this CTA's sums before it writes the next ones or ends
+  if (ranks > 1) cluster.sync();
+  else __syncthreads();
+
+  // outputs 16u + g and + 8 of the rows in slots 2t and 2t + 1
+  const T* from[2] = {nullptr, nullptr};
+  T* to[2] = {nullptr, nullptr};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (2 * t + i < count) {
+      const long long m = row0 + slots[2 * t + i];
+      from[i] = a.base ? (const T*)a.base + m * a.base_st : nullptr;
+      to[i] = (T*)a.out + m * a.out_st;
+    }
+  float base[4], next_base[4];
+  auto load_base = [&](int u, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = u * 16 + g + 8 * (i >> 1);
+      v[i] = from[i & 1] && n < a.outer ? to_float<T>(from[i & 1][n]) : 0.f;
+    }
+  };
+  if (q < blocks) load_base(q, next_base);
+  const uint32_t h_at = (uint32_t)__cvta_generic_to_shared(h) + (g * pitch) * (int)sizeof(T) + t * 16;
+  for (int u = q; u < blocks; u += of) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) base[i] = next_base[i];
+    if (u + of < blocks) load_base(u + of, next_base);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < b_pieces; ++k) {
+      copy_wait<kDepth - 1>();
+      const uint4 w0 = read_shared(at), w1 = read_shared(at + 512);
+      float sum[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int p = L::kParts - 1; p >= 0; --p) {
+        const uint4 v[1] = {read_shared(h_at + p * part * (int)sizeof(T) + k * 64)};
+        chunk_product<T, 1>(sum, w0, w1, v);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += sum[0][i];
+      copy(at);
+      next();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = u * 16 + g + 8 * (i >> 1);
+      if (to[i & 1] && n < a.outer) to[i & 1][n] = from_float<T>(base[i] + acc[i]);
+    }
+  }
+  __syncthreads();  // h and the sums are written again for the next group
+}
+
+// The second product for up to 32 rows: h [slots][pitch] in shared memory
+// (16-bit: the high parts, then the low ones), MT blocks of 16 of them; the
 // warp's blocks of 32 outputs u = q, q + of, ...
 template <typename T, int MT>
-__device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, int pitch, int part, const int* slots, int count,
-                                       int row0, int q, int of) {
+__device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, int part, const int* slots, int count, int row0, int q, int of) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int pitch = Layout<T>::pitch(a.rank);
   const T* weights = (const T*)a.b + (long long)adapter * a.outer * a.rank;
   const int blocks = (a.outer + 31) / 32;
+  constexpr int WORDS = 8 * (int)sizeof(T) / 16;
+  union Eight {
+    uint4 raw[WORDS];
+    T v[8];
+    __device__ Eight() {}
+  };
+  long long rows[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) rows[m][r] = m * 16 + g + 8 * r < count ? row0 + slots[m * 16 + g + 8 * r] : -1;
+  // base is loaded a block ahead
+  auto load_base = [&](int u, Eight (&io)[MT][2]) {
+    const int n = 32 * u + 8 * t;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const bool there = rows[m][r] >= 0 && a.base;
+        const T* from = (const T*)a.base + (there ? rows[m][r] * a.base_st + n : 0);
+        if (a.out_wide && n + 8 <= a.outer) {
+#pragma unroll
+          for (int i = 0; i < WORDS; ++i) io[m][r].raw[i] = there ? __ldcs(reinterpret_cast<const uint4*>(from) + i) : make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) io[m][r].v[e] = there && n + e < a.outer ? from[e] : from_float<T>(0.f);
+        }
+      }
+  };
+  Eight io[MT][2], ahead[MT][2];
+  if (q < blocks) load_base(q, ahead);
   for (int u = q; u < blocks; u += of) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) io[m][r].raw[i] = ahead[m][r].raw[i];
     float acc[MT][4][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -168,16 +338,19 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
       for (int j = 0; j < 4; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
     // column c of block j is output 32u + 8 (c / 2) + 2j + c % 2
     const int n0 = 32 * u + 8 * (g >> 1) + (g & 1);
-#pragma unroll 2
+    bool first = true;
     for (int k = 0; k < a.rank; k += 16) {
       const int at = k + 4 * t;
-      if constexpr (sizeof(T) == 2) {
-        uint2 w[4];
+      using Word = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+      Word w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = n0 + 2 * j < a.outer ? *reinterpret_cast<const uint2*>(weights + (long long)(n0 + 2 * j) * a.rank + at) : make_uint2(0, 0);
+      for (int j = 0; j < 4; ++j)
+        w[j] = n0 + 2 * j < a.outer ? *reinterpret_cast<const Word*>(weights + (long long)(n0 + 2 * j) * a.rank + at) : Word();
+      if (first && u + of < blocks) load_base(u + of, ahead);
+      first = false;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m) {
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
           for (int p = 1; p >= 0; --p) {
             const uint2 x0 = *reinterpret_cast<const uint2*>(h + p * part + (m * 16 + g) * pitch + at);
@@ -185,14 +358,7 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
 #pragma unroll
             for (int j = 0; j < 4; ++j) mma16(acc[m][j], x0.x, x1.x, x0.y, x1.y, w[j].x, w[j].y, T());
           }
-      } else {
-        uint4 w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = n0 + 2 * j < a.outer ? *reinterpret_cast<const uint4*>(weights + (long long)(n0 + 2 * j) * a.rank + at)
-                                      : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        } else {
           const uint4 x0 = *reinterpret_cast<const uint4*>(h + (m * 16 + g) * pitch + at);
           const uint4 x1 = *reinterpret_cast<const uint4*>(h + (m * 16 + g + 8) * pitch + at);
           float sum[4][4];
@@ -211,64 +377,113 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int slot = m * 16 + g + 8 * r;
-        if (slot >= count || n >= a.outer) continue;
-        const long long row = row0 + slots[slot];
-        const T* from = a.base ? (const T*)a.base + row * a.base_st + n : nullptr;
-        T* to = (T*)a.out + row * a.out_st + n;
-        constexpr int WORDS = 8 * (int)sizeof(T) / 16;
-        union {
-          uint4 raw[WORDS];
-          T v[8];
-        } io;
-        const bool wide = a.out_wide && n + 8 <= a.outer;
-        if (wide) {
-#pragma unroll
-          for (int i = 0; i < WORDS; ++i) io.raw[i] = from ? reinterpret_cast<const uint4*>(from)[i] : make_uint4(0, 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) io.v[e] = from && n + e < a.outer ? from[e] : from_float<T>(0.f);
-        }
+        if (rows[m][r] < 0 || n >= a.outer) continue;
+        T* to = (T*)a.out + rows[m][r] * a.out_st + n;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) io.v[2 * j + i] = from_float<T>(to_float<T>(io.v[2 * j + i]) + acc[m][j][2 * r + i]);
-        if (wide) {
+          for (int i = 0; i < 2; ++i) {
+            T& v = io[m][r].v[2 * j + i];
+            v = from_float<T>(to_float<T>(v) + acc[m][j][2 * r + i]);
+          }
+        if (a.out_wide && n + 8 <= a.outer) {
 #pragma unroll
-          for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint4*>(to)[i] = io.raw[i];
+          for (int i = 0; i < WORDS; ++i) __stcs(reinterpret_cast<uint4*>(to) + i, io[m][r].raw[i]);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (n + e < a.outer) to[e] = io.v[e];
+            if (n + e < a.outer) to[e] = io[m][r].v[e];
         }
       }
   }
 }
 
+// A group of 9 to 32 rows.
 template <typename T>
-struct Layout {
-  static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
-  static __host__ __device__ int pitch(int rank) { return rank + (int)(16 / sizeof(T)); }  // of h: rows in other banks
-  // the warps' sums, or h after them, then the sums that the cluster reads
-  static __host__ __device__ int first_bytes(int rank, int slots) {
-    const int blocks = (rank < 64 ? (rank < 32 ? 1 : 2) : (slots <= 8 ? 4 : 2)) * (slots / 8);
-    const int red = kWarps * blocks * 32 * 16, h = kParts * (slots < 16 ? 16 : slots) * pitch(rank) * (int)sizeof(T);
-    return red > h ? red : h;
+__device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& cluster, int ranks, int adapter, const int* slots, int count,
+                                          int row0, int q, int of, char* smem) {
+  using L = Layout<T>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  constexpr int NT = 4, kStage = 1024 + NT * 512, kDepth = kRing / kStage;
+  float* sums = reinterpret_cast<float*>(smem + L::sums_at(a.rank));
+  T* h = reinterpret_cast<T*>(smem);
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * kRing) + lane * 16;
+  const int bytes = (int)a.a_row, pieces = (bytes + 63) / 64, x_bytes = a.inner * (int)sizeof(T);
+  const T* rows[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) rows[n] = n * 8 + g < count ? (const T*)a.x + (long long)(row0 + slots[n * 8 + g]) * a.x_st : nullptr;
+
+  for (int r0 = 0; r0 < a.rank; r0 += 16) {  // x is read again, from L2, for every 16 ranks
+    const char* weights = a.a + ((long long)adapter * a.rank + r0 + g) * a.a_row;
+    int c_ahead = q;
+    auto copy = [&](uint32_t to) {
+      if (c_ahead < pieces) {
+        const int at = c_ahead * 64 + t * 16;
+        const int size = at < bytes ? 16 : 0, x_size = a.x_wide && at + 16 <= x_bytes ? 16 : 0;
+        copy_async(to, weights + at, size);
+        copy_async(to + 512, weights + 8 * a.a_row + at, size);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) copy_async(to + 1024 + n * 512, rows[n] ? (const char*)rows[n] + at : a.a, rows[n] ? x_size : 0);
+        c_ahead += of;
+      }
+      copy_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kDepth; ++s) copy(ring + s * kStage);
+    uint32_t at = ring;
+    float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    for (int c = q; c < pieces; c += of) {
+      copy_wait<kDepth - 1>();
+      uint4 v[NT];
+      const int byte = c * 64 + t * 16;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        v[n] = read_shared(at + 1024 + n * 512);
+        if (rows[n] && (!a.x_wide || byte + 16 > x_bytes)) v[n] = load_row<T>(rows[n], byte, a.inner);
+      }
+      float sum[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
+      chunk_product<T, NT>(sum, read_shared(at), read_shared(at + 512), v);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] += sum[n][i];
+      copy(at);
+      at = at == ring + (kDepth - 1) * kStage ? ring : at + kStage;
+    }
+    copy_wait<0>();
+    float4* red = reinterpret_cast<float4*>(smem);  // in the warps' rings
+#pragma unroll
+    for (int n = 0; n < NT; ++n) red[warp * (kRing / 16) + n * 32 + lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+    __syncthreads();
+    add_warps(red, kRing / 16, NT, NT, r0, 8 * NT, sums);
+    __syncthreads();
   }
-  static int bytes(int rank, int slots) { return first_bytes(rank, slots) + rank * slots * 4; }
-};
+  if (ranks > 1) cluster.sync();
+  const int part = 32 * L::pitch(a.rank);
+  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 32, h, part);
+  // the others have read this CTA's sums before it writes the next ones or ends
+  if (ranks > 1) cluster.sync();
+  else __syncthreads();
+  if constexpr (sizeof(T) == 2) {
+    if (count <= 16) expand<T, 1>(a, adapter, h, part, slots, count, row0, q, of);
+    else expand<T, 2>(a, adapter, h, part, slots, count, row0, q, of);
+  } else {  // (two blocks of fp32 rows do not fit the registers)
+    for (int s = 0; s < count; s += 16) expand<T, 1>(a, adapter, h + s * L::pitch(a.rank), part, slots + s, count - s, row0, q, of);
+  }
+  __syncthreads();  // h's place is the rings of the next group
+}
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) adapters_kernel(Args a) {
-  using L = Layout<T>;
+__global__ void __launch_bounds__(kThreads, 2) adapters_kernel(Args a) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int slots[kTile];
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  float4* red = reinterpret_cast<float4*>(smem);
-  T* h = reinterpret_cast<T*>(smem);
-  float* sums = reinterpret_cast<float*>(smem + L::first_bytes(a.rank, a.most_slots));
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int unit = (int)(blockIdx.x / ranks), row0 = unit / a.per_tile * kTile, first_group = unit % a.per_tile;
   begin();
 
@@ -305,48 +520,8 @@ __global__ void __launch_bounds__(kThreads) adapters_kernel(Args a) {
     }
     if (warp == 0 && (members >> lane & 1)) slots[__popc(members & ((1u << lane) - 1))] = lane;
     __syncthreads();
-    const T* rows[4];
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-      rows[n] = n * 8 + g < count ? (const T*)a.x + (long long)(row0 + slots[n * 8 + g]) * a.x_st : nullptr;
-    const int wide = count <= 8 ? 8 : count <= 16 ? 16 : 32;
-    if (wide == 8) shrink_all<T, 1>(a, adapter, rows, q, of, red, sums);
-    else if (wide == 16) shrink_all<T, 2>(a, adapter, rows, q, of, red, sums);
-    else shrink_all<T, 4>(a, adapter, rows, q, of, red, sums);
-    if (ranks > 1) cluster.sync();
-    // h, the cluster's sums times the adapter's scale; blocks of 16 rows, of
-    // which those behind the last slot are zeros
-    const float scale = a.scales[adapter];
-    const int pitch = L::pitch(a.rank), part = max(wide, 16) * pitch;
-    for (int j = tid; j < max(wide, 16) * a.rank; j += kThreads) {
-      const int s = j / a.rank, r = j - s * a.rank;
-      float v = 0.f;
-      if (s < wide) {
-        const int at = r * wide + s;
-        if (ranks > 1) {
-#pragma unroll
-          for (int c = 0; c < kMostRanks; ++c)
-            if (c < ranks) v += cluster.map_shared_rank(sums, c)[at];
-        } else {
-          v = sums[at];
-        }
-        v *= scale;
-      }
-      if constexpr (sizeof(T) == 4) {
-        h[s * pitch + r] = v;
-      } else {
-        T hi, lo;
-        two_parts(v, hi, lo);
-        h[s * pitch + r] = hi;
-        h[part + s * pitch + r] = lo;
-      }
-    }
-    // the others have read this CTA's sums before it writes the next ones or ends
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
-    if (wide <= 16) expand<T, 1>(a, adapter, h, pitch, part, slots, count, row0, q, of);
-    else expand<T, 2>(a, adapter, h, pitch, part, slots, count, row0, q, of);
-    __syncthreads();  // h's place is the warps' sums of the next group
+    if (count <= 8) few_rows<T>(a, cluster, ranks, adapter, slots, count, row0, q, of, smem);
+    else many_rows<T>(a, cluster, ranks, adapter, slots, count, row0, q, of, smem);
   }
 }
 
@@ -402,7 +577,7 @@ void launch_adapters(const pfk_adapters_params& p, cudaStream_t stream) {
   a.err = p.err;
   a.x_wide = (uintptr_t)p.x % 16 == 0 && a.x_st * es % 16 == 0;
   a.out_wide = (uintptr_t)p.out % 16 == 0 && a.out_st * es % 16 == 0 && (uintptr_t)p.base % 16 == 0 && a.base_st * es % 16 == 0;
-  a.most_slots = p.rows <= 8 ? 8 : p.rows <= 16 ? 16 : 32;
+  a.most_slots = p.rows <= 8 ? 8 : 32;
   // A tile has up to as many groups as rows or adapters; clusters for all of
   // them, which end at once where there are fewer, as long as these do not
   // become thousands of CTAs.
