@@ -64,9 +64,10 @@ struct Args {
   int* err;
   int x_wide, out_wide;  // rows may be accessed 16 bytes at a time
   int most_slots;        // 8 or 32: of a group at most
-  int per_tile;          // clusters that share a tile's groups
+  int tiles, per_tile;   // per_tile: clusters that share a tile's groups
 };
 
+constexpr int kFewBlocks = 4;  // of 16 ranks, whose sums few rows' warps leave at a time
 constexpr int kRing = 10752;  // bytes of a warp's ring: 7 stages of few rows, 3 of many
 
 // 16 bytes of a row of x from byte `at` on, zeros behind the row's end
@@ -109,14 +110,14 @@ __device__ __forceinline__ void add_warps(const float4* red, int pitch, int bloc
 }
 
 // Shared memory: the warps' rings, then (a group of few rows) the warps' sums
-// of up to two blocks of ranks and h, then the sums that the cluster reads.  A
+// of up to four blocks of ranks and h, then the sums that the cluster reads.  A
 // group of many rows has its warps' sums and h in the rings' place.
 template <typename T>
 struct Layout {
   static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
   // of a row of h: the ranks, rounded up to whole pieces of 64 bytes, and rows in other banks
   static __host__ __device__ int pitch(int rank) { return (rank * (int)sizeof(T) + 63) / 64 * (64 / (int)sizeof(T)) + 16 / (int)sizeof(T); }
-  static constexpr int kRed = kWarps * 2 * 512;
+  static constexpr int kRed = kWarps * kFewBlocks * 512;
   static __host__ __device__ int h_bytes(int rank, int slots) { return kParts * slots * pitch(rank) * (int)sizeof(T); }
   static __host__ __device__ int sums_at(int rank) { return kWarps * kRing + kRed + h_bytes(rank, 8); }
   static int bytes(int rank, int slots) { return sums_at(rank) + rank * slots * 4; }
@@ -125,12 +126,12 @@ struct Layout {
 // h [slots][pitch], the cluster's sums times the adapter's scale, in parts;
 // zeros behind the ranks.
 template <typename T>
-__device__ __forceinline__ void make_h(const Args& a, cg::cluster_group& cluster, int ranks, float scale, float* sums, int slots, T* h, int part) {
+__device__ __forceinline__ void make_h(const Args& a, cg::cluster_group& cluster, int ranks, float scale, float* sums, int slots, int count, T* h, int part) {
   const int pitch = Layout<T>::pitch(a.rank), wide = pitch - 16 / (int)sizeof(T);
   for (int j = threadIdx.x; j < slots * wide; j += kThreads) {
     const int s = j / wide, r = j - s * wide;
     float v = 0.f;
-    if (r < a.rank) {
+    if (r < a.rank && s < count) {
       const int at = r * slots + s;
       if (ranks > 1) {
 #pragma unroll
@@ -167,36 +168,42 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
   const int a_bytes = (int)a.a_row, b_bytes = a.rank * (int)sizeof(T);
   const int a_pieces = (a_bytes + 63) / 64, b_pieces = (b_bytes + 63) / 64;
   const T* row = g < count ? (const T*)a.x + (long long)(row0 + slots[g]) * a.x_st : nullptr;
-  const int x_size = row && a.x_wide ? 16 : 0;
+  const int x_size = row && a.x_wide ? 16 : 0, x_bytes = a.inner * (int)sizeof(T);
   const char* a_first = a.a + ((long long)adapter * a.rank + g) * a.a_row;
   const char* b_first = (const char*)a.b + (long long)adapter * a.outer * b_bytes;
   const int blocks = (a.outer + 15) / 16;
 
   // What the copies stand at: pieces q, q + of, ... of A's blocks of 16 rows,
   // one block after the other, then all pieces of B's blocks q, q + of, ...
-  int r_ahead = q < a_pieces ? 0 : a.rank, c_ahead = q, u_ahead = q, k_ahead = 0;
+  int r_left = q < a_pieces ? a.rank / 16 : 0, a_at = q * 64 + t * 16, u_ahead = q, b_at = t * 16;
+  const char *from_a = a_first + a_at, *from_x = (row ? (const char*)row : a.a) + a_at;
+  const char* from_b = b_first + ((long long)q * 16 + g) * b_bytes + b_at;
+  const long long a_back = 16 * a.a_row + q * 64 + t * 16, b_skip = (long long)of * 16 * b_bytes;
   auto copy = [&](uint32_t to) {
-    if (r_ahead < a.rank) {
-      const int at = c_ahead * 64 + t * 16;
-      const int size = at < a_bytes ? 16 : 0;
-      const char* from = a_first + r_ahead * a.a_row + at;
-      copy_async(to, from, size);
-      copy_async(to + 512, from + 8 * a.a_row, size);
+    if (r_left) {
+      const int size = a_at < a_bytes ? 16 : 0;
+      copy_async(to, from_a, size);
+      copy_async(to + 512, from_a + 8 * a.a_row, size);
       // rows of x end where their values do: a last piece that is not whole is read by elements
-      copy_async(to + 1024, row ? (const char*)row + at : a.a, at + 16 <= a.inner * (int)sizeof(T) ? x_size : 0);
-      c_ahead += of;
-      if (c_ahead >= a_pieces) {
-        c_ahead = q;
-        r_ahead += 16;
+      copy_async(to + 1024, from_x, a_at + 16 <= x_bytes ? x_size : 0);
+      a_at += of * 64;
+      from_a += of * 64;
+      from_x += of * 64;
+      if (a_at - t * 16 >= a_bytes) {
+        from_a += a_back - a_at;
+        a_at = q * 64 + t * 16;
+        from_x = (row ? (const char*)row : a.a) + a_at;
+        --r_left;
       }
     } else if (u_ahead < blocks) {
-      const int at = k_ahead * 64 + t * 16, n = u_ahead * 16 + g;
-      const int size = at < b_bytes ? 16 : 0;
-      const char* from = b_first + (long long)min(n, a.outer - 1) * b_bytes + at;
-      copy_async(to, from, n < a.outer ? size : 0);
-      copy_async(to + 512, n + 8 < a.outer ? from + 8 * b_bytes : from, n + 8 < a.outer ? size : 0);
-      if (++k_ahead == b_pieces) {
-        k_ahead = 0;
+      const int n = u_ahead * 16 + g, size = b_at < b_bytes ? 16 : 0;
+      copy_async(to, n < a.outer ? from_b : b_first, n < a.outer ? size : 0);
+      copy_async(to + 512, n + 8 < a.outer ? from_b + 8 * b_bytes : b_first, n + 8 < a.outer ? size : 0);
+      b_at += 64;
+      from_b += 64;
+      if (b_at - t * 16 >= b_bytes) {
+        from_b += b_skip + t * 16 - b_at;
+        b_at = t * 16;
         u_ahead += of;
       }
     }
@@ -207,15 +214,14 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
   uint32_t at = ring;
   auto next = [&]() { at = at == ring + (kDepth - 1) * kStage ? ring : at + kStage; };
 
-  for (int r0 = 0; r0 < a.rank; r0 += 32) {
-    const int some = min(2, (a.rank - r0) / 16);
+  for (int r0 = 0; r0 < a.rank; r0 += 16 * kFewBlocks) {
+    const int some = min(kFewBlocks, (a.rank - r0) / 16);
     for (int r = 0; r < some; ++r) {
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int c = q; c < a_pieces; c += of) {
+      for (int byte = q * 64 + t * 16; byte - t * 16 < a_bytes; byte += of * 64) {
         copy_wait<kDepth - 1>();
         uint4 v[1] = {read_shared(at + 1024)};
-        const int byte = c * 64 + t * 16;
-        if (row && (!a.x_wide || byte + 16 > a.inner * (int)sizeof(T))) v[0] = load_row<T>(row, byte, a.inner);
+        if (row && (!a.x_wide || byte + 16 > x_bytes)) v[0] = load_row<T>(row, byte, a.inner);
         float sum[1][4] = {{0.f, 0.f, 0.f, 0.f}};
         chunk_product<T, 1>(sum, read_shared(at), read_shared(at + 512), v);
 #pragma unroll
@@ -223,15 +229,15 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
         copy(at);
         next();
       }
-      red[(warp * 2 + r) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      red[(warp * kFewBlocks + r) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
     }
     __syncthreads();
-    add_warps(red, 64, some, 1, r0, 8, sums);
+    add_warps(red, kFewBlocks * 32, some, 1, r0, 8, sums);
     __syncthreads();
   }
   if (ranks > 1) cluster.sync();
   const int pitch = L::pitch(a.rank), part = 8 * pitch;
-  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 8, h, part);
+  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 8, count, h, part);
   // the others have read this CTA's sums before it writes the next ones or ends
   if (ranks > 1) cluster.sync();
   else __syncthreads();
@@ -246,7 +252,7 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
       from[i] = a.base ? (const T*)a.base + m * a.base_st : nullptr;
       to[i] = (T*)a.out + m * a.out_st;
     }
-  float base[4], next_base[4];
+  // base is loaded two blocks ahead
   auto load_base = [&](int u, float (&v)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -254,12 +260,17 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
       v[i] = from[i & 1] && n < a.outer ? to_float<T>(from[i & 1][n]) : 0.f;
     }
   };
-  if (q < blocks) load_base(q, next_base);
+  float base[3][4];
+  load_base(q, base[1]);
+  load_base(q + of, base[2]);
   const uint32_t h_at = (uint32_t)__cvta_generic_to_shared(h) + (g * pitch) * (int)sizeof(T) + t * 16;
   for (int u = q; u < blocks; u += of) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) base[i] = next_base[i];
-    if (u + of < blocks) load_base(u + of, next_base);
+    for (int i = 0; i < 4; ++i) {
+      base[0][i] = base[1][i];
+      base[1][i] = base[2][i];
+    }
+    load_base(u + 2 * of, base[2]);
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int k = 0; k < b_pieces; ++k) {
       copy_wait<kDepth - 1>();
@@ -278,10 +289,25 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = u * 16 + g + 8 * (i >> 1);
-      if (to[i & 1] && n < a.outer) to[i & 1][n] = from_float<T>(base[i] + acc[i]);
+      if (to[i & 1] && n < a.outer) to[i & 1][n] = from_float<T>(base[0][i] + acc[i]);
     }
   }
   __syncthreads();  // h and the sums are written again for the next group
+}
+
+// Two neighbouring values of a word of a row (fp32: of two words), plus x and y.
+__device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, __half) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(w + i));
+  const __half2 r = __floats2half2_rn(v.x + x, v.y + y);
+  w[i] = *reinterpret_cast<const unsigned*>(&r);
+}
+__device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, __nv_bfloat16) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(w[i] << 16) + x, __uint_as_float(w[i] & 0xffff0000u) + y);
+  w[i] = *reinterpret_cast<const unsigned*>(&r);
+}
+__device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, float) {
+  w[2 * i] = __float_as_uint(__uint_as_float(w[2 * i]) + x);
+  w[2 * i + 1] = __float_as_uint(__uint_as_float(w[2 * i + 1]) + y);
 }
 
 // The second product for up to 32 rows: h [slots][pitch] in shared memory
@@ -292,62 +318,84 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int pitch = Layout<T>::pitch(a.rank);
   const T* weights = (const T*)a.b + (long long)adapter * a.outer * a.rank;
-  const int blocks = (a.outer + 31) / 32;
-  constexpr int WORDS = 8 * (int)sizeof(T) / 16;
-  union Eight {
-    uint4 raw[WORDS];
-    T v[8];
-    __device__ Eight() {}
-  };
-  long long rows[MT][2];
+  const int blocks = (a.outer + 31) / 32, whole = a.out_wide ? a.outer / 32 : 0;  // blocks read and written 16 bytes at a time
+  constexpr int WORDS = 2 * (int)sizeof(T);  // of a lane's 8 outputs
+  int rows[MT][2];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int r = 0; r < 2; ++r) rows[m][r] = m * 16 + g + 8 * r < count ? row0 + slots[m * 16 + g + 8 * r] : -1;
-  // base is loaded a block ahead
-  auto load_base = [&](int u, Eight (&io)[MT][2]) {
-    const int n = 32 * u + 8 * t;
+  // base and the first 16 ranks' weights are loaded a block ahead
+  auto load_base = [&](int u, unsigned (&io)[MT][2][WORDS]) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) io[m][r][i] = 0;
+    if (!a.base) return;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const bool there = rows[m][r] >= 0 && a.base;
-        const T* from = (const T*)a.base + (there ? rows[m][r] * a.base_st + n : 0);
-        if (a.out_wide && n + 8 <= a.outer) {
+        if (rows[m][r] < 0) continue;
+        const T* from = (const T*)a.base + rows[m][r] * a.base_st + 32 * u + 8 * t;
+        if (u < whole) {
 #pragma unroll
-          for (int i = 0; i < WORDS; ++i) io[m][r].raw[i] = there ? __ldcs(reinterpret_cast<const uint4*>(from) + i) : make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < WORDS / 4; ++i) {
+            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from) + i);
+            io[m][r][4 * i] = v.x;
+            io[m][r][4 * i + 1] = v.y;
+            io[m][r][4 * i + 2] = v.z;
+            io[m][r][4 * i + 3] = v.w;
+          }
         } else {
+          T* to = reinterpret_cast<T*>(io[m][r]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) io[m][r].v[e] = there && n + e < a.outer ? from[e] : from_float<T>(0.f);
+          for (int e = 0; e < 8; ++e)
+            if (32 * u + 8 * t + e < a.outer) to[e] = from[e];
         }
       }
   };
-  Eight io[MT][2], ahead[MT][2];
-  if (q < blocks) load_base(q, ahead);
+  using Word = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+  // column c of block j is output 32u + 8 (c / 2) + 2j + c % 2
+  auto load_weights = [&](int u, int k, Word (&w)[4]) {
+    const int n0 = 32 * u + 8 * (g >> 1) + (g & 1);
+    const T* from = weights + (long long)n0 * a.rank + k + 4 * t;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = n0 + 2 * j < a.outer ? *reinterpret_cast<const Word*>(from + 2 * j * a.rank) : Word();
+  };
+  unsigned io[MT][2][WORDS], ahead[MT][2][WORDS];
+  Word next[4];
+  if (q < blocks) {
+    load_base(q, ahead);
+    load_weights(q, 0, next);
+  }
   for (int u = q; u < blocks; u += of) {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) io[m][r].raw[i] = ahead[m][r].raw[i];
+        for (int i = 0; i < WORDS; ++i) io[m][r][i] = ahead[m][r][i];
     float acc[MT][4][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
-    // column c of block j is output 32u + 8 (c / 2) + 2j + c % 2
-    const int n0 = 32 * u + 8 * (g >> 1) + (g & 1);
-    bool first = true;
     for (int k = 0; k < a.rank; k += 16) {
       const int at = k + 4 * t;
-      using Word = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
       Word w[4];
+      if (k == 0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = n0 + 2 * j < a.outer ? *reinterpret_cast<const Word*>(weights + (long long)(n0 + 2 * j) * a.rank + at) : Word();
-      if (first && u + of < blocks) load_base(u + of, ahead);
-      first = false;
+        for (int j = 0; j < 4; ++j) w[j] = next[j];
+        if (u + of < blocks) {
+          load_base(u + of, ahead);
+          load_weights(u + of, 0, next);
+        }
+      } else {
+        load_weights(u, k, w);
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         if constexpr (sizeof(T) == 2) {
@@ -372,27 +420,23 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
         }
       }
     }
-    const int n = 32 * u + 8 * t;  // the lane's 8 outputs
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        if (rows[m][r] < 0 || n >= a.outer) continue;
-        T* to = (T*)a.out + rows[m][r] * a.out_st + n;
+        if (rows[m][r] < 0) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) add_two(io[m][r], j, acc[m][j][2 * r], acc[m][j][2 * r + 1], T());
+        T* to = (T*)a.out + rows[m][r] * a.out_st + 32 * u + 8 * t;
+        if (u < whole) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            T& v = io[m][r].v[2 * j + i];
-            v = from_float<T>(to_float<T>(v) + acc[m][j][2 * r + i]);
-          }
-        if (a.out_wide && n + 8 <= a.outer) {
-#pragma unroll
-          for (int i = 0; i < WORDS; ++i) __stcs(reinterpret_cast<uint4*>(to) + i, io[m][r].raw[i]);
+          for (int i = 0; i < WORDS / 4; ++i)
+            __stcs(reinterpret_cast<uint4*>(to) + i, make_uint4(io[m][r][4 * i], io[m][r][4 * i + 1], io[m][r][4 * i + 2], io[m][r][4 * i + 3]));
         } else {
+          const T* v = reinterpret_cast<const T*>(io[m][r]);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (n + e < a.outer) to[e] = io[m][r].v[e];
+            if (32 * u + 8 * t + e < a.outer) to[e] = v[e];
         }
       }
   }
@@ -464,7 +508,7 @@ __device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& clus
   }
   if (ranks > 1) cluster.sync();
   const int part = 32 * L::pitch(a.rank);
-  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 32, h, part);
+  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 32, count, h, part);
   // the others have read this CTA's sums before it writes the next ones or ends
   if (ranks > 1) cluster.sync();
   else __syncthreads();
@@ -484,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(Args a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int unit = (int)(blockIdx.x / ranks), row0 = unit / a.per_tile * kTile, first_group = unit % a.per_tile;
+  const int unit = (int)(blockIdx.x / ranks), row0 = unit % a.tiles * kTile, first_group = unit / a.tiles;
   begin();
 
   int mine = INT_MIN;  // the lane's row's adapter
@@ -578,17 +622,23 @@ void launch_adapters(const pfk_adapters_params& p, cudaStream_t stream) {
   a.x_wide = (uintptr_t)p.x % 16 == 0 && a.x_st * es % 16 == 0;
   a.out_wide = (uintptr_t)p.out % 16 == 0 && a.out_st * es % 16 == 0 && (uintptr_t)p.base % 16 == 0 && a.base_st * es % 16 == 0;
   a.most_slots = p.rows <= 8 ? 8 : 32;
-  // A tile has up to as many groups as rows or adapters; clusters for all of
-  // them, which end at once where there are fewer, as long as these do not
-  // become thousands of CTAs.
+  // A tile has up to as many groups as rows or adapters.  A cluster for all of
+  // them, as long as these do not become thousands of CTAs: the first groups
+  // of all tiles in front, so that those of prompts start at once, then the
+  // others, which end at once where there are none (one cluster a tile took 82
+  // us for the 60 of prompts of 8191 rows: two groups where prompts meet, one
+  // after the other).
   const int64_t tiles = ceil_div(p.rows, kTile), groups = std::min<int64_t>({kTile, p.rows, p.adapters + 1});
+  const int64_t sms = device_sm_count(current_device());
+  a.tiles = (int)tiles;
   a.per_tile = (int)std::min(groups, std::max<int64_t>(1, 2048 / tiles));
   const int64_t units = tiles * a.per_tile;
   PFB_CHECK_ARG(units <= INT32_MAX / kMostRanks, "adapters: too many rows");
-  // few groups: several CTAs each, as long as all warps have something of one of the products
+  // few groups: several CTAs each, as many as the device holds at once, as long
+  // as all warps have something of one of the products
   const int64_t work = std::max(ceil_div(a.a_row, 64), ceil_div(p.outer, 32));
   int ranks = 1;
-  while (ranks < kMostRanks && units * ranks <= 512 && work > ranks * kWarps) ranks *= 2;
+  while (ranks < kMostRanks && units * ranks <= sms && work > ranks * kWarps) ranks *= 2;
   if (p.dtype == PFC_DTYPE_FLOAT32) launch_typed<float>(a, units * ranks, ranks, stream);
   else if (p.dtype == PFC_DTYPE_FLOAT16) launch_typed<__half>(a, units * ranks, ranks, stream);
   else launch_typed<__nv_bfloat16>(a, units * ranks, ranks, stream);
