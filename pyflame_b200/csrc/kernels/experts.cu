@@ -96,15 +96,26 @@ __device__ __forceinline__ void let_next_come() { asm volatile("griddepcontrol.l
 // route
 // ---------------------------------------------------------------------------
 
-// Lists the pairs by expert, in parts of at most `most`: threads of one CTA;
-// shared: [experts + pairs] ints.  The order of an expert's pairs, of which a
-// token has one at most, has no effect: their sums are apart.
+// Lists the pairs by expert, those of an expert in their order, in parts of at
+// most `most`: threads of one CTA; shared: [experts + 2 * pairs] ints.  (An
+// order that depended on timing would put a pair in one part or another, whose
+// rows' pieces are shared out among warps in another way.)
 __device__ void list_pairs(const Args& a, const int* chosen, int* shared, int most) {
-  int *hist = shared, *place = shared + a.experts;
+  int *hist = shared, *place = shared + a.experts, *expert = place + a.tokens * a.top;
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, pairs = a.tokens * a.top;
   for (int e = tid; e < a.experts; e += threads) hist[e] = 0;
+  for (int p = tid; p < pairs; p += threads) expert[p] = chosen[p];
   __syncthreads();
-  for (int p = tid; p < pairs; p += threads) place[p] = atomicAdd(&hist[chosen[p]], 1);
+  if (tid < 32) {
+    for (int base = 0; base < pairs; base += 32) {
+      const int p = base + lane, e = p < pairs ? expert[p] : -1;
+      const unsigned same = __match_any_sync(~0u, e), before = same & ((1u << lane) - 1);
+      if (e >= 0) place[p] = hist[e] + __popc(before);
+      __syncwarp();
+      if (e >= 0 && !before) hist[e] += __popc(same);
+      __syncwarp();
+    }
+  }
   __syncthreads();
   if (tid < 32) {
     int start = 0, parts = 0;
@@ -128,7 +139,7 @@ __device__ void list_pairs(const Args& a, const int* chosen, int* shared, int mo
     if (lane == 0) a.parts[0] = make_int4(parts, 0, 0, 0);
   }
   __syncthreads();
-  for (int p = tid; p < pairs; p += threads) a.pairs[hist[chosen[p]] + place[p]] = p;
+  for (int p = tid; p < pairs; p += threads) a.pairs[hist[expert[p]] + place[p]] = p;
 }
 
 // Parts of the logits of EP experts and TB tokens, over `len` values (a
@@ -751,7 +762,7 @@ void launch_typed(const pfk_experts_params& p, const Plan& w, Args a, cudaStream
     const int pairs = a.tokens * a.top;
     a.h_part = pairs * w.h_row;
     a.most_parts = (int)parts_of(p, a.tokens);
-    const size_t list = (size_t)(a.experts + pairs) * sizeof(int);
+    const size_t list = (size_t)(a.experts + 2 * pairs) * sizeof(int);
     a.tokens == 1 ? launch_route<T, 1>(a, list, stream) : launch_route<T, kRouteTokens>(a, list, stream);
     if (a.tokens > kRouteTokens) launch_following<Args>(list_kernel, dim3(1), kRouteThreads, list, stream, a);
     a.tokens <= 8 ? launch_products<T, 1>(a, stream) : launch_products<T, 2>(a, stream);
