@@ -51,13 +51,15 @@ __device__ __forceinline__ void mma8_tf32(float (&c)[4], unsigned a0, unsigned a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo: hi has the sign, the exponent and 10 bits of the mantissa, lo
-// the other 13 exactly, of which the tensor cores take the first 11: what is
-// lost is below 2^-21 of x.  (Both parts rounded to the nearest cost three
-// instructions more for each value.)  An infinity has a low part of NaN, so
-// its products are NaN.
+// x = hi + lo: hi is x rounded to tf32's 10 bits of mantissa by an integer
+// addition, lo the rest exactly, 12 bits and a sign, of which the tensor cores
+// take 11: what is lost is below 2^-22 of x and has either sign, as has the
+// product of the low parts, which is left out.  (hi by its mask alone, an
+// instruction less, has low parts of x's sign: their products' mean was 2^-22
+// of the result.)  An infinity has a low part of NaN, so its products are NaN;
+// numbers above 2^127 (2 - 2^-11) round to one.
 __device__ __forceinline__ void split_tf32(unsigned x, unsigned& hi, unsigned& lo) {
-  hi = x & 0xffffe000u;
+  hi = (x + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
 }
 
