@@ -155,14 +155,21 @@ class PagedKVCache4bit:
         """(k, v): what the cache holds at `slots` (int64 [tokens]; negative:
         zeros), [tokens, num_heads, head_dim] in `dtype` (float32 by
         default)."""
-        import torch
-        dtype = torch.float32 if dtype is None else dtype
-        _check("slots", slots, (None,), torch.int64, self.device)
-        shape = (len(slots), self.num_heads, self.head_dim)
-        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
-        p = N.Cache4ReadParamsC(self._c, _code(dtype), len(slots), slots.data_ptr(), k.data_ptr(), v.data_ptr())
+        key = (dtype, slots.dtype, slots.shape, slots.stride(), slots.get_device())
+        plan = self._plans.get(key) or self._plans.keep(key, self._read_plan(slots, dtype), slots)
+        p = N.Cache4ReadParamsC.from_buffer_copy(plan[0])
+        empty = _Bound.torch.empty_like
+        k, v = empty(plan[1]), empty(plan[1])
+        p.slots, p.k, p.v = slots.data_ptr(), k.data_ptr(), v.data_ptr()
         _call(self._read_fn, self.device, C.byref(p))
         return k, v
+
+    def _read_plan(self, slots, dtype):
+        import torch
+        dtype = torch.float32 if dtype is None else dtype
+        code = _code(dtype)
+        _check("slots", slots, (None,), torch.int64, self.device)
+        return (N.Cache4ReadParamsC(self._c, code, len(slots)), _model(self._err, (len(slots), self.num_heads, self.head_dim), dtype))
 
     def attend(self, q, block_table, seq_lens, scale: Optional[float] = None, window: int = 0, out=None,
                return_lse: bool = False):

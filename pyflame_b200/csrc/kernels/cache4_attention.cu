@@ -55,9 +55,12 @@ Plan plan_of(const pfk_cache4_attention_params& p) {
   const int64_t units = p.batch * p.cache.heads * ceil_div(group, kHeads), tiles = ceil_div(seen, 64);
   w.ranks = 0;
   w.stats_at = w.parts_at = w.bytes = 0;
-  if (tiles <= kClusterTiles && units * kMostRanks <= device_sm_count(current_device())) {
-    w.ranks = 1;
-    while (w.ranks < kMostRanks && w.ranks < tiles) w.ranks *= 2;
+  // Few units with tables for short sequences: a cluster takes each, with no
+  // list, no workspace and no second launch.
+  int ranks = 1;
+  while (ranks < kMostRanks && ranks < tiles) ranks *= 2;
+  if (tiles <= kClusterTiles && units * ranks <= 2 * device_sm_count(current_device())) {
+    w.ranks = ranks;
     return w;
   }
   w.stats_at = (int64_t)w.ctas * 16;

@@ -8,13 +8,13 @@
 // tokens memory is the bound.  Kernels, each launched as a programmatic
 // dependent of the one before:
 //
-// 1. route: a cluster of 8 CTAs for up to 4 tokens: each CTA an eighth of the
+// 1. route: a cluster of 8 CTAs for up to 8 tokens, or for 4 of more: each CTA an eighth of the
 //    experts' logits, in 64 bits, since which expert a token takes is a
 //    decision that no rounding should make (mma.sync in 64 bits takes 500
 //    cycles an instruction on this device); the first CTA gathers them through
 //    distributed shared memory and picks.  It copies x, aligned and padded,
 //    for the next kernel, and lists the (token, choice) pairs by expert.  With
-//    more than 4 tokens a kernel of one CTA lists them.
+//    more than 8 tokens a kernel of one CTA lists them.
 // 2. up: a CTA of 4 warps takes 8 gate rows and their 8 up rows of an expert,
 //    which share the 16 rows of a matrix instruction, so that a lane ends with
 //    a gate and its up value.  The warps share the summed axis, 64 bytes of a
@@ -56,7 +56,6 @@ constexpr int kMostExperts = 1024;
 constexpr int kMostTop = 32;
 constexpr int kRouteRanks = 8;
 constexpr int kRouteThreads = 256;
-constexpr int kRouteTokens = 4;  // of a cluster
 constexpr int kRouteBlock = 2048;  // values of x that it holds of a token at a time
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
@@ -97,30 +96,41 @@ __device__ __forceinline__ void let_next_come() { asm volatile("griddepcontrol.l
 // ---------------------------------------------------------------------------
 
 // Lists the pairs by expert, those of an expert in their order, in parts of at
-// most `most`: threads of one CTA; shared: [experts + 2 * pairs] ints.  (An
-// order that depended on timing would put a pair in one part or another, whose
-// rows' pieces are shared out among warps in another way.)
+// most `most`: a CTA of kRouteThreads; shared: list_ints() ints.  (An order that
+// depended on timing would put a pair in one part or another, whose rows'
+// pieces are shared out among warps in another way.)  A warp counts a run of
+// the pairs, 32 at a time.
+constexpr int kListWarps = kRouteThreads / 32;
+constexpr size_t list_ints(int64_t experts, int64_t pairs) { return (size_t)(kListWarps * experts + 2 * pairs); }
+
 __device__ void list_pairs(const Args& a, const int* chosen, int* shared, int most) {
-  int *hist = shared, *place = shared + a.experts, *expert = place + a.tokens * a.top;
-  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, pairs = a.tokens * a.top;
-  for (int e = tid; e < a.experts; e += threads) hist[e] = 0;
-  for (int p = tid; p < pairs; p += threads) expert[p] = chosen[p];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pairs = a.tokens * a.top;
+  int *counts = shared, *place = shared + kListWarps * a.experts, *expert = place + pairs;  // counts: [warp][expert]
+  const int run = (pairs + 32 * kListWarps - 1) / (32 * kListWarps) * 32;
+  for (int i = tid; i < kListWarps * a.experts; i += kRouteThreads) counts[i] = 0;
+  for (int p = tid; p < pairs; p += kRouteThreads) expert[p] = chosen[p];
   __syncthreads();
-  if (tid < 32) {
-    for (int base = 0; base < pairs; base += 32) {
-      const int p = base + lane, e = p < pairs ? expert[p] : -1;
-      const unsigned same = __match_any_sync(~0u, e), before = same & ((1u << lane) - 1);
-      if (e >= 0) place[p] = hist[e] + __popc(before);
-      __syncwarp();
-      if (e >= 0 && !before) hist[e] += __popc(same);
-      __syncwarp();
-    }
+  int* mine = counts + warp * a.experts;
+  for (int base = warp * run; base < min(pairs, (warp + 1) * run); base += 32) {
+    const int p = base + lane, e = p < pairs ? expert[p] : -1;
+    const unsigned same = __match_any_sync(~0u, e), before = same & ((1u << lane) - 1);
+    if (e >= 0) place[p] = mine[e] + __popc(before);
+    __syncwarp();
+    if (e >= 0 && !before) mine[e] += __popc(same);
+    __syncwarp();
   }
   __syncthreads();
-  if (tid < 32) {
+  for (int e = tid; e < a.experts; e += kRouteThreads) {  // how many an expert has in the runs up to and with each warp's
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kListWarps; ++w) sum += counts[w * a.experts + e], counts[w * a.experts + e] = sum;
+  }
+  __syncthreads();
+  int* all = counts + (kListWarps - 1) * a.experts;
+  if (warp == 0) {
     int start = 0, parts = 0;
     for (int base = 0; base < a.experts; base += 32) {
-      const int e = base + lane, n = e < a.experts ? hist[e] : 0, own = (n + most - 1) / most;
+      const int e = base + lane, n = e < a.experts ? all[e] : 0, own = (n + most - 1) / most;
       int sum = n, before = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -132,14 +142,17 @@ __device__ void list_pairs(const Args& a, const int* chosen, int* shared, int mo
       }
       const int first = start + sum - n;
       for (int k = 0; k < own; ++k) a.parts[1 + parts + before - own + k] = make_int4(e, first + k * most, min(most, n - k * most), 0);
-      if (e < a.experts) hist[e] = first;
+      if (e < a.experts) all[e] = first;
       start += __shfl_sync(~0u, sum, 31);
       parts += __shfl_sync(~0u, before, 31);
     }
     if (lane == 0) a.parts[0] = make_int4(parts, 0, 0, 0);
   }
   __syncthreads();
-  for (int p = tid; p < pairs; p += threads) a.pairs[hist[expert[p]] + place[p]] = p;
+  for (int p = tid; p < pairs; p += kRouteThreads) {
+    const int e = expert[p], w = p / run;
+    a.pairs[all[e] + (w ? counts[(w - 1) * a.experts + e] : 0) + place[p]] = p;
+  }
 }
 
 // Parts of the logits of EP experts and TB tokens, over `len` values (a
@@ -335,7 +348,7 @@ __global__ void __launch_bounds__(kRouteThreads) list_kernel(Args a) {
   extern __shared__ double shared[];
   let_next_come();
   begin();
-  list_pairs(a, a.chosen, reinterpret_cast<int*>(shared), a.tokens <= 8 ? 8 : 16);
+  list_pairs(a, a.chosen, reinterpret_cast<int*>(shared), 16);
 }
 
 // ---------------------------------------------------------------------------
@@ -745,10 +758,10 @@ template <typename T, int TB>
 void launch_route(const Args& a, size_t list, cudaStream_t stream) {
   static std::once_flag once[64];
   std::call_once(once[current_device()], [] {
-    PFB_CUDA(cudaFuncSetAttribute(route_kernel<T, TB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)route_smem<TB>(kMostExperts)));
+    PFB_CUDA(cudaFuncSetAttribute(route_kernel<T, TB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)std::max(route_smem<TB>(kMostExperts), list_ints(kMostExperts, TB * kMostTop) * sizeof(int))));
   });
   launch_following<Args>(route_kernel<T, TB>, dim3((unsigned)(ceil_div(a.tokens, TB) * kRouteRanks)), kRouteThreads,
-                         std::max(route_smem<TB>(a.experts), list), stream, a, kRouteRanks);
+                         a.tokens <= TB ? std::max(route_smem<TB>(a.experts), list) : route_smem<TB>(a.experts), stream, a, kRouteRanks);
 }
 
 template <typename T>
@@ -762,9 +775,17 @@ void launch_typed(const pfk_experts_params& p, const Plan& w, Args a, cudaStream
     const int pairs = a.tokens * a.top;
     a.h_part = pairs * w.h_row;
     a.most_parts = (int)parts_of(p, a.tokens);
-    const size_t list = (size_t)(a.experts + 2 * pairs) * sizeof(int);
-    a.tokens == 1 ? launch_route<T, 1>(a, list, stream) : launch_route<T, kRouteTokens>(a, list, stream);
-    if (a.tokens > kRouteTokens) launch_following<Args>(list_kernel, dim3(1), kRouteThreads, list, stream, a);
+    const size_t list = list_ints(a.experts, pairs) * sizeof(int);
+    if (a.tokens == 1) launch_route<T, 1>(a, list, stream);
+    else if (a.tokens <= 4 || a.tokens > 8) launch_route<T, 4>(a, list, stream);
+    else launch_route<T, 8>(a, list, stream);  // one cluster, which lists the pairs
+    if (a.tokens > 8) {
+      static std::once_flag once[64];
+      std::call_once(once[current_device()], [] {
+        PFB_CUDA(cudaFuncSetAttribute(list_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(list_ints(kMostExperts, kMostPairs) * sizeof(int))));
+      });
+      launch_following<Args>(list_kernel, dim3(1), kRouteThreads, list, stream, a);
+    }
     a.tokens <= 8 ? launch_products<T, 1>(a, stream) : launch_products<T, 2>(a, stream);
   }
 }
