@@ -227,7 +227,10 @@ struct Layout {
   static constexpr size_t q_bytes = (size_t)kQParts * kBlocks * 32 * 16;
   static constexpr size_t o_bytes = (size_t)kWarps * kHeads * kPitch * 4;
   static constexpr size_t smem = q_bytes + o_bytes;
-  static constexpr int kResident = W <= 64 ? 4 : W <= 128 ? 3 : 2;  // CTAs that share an SM
+  // CTAs that share an SM: more warps help (128 sequences of 5000 keys, bf16,
+  // groups of 64: 168 us with four, 185 with three), but not where 128
+  // registers a thread spill (fp16, groups of 32: 106 us for 88)
+  static constexpr int kResident = W <= 64 ? 4 : W <= 128 ? (sizeof(T) == 4 || kGroups > 2 ? 3 : 4) : 2;
 };
 
 // CLUSTER: a cluster of CTAs for each unit, each an equal part of its tiles;
@@ -628,65 +631,66 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
       float base[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i] - kShift;
-      unsigned pt[R][NG][L::kPParts][2];  // weights times steps as the second operand, of keys 0-7 and 8-15
+      float p[R][4];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float p[4];
+      for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[i] = exp2_fast(s[r][i] - base[i & 1]);
-          l[i & 1] += p[i];
+          p[r][i] = exp2_fast(s[r][i] - base[i & 1]);
+          l[i & 1] += p[r][i];
         }
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
+      for (int n = 0; n < NG; ++n) {
+        unsigned pt[R][L::kPParts][2];  // weights times steps as the second operand, of keys 0-7 and 8-15
+#pragma unroll
+        for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const unsigned w = vs[r][i][n];
             const float st = __uint_as_float(w & 0xffff0000u) * below, low = low_of<L::kCentred>(w);
-            z[n][0] = fmaf(p[2 * i], low, z[n][0]);
-            z[n][1] = fmaf(p[2 * i + 1], low, z[n][1]);
-            const float x = p[2 * i] * st, y = p[2 * i + 1] * st;
+            z[n][0] = fmaf(p[r][2 * i], low, z[n][0]);
+            z[n][1] = fmaf(p[r][2 * i + 1], low, z[n][1]);
+            const float x = p[r][2 * i] * st, y = p[r][2 * i + 1] * st;
             const unsigned hi = pack_half(x, y);
-            pt[r][n][0][i] = transpose8x8(hi);
+            pt[r][0][i] = transpose8x8(hi);
             if constexpr (L::kPParts == 2) {
               const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-              pt[r][n][1][i] = transpose8x8(pack_half(x - back.x, y - back.y));
+              pt[r][1][i] = transpose8x8(pack_half(x - back.x, y - back.y));
             }
           }
-      }
 #pragma unroll
-      for (int b = 0; b < B; ++b) {
-        constexpr int F = L::kFold;
-        float sum[2][4];
+        for (int b = n * L::kFold; b < (n + 1) * L::kFold && b < B; ++b) {
+          float sum[2][4];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          unsigned x = vc[r][0][b], y = vc[r][1][b];  // of keys 2t and 2t + 1, and of 2t + 8 and 2t + 9
-          if constexpr (!RUNS) {
-            x = __byte_perm(vc[r][0][b], vc[r][1][b], (odd & 1 ? 0x32 : 0x10) | (odd & 2 ? 0x7600 : 0x5400));
-            y = __byte_perm(vc[r][2][b], vc[r][3][b], (odd & 4 ? 0x32 : 0x10) | (odd & 8 ? 0x7600 : 0x5400));
-          }
-          unsigned e0, o0, e1, o1, e2, o2, e3, o3;
-          operands<L::kCentred>(x, e0, o0);
-          operands<L::kCentred>(y, e1, o1);
-          operands<L::kCentred>(x >> 8, e2, o2);
-          operands<L::kCentred>(y >> 8, e3, o3);
+          for (int r = 0; r < R; ++r) {
+            unsigned x = vc[r][0][b], y = vc[r][1][b];  // of keys 2t and 2t + 1, and of 2t + 8 and 2t + 9
+            if constexpr (!RUNS) {
+              x = __byte_perm(vc[r][0][b], vc[r][1][b], (odd & 1 ? 0x32 : 0x10) | (odd & 2 ? 0x7600 : 0x5400));
+              y = __byte_perm(vc[r][2][b], vc[r][3][b], (odd & 4 ? 0x32 : 0x10) | (odd & 8 ? 0x7600 : 0x5400));
+            }
+            unsigned e0, o0, e1, o1, e2, o2, e3, o3;
+            operands<L::kCentred>(x, e0, o0);
+            operands<L::kCentred>(y, e1, o1);
+            operands<L::kCentred>(x >> 8, e2, o2);
+            operands<L::kCentred>(y >> 8, e3, o3);
 #pragma unroll
-          for (int q = L::kPParts - 1; q >= 0; --q) {
-            if (r == 0 && q == L::kPParts - 1) {
-              mma_first(sum[0], e0, o0, e1, o1, pt[r][b / F][q][0], pt[r][b / F][q][1]);
-              mma_first(sum[1], e2, o2, e3, o3, pt[r][b / F][q][0], pt[r][b / F][q][1]);
-            } else {
-              mma(sum[0], e0, o0, e1, o1, pt[r][b / F][q][0], pt[r][b / F][q][1]);
-              mma(sum[1], e2, o2, e3, o3, pt[r][b / F][q][0], pt[r][b / F][q][1]);
+            for (int q = L::kPParts - 1; q >= 0; --q) {
+              if (r == 0 && q == L::kPParts - 1) {
+                mma_first(sum[0], e0, o0, e1, o1, pt[r][q][0], pt[r][q][1]);
+                mma_first(sum[1], e2, o2, e3, o3, pt[r][q][0], pt[r][q][1]);
+              } else {
+                mma(sum[0], e0, o0, e1, o1, pt[r][q][0], pt[r][q][1]);
+                mma(sum[1], e2, o2, e3, o3, pt[r][q][0], pt[r][q][1]);
+              }
             }
           }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[b][j][i] = fmaf(above, sum[j][i], o[b][j][i]);
         }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[b][j][i] = fmaf(above, sum[j][i], o[b][j][i]);
       }
-          load_v(parity_of(next));
+      load_v(parity_of(next));
       next = place();
     }
 

@@ -530,10 +530,10 @@ def test_refusals():
 def test_workspace_is_checked():
     c = pf.PagedKVCache4bit(200, 64, 8, 128)
     L = N.lib()
-    q, table = torch.zeros(4, 32, 128, device="cuda"), torch.zeros(4, 50, dtype=torch.int32, device="cuda")
-    n, need = torch.full((4,), 3000, dtype=torch.int32, device="cuda"), C.c_size_t(0)
+    q, table = torch.zeros(8, 32, 128, device="cuda"), torch.zeros(8, 50, dtype=torch.int32, device="cuda")
+    n, need = torch.full((8,), 3000, dtype=torch.int32, device="cuda"), C.c_size_t(0)
     out = torch.empty_like(q)
-    p = N.Cache4AttentionParamsC(c._c, 0, 4, 32, q.data_ptr(), 4096, 128, out.data_ptr(), 4096, 128, None, table.data_ptr(), 50, 50, n.data_ptr(), 0, 0.1)
+    p = N.Cache4AttentionParamsC(c._c, 0, 8, 32, q.data_ptr(), 4096, 128, out.data_ptr(), 4096, 128, None, table.data_ptr(), 50, 50, n.data_ptr(), 0, 0.1)
     assert L.pfk_cache4_attention_workspace(C.byref(p), C.byref(need)) == 0 and need.value > 0
     work = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
     for at, size in ((None, need.value), (work.data_ptr(), need.value - 1), (work.data_ptr() + 8, need.value)):
