@@ -252,15 +252,15 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
       from[i] = a.base ? (const T*)a.base + m * a.base_st : nullptr;
       to[i] = (T*)a.out + m * a.out_st;
     }
-  // base is loaded two blocks ahead
-  auto load_base = [&](int u, float (&v)[4]) {
+  // base is loaded two blocks ahead (and converted when it is there)
+  auto load_base = [&](int u, T (&v)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = u * 16 + g + 8 * (i >> 1);
-      v[i] = from[i & 1] && n < a.outer ? to_float<T>(from[i & 1][n]) : 0.f;
+      v[i] = from[i & 1] && n < a.outer ? from[i & 1][n] : from_float<T>(0.f);
     }
   };
-  float base[3][4];
+  T base[3][4];
   load_base(q, base[1]);
   load_base(q + of, base[2]);
   const uint32_t h_at = (uint32_t)__cvta_generic_to_shared(h) + (g * pitch) * (int)sizeof(T) + t * 16;
@@ -289,7 +289,7 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = u * 16 + g + 8 * (i >> 1);
-      if (to[i & 1] && n < a.outer) to[i & 1][n] = from_float<T>(base[0][i] + acc[i]);
+      if (to[i & 1] && n < a.outer) to[i & 1][n] = from_float<T>(to_float<T>(base[0][i]) + acc[i]);
     }
   }
   __syncthreads();  // h and the sums are written again for the next group
