@@ -109,9 +109,9 @@ __device__ __forceinline__ void add_warps(const float4* red, int pitch, int bloc
   }
 }
 
-// Shared memory: the warps' rings, then (a group of few rows) the warps' sums
-// of up to four blocks of ranks and h, then the sums that the cluster reads.  A
-// group of many rows has its warps' sums and h in the rings' place.
+// Shared memory: the warps' rings, then the warps' sums of up to four blocks
+// of ranks and h (a group of many rows has its warps' sums in the rings and h
+// here), then the sums that the cluster reads.
 template <typename T>
 struct Layout {
   static constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
@@ -119,8 +119,11 @@ struct Layout {
   static __host__ __device__ int pitch(int rank) { return (rank * (int)sizeof(T) + 63) / 64 * (64 / (int)sizeof(T)) + 16 / (int)sizeof(T); }
   static constexpr int kRed = kWarps * kFewBlocks * 512;
   static __host__ __device__ int h_bytes(int rank, int slots) { return kParts * slots * pitch(rank) * (int)sizeof(T); }
-  static __host__ __device__ int sums_at(int rank) { return kWarps * kRing + kRed + h_bytes(rank, 8); }
-  static int bytes(int rank, int slots) { return sums_at(rank) + rank * slots * 4; }
+  static __host__ __device__ int sums_at(int rank, int slots) {
+    const int few = kRed + h_bytes(rank, 8), many = slots > 8 ? h_bytes(rank, slots) : 0;
+    return kWarps * kRing + (few > many ? few : many);
+  }
+  static int bytes(int rank, int slots) { return sums_at(rank, slots) + rank * slots * 4; }
 };
 
 // h [slots][pitch], the cluster's sums times the adapter's scale, in parts;
@@ -162,7 +165,7 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
   constexpr int kStage = 1536, kDepth = kRing / kStage;
   float4* red = reinterpret_cast<float4*>(smem + kWarps * kRing);
   T* h = reinterpret_cast<T*>(smem + kWarps * kRing + L::kRed);
-  float* sums = reinterpret_cast<float*>(smem + L::sums_at(a.rank));
+  float* sums = reinterpret_cast<float*>(smem + L::sums_at(a.rank, a.most_slots));
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * kRing) + lane * 16;
 
   const int a_bytes = (int)a.a_row, b_bytes = a.rank * (int)sizeof(T);
@@ -312,9 +315,10 @@ __device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, fl
 
 // The second product for up to 32 rows: h [slots][pitch] in shared memory
 // (16-bit: the high parts, then the low ones), MT blocks of 16 of them; the
-// warp's blocks of 32 outputs u = q, q + of, ...
+// warp's blocks of 32 outputs u = q, q + of, ...; ring: the lane's place in
+// the warp's.
 template <typename T, int MT>
-__device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, int part, const int* slots, int count, int row0, int q, int of) {
+__device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, int part, const int* slots, int count, int row0, int q, int of, uint32_t ring) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int pitch = Layout<T>::pitch(a.rank);
   const T* weights = (const T*)a.b + (long long)adapter * a.outer * a.rank;
@@ -325,31 +329,42 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int r = 0; r < 2; ++r) rows[m][r] = m * 16 + g + 8 * r < count ? row0 + slots[m * 16 + g + 8 * r] : -1;
-  // base and the first 16 ranks' weights are loaded a block ahead
-  auto load_base = [&](int u, unsigned (&io)[MT][2][WORDS]) {
+  // Base comes through the warp's ring, several blocks ahead; the last block,
+  // if it is not whole, and rows that are not aligned are read by elements.
+  // The first 16 ranks' weights are loaded a block ahead.
+  constexpr int kStage = MT * 2 * WORDS / 4 * 512, kDepth = kRing / kStage;
+  static_assert(kDepth >= 2, "a block ahead at least");
+  int u_ahead = q;
+  auto copy = [&](uint32_t to) {
+    if (u_ahead < whole && a.base) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2; ++r) {
+          const T* from = (const T*)a.base + max(rows[m][r], 0) * a.base_st + 32 * u_ahead + 8 * t;
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) io[m][r][i] = 0;
-    if (!a.base) return;
+          for (int i = 0; i < WORDS / 4; ++i)
+            copy_async(to + ((m * 2 + r) * (WORDS / 4) + i) * 512, reinterpret_cast<const uint4*>(from) + i, rows[m][r] < 0 ? 0 : 16);
+        }
+    }
+    u_ahead += of;
+    copy_commit();
+  };
+  auto take_base = [&](int u, uint32_t at, unsigned (&io)[MT][2][WORDS]) {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        if (rows[m][r] < 0) continue;
-        const T* from = (const T*)a.base + rows[m][r] * a.base_st + 32 * u + 8 * t;
-        if (u < whole) {
 #pragma unroll
-          for (int i = 0; i < WORDS / 4; ++i) {
-            const uint4 v = __ldcs(reinterpret_cast<const uint4*>(from) + i);
-            io[m][r][4 * i] = v.x;
-            io[m][r][4 * i + 1] = v.y;
-            io[m][r][4 * i + 2] = v.z;
-            io[m][r][4 * i + 3] = v.w;
-          }
-        } else {
+        for (int i = 0; i < WORDS / 4; ++i) {
+          const uint4 v = u < whole && a.base ? read_shared(at + ((m * 2 + r) * (WORDS / 4) + i) * 512) : make_uint4(0, 0, 0, 0);
+          io[m][r][4 * i] = v.x;
+          io[m][r][4 * i + 1] = v.y;
+          io[m][r][4 * i + 2] = v.z;
+          io[m][r][4 * i + 3] = v.w;
+        }
+        if (u >= whole && a.base && rows[m][r] >= 0) {
+          const T* from = (const T*)a.base + rows[m][r] * a.base_st + 32 * u + 8 * t;
           T* to = reinterpret_cast<T*>(io[m][r]);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -365,19 +380,13 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = n0 + 2 * j < a.outer ? *reinterpret_cast<const Word*>(from + 2 * j * a.rank) : Word();
   };
-  unsigned io[MT][2][WORDS], ahead[MT][2][WORDS];
+  unsigned io[MT][2][WORDS];
   Word next[4];
-  if (q < blocks) {
-    load_base(q, ahead);
-    load_weights(q, 0, next);
-  }
+#pragma unroll
+  for (int s = 0; s < kDepth; ++s) copy(ring + s * kStage);
+  uint32_t ring_at = ring;
+  if (q < blocks) load_weights(q, 0, next);
   for (int u = q; u < blocks; u += of) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) io[m][r][i] = ahead[m][r][i];
     float acc[MT][4][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -389,10 +398,7 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
       if (k == 0) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = next[j];
-        if (u + of < blocks) {
-          load_base(u + of, ahead);
-          load_weights(u + of, 0, next);
-        }
+        if (u + of < blocks) load_weights(u + of, 0, next);
       } else {
         load_weights(u, k, w);
       }
@@ -420,6 +426,10 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
         }
       }
     }
+    copy_wait<kDepth - 1>();
+    take_base(u, ring_at, io);
+    copy(ring_at);
+    ring_at = ring_at == ring + (kDepth - 1) * kStage ? ring : ring_at + kStage;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -440,6 +450,7 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
         }
       }
   }
+  copy_wait<0>();
 }
 
 // A group of 9 to 32 rows.
@@ -449,8 +460,8 @@ __device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& clus
   using L = Layout<T>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   constexpr int NT = 4, kStage = 1024 + NT * 512, kDepth = kRing / kStage;
-  float* sums = reinterpret_cast<float*>(smem + L::sums_at(a.rank));
-  T* h = reinterpret_cast<T*>(smem);
+  float* sums = reinterpret_cast<float*>(smem + L::sums_at(a.rank, a.most_slots));
+  T* h = reinterpret_cast<T*>(smem + kWarps * kRing);
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * kRing) + lane * 16;
   const int bytes = (int)a.a_row, pieces = (bytes + 63) / 64, x_bytes = a.inner * (int)sizeof(T);
   const T* rows[NT];
@@ -513,12 +524,12 @@ __device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& clus
   if (ranks > 1) cluster.sync();
   else __syncthreads();
   if constexpr (sizeof(T) == 2) {
-    if (count <= 16) expand<T, 1>(a, adapter, h, part, slots, count, row0, q, of);
-    else expand<T, 2>(a, adapter, h, part, slots, count, row0, q, of);
+    if (count <= 16) expand<T, 1>(a, adapter, h, part, slots, count, row0, q, of, ring);
+    else expand<T, 2>(a, adapter, h, part, slots, count, row0, q, of, ring);
   } else {  // (two blocks of fp32 rows do not fit the registers)
-    for (int s = 0; s < count; s += 16) expand<T, 1>(a, adapter, h + s * L::pitch(a.rank), part, slots + s, count - s, row0, q, of);
+    for (int s = 0; s < count; s += 16) expand<T, 1>(a, adapter, h + s * L::pitch(a.rank), part, slots + s, count - s, row0, q, of, ring);
   }
-  __syncthreads();  // h's place is the rings of the next group
+  __syncthreads();  // h and the sums are written again for the next group
 }
 
 template <typename T>
