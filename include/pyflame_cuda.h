@@ -533,7 +533,8 @@ typedef struct pfk_cache4_append_params {
   int64_t q_heads, q_st, q_sh, qo_st, qo_sh;
   const int64_t* slots;     /* [tokens]; negative: the token is skipped, its q_out row left as it was */
   const int64_t* positions; /* [tokens]; may be NULL without rotation */
-  pfk_rotary rotary;        /* of k, in 64 bits and rounded to fp32 once, and of q */
+  pfk_rotary rotary;        /* of k, in 64 bits and rounded to fp32 once, and of q; its factor is not read */
+  double factor;            /* on cosines and sines, in 64 bits: it moves keys over the borders between codes */
 } pfk_cache4_append_params;
 /* The slots of one call are distinct: of tokens that name the same slot, parts
  * of each may remain. */

@@ -112,7 +112,7 @@ class Cache4AppendParamsC(C.Structure):
     _fields_ = [("cache", Cache4C), ("dtype", C.c_int), ("tokens", _I64), ("k", _P), ("k_st", _I64), ("k_sh", _I64), ("v", _P),
                 ("v_st", _I64), ("v_sh", _I64), ("q", _P), ("q_out", _P)] + [(n, _I64) for n in (
                     "q_heads", "q_st", "q_sh", "qo_st", "qo_sh")] + [
-        ("slots", _P), ("positions", _P), ("rotary", RotaryC)]
+        ("slots", _P), ("positions", _P), ("rotary", RotaryC), ("factor", C.c_double)]
 
 
 class Cache4ReadParamsC(C.Structure):

@@ -100,7 +100,7 @@ class PagedKVCache4bit:
         p = N.Cache4AppendParamsC.from_buffer_copy(plan[0])
         p.k, p.v, p.slots = at_k, at_v, _ = k.data_ptr(), v.data_ptr(), slots.data_ptr()
         if rotary is not None:
-            p.positions, p.rotary = positions.data_ptr(), rotary._c
+            p.positions, p.rotary, p.factor = positions.data_ptr(), rotary._c, rotary.factor
         if q is not None:
             if q_out is None:
                 q_out = q.new_zeros(q.shape)

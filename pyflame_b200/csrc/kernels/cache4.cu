@@ -51,7 +51,7 @@ struct Args {
   const int64_t* positions;
   const double* inv_freq;
   int rot, interleaved;
-  float factor;
+  double factor;
   void* out[2];  // of a read: k, v
 };
 
@@ -553,7 +553,7 @@ void launch_cache4_append(const pfk_cache4_append_params& p, cudaStream_t stream
   a.inv_freq = r.inv_freq;
   a.rot = (int)r.rotary_dim;
   a.interleaved = r.interleaved;
-  a.factor = r.factor;
+  a.factor = p.factor;
   if (p.dtype == PFC_DTYPE_FLOAT32) launch_append<float>(a, stream);
   else if (p.dtype == PFC_DTYPE_FLOAT16) launch_append<__half>(a, stream);
   else launch_append<__nv_bfloat16>(a, stream);

@@ -41,7 +41,7 @@ def test_append_refusals(native, change, word):
     v.update(change)
     p = native.Cache4AppendParamsC(cache(native, **change), v["dtype"], v["tokens"], v["tk"], v["k_st"], 64, v["tv"], 128, 64, v["q"], v["q_out"],
                                    v["q_heads"], 256, 64, v["qo_st"], 64, v["slots"], v["positions"],
-                                   native.RotaryC(v["inv"], v["rot"], v["interleaved"], 1.0))
+                                   native.RotaryC(v["inv"], v["rot"], v["interleaved"], 1.0), 1.0)
     refused(native, native.lib().pfk_cache4_append(C.byref(p), None), word)
 
 

@@ -136,6 +136,22 @@ def test_append_rotated(dtype, layout, dim, rot, heads, q_heads, tokens):
         within(out, y, HALF[dtype] * y.abs() + 2.0 ** -21 * 1.25 * 2 * q.double().abs().amax() + TINY[dtype])
 
 
+def test_the_factor_counts_in_64_bits():
+    """Many keys, rotated with a factor that fp32 does not hold: one rounding to fp32, and so the same codes."""
+    g = gen(31)
+    r = pf.RotaryEmbedding(128, scaling={"type": "yarn", "factor": 8.0, "original_max_position": 4096})
+    k, pos = randn(g, 6000, 8, 128, dtype=F16), torch.randint(0, 32768, (6000,), generator=g, device="cuda")
+    c = pf.PagedKVCache4bit(375, 16, 8, 128)
+    slots = torch.randperm(6000, generator=g, device="cuda")
+    c.append(k, k, slots, positions=pos, rotary=r)
+    a, x = pos.double()[:, None] * r.inv_freq, k.double()
+    cos, sin = (f(a)[:, None] * r.factor for f in (torch.cos, torch.sin))
+    turned = torch.cat((x[..., :64] * cos - x[..., 64:] * sin, x[..., :64] * sin + x[..., 64:] * cos), -1)
+    # angles of up to 32768 in one 64-bit number are off by 2^-38: one key in 10^4 rounds to another fp32
+    # number, and one in 10^5 of those to another code
+    assert same(c.read(slots)[0], kept(turned.float(), 64)[0])
+
+
 def test_queries_in_place_and_skipped_rows():
     g = gen(3)
     r = pf.RotaryEmbedding(64)
