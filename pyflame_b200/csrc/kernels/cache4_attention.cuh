@@ -409,18 +409,25 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
       }
     }
   };
+  // The lane's places in record 0 (RUNS: of its row among 16): the record's
+  // offset is one multiplication and addition, the other rows' an immediate.
+  const char* const lane_k = a.k + (RUNS ? g * (W / 2) : 0) + t * (4 * L::kPaired);
+  const char* const lane_v = a.v + (RUNS ? t * W : 0) + g * (4 * L::kPaired);
+  const char* const lane_ks = a.k_scales + (RUNS ? g * (4 * L::kScales) : 0);
+  const char* const lane_vs = a.v_scales + (RUNS ? g * (4 * L::kScales) : 0);
   auto load_k = [&]() {
     seen = next_seen;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const unsigned long long u = RUNS ? (unsigned long long)next_k[r][0] + 8 * i + g : next_k[r][RUNS ? 0 : i];
-        const char* at = a.k + u * (W / 2);
-        load_words<L::kPaired>(kc[r][i], at + t * (4 * L::kPaired));
-        if constexpr (B & 1) load_words<1>(kc[r][i] + L::kPaired, at + 16 * L::kPaired + 4 * t);
-        load_words<L::kScales>(kw[r][i], a.k_scales + u * (4 * L::kScales));
-        load_words<L::kScales>(vw[r][i], a.v_scales + u * (4 * L::kScales));
+        const unsigned long long u = next_k[r][RUNS ? 0 : i];
+        const int more = RUNS ? 8 * i : 0;  // rows
+        const char* at = lane_k + u * (W / 2) + more * (W / 2);
+        load_words<L::kPaired>(kc[r][i], at);
+        if constexpr (B & 1) load_words<1>(kc[r][i] + L::kPaired, at + 16 * L::kPaired - t * (4 * L::kPaired - 4));
+        load_words<L::kScales>(kw[r][i], lane_ks + u * (4 * L::kScales) + more * (4 * L::kScales));
+        load_words<L::kScales>(vw[r][i], lane_vs + u * (4 * L::kScales) + more * (4 * L::kScales));
       }
   };
   auto load_v = [&](unsigned parity) {
@@ -429,10 +436,10 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int i = 0; i < VK; ++i) {
-        const unsigned long long u = RUNS ? (unsigned long long)next_v[r][0] + 4 * i + t : next_v[r][RUNS ? 0 : i];
-        const char* at = a.v + u * W;
-        load_words<L::kPaired>(vc[r][i], at + g * (4 * L::kPaired));
-        if constexpr (B & 1) load_words<1>(vc[r][i] + L::kPaired, at + 32 * L::kPaired + 4 * g);
+        const unsigned long long u = next_v[r][RUNS ? 0 : i];
+        const char* at = lane_v + u * W + (RUNS ? 4 * i * W : 0);
+        load_words<L::kPaired>(vc[r][i], at);
+        if constexpr (B & 1) load_words<1>(vc[r][i] + L::kPaired, at + 32 * L::kPaired - g * (4 * L::kPaired - 4));
       }
   };
   // of the lane's four keys of a step's values: which are odd tokens of their pages
