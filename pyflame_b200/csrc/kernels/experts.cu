@@ -30,6 +30,13 @@
 // The rows come through a ring of asynchronous copies in shared memory for
 // each warp, whose lanes read what they copied, as operand registers
 // (streamed.cuh): the copies run ahead over the borders of rows and experts.
+//
+// Measured (device time, replayed from a graph; the bytes at 6.56 TB/s in
+// brackets): 64 tokens, 8 of 128 experts, 2048 x 768, fp16, 1.19 GB: 225 us
+// (181), of which route and list 21, up 124 and down 85; one token, 6 of 64
+// experts, 2048 x 1408, bf16, 104 MB: 34 us (15.9), route 8.7, up 15.6 and
+// down 11.4, of which 8 stay when its weights are in L2: what begins and ends
+// a kernel; five tokens, 2 of 8 experts, 768 x 2048, fp32: 40 us (17.6).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
