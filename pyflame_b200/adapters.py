@@ -66,12 +66,14 @@ class LowRankAdapters:
         a, b = a.detach(), b.detach()
         _check("a", a, (r, self.in_features), self.dtype, self.device, False)
         _check("b", b, (self.out_features, r), self.dtype, self.device, False)
-        with torch.no_grad(), torch.cuda.device(self.device):
-            self._a[i, :r, :self.in_features].copy_(a)
-            self._a[i, r:].zero_()
-            self._b[i, :, :r].copy_(b)
-            self._b[i, :, r:].zero_()
-            self._scales[i].fill_(float(scale))
+        with torch.no_grad():
+            mine_a, mine_b = self._a[i], self._b[i]
+            mine_a[:r, :self.in_features].copy_(a)
+            mine_b[:, :r].copy_(b)
+            if r < len(mine_a):
+                mine_a[r:].zero_()
+                mine_b[:, r:].zero_()
+            self._scales[i] = float(scale)
 
     def __call__(self, x, index, base=None, out=None):
         """base + the adapters' part: x [..., in_features], index int32

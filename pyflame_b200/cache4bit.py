@@ -1,5 +1,5 @@
-"""A paged key-value cache in 4 bits: a fourth of the memory of PagedKVCache in
-16-bit types, and of what attention reads.
+"""A paged key-value cache in 4 bits: little more than a fourth of the memory of
+PagedKVCache in 16-bit types, and of what attention reads.
 
   PagedKVCache4bit  append(): quantise and store new keys and values, the keys
                     rotated on the way; attend(): attention of one new token

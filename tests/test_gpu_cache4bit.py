@@ -442,6 +442,25 @@ def test_layouts(dtype):
     assert not none.any()
 
 
+@pytest.mark.parametrize("page", [16, 15])
+def test_places_beyond_32_bits(page):
+    """A cache of 9 GB of keys' codes and as much of values': tokens at both ends of it."""
+    g = gen(19)
+    pages = (1 << 25) // page
+    c = pf.PagedKVCache4bit(pages, page, 2, 256, group_size=128)
+    assert c.k.numel() * 4 > 1 << 32 and c.v.numel() * 4 > 1 << 32
+    table = torch.tensor([[pages - 1, 0, pages - 2, pages // 2]], dtype=torch.int32, device="cuda")
+    n = 4 * page - 3
+    j = torch.arange(n, device="cuda")
+    slots = table[0, j // page].long() * page + j % page
+    k, v = randn(g, n, 2, 256, dtype=F16), randn(g, n, 2, 256, dtype=F16)
+    c.append(k, v, slots)
+    got = c.read(slots)
+    assert same(got[0], kept(k.float(), 128)[0]) and same(got[1], kept(v.float(), 128)[0])
+    check_attend(c, randn(g, 1, 4, 256, dtype=F16), table, torch.tensor([n], dtype=torch.int32, device="cuda"))
+    c.check()
+
+
 def test_same_bits_streams_and_graphs():
     """The same call gives the same bits: again, on another stream while it runs, captured and replayed with new data."""
     g = gen(17)
