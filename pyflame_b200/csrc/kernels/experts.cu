@@ -34,8 +34,8 @@
 // Measured (device time, replayed from a graph; the bytes at 6.56 TB/s in
 // brackets): 64 tokens, 8 of 128 experts, 2048 x 768, fp16, 1.19 GB: 225 us
 // (181), of which route and list 21, up 124 and down 85; one token, 6 of 64
-// experts, 2048 x 1408, bf16, 104 MB: 34 us (15.9), route 8.7, up 15.6 and
-// down 11.4, of which 8 stay when its weights are in L2: what begins and ends
+// experts, 2048 x 1408, bf16, 104 MB: 32.6 us (15.9), route 8.7, up 15.6 and
+// down 10.5, of which 8 stay when its weights are in L2: what begins and ends
 // a kernel; five tokens, 2 of 8 experts, 768 x 2048, fp32: 40 us (17.6).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -538,35 +538,36 @@ __global__ void __launch_bounds__(kThreads, (Up<T, NT>::kResident)) up_kernel(Ar
   }
 }
 
-template <typename T, int NT>
+// WARPS of a CTA: with few blocks of rows, all of a block's in one CTA.
+template <typename T, int NT, int WARPS>
 struct Down {
   static constexpr int kDepth = NT == 1 ? 6 : 4;
   using R = Ring<NT * Parts<T>::kH, kDepth>;
-  static constexpr int kResident = NT == 1 ? 4 : 3;
+  static constexpr int kResident = WARPS > 4 ? 16 / WARPS : NT == 1 ? 4 : 3;
   static size_t smem(int parts, int pairs, int tokens) {
-    return (size_t)kWarps * (R::kBytes + tokens * 64) + (size_t)parts * 16 + (size_t)round_up(pairs, 4) * 4;
+    return (size_t)WARPS * (R::kBytes + tokens * 64) + (size_t)parts * 16 + (size_t)round_up(pairs, 4) * 4;
   }
 };
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(kThreads, (Down<T, NT>::kResident)) down_kernel(Args a) {
-  using D = Down<T, NT>;
+template <typename T, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, (Down<T, NT, WARPS>::kResident)) down_kernel(Args a) {
+  using D = Down<T, NT, WARPS>;
   constexpr int PARTS = Parts<T>::kH;
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = (int)(blockIdx.x / ranks) * 16, cells = a.tokens * 16;
-  float* tables = reinterpret_cast<float*>(smem + kWarps * D::R::kBytes);  // [warps][tokens][16]
-  int4* parts = reinterpret_cast<int4*>(tables + kWarps * cells);
+  float* tables = reinterpret_cast<float*>(smem + WARPS * D::R::kBytes);  // [warps][tokens][16]
+  int4* parts = reinterpret_cast<int4*>(tables + WARPS * cells);
   int* pairs = reinterpret_cast<int*>(parts + a.most_parts);
   typename D::R ring(smem + warp * D::R::kBytes);
-  for (int i = tid; i < kWarps * cells; i += kThreads) tables[i] = 0.f;
+  for (int i = tid; i < WARPS * cells; i += (WARPS * 32)) tables[i] = 0.f;
   begin();
-  for (int i = tid; i < a.most_parts; i += kThreads) parts[i] = a.parts[1 + i];
-  for (int i = tid; i < a.tokens * a.top; i += kThreads) pairs[i] = a.pairs[i];
+  for (int i = tid; i < a.most_parts; i += (WARPS * 32)) parts[i] = a.parts[1 + i];
+  for (int i = tid; i < a.tokens * a.top; i += (WARPS * 32)) pairs[i] = a.pairs[i];
   const int bytes = (int)min(a.h_row, a.down_row), pieces = (bytes + 63) / 64;
-  const int total = a.parts[0].x * pieces, q = rank * kWarps + warp, of = ranks * kWarps;
+  const int total = a.parts[0].x * pieces, q = rank * WARPS + warp, of = ranks * WARPS;
   const int p0 = (int)((long long)total * q / of), p1 = (int)((long long)total * (q + 1) / of);
   __syncthreads();
 
@@ -652,15 +653,15 @@ __global__ void __launch_bounds__(kThreads, (Down<T, NT>::kResident)) down_kerne
     __syncwarp();
   }
   __syncthreads();
-  for (int i = tid; i < cells; i += kThreads) {
+  for (int i = tid; i < cells; i += (WARPS * 32)) {
     float s = tables[i];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) s += tables[w * cells + i];
+    for (int w = 1; w < WARPS; ++w) s += tables[w * cells + i];
     tables[i] = s;
   }
   if (ranks > 1) cluster.sync();
   else __syncthreads();
-  for (int i = rank * kThreads + tid; i < cells; i += kThreads * ranks) {
+  for (int i = rank * (WARPS * 32) + tid; i < cells; i += (WARPS * 32) * ranks) {
     float s = 0.f;
     for (int r = 0; r < ranks; ++r) s += cluster.map_shared_rank(tables, r)[i];
     const int n = i >> 4, d = row + (i & 15);
@@ -733,26 +734,41 @@ int resident(F kernel, size_t most, size_t usual, std::once_flag* once, int* per
 constexpr size_t kSharedOfSm = 228 * 1024;
 constexpr int kMostPairs = kBlockTokens * kMostTop, kMostParts = kMostExperts + kMostPairs / 16;
 
-template <typename T, int NT>
-void launch_products(const Args& a, cudaStream_t stream) {
-  using U = Up<T, NT>;
-  using D = Down<T, NT>;
-  const int sms = device_sm_count(current_device()), pairs = a.tokens * a.top;
-  static std::once_flag once_up[64], once_down[64];
-  static int per_up[64], per_down[64];
-  const int per = resident(up_kernel<T, NT>, U::smem(kMostParts, kMostPairs), U::smem(64, 64), once_up, per_up);
-  const int64_t units = (int64_t)a.most_parts * ceil_div(a.inner, 8);
-  launch_following<Args>(up_kernel<T, NT>, dim3((unsigned)std::min<int64_t>(units, (int64_t)per * sms)), kThreads, U::smem(a.most_parts, pairs),
-                         stream, a);
-  resident(down_kernel<T, NT>, D::smem(kMostParts, kMostPairs, kBlockTokens), D::smem(64, 64, 8 * NT), once_down, per_down);
+template <typename T, int NT, int WARPS>
+void launch_down(const Args& a, cudaStream_t stream) {
+  using D = Down<T, NT, WARPS>;
+  static std::once_flag once[64];
+  std::call_once(once[current_device()], [] {
+    PFB_CUDA(cudaFuncSetAttribute(down_kernel<T, NT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)D::smem(kMostParts, NT == 1 ? 8 * kMostTop : kMostPairs, NT == 1 ? 8 : kBlockTokens)));
+  });
+  const int pairs = a.tokens * a.top;
   // as many CTAs as the device holds at once (a second round of few would take as
   // long as the first), but runs of at least 8 pieces for a warp
   const size_t smem = D::smem(a.most_parts, pairs, a.tokens);
   const int64_t blocks = ceil_div(a.width, 16), pieces = a.most_parts * ceil_div(a.h_row, 64);
-  const int64_t slots = std::min<int64_t>(D::kResident, (int64_t)(kSharedOfSm / (smem + 1024))) * sms;
+  const int64_t slots = std::min<int64_t>(D::kResident, (int64_t)(kSharedOfSm / (smem + 1024))) * device_sm_count(current_device());
   int ranks = 1;
-  while (ranks < 8 && blocks * (ranks + 1) <= slots && pieces >= 8 * kWarps * (ranks + 1)) ++ranks;
-  launch_following<Args>(down_kernel<T, NT>, dim3((unsigned)(blocks * ranks)), kThreads, smem, stream, a, ranks);
+  while (ranks < 8 && blocks * (ranks + 1) <= slots && pieces >= 8 * WARPS * (ranks + 1)) ++ranks;
+  launch_following<Args>(down_kernel<T, NT, WARPS>, dim3((unsigned)(blocks * ranks)), WARPS * 32, smem, stream, a, ranks);
+}
+
+template <typename T, int NT>
+void launch_products(const Args& a, cudaStream_t stream) {
+  using U = Up<T, NT>;
+  const int sms = device_sm_count(current_device()), pairs = a.tokens * a.top;
+  static std::once_flag once_up[64];
+  static int per_up[64];
+  const int per = resident(up_kernel<T, NT>, U::smem(kMostParts, kMostPairs), U::smem(64, 64), once_up, per_up);
+  const int64_t units = (int64_t)a.most_parts * ceil_div(a.inner, 8);
+  launch_following<Args>(up_kernel<T, NT>, dim3((unsigned)std::min<int64_t>(units, (int64_t)per * sms)), kThreads, U::smem(a.most_parts, pairs),
+                         stream, a);
+  const int64_t blocks = ceil_div(a.width, 16);
+  // Where CTAs of 16 warps fill the device, and nearly all of it, a block's sums
+  // need no cluster (one token, width 2048: 10.5 us for 11.4; of width 2560, 8
+  // warps without a cluster took 4 us longer, with 48 blocks 16 did 9 longer).
+  if (NT == 1 && 5 * blocks > 4 * sms && blocks <= sms) launch_down<T, NT, 16>(a, stream);
+  else launch_down<T, NT, 4>(a, stream);
 }
 
 template <int TB>
