@@ -29,8 +29,7 @@
 // key-value head and up to 8 of its query heads; its keys are cut into tiles,
 // a step of a CTA's 4 warps each; the tiles of all units form one list, of
 // which each CTA of one wave takes an equal run, and a second small kernel
-// joins the shares of units that several CTAs have, in the order of the list.
-// Few units of short sequences have a cluster of CTAs each.
+// joins the shares of units that several CTAs have, in a fixed order.  Few units of short sequences have a cluster of CTAs each.
 //
 // Step.  A warp takes 32 keys (16 of heads above 128 values, of pages that are
 // no multiple of 16 tokens, and in clusters): lane (g, t) = (lane / 4, lane %
@@ -46,7 +45,7 @@
 // Measured (device time, replayed from a graph; the bytes at 6.56 TB/s in
 // brackets): 128 sequences of 2048 to 8192 keys, bf16, 32/8 heads of 128,
 // groups of 64, 757 MB: 168 us (115); 48 of 0 to 8192, fp16, groups of 32: 88
-// us (38.5); one of 131071, 64/8 heads, bf16: 45.6 us (23); one of 333 with a
+// us (38.5); one of 131071, 64/8 heads, bf16: 43.1 us (23); one of 333 with a
 // window of 250, fp32, 20 heads of 80: 5.9 us.  The long ones are bound by
 // their instructions, 720 for a warp's 32 keys (920 with groups of 32 and
 // weights in two parts), of which 59 % of the issue slots are used: with all
@@ -820,23 +819,54 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
   }
 }
 
-constexpr int kJoinThreads = 256;
+// A join's shares are split among groups of its threads.  Few units have many
+// shares each: one CTA for a unit, of all the threads that it may have (two
+// sequences of 86832 and 696 keys on one key-value head, pages of 7: the call
+// took 42.4 us with 256 threads, 20.6 so; one of 8 units 45.7 and 43.1).  With
+// 1024 threads in a CTA for each CTA of the first kernel, most of which have
+// nothing to join, that of 8 units took 58.  Many units have few shares each,
+// and a CTA of 256 for each CTA of the first kernel, with no unit to look for.
+constexpr int kFewUnits = 64;
 
-// CTA (c, h): joins the shares of query head h of the unit that began in CTA
-// c of the first kernel and went on, in the order of the list; and writes
-// the outputs of sequence c if it is empty.
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a) {
-  __shared__ float4 acc[kJoinThreads];
-  __shared__ float2 stats[kJoinThreads / 16];
-  const int tid = threadIdx.x, c0 = blockIdx.x;
+// CTA (c, h): joins the shares of query head h of a unit that went on beyond
+// the CTA it began in, in a fixed order: with FIND the c-th such unit,
+// else the one that began in CTA c of the first kernel; and writes the outputs
+// of sequence c if it is empty.
+template <typename T, int THREADS, bool FIND>
+__global__ void __launch_bounds__(THREADS) join_kernel(Args a) {
+  __shared__ float4 acc[THREADS];
+  __shared__ float2 stats[THREADS / 16];
+  const int tid = threadIdx.x;
+  int c0 = blockIdx.x;
   begin();
   if (c0 < a.batch && span_of<64>(a, c0).tiles == 0) {
     for (int qh = blockIdx.y; qh < a.q_heads; qh += gridDim.y) {
-      for (int d = tid; d < a.head_dim; d += kJoinThreads)
+      for (int d = tid; d < a.head_dim; d += THREADS)
         ((T*)a.out)[(long long)c0 * a.o_sb + (long long)qh * a.o_sh + d] = from_float<T>(0.f);
       if (tid == 0 && a.lse) a.lse[(long long)c0 * a.q_heads + qh] = -INFINITY;
     }
+  }
+  if constexpr (FIND) {
+    __shared__ int in_warp[THREADS / 32], found;
+    if (tid == 0) found = -1;
+    int left = c0;  // such units before this CTA's that are still to come
+    for (int base = 0; base < a.ctas; base += THREADS) {
+      const bool on = base + tid < a.ctas && a.records[base + tid].w;
+      const unsigned lanes = __ballot_sync(~0u, on);
+      if (tid % 32 == 0) in_warp[tid / 32] = __popc(lanes);
+      __syncthreads();
+      int before = 0, all = 0;
+#pragma unroll
+      for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < tid / 32) before += in_warp[w];
+        all += in_warp[w];
+      }
+      if (on && before + __popc(lanes & ((1u << tid % 32) - 1)) == left) found = base + tid;
+      left -= all;
+      __syncthreads();
+    }
+    c0 = found;
+    if (c0 < 0) return;
   }
   if (c0 >= a.ctas) return;
   const int4 rec = a.records[c0];
@@ -849,7 +879,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a) {
   auto share = [&](int i) -> long long { return ((long long)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * a.heads + h; };
   const int cols = a.head_dim / 4;                            // of 4 values
   const int across = cols <= 16 ? 16 : cols <= 32 ? 32 : 64;  // threads of a share
-  const int groups = kJoinThreads / across, gi = tid / across, col = tid % across;
+  const int groups = THREADS / across, gi = tid / across, col = tid % across;
 
   // x, of maximum m, joined to (top, sum, v): one pass, each of its loads
   // independent of the others
@@ -872,11 +902,22 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a) {
       join(st.x, st.y, *reinterpret_cast<const float4*>(a.parts + share(i) * a.head_dim + col * 4));
     }
   }
-  acc[tid] = v;
-  if (col == 0) stats[gi] = make_float2(top, sum);
-  __syncthreads();
+  if constexpr (FIND) {  // many groups: by halves
+    for (int half = groups / 2; half > 0; half /= 2) {
+      if (gi >= half && gi < 2 * half) {
+        acc[tid] = v;
+        if (col == 0) stats[gi] = make_float2(top, sum);
+      }
+      __syncthreads();
+      if (gi < half) join(stats[gi + half].x, stats[gi + half].y, acc[(gi + half) * across + col]);
+    }
+  } else {
+    acc[tid] = v;
+    if (col == 0) stats[gi] = make_float2(top, sum);
+    __syncthreads();
+    for (int w = 1; gi == 0 && w < groups; ++w) join(stats[w].x, stats[w].y, acc[w * across + col]);
+  }
   if (gi == 0 && col < cols) {
-    for (int w = 1; w < groups; ++w) join(stats[w].x, stats[w].y, acc[w * across + col]);
     T* out = (T*)a.out + (long long)b * a.o_sb + (long long)qh * a.o_sh + col * 4;
     const float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -918,7 +959,11 @@ void launch_sized(Args& a, int ranks, cudaStream_t stream) {
     return;
   }
   launch_following<Args>(K::run, dim3((unsigned)a.ctas), kThreads, K::L::smem, stream, a);
-  launch_following<Args>(join_kernel<typename K::T>, dim3((unsigned)std::max(a.ctas, a.batch), (unsigned)a.heads), kJoinThreads, 0, stream, a);
+  const int64_t units = (int64_t)a.batch * a.kv_heads * a.chunks;
+  if (units <= kFewUnits && units < a.ctas)
+    launch_following<Args>(join_kernel<typename K::T, 1024, true>, dim3((unsigned)units, (unsigned)a.heads), 1024, 0, stream, a);
+  else
+    launch_following<Args>(join_kernel<typename K::T, 256, false>, dim3((unsigned)std::max(a.ctas, a.batch), (unsigned)a.heads), 256, 0, stream, a);
 }
 
 // Calls f(Kernel<...>()) for the call's sizes.  Groups as wide as the head are
