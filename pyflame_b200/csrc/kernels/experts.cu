@@ -61,7 +61,8 @@ namespace cg = cooperative_groups;
 constexpr int kBlockTokens = 128;  // tokens of one pass over the weights
 constexpr int kMostExperts = 1024;
 constexpr int kMostTop = 32;
-constexpr int kRouteRanks = 8;
+constexpr int kMostRanks = 8;  // CTAs of a cluster
+constexpr int kRouteRanks = kMostRanks;
 constexpr int kRouteThreads = 256;
 constexpr int kRouteBlock = 2048;  // values of x that it holds of a token at a time
 constexpr int kWarps = 4;
@@ -404,7 +405,7 @@ struct Up {
   static constexpr int kDepth = NT == 1 ? 8 : 6;
   using R = Ring<NT, kDepth>;
   static constexpr int kResident = 4;  // CTAs an SM
-  static size_t smem(int parts, int pairs) { return (size_t)kWarps * R::kBytes + (size_t)parts * 16 + (size_t)round_up(pairs, 4) * 4; }
+  static size_t smem(int parts, int pairs) { return (size_t)kWarps * R::kBytes + (size_t)parts * 16 + (size_t)((pairs + 3) / 4) * 16; }
 };
 
 // Units are 8 rows of a part of an expert's pairs; CTAs take them in turn.
@@ -543,9 +544,9 @@ template <typename T, int NT, int WARPS>
 struct Down {
   static constexpr int kDepth = NT == 1 ? 6 : 4;
   using R = Ring<NT * Parts<T>::kH, kDepth>;
-  static constexpr int kResident = WARPS > 4 ? 16 / WARPS : NT == 1 ? 4 : 3;
-  static size_t smem(int parts, int pairs, int tokens) {
-    return (size_t)WARPS * (R::kBytes + tokens * 64) + (size_t)parts * 16 + (size_t)round_up(pairs, 4) * 4;
+  static constexpr int kResident = WARPS > 4 ? (NT == 1 ? 16 : 8) / WARPS : NT == 1 ? 4 : 3;
+  static constexpr size_t smem(int parts, int pairs, int tokens) {
+    return (size_t)WARPS * (R::kBytes + tokens * 64) + (size_t)parts * 16 + (size_t)((pairs + 3) / 4) * 16;
   }
 };
 
@@ -738,9 +739,10 @@ template <typename T, int NT, int WARPS>
 void launch_down(const Args& a, cudaStream_t stream) {
   using D = Down<T, NT, WARPS>;
   static std::once_flag once[64];
+  constexpr size_t most = D::smem(kMostParts, NT == 1 ? 8 * kMostTop : kMostPairs, NT == 1 ? 8 : kBlockTokens);
+  static_assert(most <= 227 * 1024, "more than a CTA may have");
   std::call_once(once[current_device()], [] {
-    PFB_CUDA(cudaFuncSetAttribute(down_kernel<T, NT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)D::smem(kMostParts, NT == 1 ? 8 * kMostTop : kMostPairs, NT == 1 ? 8 : kBlockTokens)));
+    PFB_CUDA(cudaFuncSetAttribute(down_kernel<T, NT, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
   });
   const int pairs = a.tokens * a.top;
   // as many CTAs as the device holds at once (a second round of few would take as
@@ -749,7 +751,7 @@ void launch_down(const Args& a, cudaStream_t stream) {
   const int64_t blocks = ceil_div(a.width, 16), pieces = a.most_parts * ceil_div(a.h_row, 64);
   const int64_t slots = std::min<int64_t>(D::kResident, (int64_t)(kSharedOfSm / (smem + 1024))) * device_sm_count(current_device());
   int ranks = 1;
-  while (ranks < 8 && blocks * (ranks + 1) <= slots && pieces >= 8 * WARPS * (ranks + 1)) ++ranks;
+  while (ranks < kMostRanks && blocks * (ranks + 1) <= slots && pieces >= 8 * WARPS * (ranks + 1)) ++ranks;
   launch_following<Args>(down_kernel<T, NT, WARPS>, dim3((unsigned)(blocks * ranks)), WARPS * 32, smem, stream, a, ranks);
 }
 
@@ -767,7 +769,13 @@ void launch_products(const Args& a, cudaStream_t stream) {
   // Where CTAs of 16 warps fill the device, and nearly all of it, a block's sums
   // need no cluster (one token, width 2048: 10.5 us for 11.4; of width 2560, 8
   // warps without a cluster took 4 us longer, with 48 blocks 16 did 9 longer).
-  if (NT == 1 && 5 * blocks > 4 * sms && blocks <= sms) launch_down<T, NT, 16>(a, stream);
+  // Where the widest clusters leave a quarter of the device idle, 8 warps in a
+  // CTA hide more of the memory's latency than 4 (whole calls: fp32, 24 tokens,
+  // 64 experts, 128 x 1400: 37.0 us with 4, 32.8 with 8; fp16, 128 tokens, 4 of
+  // 128, 200 x 889: 85.4 and 75.5); with more blocks they cost more than they
+  // give (fp16, 41 tokens, 4 of 64, 304 x 1024: 55.3 and 61.7).
+  if (NT == 1 && 5 * blocks > 4 * sms && blocks <= sms) launch_down<T, NT, NT == 1 ? 16 : 8>(a, stream);
+  else if (4 * blocks * kMostRanks <= 3 * sms) launch_down<T, NT, 8>(a, stream);
   else launch_down<T, NT, 4>(a, stream);
 }
 
