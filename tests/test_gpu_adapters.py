@@ -141,6 +141,33 @@ def test_layouts(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("inner,outer", [(72, 56), (33, 131), (7, 3), (515, 1025), (1, 1)])
+def test_rows_at_every_place(dtype, inner, outer):
+    """Rows between NaNs, that begin on no 16 bytes: the bits of packed, aligned ones, and the NaNs stay."""
+    g = gen(inner)
+    layer, parts = make(g, 4, inner, outer, [16, 48], dtype)
+    index = torch.tensor([0] * 40 + [1] * 12 + [-1] * 9 + [2] * 3 + [-1] + [3] * 17, dtype=torch.int32, device="cuda")
+    x, base = randn(g, len(index), inner, dtype=dtype), randn(g, len(index), outer, dtype=dtype)
+    pad = lambda n: torch.zeros(len(index), (n + 15) // 8 * 8, device="cuda", dtype=dtype)
+    ax, ab = pad(inner)[:, :inner].copy_(x), pad(outer)[:, :outer].copy_(base)
+    aligned = pad(outer)[:, :outer]
+    want = check(layer, parts, ax, index, ab, out=aligned)
+    assert torch.equal(layer(x, index, base), want)
+    zero = layer(ax, index)
+    for place in range(8):
+        wide = torch.full((len(index), inner + outer + 23 + place % 3), float("nan"), device="cuda", dtype=dtype)
+        wx, wb = wide[:, place:place + inner], wide[:, place + inner + 5:place + inner + 5 + outer]
+        wx.copy_(x)
+        wb.copy_(base)
+        assert torch.equal(layer(wx, index, wb), want) and torch.equal(layer(wx, index), zero)
+        layer(wx, index, wb, out=wb)
+        assert torch.equal(wb, want) and torch.equal(wx, x)
+        wx.fill_(float("nan"))
+        wb.fill_(float("nan"))
+        assert wide.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_adapters_are_replaced(dtype):
     g = gen(4)
     layer, parts = make(g, 2, 64, 64, [32], dtype)
