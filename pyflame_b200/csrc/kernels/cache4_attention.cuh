@@ -29,7 +29,8 @@
 // key-value head and up to 8 of its query heads; its keys are cut into tiles,
 // a step of a CTA's 4 warps each; the tiles of all units form one list, of
 // which each CTA of one wave takes an equal run, and a second small kernel
-// joins the shares of units that several CTAs have, in a fixed order.  Few units of short sequences have a cluster of CTAs each.
+// joins the shares of units that several CTAs have, in a fixed order.  Few
+// units of short sequences have a cluster of CTAs each.
 //
 // Step.  A warp takes 32 keys (16 of heads above 128 values, of pages that are
 // no multiple of 16 tokens, and in clusters): lane (g, t) = (lane / 4, lane %
