@@ -33,7 +33,7 @@
 // Measured (device time, replayed from a graph; the bytes at 6.56 TB/s in
 // brackets): one row, 4096 to 4096, rank 16, bf16: 6.1 us, latency alone; 61
 // rows with 55 adapters of rank 64, 4096 to 16384, fp16, 149 MB: 38.2 us
-// (22.7); 8191 rows of five prompts, rank 16, bf16, 203 MB: 46.6 us (30.9),
+// (22.7); 8191 rows of five prompts, rank 16, bf16, 203 MB: 44.9 us (30.9),
 // where all CTAs read x and then update the outputs at about the same time.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -359,8 +359,8 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int r = 0; r < 2; ++r) rows[m][r] = m * 16 + g + 8 * r < count ? row0 + slots[m * 16 + g + 8 * r] : -1;
-  // Base comes through the warp's ring, several blocks ahead.  The first 16
-  // ranks' weights are loaded a block ahead.
+  // Base comes through the warp's ring, several blocks ahead, 16
+  // ranks' weights while the 16 before them are used.
   constexpr int PARTS = WORDS / 4 + (WIDE ? 0 : 1);  // of 16 bytes, of a lane's outputs
   constexpr int kStage = MT * 2 * PARTS * 512, kDepth = kRing / kStage;
   static_assert(kDepth >= 2, "a block ahead at least");
@@ -424,13 +424,11 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
     for (int k = 0; k < a.rank; k += 16) {
       const int at = k + 4 * t;
       Word w[4];
-      if (k == 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = next[j];
-        if (u + of < blocks) load_weights(u + of, 0, next);
-      } else {
-        load_weights(u, k, w);
-      }
+      for (int j = 0; j < 4; ++j) w[j] = next[j];
+      const bool more = k + 16 < a.rank;
+      const int u_next = more ? u : u + of;
+      if (u_next < blocks) load_weights(u_next, more ? k + 16 : 0, next);
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         if constexpr (sizeof(T) == 2) {
