@@ -505,71 +505,93 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
   copy_wait<0>();
 }
 
-// A group of 9 to 32 rows.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& cluster, int ranks, int adapter, const int* slots, int count,
-                                          int row0, int q, int of, char* smem) {
-  using L = Layout<T>;
+// Ranks r0 to r0 + 16 * RT of A's products with up to 32 rows of x, which is
+// read, from L2 but for the first time, for each of them: the warp's pieces of
+// x's axis q, q + of, ..., then the sums of all warps.
+template <typename T, bool WIDE, int RT>
+__device__ __forceinline__ void reduce(const Args& a, int adapter, const int (&rows)[4], int r0, int q, int of, uint32_t ring, char* smem, float* sums) {
+  constexpr int NT = 4, kX = WIDE ? 512 : 1024, kStage = RT * 1024 + NT * kX, kDepth = kRing / kStage;
+  static_assert(kDepth >= 2, "a piece ahead at least");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  constexpr int NT = 4, kX = WIDE ? 512 : 1024, kStage = 1024 + NT * kX, kDepth = kRing / kStage;
-  float* sums = reinterpret_cast<float*>(smem + L::sums_at(a.rank, a.most_slots));
-  T* h = reinterpret_cast<T*>(smem + kWarps * kRing);
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * kRing) + lane * 16;
   const int bytes = (int)a.a_row, pieces = (bytes + 63) / 64, x_bytes = a.inner * (int)sizeof(T);
-  const T* rows[NT];
+  const char* weights = a.a + ((long long)adapter * a.rank + r0 + g) * a.a_row;
+  int c_ahead = q;
+  auto copy = [&](uint32_t to) {
+    if (c_ahead < pieces) {
+      const int at = c_ahead * 64 + t * 16;
+      const int size = at < bytes ? 16 : 0;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) rows[n] = n * 8 + g < count ? (const T*)a.x + (long long)(row0 + slots[n * 8 + g]) * a.x_st : nullptr;
-
-  for (int r0 = 0; r0 < a.rank; r0 += 16) {  // x is read again, from L2, for every 16 ranks
-    const char* weights = a.a + ((long long)adapter * a.rank + r0 + g) * a.a_row;
-    int c_ahead = q;
-    auto copy = [&](uint32_t to) {
-      if (c_ahead < pieces) {
-        const int at = c_ahead * 64 + t * 16;
-        const int size = at < bytes ? 16 : 0;
-        copy_async(to, weights + at, size);
-        copy_async(to + 512, weights + 8 * a.a_row + at, size);
+      for (int r = 0; r < 2 * RT; ++r) copy_async(to + r * 512, weights + r * 8 * a.a_row + at, size);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int s = WIDE ? 0 : behind_16(rows[n]), left = rows[n] ? s + x_bytes - at : 0;
-          const char* from = rows[n] ? (const char*)rows[n] - s + at : a.a;
-          copy_up_to(to + 1024 + n * kX, from, left);
-          if constexpr (!WIDE) copy_up_to(to + 1536 + n * kX, from + 16, s ? left - 16 : 0);
-        }
-        c_ahead += of;
+      for (int n = 0; n < NT; ++n) {
+        const char* from = (const char*)((const T*)a.x + max(rows[n], 0) * a.x_st);
+        const int s = WIDE ? 0 : behind_16(from), left = rows[n] >= 0 ? s + x_bytes - at : 0;
+        from += at - s;
+        copy_up_to(to + RT * 1024 + n * kX, from, left);
+        if constexpr (!WIDE) copy_up_to(to + RT * 1024 + 512 + n * kX, from + 16, s ? left - 16 : 0);
       }
-      copy_commit();
-    };
+      c_ahead += of;
+    }
+    copy_commit();
+  };
 #pragma unroll
-    for (int s = 0; s < kDepth; ++s) copy(ring + s * kStage);
-    uint32_t at = ring;
-    float acc[NT][4];
+  for (int s = 0; s < kDepth; ++s) copy(ring + s * kStage);
+  uint32_t at = ring;
+  float acc[RT][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    for (int c = q; c < pieces; c += of) {
-      copy_wait<kDepth - 1>();
-      uint4 v[NT];
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) v[n] = read_row<WIDE>(at + 1024 + n * kX, behind_16(rows[n]));
+    for (int n = 0; n < NT; ++n) acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.f;
+  for (int c = q; c < pieces; c += of) {
+    copy_wait<kDepth - 1>();
+    uint4 v[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) v[n] = read_row<WIDE>(at + RT * 1024 + n * kX, behind_16((const T*)a.x + max(rows[n], 0) * a.x_st));
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
       float sum[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
-      chunk_product<T, NT>(sum, read_shared(at), read_shared(at + 512), v);
+      chunk_product<T, NT>(sum, read_shared(at + r * 1024), read_shared(at + r * 1024 + 512), v);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] += sum[n][i];
-      copy(at);
-      at = at == ring + (kDepth - 1) * kStage ? ring : at + kStage;
+        for (int i = 0; i < 4; ++i) acc[r][n][i] += sum[n][i];
     }
-    copy_wait<0>();
-    float4* red = reinterpret_cast<float4*>(smem);  // in the warps' rings
-#pragma unroll
-    for (int n = 0; n < NT; ++n) red[warp * (kRing / 16) + n * 32 + lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-    __syncthreads();
-    add_warps(red, kRing / 16, NT, NT, r0, 8 * NT, sums);
-    __syncthreads();
+    copy(at);
+    at = at == ring + (kDepth - 1) * kStage ? ring : at + kStage;
   }
+  copy_wait<0>();
+  __syncwarp();
+  float4* red = reinterpret_cast<float4*>(smem);  // in the warps' rings
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      red[warp * (kRing / 16) + (r * NT + n) * 32 + lane] = make_float4(acc[r][n][0], acc[r][n][1], acc[r][n][2], acc[r][n][3]);
+  __syncthreads();
+  add_warps(red, kRing / 16, RT * NT, NT, r0, 8 * NT, sums);
+  __syncthreads();
+}
+
+// A group of 9 to 32 rows.
+template <typename T, bool WIDE, int RT>
+__device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& cluster, int ranks, int adapter, const int* slots, int count,
+                                          int row0, int q, int of, char* smem) {
+  using L = Layout<T>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
+  constexpr int NT = 4;
+  float* sums = reinterpret_cast<float*>(smem + L::sums_at(a.rank, a.most_slots));
+  T* h = reinterpret_cast<T*>(smem + kWarps * kRing);
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * kRing) + lane * 16;
+  int rows[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) rows[n] = n * 8 + g < count ? row0 + slots[n * 8 + g] : -1;
+
+  int r0 = 0;
+  if constexpr (RT > 1)
+    for (; r0 + 16 * RT <= a.rank; r0 += 16 * RT) reduce<T, WIDE, RT>(a, adapter, rows, r0, q, of, ring, smem, sums);
+  for (; r0 < a.rank; r0 += 16) reduce<T, WIDE, 1>(a, adapter, rows, r0, q, of, ring, smem, sums);
   if (ranks > 1) cluster.sync();
   const int part = 32 * L::pitch(a.rank);
   make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 32, count, h, part);
@@ -614,7 +636,12 @@ __device__ __forceinline__ void copy_rows(const Args& a, const int* slots, int c
     }
 }
 
-template <typename T, bool WIDE>
+// RT: blocks of 16 ranks that many rows' first product takes at a time, two
+// where the rank has them (8191 rows of five prompts, 4096 to 4096, rank 64,
+// bf16: 97.9 us with one, 88.4 with two; fp32: 259 and 236, though it spills).
+// Rows that are shifted leave no room for two in the rings, and a kernel with
+// the second block's registers took 1.4 us more of the 45 of rank 16.
+template <typename T, bool WIDE, int RT>
 __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(Args a) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int slots[kTile];
@@ -654,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(Args a) {
     } else if (count <= 8) {
       few_rows<T, WIDE>(a, cluster, ranks, adapter, slots, count, row0, q, of, smem);
     } else {
-      many_rows<T, WIDE>(a, cluster, ranks, adapter, slots, count, row0, q, of, smem);
+      many_rows<T, WIDE, RT>(a, cluster, ranks, adapter, slots, count, row0, q, of, smem);
     }
   }
 }
@@ -670,13 +697,13 @@ void check(const pfk_adapters_params& p) {
   PFB_CHECK_ARG(p.a_st >= p.inner && p.a_st * es % 16 == 0, "adapters: rows of a must be padded to multiples of 16 bytes");
 }
 
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, int RT>
 void launch_typed(Args& a, int64_t ctas, int ranks, cudaStream_t stream) {
   static std::once_flag once[64];
   std::call_once(once[current_device()], [] {
-    PFB_CUDA(cudaFuncSetAttribute(adapters_kernel<T, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<T>::bytes(kMostRank, kTile)));
+    PFB_CUDA(cudaFuncSetAttribute(adapters_kernel<T, WIDE, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<T>::bytes(kMostRank, kTile)));
   });
-  launch_following<Args>(adapters_kernel<T, WIDE>, dim3((unsigned)ctas), kThreads, (size_t)Layout<T>::bytes(a.rank, a.most_slots), stream, a,
+  launch_following<Args>(adapters_kernel<T, WIDE, RT>, dim3((unsigned)ctas), kThreads, (size_t)Layout<T>::bytes(a.rank, a.most_slots), stream, a,
                          ranks);
 }
 
@@ -730,8 +757,9 @@ void launch_adapters(const pfk_adapters_params& p, cudaStream_t stream) {
   int ranks = 1;
   while (ranks < kMostRanks && units * ranks <= sms && work > ranks * kWarps) ranks *= 2;
   auto launch = [&](auto t) {
-    if (all_wide) launch_typed<decltype(t), true>(a, units * ranks, ranks, stream);
-    else launch_typed<decltype(t), false>(a, units * ranks, ranks, stream);
+    if (!all_wide) launch_typed<decltype(t), false, 1>(a, units * ranks, ranks, stream);
+    else if (p.rank < 32 || p.rows <= 8) launch_typed<decltype(t), true, 1>(a, units * ranks, ranks, stream);
+    else launch_typed<decltype(t), true, 2>(a, units * ranks, ranks, stream);
   };
   if (p.dtype == PFC_DTYPE_FLOAT32) launch(float());
   else if (p.dtype == PFC_DTYPE_FLOAT16) launch(__half());
