@@ -77,6 +77,7 @@ struct Args {
   int* err;
   int most_slots;        // 8 or 32: of a group at most
   int tiles, per_tile;   // per_tile: clusters that share a tile's groups
+  int apart;             // CTAs of a cluster take a group each where a tile has more groups than clusters
 };
 
 constexpr int kFewBlocks = 4;  // of 16 ranks, whose sums few rows' warps leave at a time
@@ -188,7 +189,7 @@ __device__ __forceinline__ void make_h(const Args& a, cg::cluster_group& cluster
 
 // A group of up to 8 rows.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& cluster, int ranks, int adapter, const int* slots, int count,
+__device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& cluster, int adapter, const int* slots, int count,
                                          int row0, int q, int of, char* smem) {
   using L = Layout<T>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -268,6 +269,7 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
     add_warps(red, kFewBlocks * 32, some, 1, r0, 8, sums);
     __syncthreads();
   }
+  const int ranks = of / kWarps;
   if (ranks > 1) cluster.sync();
   const int pitch = L::pitch(a.rank), part = 8 * pitch;
   make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 8, count, h, part);
@@ -576,7 +578,7 @@ __device__ __forceinline__ void reduce(const Args& a, int adapter, const int (&r
 
 // A group of 9 to 32 rows.
 template <typename T, bool WIDE, int RT>
-__device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& cluster, int ranks, int adapter, const int* slots, int count,
+__device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& cluster, int adapter, const int* slots, int count,
                                           int row0, int q, int of, char* smem) {
   using L = Layout<T>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
@@ -592,6 +594,7 @@ __device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& clus
   if constexpr (RT > 1)
     for (; r0 + 16 * RT <= a.rank; r0 += 16 * RT) reduce<T, WIDE, RT>(a, adapter, rows, r0, q, of, ring, smem, sums);
   for (; r0 < a.rank; r0 += 16) reduce<T, WIDE, 1>(a, adapter, rows, r0, q, of, ring, smem, sums);
+  const int ranks = of / kWarps;
   if (ranks > 1) cluster.sync();
   const int part = 32 * L::pitch(a.rank);
   make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 32, count, h, part);
@@ -648,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(Args a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int unit = (int)(blockIdx.x / ranks), row0 = unit % a.tiles * kTile, first_group = unit / a.tiles;
+  const int unit = (int)(blockIdx.x / ranks), row0 = unit % a.tiles * kTile;
   begin();
 
   int mine = INT_MIN;  // the lane's row's adapter
@@ -664,9 +667,10 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(Args a) {
   // groups by their first rows
   const unsigned firsts = __ballot_sync(~0u, mine != INT_MIN && (int)(__ffs(same) - 1) == lane);
   const int groups = __popc(firsts);
-
-  const int q = rank * kWarps + warp, of = ranks * kWarps;
-  for (int i = first_group; i < groups; i += a.per_tile) {
+  const bool alone = a.apart && groups > a.per_tile;  // the same in all CTAs of the cluster
+  const int first_group = alone ? unit / a.tiles * ranks + rank : unit / a.tiles, step = alone ? a.per_tile * ranks : a.per_tile;
+  const int q = alone ? warp : rank * kWarps + warp, of = alone ? kWarps : ranks * kWarps;
+  for (int i = first_group; i < groups; i += step) {
     unsigned left = firsts;
     for (int k = 0; k < i; ++k) left &= left - 1;
     const int leader = __ffs(left) - 1;
@@ -679,9 +683,9 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(Args a) {
       copy_rows<T, typename std::conditional<WIDE, uint4, T>::type>(a, slots, count, row0, q, of);
       __syncthreads();  // the slots are written again
     } else if (count <= 8) {
-      few_rows<T, WIDE>(a, cluster, ranks, adapter, slots, count, row0, q, of, smem);
+      few_rows<T, WIDE>(a, cluster, adapter, slots, count, row0, q, of, smem);
     } else {
-      many_rows<T, WIDE, RT>(a, cluster, ranks, adapter, slots, count, row0, q, of, smem);
+      many_rows<T, WIDE, RT>(a, cluster, adapter, slots, count, row0, q, of, smem);
     }
   }
 }
@@ -749,13 +753,25 @@ void launch_adapters(const pfk_adapters_params& p, cudaStream_t stream) {
   const int64_t sms = device_sm_count(current_device());
   a.tiles = (int)tiles;
   a.per_tile = (int)std::min(groups, std::max<int64_t>(1, 2048 / tiles));
-  const int64_t units = tiles * a.per_tile;
+  int64_t units = tiles * a.per_tile;
   PFB_CHECK_ARG(units <= INT32_MAX / kMostRanks, "adapters: too many rows");
   // few groups: several CTAs each, as many as the device holds at once, as long
   // as all warps have something of one of the products
   const int64_t work = std::max(ceil_div(a.a_row, 64), ceil_div(p.outer, 32));
   int ranks = 1;
   while (ranks < kMostRanks && units * ranks <= sms && work > ranks * kWarps) ranks *= 2;
+  // Many groups at most, but tiles of one or two would leave the device idle:
+  // the two CTAs of a cluster work on a group together or, where a tile has
+  // more groups than clusters, on one each.  4096 to 4096, rank 16, bf16, us
+  // with one CTA and with two: 3000 rows of five prompts 33.8 and 23.7, 1200
+  // 21.8 and 15.0; 3000 mixed rows of 16 adapters 126.8 and 132.9 (four CTAs:
+  // 1200 rows of prompts 17.2, of mixed adapters 61.7 for 48.4).
+  if (ranks == 1 && tiles <= sms && work > kWarps) {
+    ranks = 2;
+    a.apart = 1;
+    a.per_tile = (int)ceil_div(a.per_tile, 2);
+    units = tiles * a.per_tile;
+  }
   auto launch = [&](auto t) {
     if (!all_wide) launch_typed<decltype(t), false, 1>(a, units * ranks, ranks, stream);
     else if (p.rank < 32 || p.rows <= 8) launch_typed<decltype(t), true, 1>(a, units * ranks, ranks, stream);

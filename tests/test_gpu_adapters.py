@@ -168,6 +168,22 @@ def test_rows_at_every_place(dtype, inner, outer):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,inner,outer", [(600, 16, 640, 320), (731, 16, 1000, 97), (1200, 5, 512, 1024), (2100, 3, 1025, 65)])
+def test_tiles_of_few_and_of_many_groups(dtype, rows, n, inner, outer):
+    """Runs, mixed rows and both beside each other: groups that several CTAs share and groups that one has."""
+    g = gen(rows)
+    layer, parts = make(g, n, inner, outer, [16, 40], dtype)
+    x, base = randn(g, rows, inner, dtype=dtype), randn(g, rows, outer, dtype=dtype)
+    mixed = torch.randint(-1, n, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    runs = mixed.sort()[0]
+    both = torch.where(torch.arange(rows, device="cuda") // 100 % 2 == 0, mixed, runs)
+    for index in (runs, mixed, both):
+        got = check(layer, parts, x, index, base)
+        inside = base.clone()
+        assert torch.equal(layer(x, index, inside, out=inside), got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_adapters_are_replaced(dtype):
     g = gen(4)
     layer, parts = make(g, 2, 64, 64, [32], dtype)
