@@ -826,8 +826,10 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
 // took 42.4 us with 256 threads, 20.6 so; one of 8 units 45.7 and 43.1).  With
 // 1024 threads in a CTA for each CTA of the first kernel, most of which have
 // nothing to join, that of 8 units took 58.  Many units have few shares each,
-// and a CTA of 256 for each CTA of the first kernel, with no unit to look for.
-constexpr int kFewUnits = 64;
+// and a CTA of 256 for each CTA of the first kernel, with no unit to look for
+// (bf16, heads of 128, us in that form and in this: 16 units 23.3 and 24.3, 32
+// 24.4 and 24.7, 48 32.5 and 28.8, 128 44.9 and 34.8).
+constexpr int kFewUnits = 32;
 
 // CTA (c, h): joins the shares of query head h of a unit that went on beyond
 // the CTA it began in, in a fixed order: with FIND the c-th such unit,

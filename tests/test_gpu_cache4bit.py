@@ -333,7 +333,8 @@ def test_long_sequence(dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim,group,page,heads,each,lens", [
     (128, 64, 7, 1, 2, [20011, 0, 696]), (64, 32, 16, 2, 1, [0, 17001]), (96, 64, 48, 1, 9, [9000, 1, 0, 12345]),
-    (256, 64, 5, 1, 1, [8000]), (8, 32, 1, 3, 1, [9000, 8999]), (128, 64, 16, 21, 1, [9001, 0, 12000]), (128, 64, 16, 22, 1, [9001, 0, 12000])])
+    (256, 64, 5, 1, 1, [8000]), (8, 32, 1, 3, 1, [9000, 8999]), (128, 64, 16, 21, 1, [9001, 0, 12000]), (128, 64, 16, 22, 1, [9001, 0, 12000]),
+    (128, 64, 16, 16, 1, [9001, 700]), (128, 64, 16, 11, 1, [9001, 0, 7000])])
 def test_few_sequences_of_many_shares(dtype, dim, group, page, heads, each, lens):
     """Units that most of the device's CTAs share, empty sequences among them."""
     g = gen(dim + page + heads)
