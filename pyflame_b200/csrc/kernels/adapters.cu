@@ -13,8 +13,9 @@
 // group, few rows several CTAs: each a part of x's axis in the first product,
 // whose sums meet through distributed shared memory in the order of the
 // ranks, and a part of the outputs in the second.  What lies between the
-// products enters the second as two 16-bit parts (fp32: split tf32), so that
-// it rounds far less than the output.
+// products enters the second as two 16-bit parts, of float16 calls with a power
+// of two for each row (make_h) (fp32: split tf32), so that it rounds far less
+// than the output.
 //
 // Groups of up to 8 rows read A and B, which are most of their bytes, through
 // a ring of asynchronous copies for each warp: B's copies are on their way
@@ -44,6 +45,7 @@
 #include <cmath>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "../common.hpp"
 #include "decode.cuh"
@@ -157,40 +159,80 @@ struct Layout {
   static int bytes(int rank, int slots) { return sums_at(rank, slots) + rank * slots * 4; }
 };
 
-// h [slots][pitch], the cluster's sums times the adapter's scale, in parts;
-// zeros behind the ranks.
-template <typename T>
-__device__ __forceinline__ void make_h(const Args& a, cg::cluster_group& cluster, int ranks, float scale, float* sums, int slots, int count, T* h, int part) {
-  const int pitch = Layout<T>::pitch(a.rank), wide = pitch - 16 / (int)sizeof(T);
-  for (int j = threadIdx.x; j < slots * wide; j += kThreads) {
-    const int s = j / wide, r = j - s * wide;
-    float v = 0.f;
-    if (r < a.rank && s < count) {
-      const int at = r * slots + s;
-      if (ranks > 1) {
+// What the cluster's CTAs have of a sum: a place of `sums` in each.
+__device__ __forceinline__ float cluster_sum(cg::cluster_group& cluster, int ranks, float* sums, int at) {
+  if (ranks == 1) return sums[at];
+  float v = 0.f;
 #pragma unroll
-        for (int c = 0; c < kMostRanks; ++c)
-          if (c < ranks) v += cluster.map_shared_rank(sums, c)[at];
-      } else {
-        v = sums[at];
+  for (int c = 0; c < kMostRanks; ++c)
+    if (c < ranks) v += cluster.map_shared_rank(sums, c)[at];
+  return v;
+}
+
+// h [slots][pitch], the cluster's sums times the adapter's scale, in parts;
+// zeros behind the ranks.  fp16 parts reach from 2^-25 to 65504, not as far as
+// the sums: a warp takes a slot, whose values are multiplied by the power of two
+// that puts the largest between 2^14 and 2^15, so that the parts lose 2^-22 of a
+// value, or 2^-39 of the largest where that is more, whatever their size; its
+// inverse, in `undo`, goes on the second product's sums (61 rows of 55 adapters
+// of rank 64: 39.0 us; without, 38.5).
+template <typename T>
+__device__ __forceinline__ void make_h(const Args& a, cg::cluster_group& cluster, int ranks, float scale, float* sums, int slots, int count, T* h, int part,
+                                       float* undo) {
+  const int pitch = Layout<T>::pitch(a.rank), wide = pitch - 16 / (int)sizeof(T);
+  if constexpr (std::is_same<T, __half>::value) {
+    const int lane = threadIdx.x & 31;
+    for (int s = threadIdx.x >> 5; s < slots; s += kWarps) {
+      float v[kMostRank / 32], top = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMostRank / 32; ++i) {
+        if (32 * i >= a.rank) break;  // the same in all lanes
+        const int r = 32 * i + lane;
+        v[i] = r < a.rank && s < count ? cluster_sum(cluster, ranks, sums, r * slots + s) * scale : 0.f;
+        top = fmaxf(top, fabsf(v[i]));
       }
-      v *= scale;
+      top = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(top)));  // in the order of the numbers: none is negative
+      // its exponent, not so low that the factors leave fp32's range
+      const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);
+      const float times = __uint_as_float((unsigned)(127 + 14 - e) << 23);
+      if (lane == 0) undo[s] = __uint_as_float((unsigned)(127 - 14 + e) << 23);
+#pragma unroll
+      for (int i = 0; i < kMostRank / 32; ++i) {
+        if (32 * i >= a.rank) break;
+        T hi, lo;
+        two_parts(v[i] * times, hi, lo);
+        h[s * pitch + 32 * i + lane] = hi;
+        h[part + s * pitch + 32 * i + lane] = lo;
+      }
     }
-    if constexpr (sizeof(T) == 4) {
-      h[s * pitch + r] = v;
-    } else {
-      T hi, lo;
-      two_parts(v, hi, lo);
-      h[s * pitch + r] = hi;
-      h[part + s * pitch + r] = lo;
+  } else {
+    for (int j = threadIdx.x; j < slots * wide; j += kThreads) {
+      const int s = j / wide, r = j - s * wide;
+      const float v = r < a.rank && s < count ? cluster_sum(cluster, ranks, sums, r * slots + s) * scale : 0.f;
+      if constexpr (sizeof(T) == 4) {
+        h[s * pitch + r] = v;
+      } else {
+        T hi, lo;
+        two_parts(v, hi, lo);
+        h[s * pitch + r] = hi;
+        h[part + s * pitch + r] = lo;
+      }
     }
   }
+}
+
+// The factor on the sums of a slot's second product (bfloat16 parts and tf32
+// ones reach as far as fp32).
+template <typename T>
+__device__ __forceinline__ float undo_of(const float* undo, int slot) {
+  if constexpr (std::is_same<T, __half>::value) return undo[slot];
+  return 1.f;
 }
 
 // A group of up to 8 rows.
 template <typename T, bool WIDE>
 __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& cluster, int adapter, const int* slots, int count,
-                                         int row0, int q, int of, char* smem) {
+                                         int row0, int q, int of, char* smem, float* undo) {
   using L = Layout<T>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   constexpr int kStage = WIDE ? 1536 : 2048, kDepth = kRing / kStage;
@@ -272,7 +314,7 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
   const int ranks = of / kWarps;
   if (ranks > 1) cluster.sync();
   const int pitch = L::pitch(a.rank), part = 8 * pitch;
-  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 8, count, h, part);
+  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 8, count, h, part, undo);
   // the others have read this CTA's sums before it writes the next ones or ends
   if (ranks > 1) cluster.sync();
   else __syncthreads();
@@ -280,13 +322,16 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
   // outputs 16u + g and + 8 of the rows in slots 2t and 2t + 1
   const T* from[2] = {nullptr, nullptr};
   T* to[2] = {nullptr, nullptr};
+  float times[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 2; ++i) {
+    times[i] = undo_of<T>(undo, 2 * t + i);
     if (2 * t + i < count) {
       const long long m = row0 + slots[2 * t + i];
       from[i] = a.base ? (const T*)a.base + m * a.base_st : nullptr;
       to[i] = (T*)a.out + m * a.out_st;
     }
+  }
   // base is loaded two blocks ahead (and converted when it is there)
   auto load_base = [&](int u, T (&v)[4]) {
 #pragma unroll
@@ -324,23 +369,23 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = u * 16 + g + 8 * (i >> 1);
-      if (to[i & 1] && n < a.outer) to[i & 1][n] = from_float<T>(to_float<T>(base[0][i]) + acc[i]);
+      if (to[i & 1] && n < a.outer) to[i & 1][n] = from_float<T>(fmaf(acc[i], times[i & 1], to_float<T>(base[0][i])));
     }
   }
   __syncthreads();  // h and the sums are written again for the next group
 }
 
-// Two neighbouring values of a word of a row (fp32: of two words), plus x and y.
-__device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, __half) {
+// Two neighbouring values of a word of a row (fp32: of two words), plus x and y times f.
+__device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, float f, __half) {
   const float2 v = __half22float2(*reinterpret_cast<const __half2*>(w + i));
-  const __half2 r = __floats2half2_rn(v.x + x, v.y + y);
+  const __half2 r = __floats2half2_rn(fmaf(x, f, v.x), fmaf(y, f, v.y));
   w[i] = *reinterpret_cast<const unsigned*>(&r);
 }
-__device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, __nv_bfloat16) {
+__device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, float, __nv_bfloat16) {
   const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(w[i] << 16) + x, __uint_as_float(w[i] & 0xffff0000u) + y);
   w[i] = *reinterpret_cast<const unsigned*>(&r);
 }
-__device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, float) {
+__device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, float, float) {
   w[2 * i] = __float_as_uint(__uint_as_float(w[2 * i]) + x);
   w[2 * i + 1] = __float_as_uint(__uint_as_float(w[2 * i + 1]) + y);
 }
@@ -350,17 +395,21 @@ __device__ __forceinline__ void add_two(unsigned* w, int i, float x, float y, fl
 // warp's blocks of 32 outputs u = q, q + of, ...; ring: the lane's place in
 // the warp's, which begins at stage.
 template <typename T, int MT, bool WIDE>
-__device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, int part, const int* slots, int count, int row0, int q, int of, uint32_t ring, T* stage) {
+__device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, int part, const int* slots, const float* undo, int count, int row0, int q, int of, uint32_t ring, T* stage) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int pitch = Layout<T>::pitch(a.rank);
   const T* weights = (const T*)a.b + (long long)adapter * a.outer * a.rank;
   const int blocks = (a.outer + 31) / 32, whole = a.outer / 32;
   constexpr int WORDS = 2 * (int)sizeof(T);  // of a lane's 8 outputs
   int rows[MT][2];
+  float times[MT][2];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) rows[m][r] = m * 16 + g + 8 * r < count ? row0 + slots[m * 16 + g + 8 * r] : -1;
+    for (int r = 0; r < 2; ++r) {
+      rows[m][r] = m * 16 + g + 8 * r < count ? row0 + slots[m * 16 + g + 8 * r] : -1;
+      times[m][r] = undo_of<T>(undo, m * 16 + g + 8 * r);
+    }
   // Base comes through the warp's ring, several blocks ahead, 16
   // ranks' weights while the 16 before them are used.
   constexpr int PARTS = WORDS / 4 + (WIDE ? 0 : 1);  // of 16 bytes, of a lane's outputs
@@ -464,7 +513,7 @@ __device__ __forceinline__ void expand(const Args& a, int adapter, const T* h, i
       for (int r = 0; r < 2; ++r) {
         if (rows[m][r] < 0) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) add_two(io[m][r], j, acc[m][j][2 * r], acc[m][j][2 * r + 1], T());
+        for (int j = 0; j < 4; ++j) add_two(io[m][r], j, acc[m][j][2 * r], acc[m][j][2 * r + 1], times[m][r], T());
         if constexpr (WIDE) {
           T* to = (T*)a.out + rows[m][r] * a.out_st + 32 * u + 8 * t;
           if (u < whole) {
@@ -579,7 +628,7 @@ __device__ __forceinline__ void reduce(const Args& a, int adapter, const int (&r
 // A group of 9 to 32 rows.
 template <typename T, bool WIDE, int RT>
 __device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& cluster, int adapter, const int* slots, int count,
-                                          int row0, int q, int of, char* smem) {
+                                          int row0, int q, int of, char* smem, float* undo) {
   using L = Layout<T>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
   constexpr int NT = 4;
@@ -597,16 +646,16 @@ __device__ __forceinline__ void many_rows(const Args& a, cg::cluster_group& clus
   const int ranks = of / kWarps;
   if (ranks > 1) cluster.sync();
   const int part = 32 * L::pitch(a.rank);
-  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 32, count, h, part);
+  make_h<T>(a, cluster, ranks, a.scales[adapter], sums, 32, count, h, part, undo);
   // the others have read this CTA's sums before it writes the next ones or ends
   if (ranks > 1) cluster.sync();
   else __syncthreads();
   T* stage = reinterpret_cast<T*>(smem + warp * kRing);
   if constexpr (sizeof(T) == 2) {
-    if (count <= 16) expand<T, 1, WIDE>(a, adapter, h, part, slots, count, row0, q, of, ring, stage);
-    else expand<T, 2, WIDE>(a, adapter, h, part, slots, count, row0, q, of, ring, stage);
+    if (count <= 16) expand<T, 1, WIDE>(a, adapter, h, part, slots, undo, count, row0, q, of, ring, stage);
+    else expand<T, 2, WIDE>(a, adapter, h, part, slots, undo, count, row0, q, of, ring, stage);
   } else {  // (two blocks of fp32 rows do not fit the registers)
-    for (int s = 0; s < count; s += 16) expand<T, 1, WIDE>(a, adapter, h + s * L::pitch(a.rank), part, slots + s, count - s, row0, q, of, ring, stage);
+    for (int s = 0; s < count; s += 16) expand<T, 1, WIDE>(a, adapter, h + s * L::pitch(a.rank), part, slots + s, undo + s, count - s, row0, q, of, ring, stage);
   }
   __syncthreads();  // h and the sums are written again for the next group
 }
@@ -648,6 +697,7 @@ template <typename T, bool WIDE, int RT>
 __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(Args a) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int slots[kTile];
+  __shared__ float undo[kTile];
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -683,9 +733,9 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(Args a) {
       copy_rows<T, typename std::conditional<WIDE, uint4, T>::type>(a, slots, count, row0, q, of);
       __syncthreads();  // the slots are written again
     } else if (count <= 8) {
-      few_rows<T, WIDE>(a, cluster, adapter, slots, count, row0, q, of, smem);
+      few_rows<T, WIDE>(a, cluster, adapter, slots, count, row0, q, of, smem, undo);
     } else {
-      many_rows<T, WIDE, RT>(a, cluster, adapter, slots, count, row0, q, of, smem);
+      many_rows<T, WIDE, RT>(a, cluster, adapter, slots, count, row0, q, of, smem, undo);
     }
   }
 }

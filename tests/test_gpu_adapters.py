@@ -184,6 +184,39 @@ def test_tiles_of_few_and_of_many_groups(dtype, rows, n, inner, outer):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,inner,outer,rank", [(1, 4096, 200, 16), (7, 96, 130, 40), (16, 333, 65, 16), (70, 512, 96, 64), (40, 64, 33, 256)])
+def test_between_the_products(dtype, rows, inner, outer, rank):
+    """scale A x far from 1, which B brings back: sizes from 1e-6 to 1e8, both in one adapter, and zeros of B
+    beside them.  The tolerance is that of any other call, with half a step of float16's subnormals (2^-25), and
+    for float16 what its two parts lose of a row's small values: half of 2^-24 on a scale where the largest is
+    2^14 at least, so 2^-39 of that for each rank."""
+    g = gen(rows + rank)
+    x, base = randn(g, rows, inner, dtype=dtype), randn(g, rows, outer, dtype=dtype)
+    layer = pf.LowRankAdapters(4, inner, outer, rank, dtype=dtype)
+    parts = []
+    for i, (size, scale) in enumerate([(300.0, 350.0), (100.0, 1e6), (1e-4, 1e-2), (30.0, 4000.0)]):
+        a = (size * randn(g, rank, inner) / math.sqrt(inner)).to(dtype)  # scale a x: 1e5, 1e8, 1e-6, 1e5
+        b = (randn(g, outer, rank) * min(1e3, max(1e-7, 1 / (size * scale)))).to(dtype)
+        if i == 3:
+            a[rank // 2:] = (1e-7 * a[rank // 2:].float()).to(dtype)
+            b[:, rank // 2:] = (1e3 * randn(g, outer, rank - rank // 2)).to(dtype)
+        b[outer // 2] = 0
+        parts.append((a, b, scale))
+        layer.load(i, *parts[-1])
+    mixed = torch.arange(rows, device="cuda", dtype=torch.int32) % 4
+    for index in (mixed, mixed.sort()[0], *(torch.full_like(mixed, i) for i in range(4))):
+        got = layer(x, index, base)
+        out, mag = reference(parts, x, index, base, outer)
+        lost = torch.zeros_like(mag)
+        if dtype == F16:
+            for i, (a, b, s) in enumerate(parts):
+                hit = index == i
+                lost[hit] = 2.0 ** -39 * abs(s) * (x[hit].double() @ a.double().T).abs().amax(1, keepdim=True) * b.double().abs().sum(1)
+        within(got, out, HALF[dtype] * out.abs() + SUMS[dtype] * mag + lost + 2.0 ** -25)
+        assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_adapters_are_replaced(dtype):
     g = gen(4)
     layer, parts = make(g, 2, 64, 64, [32], dtype)
