@@ -39,7 +39,8 @@ constexpr int64_t kClusterTiles = 64;  // of 64 keys: the longest sequences that
 
 struct Plan {
   int ctas, heads;
-  bool runs;  // pages of whole runs of 16 tokens
+  bool runs;    // pages of whole runs of 16 tokens
+  bool beside;  // units whose heads fill at most half of an instruction
   int ranks;  // CTAs of a unit's cluster; 0: runs of the list of all tiles
   int64_t stats_at, parts_at, bytes;
 };
@@ -49,7 +50,8 @@ Plan plan_of(const pfk_cache4_attention_params& p) {
   const int64_t group = p.q_heads / p.cache.heads;
   w.heads = (int)std::min<int64_t>(group, kHeads);
   w.runs = p.cache.page_size % 16 == 0;
-  w.ctas = typed(p.dtype, [&](auto t) { return cache4::wave_of<decltype(t)>(cache4_width(p.cache.head_dim), p.cache.group, w.runs); });
+  w.beside = w.heads <= kHeads / 2;
+  w.ctas = typed(p.dtype, [&](auto t) { return cache4::wave_of<decltype(t)>(cache4_width(p.cache.head_dim), p.cache.group, w.runs, w.beside); });
   int64_t seen = std::min<int64_t>(p.table_width * p.cache.page_size, INT32_MAX);
   if (p.window) seen = std::min<int64_t>(seen, std::min<int64_t>(p.window, INT32_MAX) + 64);
   const int64_t units = p.batch * p.cache.heads * ceil_div(group, kHeads), tiles = ceil_div(seen, 64);
@@ -123,7 +125,7 @@ void launch_cache4_attention(const pfk_cache4_attention_params& p, cudaStream_t 
   a.parts = (float*)(ws + w.parts_at);
   a.ctas = w.ctas;
   a.heads = w.heads;
-  typed(p.dtype, [&](auto t) { cache4::launch_of<decltype(t)>(a, cache4_width(c.head_dim), c.group, w.runs, w.ranks, stream); });
+  typed(p.dtype, [&](auto t) { cache4::launch_of<decltype(t)>(a, cache4_width(c.head_dim), c.group, w.runs, w.beside, w.ranks, stream); });
 }
 
 }  // namespace pfb

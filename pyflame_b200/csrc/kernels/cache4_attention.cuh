@@ -19,8 +19,14 @@
 // in 2^14 ... 2^15 and a sixteenth of that beside the codes that count sixteen
 // times: exact for fp16 and bf16 down to 2^-20 of the head's largest, and in
 // two parts (2^-22) for fp32.  p step enters as 2^8 p step over a power of two
-// above the largest step so far, in two parts for fp32 and fp16 and in one,
-// 2^-12, for bf16 outputs, 2^-9.  For fp32 the codes are centred, c - 8 (four
+// above the largest step so far, in two parts (2^-22): one alone, 2^-11, showed
+// in bf16 outputs, whose error rose from 1.64e-3 to 1.72e-3.  An instruction has
+// eight columns: a unit of up to four heads has its high parts in the first
+// four and its low ones in the others, which calls for the same scores again
+// there and for no more instructions on the tensor cores (128 sequences, bf16:
+// 178 us; one part took 169, two instructions 200); more heads take two
+// instructions (one sequence of 131071, 8 heads a unit, bf16: 50.5 us; one part
+// took 43).  For fp32 the codes are centred, c - 8 (four
 // instructions a word more): with many keys the values average out, and the
 // large part that codes from 0 on have in common lost 5e-5 of what remains to
 // the tensor cores' truncation.
@@ -107,9 +113,9 @@ struct Args {
 // CTAs of one wave of a call's kernel, and its launch; defined for each type
 // in a file of its own.
 template <typename T>
-int wave_of(int width, int64_t group, bool runs);
+int wave_of(int width, int64_t group, bool runs, bool beside);
 template <typename T>
-void launch_of(Args& a, int width, int64_t group, bool runs, int ranks, cudaStream_t stream);
+void launch_of(Args& a, int width, int64_t group, bool runs, bool beside, int ranks, cudaStream_t stream);
 
 }  // namespace cache4
 }  // namespace pfb
@@ -176,6 +182,10 @@ __device__ __forceinline__ unsigned pack_half(float x, float y) {
   return *reinterpret_cast<const unsigned*>(&v);
 }
 
+// What of x the first of two fp16 numbers holds: 11 bits of it (below 2^-14,
+// steps of 2^-24).
+__device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+
 __device__ __forceinline__ unsigned long long divide(unsigned long long a, unsigned long long b) {
   return ((a | b) >> 32) ? a / b : (unsigned)a / (unsigned)b;
 }
@@ -222,8 +232,9 @@ __device__ __forceinline__ void load_words(unsigned* to, const char* p) {
   }
 }
 
-// T: of queries and output; W: the head's values with padding; G: a group's.
-template <typename T, int W, int G, bool RUNS>
+// T: of queries and output; W: the head's values with padding; G: a group's;
+// BESIDE: units of up to 4 heads, with both parts of a weight in one instruction.
+template <typename T, int W, int G, bool RUNS, bool BESIDE>
 struct Layout {
   static constexpr int kBlocks = W / 32;
   static constexpr int kPaired = kBlocks & ~1;
@@ -231,7 +242,7 @@ struct Layout {
   static constexpr int kGroups = (kBlocks + kFold - 1) / kFold;
   static constexpr int kScales = kGroups <= 1 ? 1 : kGroups <= 2 ? 2 : kGroups <= 4 ? 4 : 8;  // words of a record
   static constexpr int kQParts = sizeof(T) == 4 ? 2 : 1;
-  static constexpr int kPParts = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
+  static constexpr int kPParts = BESIDE ? 1 : 2;  // instructions for a weight's parts
   static constexpr bool kCentred = sizeof(T) == 4;
   // what the codes' operands and q's scaling leave to multiply with
   static constexpr int kQShift = kCentred ? -14 : 10;  // of 2, with q's exponent
@@ -243,18 +254,19 @@ struct Layout {
   static constexpr size_t o_bytes = (size_t)kWarps * kHeads * kPitch * 4;
   static constexpr size_t smem = q_bytes + o_bytes;
   // CTAs that share an SM: more warps help (128 sequences of 5000 keys, bf16,
-  // groups of 64: 168 us with four, 185 with three), but not where 128
-  // registers a thread spill (fp16, groups of 32: 106 us for 88)
-  static constexpr int kResident = W <= 64 ? 4 : W <= 128 ? (sizeof(T) == 4 || kGroups > 2 ? 3 : 4) : 2;
+  // groups of 64: 178 us with four, 192 with three), but not where 128
+  // registers a thread spill (fp16, groups of 32: 106 us for 88; one of 131071
+  // keys, 8 heads a unit, bf16: 51.3 us for 50.3)
+  static constexpr int kResident = W <= 64 ? 4 : W <= 128 ? (sizeof(T) == 2 && kGroups <= 2 && BESIDE ? 4 : 3) : 2;
 };
 
 // CLUSTER: a cluster of CTAs for each unit, each an equal part of its tiles;
 // otherwise runs of the list of all tiles.  RUNS: pages are multiples of 16
 // tokens, so that 16 keys of a step follow one another in memory: a lane's
 // rows are at fixed distances, and only the first's place is looked up.
-template <typename T, int W, int G, bool CLUSTER, bool RUNS>
-__global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) attend_kernel(Args a) {
-  using L = Layout<T, W, G, RUNS>;
+template <typename T, int W, int G, bool CLUSTER, bool RUNS, bool BESIDE>
+__global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kResident)) attend_kernel(Args a) {
+  using L = Layout<T, W, G, RUNS, BESIDE>;
   constexpr int R = L::kRows, B = L::kBlocks, NG = L::kGroups;
   extern __shared__ __align__(16) char smem[];
   uint4* qs = reinterpret_cast<uint4*>(smem);  // [part][block][lane]
@@ -269,6 +281,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
+  const float low_half = t >> 1;  // BESIDE: whether the lane's weights are the low parts
   begin();
   const int per_row = a.kv_heads * a.chunks;
   int row, unit, tile;  // unit: of the row
@@ -464,17 +477,18 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
     return (odds >> (2 * t) & 3u) | (odds >> (8 + 2 * t) & 3u) << 2;
   };
   // Q in the order of the second operand's registers: a warp takes two heads
+  // (BESIDE: heads 4 to 7 are 0 to 3 again)
   auto stage_q = [&](int row, int first_q, int heads) {
     const T* qp = (const T*)a.q + (long long)row * a.q_sb + (long long)first_q * a.q_sh;
     __half* to = reinterpret_cast<__half*>(qs);
 #pragma unroll
     for (int i = 0; i < kHeads / kWarps; ++i) {
-      const int h = warp * (kHeads / kWarps) + i;
+      const int h = warp * (kHeads / kWarps) + i, from = BESIDE ? h & 3 : h;
       float x[B], top = 0.f;
 #pragma unroll
       for (int j = 0; j < B; ++j) {
         const int d = 32 * j + lane;
-        x[j] = h < heads && d < a.head_dim ? to_float<T>(qp[h * a.q_sh + d]) : 0.f;
+        x[j] = from < heads && d < a.head_dim ? to_float<T>(qp[from * a.q_sh + d]) : 0.f;
         top = fmaxf(top, fabsf(x[j]));
       }
 #pragma unroll
@@ -528,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
     }
     __syncthreads();
 
-    // A lane has query heads 2t and 2t + 1; of o the values 32b + 4g + 2j (o[..][0..1]) and the next, sixteenfold
+    // A lane has query heads 2t and 2t + 1 (BESIDE: lanes 2 and 3 of four those of 0 and 1 again, for the low parts); of o the values 32b + 4g + 2j (o[..][0..1]) and the next, sixteenfold
     float m[2], l[2], z[NG][2], o[B][2][4], f[2], qsum[NG][2];
     unsigned e = 0;  // a power of two above the largest step of values so far: its exponent, less 1; the power, and its inverse
     float above = 0x1p-126f, below = 0x1p126f;
@@ -673,10 +687,12 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
             z[n][0] = fmaf(p[r][2 * i], low, z[n][0]);
             z[n][1] = fmaf(p[r][2 * i + 1], low, z[n][1]);
             const float x = p[r][2 * i] * st, y = p[r][2 * i + 1] * st;
-            const unsigned hi = pack_half(x, y);
-            pt[r][0][i] = transpose8x8(hi);
-            if constexpr (L::kPParts == 2) {
+            if constexpr (BESIDE) {  // the high parts times -1, or the low ones
+              pt[r][0][i] = transpose8x8(pack_half(fmaf(x, low_half, -high_part(x)), fmaf(y, low_half, -high_part(y))));
+            } else {
+              const unsigned hi = pack_half(x, y);
               const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+              pt[r][0][i] = transpose8x8(hi);
               pt[r][1][i] = transpose8x8(pack_half(x - back.x, y - back.y));
             }
           }
@@ -716,6 +732,15 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
       next = place();
     }
 
+    if constexpr (BESIDE) {  // lanes of heads 0 to 3 take the low parts' sums and the others' of the high ones
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[b][j][i] = __shfl_xor_sync(~0u, o[b][j][i], 2) - o[b][j][i];
+    }
+
     // join the warps
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -726,6 +751,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS>::kResident)) 
 #pragma unroll
         for (int n = 0; n < NG; ++n) z[n][i] += __shfl_xor_sync(~0u, z[n][i], off);
       }
+      if (BESIDE && t >= 2) continue;
       if (g == 0) {
         ms[h] = m[i];
         ls[h] = l[i];
@@ -929,13 +955,13 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Args a) {
   }
 }
 
-template <typename T_, int W, int G, bool RUNS>
+template <typename T_, int W, int G, bool RUNS, bool BESIDE>
 struct Kernel {
   using T = T_;
-  using L = Layout<T, W, G, RUNS>;
-  using LC = Layout<T, W, G, false>;  // of the clusters' kernel
-  static constexpr auto run = attend_kernel<T, W, G, false, RUNS>;
-  static constexpr auto run_cluster = attend_kernel<T, W, G, true, false>;
+  using L = Layout<T, W, G, RUNS, BESIDE>;
+  using LC = Layout<T, W, G, false, false>;  // of the clusters' kernel
+  static constexpr auto run = attend_kernel<T, W, G, false, RUNS, BESIDE>;
+  static constexpr auto run_cluster = attend_kernel<T, W, G, true, false, false>;
 };
 
 // CTAs of one wave of a kernel on the current device, asked once per device.
@@ -971,39 +997,39 @@ void launch_sized(Args& a, int ranks, cudaStream_t stream) {
 
 // Calls f(Kernel<...>()) for the call's sizes.  Groups as wide as the head are
 // one group, whatever their size.
-template <typename T, bool RUNS, class F>
+template <typename T, bool RUNS, bool BESIDE, class F>
 void dispatch_sized(int width, int64_t group, F&& f) {
   if (width == 64) {
-    group == 32 ? f(Kernel<T, 64, 32, RUNS>()) : f(Kernel<T, 64, 64, RUNS>());
+    group == 32 ? f(Kernel<T, 64, 32, RUNS, BESIDE>()) : f(Kernel<T, 64, 64, RUNS, BESIDE>());
   } else if (width == 96) {
-    if (group == 32) f(Kernel<T, 96, 32, RUNS>());
-    else group == 64 ? f(Kernel<T, 96, 64, RUNS>()) : f(Kernel<T, 96, 128, RUNS>());
+    if (group == 32) f(Kernel<T, 96, 32, RUNS, BESIDE>());
+    else group == 64 ? f(Kernel<T, 96, 64, RUNS, BESIDE>()) : f(Kernel<T, 96, 128, RUNS, BESIDE>());
   } else if (width == 128) {
-    if (group == 32) f(Kernel<T, 128, 32, RUNS>());
-    else group == 64 ? f(Kernel<T, 128, 64, RUNS>()) : f(Kernel<T, 128, 128, RUNS>());
+    if (group == 32) f(Kernel<T, 128, 32, RUNS, BESIDE>());
+    else group == 64 ? f(Kernel<T, 128, 64, RUNS, BESIDE>()) : f(Kernel<T, 128, 128, RUNS, BESIDE>());
   } else {
-    if (group == 32) f(Kernel<T, 256, 32, RUNS>());
-    else group == 64 ? f(Kernel<T, 256, 64, RUNS>()) : f(Kernel<T, 256, 128, RUNS>());
+    if (group == 32) f(Kernel<T, 256, 32, RUNS, BESIDE>());
+    else group == 64 ? f(Kernel<T, 256, 64, RUNS, BESIDE>()) : f(Kernel<T, 256, 128, RUNS, BESIDE>());
   }
 }
 template <typename T, class F>
-void dispatch(int width, int64_t group, bool runs, F&& f) {
-  if (runs) dispatch_sized<T, true>(width, group, f);
-  else dispatch_sized<T, false>(width, group, f);
+void dispatch(int width, int64_t group, bool runs, bool beside, F&& f) {
+  if (runs) beside ? dispatch_sized<T, true, true>(width, group, f) : dispatch_sized<T, true, false>(width, group, f);
+  else beside ? dispatch_sized<T, false, true>(width, group, f) : dispatch_sized<T, false, false>(width, group, f);
 }
 
 }  // namespace
 
 template <typename T>
-int wave_of(int width, int64_t group, bool runs) {
+int wave_of(int width, int64_t group, bool runs, bool beside) {
   int ctas = 0;
-  dispatch<T>(width, group, runs, [&](auto k) { ctas = wave<decltype(k)>(); });
+  dispatch<T>(width, group, runs, beside, [&](auto k) { ctas = wave<decltype(k)>(); });
   return ctas;
 }
 
 template <typename T>
-void launch_of(Args& a, int width, int64_t group, bool runs, int ranks, cudaStream_t stream) {
-  dispatch<T>(width, group, runs, [&](auto k) { launch_sized<decltype(k)>(a, ranks, stream); });
+void launch_of(Args& a, int width, int64_t group, bool runs, bool beside, int ranks, cudaStream_t stream) {
+  dispatch<T>(width, group, runs, beside, [&](auto k) { launch_sized<decltype(k)>(a, ranks, stream); });
 }
 
 }  // namespace cache4

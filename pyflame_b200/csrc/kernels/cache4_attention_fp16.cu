@@ -6,8 +6,8 @@
 namespace pfb {
 namespace cache4 {
 
-template int wave_of<__half>(int, int64_t, bool);
-template void launch_of<__half>(Args&, int, int64_t, bool, int, cudaStream_t);
+template int wave_of<__half>(int, int64_t, bool, bool);
+template void launch_of<__half>(Args&, int, int64_t, bool, bool, int, cudaStream_t);
 
 }  // namespace cache4
 }  // namespace pfb
