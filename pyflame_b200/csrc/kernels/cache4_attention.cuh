@@ -21,12 +21,12 @@
 // two parts (2^-22) for fp32.  p step enters as 2^8 p step over a power of two
 // above the largest step so far, in two parts (2^-22): one alone, 2^-11, showed
 // in bf16 outputs, whose error rose from 1.64e-3 to 1.72e-3.  An instruction has
-// eight columns: a unit of up to four heads has its high parts in the first
-// four and its low ones in the others, which calls for the same scores again
-// there and for no more instructions on the tensor cores (128 sequences, bf16:
-// 178 us; one part took 169, two instructions 200); more heads take two
-// instructions (one sequence of 131071, 8 heads a unit, bf16: 50.5 us; one part
-// took 43).  For fp32 the codes are centred, c - 8 (four
+// eight columns: a unit of up to four heads has the two parts of a head side by
+// side, so that a lane has the weights of one head and adds both parts' sums
+// (128 sequences, bf16: 166 us; two instructions took 200, and one part alone,
+// with two heads a lane, 169); more heads take two instructions (one sequence
+// of 131071, 8 heads a unit, bf16: 50.5 us; one part took 43).  For fp32 the
+// codes are centred, c - 8 (four
 // instructions a word more): with many keys the values average out, and the
 // large part that codes from 0 on have in common lost 5e-5 of what remains to
 // the tensor cores' truncation.
@@ -182,10 +182,6 @@ __device__ __forceinline__ unsigned pack_half(float x, float y) {
   return *reinterpret_cast<const unsigned*>(&v);
 }
 
-// What of x the first of two fp16 numbers holds: 11 bits of it (below 2^-14,
-// steps of 2^-24).
-__device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
-
 __device__ __forceinline__ unsigned long long divide(unsigned long long a, unsigned long long b) {
   return ((a | b) >> 32) ? a / b : (unsigned)a / (unsigned)b;
 }
@@ -243,6 +239,7 @@ struct Layout {
   static constexpr int kScales = kGroups <= 1 ? 1 : kGroups <= 2 ? 2 : kGroups <= 4 ? 4 : 8;  // words of a record
   static constexpr int kQParts = sizeof(T) == 4 ? 2 : 1;
   static constexpr int kPParts = BESIDE ? 1 : 2;  // instructions for a weight's parts
+  static constexpr int kOwn = BESIDE ? 1 : 2;     // heads of a lane
   static constexpr bool kCentred = sizeof(T) == 4;
   // what the codes' operands and q's scaling leave to multiply with
   static constexpr int kQShift = kCentred ? -14 : 10;  // of 2, with q's exponent
@@ -254,9 +251,9 @@ struct Layout {
   static constexpr size_t o_bytes = (size_t)kWarps * kHeads * kPitch * 4;
   static constexpr size_t smem = q_bytes + o_bytes;
   // CTAs that share an SM: more warps help (128 sequences of 5000 keys, bf16,
-  // groups of 64: 178 us with four, 192 with three), but not where 128
-  // registers a thread spill (fp16, groups of 32: 106 us for 88; one of 131071
-  // keys, 8 heads a unit, bf16: 51.3 us for 50.3)
+  // groups of 64: 166 us with four), but not where 128 registers a thread spill
+  // (fp16, groups of 32: 106 us for 88; one of 131071 keys, 8 heads a unit, bf16:
+  // 51.3 us for 50.3)
   static constexpr int kResident = W <= 64 ? 4 : W <= 128 ? (sizeof(T) == 2 && kGroups <= 2 && BESIDE ? 4 : 3) : 2;
 };
 
@@ -267,7 +264,7 @@ struct Layout {
 template <typename T, int W, int G, bool CLUSTER, bool RUNS, bool BESIDE>
 __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kResident)) attend_kernel(Args a) {
   using L = Layout<T, W, G, RUNS, BESIDE>;
-  constexpr int R = L::kRows, B = L::kBlocks, NG = L::kGroups;
+  constexpr int R = L::kRows, B = L::kBlocks, NG = L::kGroups, H = L::kOwn;
   extern __shared__ __align__(16) char smem[];
   uint4* qs = reinterpret_cast<uint4*>(smem);  // [part][block][lane]
   float* os = reinterpret_cast<float*>(smem + L::q_bytes);
@@ -281,7 +278,6 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const float low_half = t >> 1;  // BESIDE: whether the lane's weights are the low parts
   begin();
   const int per_row = a.kv_heads * a.chunks;
   int row, unit, tile;  // unit: of the row
@@ -477,13 +473,13 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
     return (odds >> (2 * t) & 3u) | (odds >> (8 + 2 * t) & 3u) << 2;
   };
   // Q in the order of the second operand's registers: a warp takes two heads
-  // (BESIDE: heads 4 to 7 are 0 to 3 again)
+  // (BESIDE: each twice)
   auto stage_q = [&](int row, int first_q, int heads) {
     const T* qp = (const T*)a.q + (long long)row * a.q_sb + (long long)first_q * a.q_sh;
     __half* to = reinterpret_cast<__half*>(qs);
 #pragma unroll
     for (int i = 0; i < kHeads / kWarps; ++i) {
-      const int h = warp * (kHeads / kWarps) + i, from = BESIDE ? h & 3 : h;
+      const int h = warp * (kHeads / kWarps) + i, from = BESIDE ? h >> 1 : h;
       float x[B], top = 0.f;
 #pragma unroll
       for (int j = 0; j < B; ++j) {
@@ -542,12 +538,13 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
     }
     __syncthreads();
 
-    // A lane has query heads 2t and 2t + 1 (BESIDE: lanes 2 and 3 of four those of 0 and 1 again, for the low parts); of o the values 32b + 4g + 2j (o[..][0..1]) and the next, sixteenfold
-    float m[2], l[2], z[NG][2], o[B][2][4], f[2], qsum[NG][2];
+    // A lane has query heads 2t and 2t + 1 (BESIDE: t); of o the values 32b + 4g + 2j, and behind the heads' the next
+    // ones, sixteenfold
+    float m[H], l[H], z[NG][H], o[B][2][2 * H], f[H], qsum[NG][H];
     unsigned e = 0;  // a power of two above the largest step of values so far: its exponent, less 1; the power, and its inverse
     float above = 0x1p-126f, below = 0x1p126f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < H; ++i) {
       m[i] = -INFINITY;
       l[i] = 0.f;
       f[i] = factors[2 * t + i];
@@ -560,10 +557,12 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) o[b][j][0] = o[b][j][1] = o[b][j][2] = o[b][j][3] = 0.f;
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 2 * H; ++i) o[b][j][i] = 0.f;
 
     for (int step = 0; step < count; ++step) {
-      float s[R][4], lows[R][4];
+      float s[R][2 * H], lows[R][2 * H];  // of a key and the one 8 on, H heads each
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         float sum[R][4];
@@ -593,11 +592,11 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const unsigned w = kw[r][i >> 1][n];
-            const float step = __uint_as_float(w & 0xffff0000u), low = low_of<L::kCentred>(w);
-            s[r][i] = n ? fmaf(step, sum[r][i], s[r][i]) : step * sum[r][i];
-            lows[r][i] = n ? fmaf(low, qsum[n][i & 1], lows[r][i]) : low * qsum[n][i & 1];
+          for (int i = 0; i < 2 * H; ++i) {
+            const unsigned w = kw[r][i / H][n];
+            const float step = __uint_as_float(w & 0xffff0000u), low = low_of<L::kCentred>(w), x = sum[r][BESIDE ? 2 * i : i];
+            s[r][i] = n ? fmaf(step, x, s[r][i]) : step * x;
+            lows[r][i] = n ? fmaf(low, qsum[n][i % H], lows[r][i]) : low * qsum[n][i % H];
           }
       }
       // the values' scales are kept: the next keys' come with their keys
@@ -611,14 +610,15 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[r][i] = fmaf(s[r][i], f[i & 1], lows[r][i]);
+        for (int i = 0; i < 2 * H; ++i) s[r][i] = fmaf(s[r][i], f[i % H], lows[r][i]);
       if (seen != kAll) {  // the same in all lanes
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             if (seen >> (16 * r + 8 * i + g) & 1) continue;
-            s[r][2 * i] = s[r][2 * i + 1] = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < H; ++h) s[r][H * i + h] = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NG; ++n) vs[r][i][n] = 0;
           }
@@ -628,20 +628,25 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 
       // The maxima move, and with them all sums, only where a score is far
       // above them, and the power above the steps only where a step is.
-      float top[2] = {-INFINITY, -INFINITY};
+      float top[H];
       unsigned largest = 0;
+      bool rises = false;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+      for (int i = 0; i < H; ++i) {
+        top[i] = s[0][i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top[i & 1] = fmaxf(top[i & 1], s[r][i]);
+        for (int k = 1; k < 2 * R; ++k) top[i] = fmaxf(top[i], s[k >> 1][H * (k & 1) + i]);
+        rises |= top[i] > m[i] + kSlack;
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int n = 0; n < NG; ++n) largest = max(largest, vs[r][i][n]);
-      }
-      if (__any_sync(~0u, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack || largest >> 23 > e)) {
+      if (__any_sync(~0u, rises || largest >> 23 > e)) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < H; ++i) {
           top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 4));
           top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 8));
           top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 16));
@@ -656,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               o[b][j][i] *= down;
-              o[b][j][i + 2] *= down;
+              o[b][j][i + H] *= down;
             }
         }
         // a NaN's exponent counts as the largest that a step has
@@ -664,16 +669,16 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
         above = __uint_as_float((e + 1) << 23);
         below = __uint_as_float((253u - e) << 23);
       }
-      float base[2];
+      float base[H];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i] - kShift;
-      float p[R][4];
+      for (int i = 0; i < H; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i] - kShift;
+      float p[R][2 * H];
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[r][i] = exp2_fast(s[r][i] - base[i & 1]);
-          l[i & 1] += p[r][i];
+        for (int i = 0; i < 2 * H; ++i) {
+          p[r][i] = exp2_fast(s[r][i] - base[i % H]);
+          l[i % H] += p[r][i];
         }
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
@@ -684,12 +689,14 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
           for (int i = 0; i < 2; ++i) {
             const unsigned w = vs[r][i][n];
             const float st = __uint_as_float(w & 0xffff0000u) * below, low = low_of<L::kCentred>(w);
-            z[n][0] = fmaf(p[r][2 * i], low, z[n][0]);
-            z[n][1] = fmaf(p[r][2 * i + 1], low, z[n][1]);
-            const float x = p[r][2 * i] * st, y = p[r][2 * i + 1] * st;
-            if constexpr (BESIDE) {  // the high parts times -1, or the low ones
-              pt[r][0][i] = transpose8x8(pack_half(fmaf(x, low_half, -high_part(x)), fmaf(y, low_half, -high_part(y))));
+#pragma unroll
+            for (int h = 0; h < H; ++h) z[n][h] = fmaf(p[r][H * i + h], low, z[n][h]);
+            const float x = p[r][H * i] * st;
+            if constexpr (BESIDE) {  // both parts, next to each other
+              const float hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);  // 11 bits of x
+              pt[r][0][i] = transpose8x8(pack_half(hi, x - hi));
             } else {
+              const float y = p[r][H * i + 1] * st;
               const unsigned hi = pack_half(x, y);
               const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
               pt[r][0][i] = transpose8x8(hi);
@@ -725,33 +732,23 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[b][j][i] = fmaf(above, sum[j][i], o[b][j][i]);
+            for (int i = 0; i < 2 * H; ++i) o[b][j][i] = fmaf(above, BESIDE ? sum[j][2 * i] + sum[j][2 * i + 1] : sum[j][i], o[b][j][i]);
         }
       }
       load_v(parity_of(next));
       next = place();
     }
 
-    if constexpr (BESIDE) {  // lanes of heads 0 to 3 take the low parts' sums and the others' of the high ones
-#pragma unroll
-      for (int b = 0; b < B; ++b)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[b][j][i] = __shfl_xor_sync(~0u, o[b][j][i], 2) - o[b][j][i];
-    }
-
     // join the warps
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int h = warp * kHeads + 2 * t + i;
+    for (int i = 0; i < H; ++i) {
+      const int h = warp * kHeads + H * t + i;
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) {
         l[i] += __shfl_xor_sync(~0u, l[i], off);
 #pragma unroll
         for (int n = 0; n < NG; ++n) z[n][i] += __shfl_xor_sync(~0u, z[n][i], off);
       }
-      if (BESIDE && t >= 2) continue;
       if (g == 0) {
         ms[h] = m[i];
         ls[h] = l[i];
@@ -761,9 +758,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
         const float low = z[b / L::kFold][i];
         float4 v;
         v.x = fmaf(o[b][0][i], L::kEven, low);
-        v.y = fmaf(o[b][0][i + 2], L::kOdd, low);
+        v.y = fmaf(o[b][0][i + H], L::kOdd, low);
         v.z = fmaf(o[b][1][i], L::kEven, low);
-        v.w = fmaf(o[b][1][i + 2], L::kOdd, low);
+        v.w = fmaf(o[b][1][i + H], L::kOdd, low);
         *reinterpret_cast<float4*>(os + (size_t)h * L::kPitch + 32 * b + 4 * g) = v;
       }
     }
