@@ -18,14 +18,16 @@
 // q enters as fp16 numbers scaled by a power of two for each head, its largest
 // in 2^14 ... 2^15 and a sixteenth of that beside the codes that count sixteen
 // times: exact for fp16 and bf16 down to 2^-20 of the head's largest, and in
-// two parts (2^-22) for fp32.  p step enters as 2^8 p step over a power of two
-// above the largest step so far, in two parts (2^-22): one alone, 2^-11, showed
-// in bf16 outputs, whose error rose from 1.64e-3 to 1.72e-3.  An instruction has
+// two parts (2^-22) for fp32.  p step enters as a multiple of a power of two
+// that follows the largest product of its head and group so far (the largest
+// step may be that of a key without weight), in two parts, which lose 2^-22 of
+// a product, or 2^-25 of that power, of which the largest is near 2^8: one alone,
+// 2^-11, showed in bf16 outputs, whose error rose from 1.64e-3 to 1.72e-3.  An instruction has
 // eight columns: a unit of up to four heads has the two parts of a head side by
 // side, so that a lane has the weights of one head and adds both parts' sums
-// (128 sequences, bf16: 166 us; two instructions took 200, and one part alone,
+// (128 sequences, bf16: 165 us; two instructions took 200, and one part alone,
 // with two heads a lane, 169); more heads take two instructions (one sequence
-// of 131071, 8 heads a unit, bf16: 50.5 us; one part took 43).  For fp32 the
+// of 131071, 8 heads a unit, bf16: 53 us; one part took 43).  For fp32 the
 // codes are centred, c - 8 (four
 // instructions a word more): with many keys the values average out, and the
 // large part that codes from 0 on have in common lost 5e-5 of what remains to
@@ -133,7 +135,12 @@ constexpr unsigned kNone = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kShift = 8.f;  // weights are held as 2^8 exp(s - m)
-constexpr float kSlack = 7.f;  // of 2: m moves when a score is this far above it (a weight is below 2^15)
+constexpr float kSlack = 3.f;  // of 2: m moves when a score is this far above it (a weight is below 2^11)
+// Weights times steps enter as multiples of a power of two, their unit: below
+// 2^8 of it when it is chosen, and below 2^15 as long as the steps' bits are
+// below the unit's and kRoom.  The least unit, with whose inverse a weight stays
+// below 2^127, and a power of two's bits and its inverse's together.
+constexpr unsigned kRoom = (unsigned)(12 - (int)kShift) << 23, kLeastUnit = (127 - 112) << 23, kOneSquared = (2 * 127u) << 23;
 
 struct Span {
   int begin, end, tiles;  // seen keys, and the tiles that cover them
@@ -251,9 +258,9 @@ struct Layout {
   static constexpr size_t o_bytes = (size_t)kWarps * kHeads * kPitch * 4;
   static constexpr size_t smem = q_bytes + o_bytes;
   // CTAs that share an SM: more warps help (128 sequences of 5000 keys, bf16,
-  // groups of 64: 166 us with four), but not where 128 registers a thread spill
-  // (fp16, groups of 32: 106 us for 88; one of 131071 keys, 8 heads a unit, bf16:
-  // 51.3 us for 50.3)
+  // groups of 64: 165 us with four, 170 with three), but not where 128
+  // registers a thread spill (fp16, groups of 32: 84 us for 80; one of 131071
+  // keys, 8 heads a unit, bf16: 51.3 us for 50.3)
   static constexpr int kResident = W <= 64 ? 4 : W <= 128 ? (sizeof(T) == 2 && kGroups <= 2 && BESIDE ? 4 : 3) : 2;
 };
 
@@ -541,8 +548,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
     // A lane has query heads 2t and 2t + 1 (BESIDE: t); of o the values 32b + 4g + 2j, and behind the heads' the next
     // ones, sixteenfold
     float m[H], l[H], z[NG][H], o[B][2][2 * H], f[H], qsum[NG][H];
-    unsigned e = 0;  // a power of two above the largest step of values so far: its exponent, less 1; the power, and its inverse
-    float above = 0x1p-126f, below = 0x1p126f;
+    unsigned unit_of[NG][H];  // what a head's weights times a group's steps are multiples of: a power of two, its bits
 #pragma unroll
     for (int i = 0; i < H; ++i) {
       m[i] = -INFINITY;
@@ -551,6 +557,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         z[n][i] = 0.f;
+        unit_of[n][i] = kLeastUnit;
         qsum[n][i] = q_sums[n][2 * t + i];
       }
     }
@@ -627,10 +634,11 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
       load_k();
 
       // The maxima move, and with them all sums, only where a score is far
-      // above them, and the power above the steps only where a step is.
+      // above them; the units of weights times steps, then or where a step is
+      // so large that a product might leave fp16's range: to 2^-8 of the largest
+      // product, or up to 2^8 more where that spares the next steps as large.
       float top[H];
-      unsigned largest = 0;
-      bool rises = false;
+      bool rises = false, large = false;
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         top[i] = s[0][i];
@@ -639,35 +647,57 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
         rises |= top[i] > m[i] + kSlack;
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int n = 0; n < NG; ++n) {
+        unsigned largest = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int r = 0; r < R; ++r) largest = max(largest, max(vs[r][0][n], vs[r][1][n]));
+        large |= largest >= min(unit_of[n][0], unit_of[n][H - 1]) + kRoom;
+      }
+      const bool moved = __any_sync(~0u, rises);
+      if (moved || __any_sync(~0u, large)) {
+        if (moved) {
 #pragma unroll
-          for (int n = 0; n < NG; ++n) largest = max(largest, vs[r][i][n]);
-      if (__any_sync(~0u, rises || largest >> 23 > e)) {
+          for (int i = 0; i < H; ++i) {
+            top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 4));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 8));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 16));
+            const float to = fmaxf(m[i], top[i]);
+            const float down = to == -INFINITY ? 1.f : exp2_fast(m[i] - to);
+            m[i] = to;
+            l[i] *= down;
 #pragma unroll
-        for (int i = 0; i < H; ++i) {
-          top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 4));
-          top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 8));
-          top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 16));
-          const float to = fmaxf(m[i], top[i]);
-          const float down = to == -INFINITY ? 1.f : exp2_fast(m[i] - to);
-          m[i] = to;
-          l[i] *= down;
+            for (int n = 0; n < NG; ++n) z[n][i] *= down;
 #pragma unroll
-          for (int n = 0; n < NG; ++n) z[n][i] *= down;
+            for (int b = 0; b < B; ++b)
 #pragma unroll
-          for (int b = 0; b < B; ++b)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              o[b][j][i] *= down;
-              o[b][j][i + H] *= down;
-            }
+              for (int j = 0; j < 2; ++j) {
+                o[b][j][i] *= down;
+                o[b][j][i + H] *= down;
+              }
+          }
         }
-        // a NaN's exponent counts as the largest that a step has
-        e = max(e, min(__reduce_max_sync(~0u, largest) >> 23, 252u));
-        above = __uint_as_float((e + 1) << 23);
-        below = __uint_as_float((253u - e) << 23);
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int i = 0; i < H; ++i) {
+            // exponents: of the largest product (which is below 2^(product - 252)), and of the largest step
+            int product = 0, step = 0;
+#pragma unroll
+            for (int k = 0; k < 2 * R; ++k) {
+              const float weight = exp2_fast(s[k >> 1][H * (k & 1) + i] - (m[i] == -INFINITY ? 0.f : m[i] - kShift));
+              const int u = __float_as_uint(weight) >> 23, v = vs[k >> 1][k & 1][n] >> 23;
+              if (u && v) product = max(product, u + v);
+              step = max(step, v);
+            }
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+              product = max(product, __shfl_xor_sync(~0u, product, off));
+              step = max(step, __shfl_xor_sync(~0u, step, off));
+            }
+            const int enough = product - 133, unit = max(enough, min(step + (int)kShift - 7, enough + 8));
+            const unsigned to = (unsigned)min(max(unit, (int)(kLeastUnit >> 23)), 253) << 23;
+            unit_of[n][i] = moved ? to : max(to, unit_of[n][i]);
+          }
       }
       float base[H];
 #pragma unroll
@@ -688,15 +718,15 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const unsigned w = vs[r][i][n];
-            const float st = __uint_as_float(w & 0xffff0000u) * below, low = low_of<L::kCentred>(w);
+            const float st = __uint_as_float(w & 0xffff0000u), low = low_of<L::kCentred>(w);
 #pragma unroll
             for (int h = 0; h < H; ++h) z[n][h] = fmaf(p[r][H * i + h], low, z[n][h]);
-            const float x = p[r][H * i] * st;
+            const float x = p[r][H * i] * __uint_as_float(kOneSquared - unit_of[n][0]) * st;
             if constexpr (BESIDE) {  // both parts, next to each other
               const float hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);  // 11 bits of x
               pt[r][0][i] = transpose8x8(pack_half(hi, x - hi));
             } else {
-              const float y = p[r][H * i + 1] * st;
+              const float y = p[r][H * i + 1] * __uint_as_float(kOneSquared - unit_of[n][H - 1]) * st;
               const unsigned hi = pack_half(x, y);
               const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
               pt[r][0][i] = transpose8x8(hi);
@@ -732,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 2 * H; ++i) o[b][j][i] = fmaf(above, BESIDE ? sum[j][2 * i] + sum[j][2 * i + 1] : sum[j][i], o[b][j][i]);
+            for (int i = 0; i < 2 * H; ++i) o[b][j][i] = fmaf(__uint_as_float(unit_of[n][i % H]), BESIDE ? sum[j][2 * i] + sum[j][2 * i + 1] : sum[j][i], o[b][j][i]);
         }
       }
       load_v(parity_of(next));
