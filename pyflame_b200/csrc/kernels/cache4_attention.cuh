@@ -134,13 +134,14 @@ constexpr int kThreads = kWarps * 32;
 constexpr unsigned kNone = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kShift = 8.f;  // weights are held as 2^8 exp(s - m)
-constexpr float kSlack = 3.f;  // of 2: m moves when a score is this far above it (a weight is below 2^11)
+// Weights are held as 2^-24 exp(s - m): sums over values of 2^126, sixteen
+// times as large where codes count sixteen times, stay in fp32's range for 2^18
+// keys at the least.
+constexpr float kShift = -24.f;
+constexpr float kSlack = 3.f;  // of 2: m moves when a score is this far above it (a weight is below 2^-21)
 // Weights times steps enter as multiples of a power of two, their unit: below
 // 2^8 of it when it is chosen, and below 2^15 as long as the steps' bits are
-// below the unit's and kRoom.  The least unit, with whose inverse a weight stays
-// below 2^127, and a power of two's bits and its inverse's together.
-constexpr unsigned kRoom = (unsigned)(12 - (int)kShift) << 23, kLeastUnit = (127 - 112) << 23, kOneSquared = (2 * 127u) << 23;
+// below the unit's and kRoom (Layout).
 
 struct Span {
   int begin, end, tiles;  // seen keys, and the tiles that cover them
@@ -250,7 +251,12 @@ struct Layout {
   static constexpr bool kCentred = sizeof(T) == 4;
   // what the codes' operands and q's scaling leave to multiply with
   static constexpr int kQShift = kCentred ? -14 : 10;  // of 2, with q's exponent
-  static constexpr float kEven = kCentred ? 1.f : 0x1p24f, kOdd = kCentred ? 1.f : 0x1p20f;
+  static constexpr float kOdd = kCentred ? 1.f : 0x1p-4f;
+  // Units are held times what the codes' operands leave, 2^24, so that sums do not leave fp32's range: the least one's
+  // bits, how far a step's may be above a unit's, and those of a unit and of its inverse, without that factor, together.
+  static constexpr int kLeft = kCentred ? 0 : 24;
+  static constexpr unsigned kLeastUnit = (unsigned)(1 + kLeft) << 23, kRoom = (unsigned)(12 - (int)kShift - kLeft) << 23;
+  static constexpr unsigned kInverse = (unsigned)(2 * 127 + kLeft) << 23;
   static constexpr int kRows = RUNS && W <= 128 ? 2 : 1;  // blocks of 16 keys of a warp's step
   static constexpr int kTile = 16 * kRows * kWarps;
   static constexpr int kPitch = W + 4;
@@ -557,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         z[n][i] = 0.f;
-        unit_of[n][i] = kLeastUnit;
+        unit_of[n][i] = L::kLeastUnit;
         qsum[n][i] = q_sums[n][2 * t + i];
       }
     }
@@ -651,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
         unsigned largest = 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) largest = max(largest, max(vs[r][0][n], vs[r][1][n]));
-        large |= largest >= min(unit_of[n][0], unit_of[n][H - 1]) + kRoom;
+        large |= largest >= min(unit_of[n][0], unit_of[n][H - 1]) + L::kRoom;
       }
       const bool moved = __any_sync(~0u, rises);
       if (moved || __any_sync(~0u, large)) {
@@ -694,8 +700,8 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
               product = max(product, __shfl_xor_sync(~0u, product, off));
               step = max(step, __shfl_xor_sync(~0u, step, off));
             }
-            const int enough = product - 133, unit = max(enough, min(step + (int)kShift - 7, enough + 8));
-            const unsigned to = (unsigned)min(max(unit, (int)(kLeastUnit >> 23)), 253) << 23;
+            const int enough = product - 133 + L::kLeft, unit = max(enough, min(step + (int)kShift - 7 + L::kLeft, enough + 8));
+            const unsigned to = (unsigned)min(max(unit, (int)(L::kLeastUnit >> 23)), 253) << 23;
             unit_of[n][i] = moved ? to : max(to, unit_of[n][i]);
           }
       }
@@ -721,12 +727,12 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
             const float st = __uint_as_float(w & 0xffff0000u), low = low_of<L::kCentred>(w);
 #pragma unroll
             for (int h = 0; h < H; ++h) z[n][h] = fmaf(p[r][H * i + h], low, z[n][h]);
-            const float x = p[r][H * i] * __uint_as_float(kOneSquared - unit_of[n][0]) * st;
+            const float x = p[r][H * i] * __uint_as_float(L::kInverse - unit_of[n][0]) * st;
             if constexpr (BESIDE) {  // both parts, next to each other
               const float hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);  // 11 bits of x
               pt[r][0][i] = transpose8x8(pack_half(hi, x - hi));
             } else {
-              const float y = p[r][H * i + 1] * __uint_as_float(kOneSquared - unit_of[n][H - 1]) * st;
+              const float y = p[r][H * i + 1] * __uint_as_float(L::kInverse - unit_of[n][H - 1]) * st;
               const unsigned hi = pack_half(x, y);
               const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
               pt[r][0][i] = transpose8x8(hi);
@@ -787,9 +793,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
       for (int b = 0; b < B; ++b) {
         const float low = z[b / L::kFold][i];
         float4 v;
-        v.x = fmaf(o[b][0][i], L::kEven, low);
+        v.x = o[b][0][i] + low;
         v.y = fmaf(o[b][0][i + H], L::kOdd, low);
-        v.z = fmaf(o[b][1][i], L::kEven, low);
+        v.z = o[b][1][i] + low;
         v.w = fmaf(o[b][1][i + H], L::kOdd, low);
         *reinterpret_cast<float4*>(os + (size_t)h * L::kPitch + 32 * b + 4 * g) = v;
       }

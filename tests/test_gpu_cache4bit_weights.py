@@ -90,3 +90,18 @@ def test_groups_of_different_sizes(dtype, ratio, n, heads):
     v = randn(g, n, 1, 64) * (2.0 ** 12 if dtype == F16 else 1.0)
     v[..., 32:] *= ratio
     check_far_apart(*far_apart(g, dtype, n, heads, 16, v, []))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,heads", [(70, 2), (9000, 4), (9000, 8)])
+def test_values_at_both_ends_of_the_type(dtype, n, heads):
+    """Values next to the largest that are kept, 2^126, and next to the smallest steps."""
+    g = gen(n + 1)
+    for size in (2.0 ** 14,) if dtype == F16 else (2.0 ** 122, 2.0 ** -100):
+        v = size * (torch.rand(n, 1, 64, generator=g, device="cuda") - 0.5)
+        check_far_apart(*far_apart(g, dtype, n, heads, 16, v, []))
+    if dtype != F16:  # both: the large ones without weight
+        v = 2.0 ** -60 * randn(g, n, 1, 64)
+        v[3] = 2.0 ** 120 * torch.rand(1, 64, generator=g, device="cuda")
+        c, q, table, lens = far_apart(g, dtype, n, 1, 16, v, [(3, -200.0)])
+        check_far_apart(c, q, table, lens)
