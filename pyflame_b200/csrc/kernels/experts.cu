@@ -20,7 +20,8 @@
 //    a gate and its up value.  The warps share the summed axis, 64 bytes of a
 //    row at a time (256 consecutive bytes a CTA).  What leaves is w act(g) u
 //    in two 16-bit parts (one fp32 value): a single one would round as
-//    coarsely as the output does.
+//    coarsely as the output does.  fp16 parts reach from 2^-25 to 65504: 8
+//    values (a unit's of a pair) have a power of two of their own (Scaled).
 // 3. down: a cluster for 16 rows of the output.  All (expert, 64 bytes) pieces
 //    of those rows form one list, of which each warp of the cluster takes an
 //    equal run; at an expert's end it adds what it has to its own table of
@@ -46,6 +47,7 @@
 #include <cmath>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "../common.hpp"
 #include "act.cuh"
@@ -88,11 +90,36 @@ struct Args {
   long long x_row;
   char* h;  // [parts][tokens * top][h_row bytes], zeros behind inner
   long long h_row, h_part;
-  // parts of experts' pairs: how many, then of each: expert, first of its pairs, their number (at most 8 NT)
+  // fp16: exponents of the powers of two on 8 values of h each, [tokens * top][e_row]
+  signed char* e;
+  long long e_row;
+  // parts of experts' pairs: how many, then of each: expert, first of its pairs, their number (at most 8 NT),
+  // whether a power of two of theirs is not 2^0
   int4* parts;
   int* pairs;  // [tokens * top] by expert
   int most_parts;
 };
+
+// fp16 intermediate values are held times 2^10, and 8 of them over a power of two
+// of their own, 2^e: 2^0 where the largest is then from 2^-8 to 65504, or that
+// with e a multiple of 8 which puts it between 2^7 and 2^15, so that a value
+// loses 2^-22, or 2^-17 of the largest of the 8.  Zeros have the least exponent.
+// Products add four of them up (64 bytes of a row): with powers that differ,
+// which multiples of 8 seldom do, the values are multiplied by what they are
+// below the largest.  The down products look at the powers of a part only where
+// one is not 2^0, as seldom happens to values from 2^-18 to 2^6 (64 tokens, 8 of
+// 128 experts, 2048 x 768: 231 us; with a few values of 10^4 in all parts 253, with
+// all values near 10^-9 272).
+template <typename T>
+struct Scaled {
+  static constexpr bool kIs = std::is_same<T, __half>::value;
+  static constexpr float kTimes = kIs ? 1024.f : 1.f;
+};
+constexpr int kZeros = -128;
+__device__ __forceinline__ int exponent_for(float largest) {
+  if (largest == 0.f) return kZeros;
+  return largest >= 0x1p-8f && largest <= 65504.f ? 0 : max(((int)(__float_as_uint(largest) >> 23) - 127 - 7) & ~7, -120);
+}
 
 // Lets the next kernel come up while this one works: the kernels in front of
 // another leave room for its CTAs, or their own are all there already.  The
@@ -381,22 +408,58 @@ struct Ring {
   }
 };
 
+// Eight fp16 numbers times two, the same.
+__device__ __forceinline__ uint4& times_half(uint4& v, unsigned by) {
+  const __half2 f = *reinterpret_cast<const __half2*>(&by);
+  unsigned* w = &v.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(w + i), f);
+    w[i] = *reinterpret_cast<const unsigned*>(&x);
+  }
+  return v;
+}
+
 // What the vectors of a piece add up to with its rows, added to acc in fp32,
 // rounded to nearest: the tensor cores truncate what they add.
-template <typename T, int NT, int PARTS, class R>
-__device__ __forceinline__ void take_piece(float (&acc)[NT][4], uint32_t at, bool second) {
+// SCALED: exponents: of the four powers of two of each of the lane's vectors.
+template <typename T, int NT, int PARTS, bool SCALED, class R>
+__device__ __forceinline__ void take_piece(float (&acc)[NT][4], uint32_t at, bool second, const int (&exponents)[NT]) {
   const uint4 a0 = R::read(at), a1 = R::read(at + 512);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     if (n && !second) continue;  // the same in all lanes
     float sum[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+    float times[2] = {1.f, 1.f};  // of the vectors 2t and 2t + 1
+    uint4 b[PARTS];
 #pragma unroll
-    for (int p = PARTS - 1; p >= 0; --p) {
-      const uint4 b[1] = {R::read(at + 1024 + (p * NT + n) * 512)};
-      chunk_product<T, 1>(sum, a0, a1, b);
+    for (int p = 0; p < PARTS; ++p) b[p] = R::read(at + 1024 + (p * NT + n) * 512);
+    if constexpr (SCALED) {
+      const int e = exponents[n];
+      if (__any_sync(~0u, e != 0)) {
+        const int t = threadIdx.x & 3, own = (signed char)(e >> (8 * t));
+        const int most = max(max((int)(signed char)e, (int)(signed char)(e >> 8)), max((int)(signed char)(e >> 16), e >> 24));
+        const int down = own - most;
+        if (__any_sync(~0u, down != 0 && own != kZeros)) {
+          // 2^down as a product of two fp16 numbers; below 2^-38, 0
+          const int rest = min(max(down, -40) + 14, 0);
+          const unsigned first = (unsigned)(15 + max(down, -14)) << 10;
+          const unsigned second = rest >= -14 ? (unsigned)(15 + rest) << 10 : rest >= -24 ? 1u << (24 + rest) : 0u;
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) times_half(times_half(b[p], first << 16 | first), second << 16 | second);
+        }
+        const float mine = __uint_as_float((unsigned)(127 + max(most, -126)) << 23);
+        times[0] = __shfl_sync(~0u, mine, 8 * t);
+        times[1] = __shfl_sync(~0u, mine, 8 * t + 4);
+      }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) acc[n][r] += sum[0][r];
+    for (int p = PARTS - 1; p >= 0; --p) {
+      const uint4 one[1] = {b[p]};
+      chunk_product<T, 1>(sum, a0, a1, one);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[n][r] = SCALED ? fmaf(sum[0][r], times[r & 1], acc[n][r]) : acc[n][r] + sum[0][r];
   }
 }
 
@@ -479,20 +542,19 @@ __global__ void __launch_bounds__(kThreads, (Up<T, NT>::kResident)) up_kernel(Ar
   for (int s = 0; s < U::kDepth; ++s) copy(at + s * U::R::kStage);
 
   int turn = 0;
+  int told = -1;
   for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
     const int i = unit / blocks, f = (unit - i * blocks) * 8 + g;
     const int4 p = parts[i];
-    // of the block of vectors that this warp finishes
-    int pair[2] = {-1, -1};
-    float weight[2];
-    if (warp < NT) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int slot = warp * 8 + 2 * t + k;
-        if (slot < p.z) {
-          pair[k] = pairs[p.y + slot];
-          weight[k] = a.weights[pair[k]];
-        }
+    // The warp finishes vectors 2t + k of block n, a value of the unit's each lane: all of them for 16 vectors, two for 8.
+    const int n = warp >> 1, k = warp & 1;
+    int pair = -1;
+    float weight = 0.f;
+    if (warp < 2 * NT) {
+      const int slot = n * 8 + 2 * t + k;
+      if (slot < p.z) {
+        pair = pairs[p.y + slot];
+        weight = a.weights[pair] * Scaled<T>::kTimes;
       }
     }
     float acc[NT][4];
@@ -500,32 +562,46 @@ __global__ void __launch_bounds__(kThreads, (Up<T, NT>::kResident)) up_kernel(Ar
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     for (int c = warp; c < pieces; c += kWarps) {
       copy_wait<U::kDepth - 1>();
-      take_piece<T, NT, 1, typename U::R>(acc, at, p.z > 8);
+      take_piece<T, NT, 1, false, typename U::R>(acc, at, p.z > 8, {});
       copy(at);
       at = at == ring.base + (U::kDepth - 1) * U::R::kStage ? ring.base : at + U::R::kStage;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) red[turn][warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
     __syncthreads();
-    static_assert(NT <= kWarps, "a warp finishes a block of vectors");
-    if (warp < NT) {
-      float4 s = red[turn][0][warp][lane];
+    static_assert(2 * NT <= kWarps, "a warp finishes half of a block of vectors");
+    if (warp < 2 * NT) {
+      const float* from = reinterpret_cast<const float*>(&red[turn][0][n][lane]) + k;
+      float gv = 0.f, uv = 0.f;
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) {
-        const float4 v = red[turn][w][warp][lane];
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
+      for (int w = 0; w < kWarps; ++w) {
+        gv += from[w * NT * 128];
+        uv += from[w * NT * 128 + 2];
       }
+      const float act = a.act ? act_apply<2>(gv) : act_apply<5>(gv);
+      // rows behind the last are zeros (their sums are)
+      float v = pair >= 0 && f < a.inner ? act * uv * weight : 0.f;
+      if constexpr (Scaled<T>::kIs) {
+        float largest = fabsf(v);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (pair[k] < 0) continue;
-        const float gv = k ? s.y : s.x, uv = k ? s.w : s.z;
-        const float act = a.act ? act_apply<2>(gv) : act_apply<5>(gv);
-        // rows behind the last are zeros (their sums are)
-        const float v = f < a.inner ? act * uv * weight[k] : 0.f;
-        T* to = reinterpret_cast<T*>(a.h + pair[k] * a.h_row) + f;
+        for (int o = 4; o < 32; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, o));
+        const int e = exponent_for(largest);
+        if (e != 0 && e != kZeros) {
+          v *= __uint_as_float((unsigned)(127 - e) << 23);
+          if (g == 0 && told != i) {
+            a.parts[1 + i].w = 1;
+            told = i;
+          }
+        }
+        if (g == 0 && pair >= 0) {
+          signed char* to = a.e + pair * a.e_row + (unit - i * blocks);
+          *to = (signed char)e;
+          if (unit - i * blocks == blocks - 1)  // up to whole pieces
+            for (int c = blocks; c < a.e_row; ++c) *++to = kZeros;
+        }
+      }
+      if (pair >= 0) {
+        T* to = reinterpret_cast<T*>(a.h + pair * a.h_row) + f;
         if constexpr (sizeof(T) == 4) {
           *to = v;
         } else {
@@ -623,23 +699,40 @@ __global__ void __launch_bounds__(WARPS * 32, (Down<T, NT, WARPS>::kResident)) d
     ahead.part = p0 / pieces;
     aim(p0 - ahead.part * pieces);
   }
+  float* table = tables + warp * cells;
   uint32_t at = ring.base;
 #pragma unroll
   for (int s = 0; s < D::kDepth; ++s) copy(at + s * D::R::kStage);
-
-  float* table = tables + warp * cells;
   for (int p = p0; p < p1;) {
     const int i = p / pieces, end = min(p1, (i + 1) * pieces);
     const int4 e = parts[i];
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    for (; p < end; ++p) {
-      copy_wait<D::kDepth - 1>();
-      take_piece<T, NT, PARTS, typename D::R>(acc, at, e.z > 8);
-      copy(at);
-      at = at == ring.base + (D::kDepth - 1) * D::R::kStage ? ring.base : at + D::R::kStage;
-    }
+    auto run = [&](auto scaled) {
+      constexpr bool SCALED = decltype(scaled)::value;
+      int exponents[NT] = {};
+      const signed char* from[NT];
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) from[n] = a.e + (long long)pairs[e.y + min(n * 8 + g, e.z - 1)] * a.e_row + (p - i * pieces) * 4;
+      }
+      for (; p < end; ++p) {
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            exponents[n] = *reinterpret_cast<const int*>(from[n]);
+            from[n] += 4;
+          }
+        }
+        copy_wait<D::kDepth - 1>();
+        take_piece<T, NT, PARTS, SCALED, typename D::R>(acc, at, e.z > 8, exponents);
+        copy(at);
+        at = at == ring.base + (D::kDepth - 1) * D::R::kStage ? ring.base : at + D::R::kStage;
+      }
+    };
+    if constexpr (Scaled<T>::kIs) e.w ? run(std::true_type()) : run(std::false_type());
+    else run(std::false_type());
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -666,7 +759,7 @@ __global__ void __launch_bounds__(WARPS * 32, (Down<T, NT, WARPS>::kResident)) d
     float s = 0.f;
     for (int r = 0; r < ranks; ++r) s += cluster.map_shared_rank(tables, r)[i];
     const int n = i >> 4, d = row + (i & 15);
-    if (d < a.width) ((T*)a.y)[n * a.y_st + d] = from_float<T>(s);
+    if (d < a.width) ((T*)a.y)[n * a.y_st + d] = from_float<T>(s * (1.f / Scaled<T>::kTimes));
   }
   if (ranks > 1) cluster.sync();  // the others' reads of this CTA's table are over
 }
@@ -691,8 +784,8 @@ void check(const pfk_experts_params& p) {
 }
 
 struct Plan {
-  int64_t block, x_row, h_row, h_part;  // of a pass
-  int64_t most_parts, h_at, parts_at, pairs_at, chosen_at, weights_at, bytes;
+  int64_t block, x_row, h_row, h_part, e_row;  // of a pass
+  int64_t most_parts, h_at, e_at, parts_at, pairs_at, chosen_at, weights_at, bytes;
 };
 
 // At most so many parts of experts' pairs.
@@ -711,7 +804,9 @@ Plan plan_of(const pfk_experts_params& p) {
   w.h_row = round_up(round_up(p.inner, 8) * es, 16);
   w.h_part = pairs * w.h_row;
   w.h_at = round_up(w.block * w.x_row, 128);
-  w.parts_at = round_up(w.h_at + w.h_part * (es == 2 ? 2 : 1), 128);
+  w.e_row = p.dtype == PFC_DTYPE_FLOAT16 ? round_up(ceil_div(p.inner, 8), 4) : 0;
+  w.e_at = round_up(w.h_at + w.h_part * (es == 2 ? 2 : 1), 128);
+  w.parts_at = round_up(w.e_at + pairs * w.e_row, 128);
   w.pairs_at = round_up(w.parts_at + (w.most_parts + 1) * (int64_t)sizeof(int4), 128);
   w.chosen_at = round_up(w.pairs_at + pairs * 4, 128);
   w.weights_at = round_up(w.chosen_at + pairs * 4, 128);
@@ -860,6 +955,8 @@ void launch_experts(const pfk_experts_params& p, cudaStream_t stream) {
   a.x_row = w.x_row;
   a.h = ws + w.h_at;
   a.h_row = w.h_row;
+  a.e = (signed char*)(ws + w.e_at);
+  a.e_row = w.e_row;
   a.parts = (int4*)(ws + w.parts_at);
   a.pairs = (int*)(ws + w.pairs_at);
   a.chosen = (int*)(ws + w.chosen_at);

@@ -79,9 +79,8 @@ class MixtureOfExperts:
         chosen experts, int32 [..., top_k], best first, and their weights,
         float32.  `out` may be x and otherwise shares no memory with it.  Rows
         at one stride are read where they are.  An infinity or NaN in x or in
-        a chosen expert's weights may make the results that depend on it NaN;
-        in float16 a product of gate and up above 65504 in size is an
-        infinity."""
+        a chosen expert's weights may make the results that depend on it
+        NaN."""
         if _Bound.forward._current_level >= 0:  # inside forward-mode differentiation
             _no_tangents(x=x, out=out)
         torch = _Bound.torch

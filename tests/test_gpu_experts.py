@@ -249,6 +249,43 @@ def test_large_intermediate_values(dtype):
         check(layer, big, (router, gate_up, down))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,e,top,d,f", [(1, 8, 4, 64, 100), (6, 4, 2, 2048, 33), (8, 8, 3, 72, 256), (9, 4, 2, 128, 64), (40, 6, 3, 96, 200), (130, 3, 2, 40, 24),
+                                              (64, 16, 2, 333, 77)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_between_the_products(dtype, tokens, e, top, d, f, mixed):
+    """Products of gate and up from 1e-7 to 1e8 in size, which down brings back: by expert, and, `mixed`, also from one
+    value to the next.  In float16 the parts of 8 values, which come in steps of 2^-24, have a power of two that leaves
+    the largest at 2^-8 at least: they lose 2^-17 of it, and so does what makes the powers of 32 values the same:
+    2^-16 of the largest of 32 for each."""
+    g = gen(tokens + f)
+    router, gate_up, down = (w.float() for w in weights(g, e, d, f, dtype))
+    size = torch.tensor([1.0, 3e3, 1e-3, 40.0, 0.05], device="cuda")[torch.arange(e, device="cuda") % 5]
+    size = size[:, None].expand(e, f).clone()
+    if mixed:
+        size *= 2.0 ** torch.randint(-4, 3, (e, f), generator=g, device="cuda")
+    gate_up = (gate_up * torch.cat([size, size], 1)[..., None]).clamp(-6e4, 6e4).to(dtype)
+    if mixed:
+        gate_up[:, :f:5] = 0
+    down = (down / (size * size).clamp(1e-7, 1e5)[:, None]).clamp(-6e4, 6e4).to(dtype)
+    x = randn(g, tokens, d, dtype=dtype)
+    ws = router.to(dtype), gate_up, down
+    layer = pf.MixtureOfExperts(*ws, top)
+    y, chosen, part = layer(x, return_routing=True)
+    want, mag, c, p = reference(x, *ws, top, True, "silu")
+    assert torch.equal(chosen.long(), c)
+    lost = torch.zeros_like(mag)
+    if dtype == F16:
+        for i in range(e):
+            n, j = (c == i).nonzero(as_tuple=True)
+            both = x[n].double() @ gate_up[i].double().T
+            h = torch.nn.functional.silu(both[:, :f]) * both[:, f:] * p[n, j][:, None]
+            pad = lambda t: torch.nn.functional.pad(t.abs(), (0, -f % 32)).unflatten(-1, (-1, 32))
+            lost.index_add_(0, n, 2.0 ** -16 * pad(h).amax(-1) @ pad(down[i].double()).sum(-1).T)
+    within(y, want, HALF[dtype] * want.abs() + 2.0 ** -15 * mag + TINY[dtype] + lost)
+    assert y.isfinite().all() and torch.equal(layer(x), y)
+
+
 def test_refusals():
     g = gen(10)
     r, u, d = weights(g, 4, 64, 32, F16)
