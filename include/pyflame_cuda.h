@@ -582,7 +582,7 @@ typedef struct pfk_adapters_params {
   int64_t base_st;
   void* out; /* [rows][outer]; may be base (same pointer and stride), not overlap base or x otherwise */
   int64_t out_st;
-  const void* a; /* [adapters][rank][a_st], zeros behind inner; 16-byte aligned rows */
+  const void* a; /* [adapters][rank][a_st], zeros behind inner up to the next 16 bytes; 16-byte aligned rows */
   int64_t a_st;
   const void* b; /* [adapters][outer][rank], 16-byte aligned */
   const float* scales; /* [adapters] */

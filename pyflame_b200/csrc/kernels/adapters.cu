@@ -73,7 +73,8 @@ struct Args {
   void* out;
   long long out_st;
   const char* a;
-  long long a_row;  // bytes
+  long long a_row;  // bytes from a row to the next; of them a_bytes count, zeros behind inner up to 16 bytes
+  int a_bytes;
   const void* b;
   const float* scales;
   int* err;
@@ -241,7 +242,7 @@ __device__ __forceinline__ void few_rows(const Args& a, cg::cluster_group& clust
   float* sums = reinterpret_cast<float*>(smem + L::sums_at(a.rank, a.most_slots));
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * kRing) + lane * 16;
 
-  const int a_bytes = (int)a.a_row, b_bytes = a.rank * (int)sizeof(T);
+  const int a_bytes = a.a_bytes, b_bytes = a.rank * (int)sizeof(T);
   const int a_pieces = (a_bytes + 63) / 64, b_pieces = (b_bytes + 63) / 64;
   const T* row = g < count ? (const T*)a.x + (long long)(row0 + slots[g]) * a.x_st : nullptr;
   const int x_shift = WIDE ? 0 : behind_16(row), x_bytes = row ? x_shift + a.inner * (int)sizeof(T) : 0;  // from the 16 bytes that the row begins in
@@ -564,7 +565,7 @@ __device__ __forceinline__ void reduce(const Args& a, int adapter, const int (&r
   constexpr int NT = 4, kX = WIDE ? 512 : 1024, kStage = RT * 1024 + NT * kX, kDepth = kRing / kStage;
   static_assert(kDepth >= 2, "a piece ahead at least");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int bytes = (int)a.a_row, pieces = (bytes + 63) / 64, x_bytes = a.inner * (int)sizeof(T);
+  const int bytes = a.a_bytes, pieces = (bytes + 63) / 64, x_bytes = a.inner * (int)sizeof(T);
   const char* weights = a.a + ((long long)adapter * a.rank + r0 + g) * a.a_row;
   int c_ahead = q;
   auto copy = [&](uint32_t to) {
@@ -787,6 +788,7 @@ void launch_adapters(const pfk_adapters_params& p, cudaStream_t stream) {
   }
   a.a = (const char*)p.a;
   a.a_row = p.a_st * es;
+  a.a_bytes = (int)round_up(p.inner * es, 16);
   a.b = p.b;
   a.scales = p.scales;
   a.err = p.err;
@@ -807,7 +809,7 @@ void launch_adapters(const pfk_adapters_params& p, cudaStream_t stream) {
   PFB_CHECK_ARG(units <= INT32_MAX / kMostRanks, "adapters: too many rows");
   // few groups: several CTAs each, as many as the device holds at once, as long
   // as all warps have something of one of the products
-  const int64_t work = std::max(ceil_div(a.a_row, 64), ceil_div(p.outer, 32));
+  const int64_t work = std::max(ceil_div(a.a_bytes, 64), ceil_div(p.outer, 32));
   int ranks = 1;
   while (ranks < kMostRanks && units * ranks <= sms && work > ranks * kWarps) ranks *= 2;
   // Many groups at most, but tiles of one or two would leave the device idle:

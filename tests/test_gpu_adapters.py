@@ -8,6 +8,7 @@ of the sum of magnitudes S = |scale| sum_r |B| sum_k |A| |x|.  What lies between
 the products is held to 2^-17 in bfloat16's two parts: 2^-15 of S in all, and
 2^-16 in the other types.
 """
+import ctypes as C
 import math
 
 import pytest
@@ -214,6 +215,28 @@ def test_between_the_products(dtype, rows, inner, outer, rank):
                 lost[hit] = 2.0 ** -39 * abs(s) * (x[hit].double() @ a.double().T).abs().amax(1, keepdim=True) * b.double().abs().sum(1)
         within(got, out, HALF[dtype] * out.abs() + SUMS[dtype] * mag + lost + 2.0 ** -25)
         assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 3, 20, 70])
+@pytest.mark.parametrize("inner", [64, 100, 333])
+def test_rows_of_a_wider_than_x(dtype, rows, inner):
+    """The C entry point takes rows of a at any distance: what lies behind their zeros, here NaN, is not read."""
+    g, outer, rank = gen(rows + inner), 48, 16
+    layer, parts = make(g, 2, inner, outer, [rank], dtype)
+    x, base = randn(g, rows, inner, dtype=dtype), randn(g, rows, outer, dtype=dtype)
+    index = torch.arange(rows, device="cuda", dtype=torch.int32) % 2
+    want = check(layer, parts, x, index, base)
+    per = 16 // x.element_size()
+    real = -(-inner // per) * per
+    a = torch.full((2, rank, real + 40 * per), float("nan"), device="cuda", dtype=dtype)
+    a[..., :real] = layer._a[..., :real]
+    out = torch.empty_like(base)
+    p = N.AdaptersParamsC.from_buffer_copy(layer._base)
+    p.rows, p.x, p.x_st, p.index, p.base, p.base_st = rows, x.data_ptr(), inner, index.data_ptr(), base.data_ptr(), outer
+    p.out, p.out_st, p.a, p.a_st = out.data_ptr(), outer, a.data_ptr(), a.shape[-1]
+    N.check(N.lib().pfk_adapters(C.byref(p), torch.cuda.current_stream().cuda_stream))
+    within(out, want.double(), HALF[dtype] * 2 * want.double().abs() + 2 * SUMS[dtype] * reference(parts, x, index, base, outer)[1])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
