@@ -927,6 +927,7 @@ void launch_experts(const pfk_experts_params& p, cudaStream_t stream) {
   check(p);
   if (p.tokens == 0) return;
   PFB_CHECK_ARG(p.x && p.y && p.router && p.gate_up && p.down, "experts: null pointer");
+  PFB_CHECK_ARG(p.y != p.x || p.tokens == 1 || p.y_st == p.x_st, "experts: y shares x's memory with another stride");
   PFB_CHECK_ARG((uintptr_t)p.router % 16 == 0 && (uintptr_t)p.gate_up % 16 == 0 && (uintptr_t)p.down % 16 == 0,
                 "experts: weights must be 16-byte aligned");
   const Plan w = plan_of(p);

@@ -108,6 +108,12 @@ def test_experts_refusals(native, change, word):
     refused(native, native.lib().pfk_experts(C.byref(p), None), word)
 
 
+def test_experts_in_place_at_another_stride(native):
+    """Refused: rows of a later pass would be written before they are read."""
+    p = native.ExpertsParamsC(0, 0, 1, 300, 64, 32, 8, 2, FAKE, 64, FAKE, 64, FAKE, 64, FAKE, 32, FAKE, 72, None, None, FAKE, 1 << 30)
+    refused(native, native.lib().pfk_experts(C.byref(p), None), "stride")
+
+
 def test_null_parameters(native):
     L, n = native.lib(), C.c_size_t(0)
     for f in (L.pfk_cache4_append, L.pfk_cache4_read, L.pfk_cache4_attention, L.pfk_adapters, L.pfk_experts):
