@@ -616,7 +616,8 @@ typedef struct pfk_experts_params {
 PFC_API int pfk_experts_workspace(const pfk_experts_params* p, size_t* bytes);
 /* y = sum over the `top` experts with the largest router logits (taken in 64
  * bits) of weight * down (act(gate x) * (up x)).  A NaN among the logits
- * counts as the lowest.  The weights are read once for every 128 tokens. */
+ * counts as the lowest.  Up to 8 tokens read an expert's weights once, more once
+ * for every 16 of the tokens that chose it, 128 tokens at a time. */
 PFC_API int pfk_experts(const pfk_experts_params* p, void* stream);
 
 #ifdef __cplusplus

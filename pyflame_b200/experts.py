@@ -29,8 +29,9 @@ class MixtureOfExperts:
 
     The router is copied (as float32).  gate_up and down are used where they
     are, if they are dense and their rows multiples of 16 bytes, else copied
-    once.  For the tokens of a decoding step: the chosen experts' weights are
-    read once for every 128 tokens.
+    once.  For the tokens of a decoding step: up to 8 tokens read their experts'
+    weights once, more once for every 16 of the tokens that chose the expert
+    (from L2 again where they are still there), 128 at a time.
     """
 
     def __init__(self, router, gate_up, down, top_k: int, renormalize: bool = True, activation: str = "silu"):
