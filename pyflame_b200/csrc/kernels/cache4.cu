@@ -314,8 +314,10 @@ __device__ __forceinline__ void store_rows(const Args& a, const double2* turns, 
   }
 }
 
-// Queries: a thread turns two chunks of 8 values that turn together, or
-// copies two.  Both are read before either is written: q_out may be q.
+// Queries, whose roundings decide nothing, in fp32 with cosines and sines
+// rounded to it: three roundings of 2^-24 of a pair's size.  A thread turns two
+// chunks of 8 values that turn together, or copies two.  Both are read before
+// either is written: q_out may be q.
 template <typename T, bool WIDE>
 __device__ __forceinline__ void turn_queries(const Args& a, const float2* turns, const Place* places, int first, int mine,
                                              int head_first, int head_last) {

@@ -217,6 +217,14 @@ __device__ __forceinline__ float low_of(unsigned scales) {
   return CENTRED ? fmaf(__uint_as_float(scales & 0xffff0000u), 8.f, low) : low;
 }
 
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
 // WORDS 32-bit words from p, aligned to their number's largest power of two
 // (up to 4)
 template <int WORDS>

@@ -1,5 +1,7 @@
 // Products of matrix rows that stream from memory with a few vectors, on
-// mma.sync, straight from global memory into operand registers.
+// mma.sync: rows and vectors come by asynchronous copies into shared memory,
+// where each lane finds its operand registers as it copied them (adapters.cu's
+// second product of many rows loads its weights straight into registers).
 //
 // A chunk is 64 bytes of a row.  Lane (g, t) = (lane / 4, lane % 4) of a warp
 // holds bytes 16t ... 16t + 15 of a chunk of rows g and g + 8 of 16 matrix
@@ -20,14 +22,6 @@
 
 namespace pfb {
 namespace {
-
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
 
 __device__ __forceinline__ void mma16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
                                       unsigned b1, __half) {
@@ -122,8 +116,9 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// v as a 16-bit part and the rest of it, 2^-17 of v in bfloat16 and 2^-22 in
-// float16; an infinity has no rest (its NaN would hide it)
+// v as a 16-bit part and the rest of it, which leave 2^-17 of v in bfloat16, and
+// in float16, up to 65504, 2^-22 of v or 2^-25, whichever is more; an infinity
+// has no rest (its NaN would hide it)
 template <typename T>
 __device__ __forceinline__ void two_parts(float v, T& hi, T& lo) {
   hi = from_float<T>(v);
