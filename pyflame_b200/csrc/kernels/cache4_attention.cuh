@@ -136,8 +136,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Weights are held as 2^-24 exp(s - m): sums over values of 2^126, sixteen
 // times as large where codes count sixteen times, stay in fp32's range for 2^18
-// keys at the least.
-constexpr float kShift = -24.f;
+// keys at the least.  (Multiplied: in the exponential's argument, 24 would leave
+// 2^-20 of it to rounding, fp32 outputs an error of 4.1e-7 for 2.3e-7.)
+constexpr int kShift = -24;
+constexpr float kWeight = 0x1p-24f;
 constexpr float kSlack = 3.f;  // of 2: m moves when a score is this far above it (a weight is below 2^-21)
 // Weights times steps enter as multiples of a power of two, their unit: below
 // 2^8 of it when it is chosen, and below 2^15 as long as the steps' bits are
@@ -263,7 +265,7 @@ struct Layout {
   // Units are held times what the codes' operands leave, 2^24, so that sums do not leave fp32's range: the least one's
   // bits, how far a step's may be above a unit's, and those of a unit and of its inverse, without that factor, together.
   static constexpr int kLeft = kCentred ? 0 : 24;
-  static constexpr unsigned kLeastUnit = (unsigned)(1 + kLeft) << 23, kRoom = (unsigned)(12 - (int)kShift - kLeft) << 23;
+  static constexpr unsigned kLeastUnit = (unsigned)(1 + kLeft) << 23, kRoom = (unsigned)(12 - kShift - kLeft) << 23;
   static constexpr unsigned kInverse = (unsigned)(2 * 127 + kLeft) << 23;
   static constexpr int kRows = RUNS && W <= 128 ? 2 : 1;  // blocks of 16 keys of a warp's step
   static constexpr int kTile = 16 * kRows * kWarps;
@@ -698,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
             int product = 0, step = 0;
 #pragma unroll
             for (int k = 0; k < 2 * R; ++k) {
-              const float weight = exp2_fast(s[k >> 1][H * (k & 1) + i] - (m[i] == -INFINITY ? 0.f : m[i] - kShift));
+              const float weight = exp2_fast(s[k >> 1][H * (k & 1) + i] - (m[i] == -INFINITY ? 0.f : m[i])) * kWeight;
               const int u = __float_as_uint(weight) >> 23, v = vs[k >> 1][k & 1][n] >> 23;
               if (u && v) product = max(product, u + v);
               step = max(step, v);
@@ -708,20 +710,20 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
               product = max(product, __shfl_xor_sync(~0u, product, off));
               step = max(step, __shfl_xor_sync(~0u, step, off));
             }
-            const int enough = product - 133 + L::kLeft, unit = max(enough, min(step + (int)kShift - 7 + L::kLeft, enough + 8));
+            const int enough = product - 133 + L::kLeft, unit = max(enough, min(step + kShift - 7 + L::kLeft, enough + 8));
             const unsigned to = (unsigned)min(max(unit, (int)(L::kLeastUnit >> 23)), 253) << 23;
             unit_of[n][i] = moved ? to : max(to, unit_of[n][i]);
           }
       }
       float base[H];
 #pragma unroll
-      for (int i = 0; i < H; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i] - kShift;
+      for (int i = 0; i < H; ++i) base[i] = m[i] == -INFINITY ? 0.f : m[i];
       float p[R][2 * H];
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int i = 0; i < 2 * H; ++i) {
-          p[r][i] = exp2_fast(s[r][i] - base[i % H]);
+          p[r][i] = exp2_fast(s[r][i] - base[i % H]) * kWeight;
           l[i % H] += p[r][i];
         }
 #pragma unroll
@@ -830,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
         if (d == 0) part[h] = make_float2(most, sum);
       } else if (whole) {
         ((T*)a.out)[(long long)row * a.o_sb + (long long)(first_q + h) * a.o_sh + d] = from_float<T>(sum == 0.f ? 0.f : v / sum);
-        if (d == 0 && a.lse) a.lse[(long long)row * a.q_heads + first_q + h] = sum == 0.f ? -INFINITY : (most + log2f(sum) - kShift) * kLn2;
+        if (d == 0 && a.lse) a.lse[(long long)row * a.q_heads + first_q + h] = sum == 0.f ? -INFINITY : (most + log2f(sum * (1.f / kWeight))) * kLn2;
       } else {
         a.parts[(share + h) * a.head_dim + d] = v;
         if (d == 0) a.stats[share + h] = make_float2(most, sum);
@@ -879,7 +881,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
         sum += by * st[r].y;
       }
       ((T*)a.out)[(long long)row * a.o_sb + (long long)(first_q + h) * a.o_sh + d] = from_float<T>(sum == 0.f ? 0.f : all / sum);
-      if (d == 0 && a.lse) a.lse[(long long)row * a.q_heads + first_q + h] = sum == 0.f ? -INFINITY : (most + log2f(sum) - kShift) * kLn2;
+      if (d == 0 && a.lse) a.lse[(long long)row * a.q_heads + first_q + h] = sum == 0.f ? -INFINITY : (most + log2f(sum * (1.f / kWeight))) * kLn2;
     }
     cluster.sync();  // the others' reads of this CTA's part are over
   } else if (tid == 0) {
@@ -992,7 +994,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Args a) {
     const float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) out[e] = from_float<T>(sum == 0.f ? 0.f : r[e] / sum);
-    if (col == 0 && a.lse) a.lse[(long long)b * a.q_heads + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum) - kShift) * kLn2;
+    if (col == 0 && a.lse) a.lse[(long long)b * a.q_heads + qh] = sum == 0.f ? -INFINITY : (top + log2f(sum * (1.f / kWeight))) * kLn2;
   }
 }
 
