@@ -33,8 +33,8 @@
 //
 // Measured (device time, replayed from a graph; the bytes at 6.56 TB/s in
 // brackets): one row, 4096 to 4096, rank 16, bf16: 6.1 us, latency alone; 61
-// rows with 55 adapters of rank 64, 4096 to 16384, fp16, 149 MB: 38.2 us
-// (22.7); 8191 rows of five prompts, rank 16, bf16, 203 MB: 44.9 us (30.9),
+// rows with 55 adapters of rank 64, 4096 to 16384, fp16, 149 MB: 39.2 us
+// (22.7); 8191 rows of five prompts, rank 16, bf16, 203 MB: 45.1 us (30.9),
 // where all CTAs read x and then update the outputs at about the same time.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

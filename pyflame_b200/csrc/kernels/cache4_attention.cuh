@@ -53,12 +53,12 @@
 //
 // Measured (device time, replayed from a graph; the bytes at 6.56 TB/s in
 // brackets): 128 sequences of 2048 to 8192 keys, bf16, 32/8 heads of 128,
-// groups of 64, 757 MB: 168 us (115); 48 of 0 to 8192, fp16, groups of 32: 88
-// us (38.5); one of 131071, 64/8 heads, bf16: 43.1 us (23); one of 333 with a
-// window of 250, fp32, 20 heads of 80: 5.9 us.  The long ones are bound by
-// their instructions, 720 for a warp's 32 keys (920 with groups of 32 and
-// weights in two parts), of which 59 % of the issue slots are used: with all
-// keys in L2 they take as long.
+// groups of 64, 757 MB: 166 us (115); 48 of 0 to 8192, fp16, groups of 32: 81
+// us (38.5); one of 131071, 64/8 heads, bf16: 53 us (23); one of 333 with a
+// window of 250, fp32, 20 heads of 80: 6.1 us.  The long ones are bound by their
+// instructions, 590 for a warp's 32 keys (groups of 32 750, 8 heads 770), and by
+// what few warps an SM, 12 or 16, hide of latencies: 52 to 58 % of the issue
+// slots are used.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -890,14 +890,12 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
 }
 
 // A join's shares are split among groups of its threads.  Few units have many
-// shares each: one CTA for a unit, of all the threads that it may have (two
-// sequences of 86832 and 696 keys on one key-value head, pages of 7: the call
-// took 42.4 us with 256 threads, 20.6 so; one of 8 units 45.7 and 43.1).  With
-// 1024 threads in a CTA for each CTA of the first kernel, most of which have
-// nothing to join, that of 8 units took 58.  Many units have few shares each,
-// and a CTA of 256 for each CTA of the first kernel, with no unit to look for
-// (bf16, heads of 128, us in that form and in this: 16 units 23.3 and 24.3, 32
-// 24.4 and 24.7, 48 32.5 and 28.8, 128 44.9 and 34.8).
+// shares each: one CTA for a unit, of all the threads that it may have.  Many
+// units have few shares each, and a CTA of 256 for each CTA of the first kernel,
+// with no unit to look for (whole calls, bf16, heads of 128, us in the first form
+// and in the second: 1 unit of 60000 keys 16.7 and 24.4, 8 33.8 and 35.1, 16 of
+// up to 30000 22.9 and 23.6, 32 of up to 16384 23.9 and 24.1, 48 32.5 and 28.8,
+// 128 44.6 and 34.4).
 constexpr int kFewUnits = 32;
 
 // CTA (c, h): joins the shares of query head h of a unit that went on beyond

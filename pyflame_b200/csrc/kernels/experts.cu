@@ -33,8 +33,8 @@
 // (streamed.cuh): the copies run ahead over the borders of rows and experts.
 //
 // Measured (device time, replayed from a graph; the bytes at 6.56 TB/s in
-// brackets): 64 tokens, 8 of 128 experts, 2048 x 768, fp16, 1.19 GB: 225 us
-// (181), of which route and list 21, up 124 and down 85; one token, 6 of 64
+// brackets): 64 tokens, 8 of 128 experts, 2048 x 768, fp16, 1.19 GB: 231 us
+// (181), of which route and list 22, up 132 and down 84; one token, 6 of 64
 // experts, 2048 x 1408, bf16, 104 MB: 32.6 us (15.9), route 8.7, up 15.6 and
 // down 10.5, of which 8 stay when its weights are in L2: what begins and ends
 // a kernel; five tokens, 2 of 8 experts, 768 x 2048, fp32: 40 us (17.6).
