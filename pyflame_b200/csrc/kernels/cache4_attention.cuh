@@ -21,17 +21,17 @@
 // two parts (2^-22) for fp32.  p step enters as a multiple of a power of two
 // that follows the largest product of its head and group so far (the largest
 // step may be that of a key without weight), in two parts, which lose 2^-22 of
-// a product, or 2^-25 of that power, of which the largest is near 2^8: one alone,
-// 2^-11, showed in bf16 outputs, whose error rose from 1.64e-3 to 1.72e-3.  An instruction has
-// eight columns: a unit of up to four heads has the two parts of a head side by
-// side, so that a lane has the weights of one head and adds both parts' sums
-// (128 sequences, bf16: 165 us; two instructions took 200, and one part alone,
-// with two heads a lane, 169); more heads take two instructions (one sequence
-// of 131071, 8 heads a unit, bf16: 53 us; one part took 43).  For fp32 the
-// codes are centred, c - 8 (four
-// instructions a word more): with many keys the values average out, and the
-// large part that codes from 0 on have in common lost 5e-5 of what remains to
-// the tensor cores' truncation.
+// a product (2^-21 where 16-bit calls truncate the high one), or 2^-25 of that
+// power, of which the largest is near 2^8: one alone, 2^-11, showed in bf16
+// outputs, whose error rose from 1.66e-3 to 1.72e-3.  An instruction has eight
+// columns: a unit of up to four heads has the two parts of a head side by side,
+// so that a lane has the weights of one head and adds both parts' sums (128
+// sequences, bf16: 166 us; two instructions took 200, and one part alone, with
+// two heads a lane, 169); more heads take two instructions (one sequence of
+// 131071, 8 heads a unit, bf16: 53 us; one part took 43).  For fp32 the codes
+// are centred, c - 8 (four instructions a word more): with many keys the values
+// average out, and the large part that codes from 0 on have in common lost 5e-5
+// of what remains to the tensor cores' truncation.
 //
 // Work.  As for the cache in the model's type: a unit is one sequence, one
 // key-value head and up to 8 of its query heads; its keys are cut into tiles,
@@ -258,6 +258,7 @@ struct Layout {
   static constexpr int kQParts = sizeof(T) == 4 ? 2 : 1;
   static constexpr int kPParts = BESIDE ? 1 : 2;  // instructions for a weight's parts
   static constexpr int kOwn = BESIDE ? 1 : 2;     // heads of a lane
+  static constexpr unsigned kRound = sizeof(T) == 4 ? 0x1000 : 0;  // BESIDE: high parts are rounded, or truncated
   static constexpr bool kCentred = sizeof(T) == 4;
   // what the codes' operands and q's scaling leave to multiply with
   static constexpr int kQShift = kCentred ? -14 : 10;  // of 2, with q's exponent
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
             for (int h = 0; h < H; ++h) z[n][h] = fmaf(p[r][H * i + h], low, z[n][h]);
             const float x = p[r][H * i] * __uint_as_float(L::kInverse - unit_of[n][0]) * st;
             if constexpr (BESIDE) {  // both parts, next to each other
-              const float hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);  // 11 bits of x
+              const float hi = __uint_as_float((__float_as_uint(x) + L::kRound) & 0xffffe000u);  // 11 bits of x
               pt[r][0][i] = transpose8x8(pack_half(hi, x - hi));
             } else {
               const float y = p[r][H * i + 1] * __uint_as_float(L::kInverse - unit_of[n][H - 1]) * st;
