@@ -516,7 +516,10 @@ __global__ void __launch_bounds__(kThreads, (Layout<T, W, G, RUNS, BESIDE>::kRes
       // its exponent, not so low that the factor leaves fp32's range
       const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);
       const float times = __uint_as_float((unsigned)(127 + 14 - e) << 23);
-      if (lane == 0) factors[h] = a.scale * kLog2e * exp2f((float)(e + L::kQShift));
+      if (lane == 0) {  // times 2^(e + kQShift), in two steps: the power alone may leave fp32's range
+        const int half = (e + L::kQShift) >> 1, rest = e + L::kQShift - half;
+        factors[h] = a.scale * kLog2e * __uint_as_float((unsigned)(127 + half) << 23) * __uint_as_float((unsigned)(127 + rest) << 23);
+      }
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < B; ++j) {

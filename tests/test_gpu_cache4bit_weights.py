@@ -9,7 +9,7 @@ import torch
 
 import pyflame_b200 as pf
 
-from .test_gpu_cache4bit import F16, HALF, TINY, TYPES, fill, gen, randn, reference, within
+from .test_gpu_cache4bit import BF16, F16, F32, HALF, TINY, TYPES, check_attend, fill, gen, randn, reference, within
 
 pytestmark = pytest.mark.gpu
 WEIGHT = 2.0 ** -18
@@ -105,3 +105,13 @@ def test_values_at_both_ends_of_the_type(dtype, n, heads):
         v[3] = 2.0 ** 120 * torch.rand(1, 64, generator=g, device="cuda")
         c, q, table, lens = far_apart(g, dtype, n, 1, 16, v, [(3, -200.0)])
         check_far_apart(c, q, table, lens)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("each,lens", [(2, [70]), (4, [9000, 5]), (8, [9000, 5])])
+def test_queries_next_to_the_largest_numbers(dtype, each, lens):
+    """Queries of 2^118 and a scale that brings their scores back."""
+    g = gen(each)
+    c, table, n = fill(g, lens, 16, 1, 64, 64, dtype)
+    q = (2.0 ** 118 * randn(g, len(lens), each, 64)).to(dtype)
+    check_attend(c, q, table, n, scale=2.0 ** -121)
