@@ -26,7 +26,7 @@
 // outputs, whose error rose from 1.66e-3 to 1.72e-3.  An instruction has eight
 // columns: a unit of up to four heads has the two parts of a head side by side,
 // so that a lane has the weights of one head and adds both parts' sums (128
-// sequences, bf16: 166 us; two instructions took 200, and one part alone, with
+// sequences, bf16: 165 us; two instructions took 200, and one part alone, with
 // two heads a lane, 169); more heads take two instructions (one sequence of
 // 131071, 8 heads a unit, bf16: 53 us; one part took 43).  For fp32 the codes
 // are centred, c - 8 (four instructions a word more): with many keys the values
@@ -53,9 +53,9 @@
 //
 // Measured (device time, replayed from a graph; the bytes at 6.56 TB/s in
 // brackets): 128 sequences of 2048 to 8192 keys, bf16, 32/8 heads of 128,
-// groups of 64, 757 MB: 166 us (115); 48 of 0 to 8192, fp16, groups of 32: 81
+// groups of 64, 757 MB: 165 us (115); 48 of 0 to 8192, fp16, groups of 32: 79
 // us (38.5); one of 131071, 64/8 heads, bf16: 53 us (23); one of 333 with a
-// window of 250, fp32, 20 heads of 80: 6.1 us.  The long ones are bound by their
+// window of 250, fp32, 20 heads of 80: 5.9 us.  The long ones are bound by their
 // instructions, 590 for a warp's 32 keys (groups of 32 750, 8 heads 770), and by
 // what few warps an SM, 12 or 16, hide of latencies: 52 to 58 % of the issue
 // slots are used.
